@@ -137,6 +137,87 @@ int tlg_dev_xent(const float *logits, const int *tgt, float *dlogits, float *los
 int tlg_dev_xent_rows(const float *logits, const int *tgt, float *dlogits, double *rows, float scale, int N, int V,
                       void *stream);
 
+/* ---- rows of logits: log probabilities and distillation ------------------
+ * Operators over logits [N][V] of element type `type`, row n at logits + n * ld
+ * elements (ld >= V; what lies between the rows is neither read nor written).
+ * V is 1 .. TLG_VOCAB_MAX and need not be a multiple of anything; pointers
+ * need the alignment of their elements only.  Sums are fp32 or wider and every
+ * output is rounded once.  Only the caller's buffers are used: calls may
+ * overlap on any streams as long as their outputs and workspaces differ, and
+ * any call can be captured into a graph.  Results do not depend on the number
+ * of rows beside a row, except for the order of its fp32 sums.
+ *
+ * A logit of -inf is a masked token (probability 0).  A row of nothing but
+ * -inf has no distribution: its log probabilities are -inf, its entropy 0, its
+ * gradient 0.  A NaN or +inf makes its row's results NaN.  Token ids below 0
+ * mean "none" (padding), ids from V on make their result or row NaN.  A
+ * gradient row whose coefficients are all zero (a padded row) is written as
+ * zeros whatever its logits hold. */
+enum { TLG_F32 = 0, TLG_F16 = 1, TLG_BF16 = 2 };     /* element types (IEEE fp32 and fp16, bfloat16) */
+#define TLG_VOCAB_MAX (1 << 20)                       /* columns of a row */
+#define TLG_VOCAB_IDS 64                              /* given tokens of a row */
+#define TLG_VOCAB_TOP 128                             /* alternatives, teacher entries of a row */
+
+/* Log probabilities of given tokens with entropy and top alternatives (the
+ * reference's `score` and `nll` commands sum such log probabilities over a
+ * text; no counterpart as one call).  With z = scale * x, scale =
+ * 1 / temperature > 0, of each row x:
+ *   logp[n][j]   = log softmax(z)[ids[n][j]], j < M (0 for an id below 0)
+ *   lse2[n]      = {max x, log sum_v e^(scale (x_v - max x))}: the log-sum-exp
+ *                  scale * lse2[0] + lse2[1] in two parts, whose sum would lose
+ *                  the digits a large maximum takes
+ *   entropy[n]   = -sum_v p_v log p_v
+ *   top_ids[n][], top_logp[n][]: the K largest unmasked x in descending order,
+ *                  the lower index first among equals, and their log
+ *                  probabilities; -1 and -inf where fewer are left
+ * lse2 and entropy may be NULL; M <= TLG_VOCAB_IDS, K <= TLG_VOCAB_TOP, either
+ * may be 0.  ws: tlg_logprobs_ws_bytes(type, N, V, K) bytes, 16-byte aligned,
+ * of any content (NULL when that is 0). */
+size_t tlg_logprobs_ws_bytes(int type, int N, int V, int K);
+int tlg_dev_logprobs(const void *logits, int type, long long ld, int N, int V, float scale, const int *ids, int M,
+                     float *logp, float *lse2, float *entropy, int K, int *top_ids, float *top_logp, void *ws,
+                     size_t ws_bytes, void *stream);
+
+/* The gradient of tlg_dev_logprobs' outputs with respect to the logits, e.g.
+ * of a policy-gradient loss with an entropy bonus: with the gradients dlogp
+ * [N][M], dlse [N] (of scale * lse2[0] + lse2[1]) and dentropy [N] (each may be
+ * NULL: zero; dlogp only with M = 0),
+ *   dz_v = sum_j dlogp_j (1{v = ids_j} - p_v) + dlse p_v
+ *          - dentropy p_v (log p_v + entropy)
+ * and dlogits = scale * dz, of the logits' type, rows ldd elements apart; it
+ * may be the logits themselves (same address and ld), else it must not overlap
+ * them.  lse2 and entropy (with dentropy) are the forward's.  An id given twice
+ * counts twice. */
+int tlg_dev_logprobs_bwd(const void *logits, int type, long long ld, int N, int V, float scale, const int *ids, int M,
+                         const float *lse2, const float *entropy, const float *dlogp, const float *dlse,
+                         const float *dentropy, void *dlogits, long long ldd, void *stream);
+
+/* Distillation from a teacher's top log probabilities, with the hard-target
+ * cross-entropy, loss and gradient in one call (as tlg_dev_xent is for the
+ * latter alone).  The teacher gives row n K tokens t_ids[n][] and their log
+ * probabilities t_logp[n][] at temperature temp, as tlg_dev_logprobs(scale =
+ * 1 / temp) writes them; a negative id is no entry, an id given twice counts at
+ * its first place.  With S the row's ids, p = softmax(x / temp):
+ *   rows[n] = w_kd temp^2 KL_n + w_ce CE_n,  CE_n = -log softmax(x)[tgt[n]]
+ *   tail 0: q = the entries' e^t_logp normalised to sum 1,
+ *           KL = sum_{k in S} q_k (log q_k - log p_k)
+ *   tail 1: q_k = e^t_logp_k, and what they leave, q_r = max(0, 1 - sum q_k), is
+ *           one more outcome: + q_r (log q_r - log p_r), p_r = sum_{v not in S}
+ *           p_v; no remainder when S is the whole vocabulary
+ *   dlogits_v = scale d rows[n] / d x_v
+ *         = scale (w_kd temp (Q p_v - q_v) + w_ce (softmax(x)_v - 1{v = tgt}))
+ *           with Q = sum q (+ q_r), outside S Q - q_r / p_r (tail 1)
+ * and loss[0] = the mean of rows over the N rows (summed in double).  Rows
+ * without an entry have KL 0, with a negative target CE 0.  rows may be NULL
+ * (then loss too) if dlogits is given, and dlogits if rows is; dlogits as in
+ * tlg_dev_logprobs_bwd.  t_ids and t_logp may be NULL with K = 0, tgt with
+ * w_ce = 0.  ws: tlg_distill_ws_bytes(type, N, V) bytes, 16-byte aligned, of
+ * any content (NULL when that is 0). */
+size_t tlg_distill_ws_bytes(int type, int N, int V);
+int tlg_dev_distill(const void *logits, int type, long long ld, int N, int V, const int *t_ids, const float *t_logp,
+                    int K, int tail, float temp, float w_kd, const int *tgt, float w_ce, float *rows, float *loss,
+                    void *dlogits, long long ldd, float scale, void *ws, size_t ws_bytes, void *stream);
+
 /* global_gradnorm, tinylm.c:1171-1176: norm[0] = sqrt(sum G^2) (double sum). */
 int tlg_dev_gradnorm(const float *G, size_t n, float *norm, void *stream);
 /* tlg_dev_gradnorm that also sets loss[0] = the mean of rows[0, N) from

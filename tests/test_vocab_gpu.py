@@ -1,0 +1,815 @@
+"""GPU tests of the operators over rows of logits (include/tltrain.h): log
+probabilities with entropy and alternatives, their gradient, distillation,
+against plain float64 evaluations of their definitions.
+
+Tolerances.  eps = 2^-24, half a step of fp32.  An exponential e^z', z' = s (x -
+m), is formed from the rounded difference, a product with a rounded constant
+and a hardware exponential of one unit in the last place: relative error
+<= eps (4 |z'| + 3).  A sum of a row runs over at most C(V) = 64 + V / 256
+sequential fp32 additions, rescalings among them, each off by eps at most.  With
+weights p the mean |z'| is entropy - log S <= log V, so S is off by rho = eps (4
+log V + 3 + C) relative and log S by rho + 2 eps |log S| absolute.  The other
+bounds follow from these term by term, as written at each check.  Outputs in
+fp16 or bf16 add the half step of their type (fp16 below its normal range
+2^-25 absolute).
+"""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+EPS = 2.0 ** -24
+F32, F16, BF16 = 0, 1, 2
+NAMES = {F32: "f32", F16: "f16", BF16: "bf16"}
+
+
+def _t():
+    import torch
+    return torch
+
+
+def dtype(ty):
+    t = _t()
+    return {F32: t.float32, F16: t.float16, BF16: t.bfloat16}[ty]
+
+
+def half_step(ty):
+    return {F32: EPS, F16: 2.0 ** -11, BF16: 2.0 ** -8}[ty]
+
+
+def tiny(ty):
+    """Half the smallest step of the type, where relative bounds end."""
+    return {F32: 2.0 ** -126, F16: 2.0 ** -25, BF16: 2.0 ** -126}[ty]
+
+
+def stream():
+    return _t().cuda.current_stream().cuda_stream
+
+
+def chain(V):
+    return 64 + V / 256
+
+
+def rho(V):
+    return EPS * (4 * math.log(V + 1) + 3 + chain(V))
+
+
+def rows_of(ty, N, V, ld=None, off=0, seed=0, spread=2.5, fill=float("nan")):
+    """Logits [N][V] in rows ld apart that start `off` elements into a buffer,
+    with `fill` between and around them."""
+    t = _t()
+    ld = ld or V
+    g = t.Generator().manual_seed(seed + 7919 * V + N)
+    buf = t.full((off + N * ld + 16,), fill, dtype=dtype(ty))
+    x = t.as_strided(buf, (N, V), (ld, 1), off)
+    x.copy_((spread * t.randn(N, V, generator=g)).to(dtype(ty)))
+    return buf, (N, V), (ld, 1), off
+
+
+def on_gpu(rows):
+    buf, shape, strides, off = rows
+    b = buf.cuda()
+    return b, _t().as_strided(b, shape, strides, off)
+
+
+def like_rows(x, ty, fill=float("nan")):
+    """A gradient buffer of x's layout, filled."""
+    t = _t()
+    b = t.full((x.storage_offset() + x.shape[0] * x.stride(0) + 16,), fill, dtype=dtype(ty), device="cuda")
+    return b, t.as_strided(b, tuple(x.shape), (x.stride(0), 1), x.storage_offset())
+
+
+def f64(x):
+    return x.detach().cpu().double().numpy()
+
+
+# ------------------------------------------------------------- definitions --
+def ref_logp(x, scale):
+    """x [N][V] float64 -> (log probabilities, m, log S, entropy)."""
+    with np.errstate(all="ignore"):
+        m = x.max(1, keepdims=True)
+        z = np.where(np.isneginf(m), -np.inf, (x - m) * scale)
+        z[np.isnan(x)] = np.nan
+        S = np.exp(z).sum(1, keepdims=True)
+        lp = z - np.log(S)
+        lp[np.isneginf(m[:, 0])] = -np.inf
+        p = np.exp(lp)
+        H = -np.where(p > 0, p * lp, 0.0).sum(1)
+        H = np.where(np.isnan(S[:, 0]), np.nan, H)
+    return lp, m[:, 0], np.log(S[:, 0]), H
+
+
+def ref_top(x, K):
+    """The K largest unmasked values of every row, the lower index first among
+    equals; -1 where fewer are left."""
+    out = np.full((x.shape[0], K), -1, np.int64)
+    for n, row in enumerate(x):
+        order = np.argsort(-row, kind="stable")
+        order = order[row[order] > -np.inf][:K]
+        out[n, :len(order)] = order
+    return out
+
+
+def ref_bwd(x, scale, ids, dlogp, dlse, dent):
+    lp, _, _, H = ref_logp(x, scale)
+    p = np.exp(lp)
+    d = p * (dlse - np.where(ids >= 0, dlogp, 0.0).sum(1))[:, None]
+    d -= dent[:, None] * np.where(p > 0, p * (np.where(p > 0, lp, 0.0) + H[:, None]), 0.0)
+    for n in range(x.shape[0]):
+        if np.isneginf(x[n]).all():
+            continue
+        for j, i in enumerate(ids[n]):
+            if i >= 0:
+                d[n, i] += dlogp[n, j]
+    return d * scale
+
+
+def ref_distill(x, ids, tl, tail, tau, w_kd, tgt, w_ce):
+    """(rows, d rows / d x) in float64."""
+    N, V = x.shape
+    rows, grad = np.zeros(N), np.zeros((N, V))
+    lp, lp1 = ref_logp(x, 1.0 / tau)[0], ref_logp(x, 1.0)[0]
+    for n in range(N):
+        q, seen = np.zeros(V), np.zeros(V, bool)
+        for i, l in zip(ids[n], tl[n]):
+            if i >= 0 and not seen[i]:
+                seen[i], q[i] = True, math.exp(l)
+        p = np.exp(lp[n])
+        qr = 0.0
+        if not tail:
+            q = q / q.sum() if q.sum() > 0 else q
+        elif seen.any() and not seen.all():
+            qr = max(0.0, 1.0 - q.sum())
+        on = q > 0
+        kl = (q[on] * (np.log(q[on]) - lp[n][on])).sum()
+        mass = (q.sum() + qr) * np.ones(V)
+        if qr > 0:
+            pr = p[~seen].sum()
+            with np.errstate(all="ignore"):
+                kl += qr * (math.log(qr) - np.log(pr))
+                mass[~seen] = (q.sum() + qr) - (qr / pr if pr > 0 else 0.0)
+        rows[n] = w_kd * tau * tau * kl
+        grad[n] = w_kd * tau * (mass * p - q)
+        if w_ce and tgt[n] >= 0:
+            rows[n] -= w_ce * lp1[n, tgt[n]]
+            grad[n] += w_ce * np.exp(lp1[n])
+            grad[n, tgt[n]] -= w_ce
+    return rows, grad
+
+
+# ------------------------------------------------------------------- calls --
+class Out:
+    pass
+
+
+def logprobs(lib, x, ty, scale, ids, K, ws_fill=255):
+    t = _t()
+    N, V = x.shape
+    o = Out()
+    M = 0 if ids is None else ids.shape[1]
+    nan = float("nan")
+    o.logp = t.full((N, M), nan, device="cuda")
+    o.lse2 = t.full((N, 2), nan, device="cuda")
+    o.entropy = t.full((N,), nan, device="cuda")
+    o.top_ids = t.full((N, K), -77, device="cuda", dtype=t.int32)
+    o.top_logp = t.full((N, K), nan, device="cuda")
+    nb = lib.tlg_logprobs_ws_bytes(ty, N, V, K)
+    o.ws = t.full((nb + 16,), ws_fill, device="cuda", dtype=t.uint8)
+    lib.logprobs(x.data_ptr(), ty, x.stride(0), N, V, scale, ids.data_ptr() if M else None, M, o.logp.data_ptr(),
+                 o.lse2.data_ptr(), o.entropy.data_ptr(), K, o.top_ids.data_ptr(), o.top_logp.data_ptr(),
+                 o.ws.data_ptr(), nb, stream())
+    return o
+
+
+def logprobs_bwd(lib, x, ty, scale, ids, lse2, entropy, dlogp, dlse, dent, d):
+    M = 0 if ids is None else ids.shape[1]
+
+    def p(v):
+        return None if v is None else v.data_ptr()
+    lib.logprobs_bwd(x.data_ptr(), ty, x.stride(0), x.shape[0], x.shape[1], scale, p(ids), M, p(lse2), p(entropy),
+                     p(dlogp), p(dlse), p(dent), d.data_ptr(), d.stride(0), stream())
+
+
+def distill(lib, x, ty, t_ids, t_logp, tail, tau, w_kd, tgt, w_ce, d, scale=1.0, ws_fill=255):
+    t = _t()
+    N, V = x.shape
+    K = 0 if t_ids is None else t_ids.shape[1]
+    o = Out()
+    o.rows = t.full((N,), float("nan"), device="cuda")
+    o.loss = t.full((1,), float("nan"), device="cuda")
+    nb = lib.tlg_distill_ws_bytes(ty, N, V)
+    o.ws = t.full((nb + 16,), ws_fill, device="cuda", dtype=t.uint8)
+    lib.distill(x.data_ptr(), ty, x.stride(0), N, V, t_ids.data_ptr() if K else None,
+                t_logp.data_ptr() if K else None, K, int(tail), tau, w_kd, None if tgt is None else tgt.data_ptr(),
+                w_ce, o.rows.data_ptr(), o.loss.data_ptr(), None if d is None else d.data_ptr(),
+                0 if d is None else d.stride(0), scale, o.ws.data_ptr(), nb, stream())
+    return o
+
+
+# ------------------------------------------------------------------ checks --
+def close(got, want, tol, what):
+    """got within tol of want element by element; infinities and NaN equal."""
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    inf = np.isinf(want)
+    assert np.array_equal(got[inf], want[inf]), what
+    err, bar = np.abs(got - want)[fin], np.broadcast_to(tol, want.shape)[fin]
+    if err.size:
+        k = int(np.argmax(err - bar))
+        assert (err <= bar).all(), (what, "worst", err[k], "allowed", bar[k])
+
+
+def check_logprobs(o, x, scale, ids, K):
+    X = f64(x)
+    V = X.shape[1]
+    lp, m, ls, H = ref_logp(X, scale)
+    bad = np.isnan(ls)
+    tol_ls = rho(V) + 2 * EPS * np.abs(np.where(np.isfinite(ls), ls, 0.0))
+    close(f64(o.lse2)[:, 0], np.where(bad, np.nan, m), 0.0, "max")
+    close(f64(o.lse2)[:, 1], np.where(np.isneginf(m), -np.inf, ls), tol_ls, "log sum")
+
+    def tol_lp(v):       # two roundings of z', log S, the final one
+        v = np.where(np.isfinite(v), np.abs(v), 0.0)
+        return 4 * EPS * (v + np.abs(np.where(np.isfinite(ls), ls, 0.0))[:, None]) + tol_ls[:, None]
+    if ids is not None and ids.shape[1]:
+        I = ids.cpu().numpy()
+        want = np.take_along_axis(lp, np.clip(I, 0, V - 1), 1)
+        want = np.where(I < 0, 0.0, np.where(I >= V, np.nan, want))
+        close(f64(o.logp), want, tol_lp(want), "logp")
+    # H = log S - u / S, both sums rho-close; |u / S| <= log V
+    lv = math.log(V + 1)
+    tol_H = tol_ls + 2 * (rho(V) + 4 * EPS) * lv + 2 * EPS * np.abs(np.where(np.isfinite(H), H, 0.0))
+    close(f64(o.entropy), np.where(np.isneginf(m), 0.0, H), tol_H, "entropy")
+    if K:
+        top = ref_top(X, K)
+        top[bad] = -1
+        assert np.array_equal(o.top_ids.cpu().numpy(), top), "top ids"
+        want = np.where(top < 0, -np.inf, np.take_along_axis(lp, np.clip(top, 0, V - 1), 1))
+        want[bad] = np.nan
+        close(f64(o.top_logp), want, tol_lp(want), "top logp")
+
+
+def some_ids(N, V, M, seed, none=True):
+    t = _t()
+    g = t.Generator().manual_seed(seed)
+    ids = t.randint(0, V, (N, M), generator=g, dtype=t.int32)
+    if none and N > 1:
+        ids[N // 2, 0] = -1
+    return ids.cuda()
+
+
+SIZES = [(1, 1, 1), (3, 2, 2), (2, 3, 5), (5, 7, 4), (4, 31, 40), (3, 64, 64), (9, 65, 8), (2, 255, 128), (3, 257, 20),
+         (5, 1000, 16), (7, 2047, 33), (130, 2048, 8), (3, 2049, 128), (2, 4097, 60), (6, 8191, 5), (1, 16384, 128),
+         (3, 32003, 32), (1, 65537, 20), (2, 131072, 100)]
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V,K", SIZES)
+def test_logprobs(lib, ty, N, V, K):
+    print("logprobs", NAMES[ty], N, V, K, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V))
+    M = 1 + V % 3
+    ids = some_ids(N, V, M, V)
+    for scale in (1.0, 1.0 / 0.7):
+        check_logprobs(logprobs(lib, x, ty, scale, ids, K), x, scale, ids, K)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V,ld,off", [(3, 1000, 1003, 1), (2, 2048, 2051, 3), (5, 333, 340, 7), (2, 40001, 40010, 5),
+                                        (300, 777, 900, 2)])
+def test_logprobs_any_alignment_and_stride(lib, ty, N, V, ld, off):
+    """Rows that start at every element offset; NaN lies between the rows."""
+    print("alignment", NAMES[ty], N, V, ld, off, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, ld, off))
+    ids = some_ids(N, V, 2, V)
+    check_logprobs(logprobs(lib, x, ty, 1.0, ids, 10), x, 1.0, ids, 10)
+
+
+def test_logprobs_optional_outputs(lib):
+    """No given tokens, no alternatives, no statistics asked for: what is
+    written is the same."""
+    t = _t()
+    for N, V in ((3, 300), (1, 70000), (300, 3000)):
+        _, x = on_gpu(rows_of(F32, N, V))
+        ids = some_ids(N, V, 1, 3)
+        full = logprobs(lib, x, F32, 1.0, ids, 9)
+        nb = lib.tlg_logprobs_ws_bytes(F32, N, V, 0)
+        ws = t.empty(nb + 16, dtype=t.uint8, device="cuda")
+        lg = t.full((N, 1), float("nan"), device="cuda")
+        lib.logprobs(x.data_ptr(), F32, V, N, V, 1.0, ids.data_ptr(), 1, lg.data_ptr(), None, None, 0, None, None,
+                     ws.data_ptr(), nb, stream())
+        ent = t.full((N,), float("nan"), device="cuda")
+        lib.logprobs(x.data_ptr(), F32, V, N, V, 1.0, None, 0, None, None, ent.data_ptr(), 0, None, None,
+                     ws.data_ptr(), nb, stream())
+        tol = 2 * (rho(V) + 8 * EPS * 20)
+        close(f64(lg), f64(full.logp), tol, "logp alone")
+        close(f64(ent), f64(full.entropy), tol * math.log(V), "entropy alone")
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V", [(4, 100), (4, 2048), (3, 40000), (260, 5000)])
+def test_ties_go_to_the_lowest_index(lib, ty, N, V):
+    """Rows of equal values, of few different values, of both zeros."""
+    t = _t()
+    print("ties", NAMES[ty], N, V, flush=True)
+    g = t.Generator().manual_seed(5)
+    x = t.zeros(N, V)
+    x[1] = t.randint(0, 3, (V,), generator=g).float()
+    x[2] = t.where(t.rand(V, generator=g) < 0.5, -0.0, 0.0)
+    if N > 3:
+        x[3] = -t.randint(0, V // 50 + 1, (V,), generator=g).float() / 16
+    x = x.to(dtype(ty)).cuda()
+    for K in (1, 7, 64, 128):
+        check_logprobs(logprobs(lib, x, ty, 1.0, None, K), x, 1.0, None, K)
+
+
+@pytest.mark.parametrize("ty", [F32, BF16])
+@pytest.mark.parametrize("step", [1, 4, 8, 64 * 4, 64 * 8, 256 * 4, 256 * 8, 1024 * 4, 1024 * 8])
+def test_alternatives_that_lie_together(lib, ty, step):
+    """The largest values all in one column of the row's vectors (the same
+    thread's, whatever the kernel's width), ascending and descending, and rows
+    in sorted order: far more candidates than a random row has."""
+    t = _t()
+    print("together", NAMES[ty], step, flush=True)
+    for V in (2048, 60000):
+        g = t.Generator().manual_seed(step)
+        x = t.randn(4, V, generator=g)
+        at = t.arange(3 if V > 3 else 0, V, step)[:700]
+        x[0, at] = 20.0 + t.arange(len(at)) / 16
+        x[1, at] = 90.0 - t.arange(len(at)) / 16
+        x[2] = t.arange(V) / 4096
+        x[3] = -t.arange(V) / 4096
+        x = x.to(dtype(ty)).cuda()
+        for K in (5, 128):
+            check_logprobs(logprobs(lib, x, ty, 1.0, None, K), x, 1.0, None, K)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("V", [5, 300, 2048, 33001])
+@pytest.mark.parametrize("N", [8, 520])
+def test_masked_rows_infinities_and_nan(lib, ty, V, N):
+    """Rows that the mask leaves nothing or little of, the type's lowest value
+    as a mask, NaN and infinities, in the first eight of N rows."""
+    t = _t()
+    if N * V > 1 << 23:
+        N = 200
+    print("masked", NAMES[ty], N, V, flush=True)
+    lo = t.finfo(dtype(ty)).min
+    g = t.Generator().manual_seed(V)
+    x = 2 * t.randn(N, V, generator=g)
+    x[0] = -math.inf
+    x[1] = -math.inf
+    x[1, V - 1] = 3.0
+    x[2] = lo
+    x[3, : V - 2] = lo
+    x[4, V // 2] = math.nan
+    x[5, V // 3] = math.inf
+    x[6, t.rand(V, generator=g) < 0.9] = -math.inf
+    x[7] = -math.inf
+    x[7, 0], x[7, V // 2] = lo, -math.inf
+    x = x.to(dtype(ty)).cuda()
+    ids = some_ids(N, V, 3, V)
+    ids[2, 1] = V + 3
+    ids[0, 0], ids[0, 1] = 0, -1
+    check_logprobs(logprobs(lib, x, ty, 1.0, ids, 12), x, 1.0, ids, 12)
+
+
+def test_extreme_temperatures(lib):
+    """Almost greedy and almost uniform distributions."""
+    _, x = on_gpu(rows_of(F32, 5, 3000))
+    ids = some_ids(5, 3000, 2, 1)
+    for scale in (1e-4, 50.0, 2000.0):
+        check_logprobs(logprobs(lib, x, F32, scale, ids, 6), x, scale, ids, 6)
+
+
+# ---------------------------------------------------------------- gradient --
+def grad_tol(ty, X, scale, want, c0, c1, H, factor):
+    """|d p| <= p eps (4 |z'| + 2 |log S| + 8) for the recomputed probabilities,
+    its products with the coefficients, and the output's rounding."""
+    lp, _, ls, _ = ref_logp(X, scale)
+    with np.errstate(all="ignore"):
+        p = np.where(np.isfinite(lp), np.exp(lp), 0.0)
+        a = np.where(np.isfinite(lp), np.abs(lp), 0.0)
+        l = np.abs(np.where(np.isfinite(ls), ls, 0.0))[:, None]
+        h = np.abs(H)[:, None]
+        relp = EPS * (4 * (a + l) + 2 * l + 8)
+        t = p * (np.abs(c0)[:, None] * (relp + 80 * EPS) +
+                 np.abs(c1)[:, None] * (relp * (a + h) + 8 * EPS * (a + l + h + 1)))
+    return factor * t * 1.01 + (half_step(ty) * 1.01 + 70 * EPS) * np.abs(want) + tiny(ty)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V,M,pad,off", [(1, 1, 1, 0, 0), (3, 2, 2, 1, 1), (5, 65, 64, 0, 0), (4, 1000, 3, 3, 1),
+                                           (130, 2048, 1, 0, 0), (7, 2049, 5, 8, 3), (2, 40001, 4, 9, 5),
+                                           (1, 131072, 1, 0, 0)])
+def test_logprobs_bwd(lib, ty, N, V, M, pad, off):
+    t = _t()
+    print("logprobs_bwd", NAMES[ty], N, V, M, pad, off, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, off))
+    ids = some_ids(N, V, M, V)
+    g = t.Generator().manual_seed(V + 1)
+    dlogp, dlse, dent = (t.randn(*s, generator=g).cuda() for s in ((N, M), (N,), (N,)))
+    scale = 1.0 / 1.3
+    X = f64(x)
+    _, m, ls, H = ref_logp(X, scale)
+    lse2 = t.tensor(np.stack([m, ls], 1), dtype=t.float32, device="cuda")
+    ent = t.tensor(H, dtype=t.float32, device="cuda")
+    I, dl = ids.cpu().numpy(), f64(dlogp)
+    for use_lse, use_ent in ((True, True), (False, False), (False, True)):
+        a, b = (f64(dlse) if use_lse else np.zeros(N)), (f64(dent) if use_ent else np.zeros(N))
+        buf, d = like_rows(x, ty)
+        logprobs_bwd(lib, x, ty, scale, ids, lse2, ent, dlogp, dlse if use_lse else None, dent if use_ent else None, d)
+        want = ref_bwd(X, scale, I, dl, a, b)
+        c0 = np.abs(np.where(I >= 0, dl, 0.0)).sum(1) + np.abs(a)
+        tol = grad_tol(ty, X, scale, want, c0, b, H, scale)
+        # the given tokens' own terms cancel against p's
+        for n in range(N):
+            for j, i in enumerate(I[n]):
+                if i >= 0:
+                    tol[n, i] += scale * abs(dl[n, j]) * (M + 4) * EPS
+        close(f64(d), want, tol, "dlogits")
+        guard = buf.clone()
+        t.as_strided(guard, tuple(d.shape), (d.stride(0), 1), d.storage_offset()).fill_(float("nan"))
+        assert bool(t.isnan(guard).all()), "wrote outside its rows"
+
+
+def test_logprobs_bwd_in_place_and_repeated_ids(lib):
+    t = _t()
+    for ty in (F32, F16, BF16):
+        for N, V in ((70, 2051), (2, 50000)):
+            buf, x = on_gpu(rows_of(ty, N, V, V + 5, 1))
+            ids = some_ids(N, V, 6, 9)
+            ids[:, 3] = ids[:, 1]
+            f = logprobs(lib, x, ty, 1.0, ids, 0)
+            dlogp = t.randn(N, 6, device="cuda")
+            dent = t.randn(N, device="cuda")
+            _, d = like_rows(x, ty)
+            logprobs_bwd(lib, x, ty, 1.0, ids, f.lse2, f.entropy, dlogp, None, dent, d)
+            merged = ids.clone()
+            merged[:, 3] = -1
+            dm = dlogp.clone()
+            dm[:, 1] += dm[:, 3]
+            _, d2 = like_rows(x, ty)
+            logprobs_bwd(lib, x, ty, 1.0, merged, f.lse2, f.entropy, dm, None, dent, d2)
+            # the same sum in another order: a few roundings of the coefficients
+            lim = 16 * EPS * float(dlogp.abs().sum(1).max()) + half_step(ty) * 2.1 * float(d.abs().max())
+            assert float((d.double() - d2.double()).abs().max()) <= lim
+            logprobs_bwd(lib, x, ty, 1.0, ids, f.lse2, f.entropy, dlogp, None, dent, x)      # in place
+            assert t.equal(x, d)
+
+
+def test_logprobs_bwd_special_rows(lib):
+    """Masked rows give 0, padded rows 0 over any logits, NaN rows and token
+    ids past the vocabulary NaN."""
+    t = _t()
+    for N, V in ((8, 300), (8, 70001), (600, 2048)):
+        _, x = on_gpu(rows_of(F32, N, V))
+        x[0] = -math.inf
+        x[1, 5] = math.nan
+        x[2, 7] = math.nan
+        x[3, : V // 2] = -math.inf
+        ids = some_ids(N, V, 2, 4, none=False)
+        ids[0] = t.tensor([0, 3])
+        ids[2] = -1
+        ids[4, 1] = V
+        f = logprobs(lib, x, F32, 1.0, ids, 0)
+        dlogp, dent = t.randn(N, 2, device="cuda"), t.randn(N, device="cuda")
+        dent[2] = 0.0
+        _, d = like_rows(x, F32)
+        logprobs_bwd(lib, x, F32, 1.0, ids, f.lse2, f.entropy, dlogp, None, dent, d)
+        assert bool((d[0] == 0).all()) and bool((d[2] == 0).all())
+        assert bool(t.isnan(d[1]).all()) and bool(t.isnan(d[4]).all())
+        part = ids[3, 0] >= V // 2
+        assert bool((d[3, : V // 2][t.arange(V // 2, device="cuda") != ids[3, 0]][:100].isfinite()).all()) or part
+        assert bool(d[5:].isfinite().all())
+
+
+def test_logprobs_gradient_against_differences(lib):
+    """Directional central differences of the kernel's own forward."""
+    t = _t()
+    N, V, h = 6, 1500, 1.0 / 64
+    _, x = on_gpu(rows_of(F32, N, V))
+    ids = some_ids(N, V, 2, 11, none=False)
+    dlogp, dlse, dent = t.randn(N, 2, device="cuda"), t.randn(N, device="cuda"), t.randn(N, device="cuda")
+
+    def value(y):
+        o = logprobs(lib, y, F32, 0.8, ids, 0)
+        lse = 0.8 * o.lse2[:, 0].double() + o.lse2[:, 1].double()
+        return (dlogp.double() * o.logp.double()).sum(1) + dlse.double() * lse + dent.double() * o.entropy.double()
+    f = logprobs(lib, x, F32, 0.8, ids, 0)
+    _, d = like_rows(x, F32)
+    logprobs_bwd(lib, x, F32, 0.8, ids, f.lse2, f.entropy, dlogp, dlse, dent, d)
+    v = (t.randn(N, V, device="cuda") * 4).round().clamp(-8, 8) / 4          # x +- h v in few bits
+    num = (value(x + h * v) - value(x - h * v)) / (2 * h)
+    ana = (d.double() * v.double()).sum(1)
+    # third derivatives of these sums are at most a few times |v|^3 (cumulants of
+    # a variable in [-2, 2], entropy's with a factor log V); fp32 values / h
+    c = (dlogp.abs().sum(1) + dlse.abs() + dent.abs() * math.log(V)).double() + 1
+    bar = c * (h * h / 6 * 8 * 8 + 4 * (rho(V) * 2 * math.log(V) + 60 * EPS) / h)
+    assert bool(((num - ana).abs() <= bar).all()), (num, ana, bar)
+    assert float((ana.abs() / bar).max()) > 3, "differences that could not fail"
+
+
+# -------------------------------------------------------------- distillation --
+def teacher(x, K, tau, seed=1, noise=0.5):
+    t = _t()
+    g = t.Generator().manual_seed(seed)
+    y = (x.float().cpu().nan_to_num(0.0, 0.0, -30.0) + noise * t.randn(tuple(x.shape), generator=g)).double() / tau
+    lp = t.log_softmax(y, 1)
+    K1 = min(K, x.shape[1])
+    v, i = t.topk(lp, K1, dim=1)
+    ids, tl = t.full((x.shape[0], K), -1, dtype=t.int32), t.zeros(x.shape[0], K)
+    ids[:, :K1], tl[:, :K1] = i.int(), v.float()
+    return ids.cuda(), tl.cuda()
+
+
+def check_distill(o, d, ty, x, ids, tl, tail, tau, w_kd, tgt, w_ce, scale):
+    X = f64(x)
+    N, V = X.shape
+    I = np.zeros((N, 0), np.int64) if ids is None else ids.cpu().numpy()
+    T = np.zeros((N, 0)) if tl is None else f64(tl)
+    G = None if tgt is None else tgt.cpu().numpy()
+    rows, grad = ref_distill(X, I, T, tail, tau, w_kd, G, w_ce)
+    lp, _, ls, _ = ref_logp(X, 1.0 / tau)
+    lp1, _, ls1, _ = ref_logp(X, 1.0)
+    # rows: log probabilities off by tol_lp each, weighted by sum q = 1 (and the
+    # remainder's log p_r by rho twice); teacher terms are in 64 bits
+    fin = np.isfinite(rows)
+    a = np.where(np.isfinite(lp), np.abs(lp), 0.0).max(1) if V < 100000 else np.full(N, 60.0)
+    a1 = np.where(np.isfinite(lp1), np.abs(lp1), 0.0).max(1) if V < 100000 else np.full(N, 60.0)
+    tol = w_kd * tau * tau * (3 * rho(V) + 6 * EPS * (a + np.abs(ls))) + \
+        w_ce * (2 * rho(V) + 6 * EPS * (a1 + np.abs(ls1))) + 2 * EPS * np.abs(np.where(fin, rows, 0.0))
+    close(f64(o.rows), rows, tol, "rows")
+    if fin.all():
+        close(f64(o.loss), [rows.mean()], tol.mean() + 2 * EPS * abs(rows.mean()), "loss")
+    if d is None:
+        return
+    want = scale * grad
+    p, p1 = np.exp(lp), np.exp(lp1)
+    # p: exponentials and S; the remainder's Q - q_r / p_r carries 2 rho of its parts
+    with np.errstate(all="ignore"):
+        z, z1 = np.where(p > 0, np.abs(lp), 0.0), np.where(p1 > 0, np.abs(lp1), 0.0)
+        relp = EPS * (4 * (z + np.abs(ls)[:, None]) + 12) + rho(V)
+        relp1 = EPS * (4 * (z1 + np.abs(ls1)[:, None]) + 12) + rho(V)
+    ratio = np.ones(N)
+    if tail:
+        for n in range(N):
+            S = np.unique(I[n][I[n] >= 0])
+            out = np.delete(p[n], S).sum()
+            q = sum(math.exp(T[n, list(I[n]).index(s)]) for s in S)
+            ratio[n] = 2 + (max(0.0, 1 - q) / out if out > 0 else 0.0)
+    q = np.zeros((N, V))
+    for n in range(N):
+        q[n, I[n][I[n] >= 0]] = 1.0
+    bar = abs(scale) * (w_kd * tau * (p * ratio[:, None] * (relp + 3 * rho(V)) + q * 4 * EPS) +
+                        w_ce * (p1 * relp1 + 4 * EPS * (p1 > 1e-30)) * (0 if G is None else 1))
+    bar = bar + (half_step(ty) * 1.01 + 8 * EPS) * np.abs(want) + tiny(ty)
+    close(f64(d), want, bar, "dlogits")
+
+
+KD = [  # N, V, K, tail, tau, w_kd, w_ce, pad, off
+    (1, 2, 1, False, 1.0, 1.0, 0.0, 0, 0), (3, 5, 4, True, 1.0, 1.0, 0.5, 2, 1), (2, 7, 9, True, 2.0, 0.5, 0.5, 0, 0),
+    (5, 64, 64, False, 1.0, 1.0, 1.0, 0, 0), (4, 257, 20, True, 1.5, 1.0, 0.0, 1, 3), (3, 1000, 128, True, 1.0, 1.0, 0.3, 3, 1),
+    (70, 2048, 8, False, 2.0, 0.7, 0.3, 0, 0), (300, 2048, 32, True, 1.0, 1.0, 0.5, 0, 0), (9, 2051, 16, False, 0.7, 1.0, 0.0, 6, 5),
+    (2, 8192, 50, True, 1.0, 1.0, 0.0, 0, 0), (3, 16385, 64, False, 1.0, 1.0, 1.0, 3, 2), (2, 40001, 50, True, 1.0, 1.0, 0.5, 9, 5),
+    (1, 131072, 100, True, 1.0, 1.0, 0.0, 0, 0), (257, 5003, 12, True, 2.0, 1.0, 0.5, 0, 0), (2, 70000, 0, False, 1.0, 1.0, 1.0, 0, 0)]
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V,K,tail,tau,w_kd,w_ce,pad,off", KD)
+def test_distill(lib, ty, N, V, K, tail, tau, w_kd, w_ce, pad, off):
+    t = _t()
+    print("distill", NAMES[ty], N, V, K, tail, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, off))
+    ids, tl = teacher(x, K, tau) if K else (None, None)
+    tgt = t.randint(0, V, (N,), generator=t.Generator().manual_seed(2), dtype=t.int32).cuda()
+    if K and N > 1:
+        tgt[1] = ids[1, 0]                     # a target that the teacher names too
+    if N > 2:
+        tgt[2] = -1
+    if K and N > 4:
+        ids[3] = -1
+        ids[4], tgt[4] = -1, -1                # a padded row
+    scale = 1.0 / N
+    buf, d = like_rows(x, ty)
+    o = distill(lib, x, ty, ids, tl, tail, tau, w_kd, tgt if w_ce else None, w_ce, d, scale)
+    check_distill(o, d, ty, x, ids, tl, tail, tau, w_kd, tgt if w_ce else None, w_ce, scale)
+    guard = buf.clone()
+    t.as_strided(guard, tuple(d.shape), (d.stride(0), 1), d.storage_offset()).fill_(float("nan"))
+    assert bool(t.isnan(guard).all()), "wrote outside its rows"
+    # the loss alone, and in place
+    o2 = distill(lib, x, ty, ids, tl, tail, tau, w_kd, tgt if w_ce else None, w_ce, None, scale)
+    assert t.equal(o2.rows, o.rows) and t.equal(o2.loss, o.loss)
+    o3 = distill(lib, x, ty, ids, tl, tail, tau, w_kd, tgt if w_ce else None, w_ce, x, scale)
+    assert t.equal(o3.rows, o.rows) and t.equal(x, d)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("N,V", [(12, 300), (12, 50003), (530, 2048)])
+def test_distill_special_rows(lib, tail, N, V):
+    """Repeated ids, entries without mass, a support that is all the student
+    has, padding over NaN, masked and NaN rows, ids past the vocabulary."""
+    t = _t()
+    print("distill special", tail, N, V, flush=True)
+    _, x = on_gpu(rows_of(F32, N, V, spread=1.5))
+    K = 10
+    ids, tl = teacher(x, K, 1.0)
+    tgt = ids[:, 1].clone()
+    ids[0, 4], ids[0, 7] = ids[0, 2], ids[0, 2]      # the first place counts
+    tl[1, 3] = -math.inf                             # an entry of the support without mass
+    ids[2], tgt[2] = -1, -1                          # a padded row over NaN
+    x[2] = math.nan
+    x[3] = -math.inf                                 # nothing left
+    ids[3], tgt[3] = -1, -1
+    x[4, 9] = math.nan
+    ids[5, 6] = V
+    tl[6] = -math.inf
+    x[7, ids[7, 0].long()] = -math.inf               # the student excludes what the teacher wants
+    tgt[7] = ids[7, 5]
+    tl[8] = tl[8] + 2.0                              # more mass than one
+    keep = x[9, ids[9].long()].clone()               # outside the support nothing is left
+    x[9] = -math.inf
+    x[9, ids[9].long()] = keep
+    _, d = like_rows(x, F32)
+    o = distill(lib, x, F32, ids, tl, tail, 1.0, 1.0, tgt, 0.5, d)
+    rows = f64(o.rows)
+    assert rows[2] == 0 and bool((d[2] == 0).all())
+    assert rows[3] == 0 and bool((d[3] == 0).all())
+    assert np.isnan(rows[4]) and bool(t.isnan(d[4]).all())
+    assert np.isnan(rows[5]) and bool(t.isnan(d[5]).all())
+    assert rows[7] == math.inf
+    good = [0, 1, 6, 7, 8, 9, 10, 11] + list(range(12, N))
+    sub = x[good]
+    o.rows, dd = o.rows[good], d[good]
+    o.loss = o.rows.mean().reshape(1)
+    check_distill(o, dd, F32, sub, ids[good], tl[good], tail, 1.0, 1.0, tgt[good], 0.5, 1.0)
+
+
+def test_distill_targets_past_the_vocabulary(lib):
+    t = _t()
+    _, x = on_gpu(rows_of(F32, 3, 100))
+    tgt = t.tensor([5, 100, 7], dtype=t.int32, device="cuda")
+    _, d = like_rows(x, F32)
+    o = distill(lib, x, F32, None, None, False, 1.0, 1.0, tgt, 1.0, d)
+    assert np.isnan(f64(o.rows)).tolist() == [False, True, False]
+    assert bool(t.isnan(d[1]).all()) and bool(d[0].isfinite().all()) and bool(d[2].isfinite().all())
+
+
+def test_distill_gradient_against_differences(lib):
+    t = _t()
+    N, V, K, h = 6, 1500, 24, 1.0 / 64
+    for tail, tau in ((False, 2.0), (True, 1.0)):
+        _, x = on_gpu(rows_of(F32, N, V))
+        ids, tl = teacher(x, K, tau, noise=1.5)
+        tgt = t.randint(0, V, (N,), dtype=t.int32).cuda()
+        _, d = like_rows(x, F32)
+        distill(lib, x, F32, ids, tl, tail, tau, 1.0, tgt, 0.5, d)
+        v = (t.randn(N, V, device="cuda") * 4).round().clamp(-8, 8) / 4
+        up = distill(lib, x + h * v, F32, ids, tl, tail, tau, 1.0, tgt, 0.5, None).rows.double()
+        dn = distill(lib, x - h * v, F32, ids, tl, tail, tau, 1.0, tgt, 0.5, None).rows.double()
+        num, ana = (up - dn) / (2 * h), (d.double() * v.double()).sum(1)
+        # cumulants of a variable in [-2, 2] (third: at most 16), for log S, the
+        # remainder's log sum and the CE's log S; fp32 values / h
+        bar = h * h / 6 * 16 * (tau * tau * 2 + 1) + 2 * (tau * tau + 1) * (3 * rho(V) + 6 * EPS * 40) / h
+        assert float((num - ana).abs().max()) <= bar, (num, ana, bar)
+        assert float(ana.abs().max()) > 2 * bar, "differences that could not fail"
+
+
+def test_cross_entropy_alone_is_xent(lib):
+    """K = 0 and w_ce = 1 is tlg_dev_xent without its 1e-12."""
+    t = _t()
+    N, V = 300, 2048
+    _, x = on_gpu(rows_of(F32, N, V))
+    tgt = t.randint(0, V, (N,), dtype=t.int32).cuda()
+    _, d = like_rows(x, F32)
+    o = distill(lib, x, F32, None, None, False, 1.0, 1.0, tgt, 1.0, d, 1.0 / N)
+    d2, loss = t.empty_like(d), t.empty(1, device="cuda")
+    lib.check(lib.tlg_dev_xent(x.data_ptr(), tgt.data_ptr(), d2.data_ptr(), loss.data_ptr(), 1.0 / N, N, V, stream()),
+              "xent")
+    assert abs(float(loss) - float(o.loss)) <= (4 * rho(V) + 200 * EPS) * float(loss) + 1e-12 * V * 1e6
+    assert float((d - d2).abs().max()) <= (2 * rho(V) + 100 * EPS) / N
+
+
+# ------------------------------------------------- graphs, streams, repeats --
+@pytest.mark.parametrize("N,V", [(2, 60000), (40, 2048), (600, 3001)])
+def test_same_bits_every_time(lib, N, V):
+    """Equal calls give equal bits, whatever the workspace held before."""
+    t = _t()
+    for ty in (F32, BF16):
+        _, x = on_gpu(rows_of(ty, N, V))
+        ids = some_ids(N, V, 2, 1)
+        a, b = logprobs(lib, x, ty, 1.0, ids, 30, 255), logprobs(lib, x, ty, 1.0, ids, 30, 0)
+        for n in ("logp", "lse2", "entropy", "top_ids", "top_logp"):
+            assert t.equal(getattr(a, n).nan_to_num(7.0), getattr(b, n).nan_to_num(7.0)), n
+        tids, tl = teacher(x, 16, 1.0)
+        _, d1 = like_rows(x, ty)
+        _, d2 = like_rows(x, ty)
+        p, q = (distill(lib, x, ty, tids, tl, True, 1.0, 1.0, None, 0.0, d, ws_fill=f)
+                for d, f in ((d1, 255), (d2, 0)))
+        assert t.equal(d1, d2) and t.equal(p.rows, q.rows) and t.equal(p.loss, q.loss)
+
+
+@pytest.mark.parametrize("N,V", [(1, 60000), (48, 2048), (600, 3001)])
+def test_scoring_then_distillation_captured(lib, N, V):
+    """A teacher's scores into a student's distillation and a policy gradient,
+    captured once and replayed with new logits between eager calls: every
+    replay equals the eager chain bit for bit."""
+    t = _t()
+    ty, K = BF16, 12
+    tx, sx = (t.empty(N, V, dtype=t.bfloat16, device="cuda") for _ in range(2))
+    ids = some_ids(N, V, 1, 3)
+    f = dict(device="cuda")
+    dlogp = t.full((N, 1), -1.0 / N, **f)
+    dent = t.full((N,), -0.01 / N, **f)
+
+    class B:
+        def __init__(self):
+            self.logp, self.lse2, self.ent = t.zeros(N, 1, **f), t.zeros(N, 2, **f), t.zeros(N, **f)
+            self.ti, self.tl = t.zeros(N, K, dtype=t.int32, **f), t.zeros(N, K, **f)
+            self.rows, self.loss = t.zeros(N, **f), t.zeros(1, **f)
+            self.d, self.d2 = t.zeros(N, V, dtype=t.bfloat16, **f), t.zeros(N, V, dtype=t.bfloat16, **f)
+            self.nb = lib.tlg_logprobs_ws_bytes(ty, N, V, K)
+            self.nk = lib.tlg_distill_ws_bytes(ty, N, V)
+            self.ws = t.zeros(max(self.nb, self.nk) + 16, dtype=t.uint8, **f)
+
+        def run(self):
+            st = stream()
+            lib.logprobs(tx.data_ptr(), ty, V, N, V, 0.5, None, 0, None, None, None, K, self.ti.data_ptr(),
+                         self.tl.data_ptr(), self.ws.data_ptr(), self.nb, st)
+            lib.distill(sx.data_ptr(), ty, V, N, V, self.ti.data_ptr(), self.tl.data_ptr(), K, 1, 2.0, 1.0, None, 0.0,
+                        self.rows.data_ptr(), self.loss.data_ptr(), self.d.data_ptr(), V, 1.0 / N,
+                        self.ws.data_ptr(), self.nk, st)
+            lib.logprobs(sx.data_ptr(), ty, V, N, V, 1.0, ids.data_ptr(), 1, self.logp.data_ptr(),
+                         self.lse2.data_ptr(), self.ent.data_ptr(), 0, None, None, self.ws.data_ptr(), self.nb, st)
+            lib.logprobs_bwd(sx.data_ptr(), ty, V, N, V, 1.0, ids.data_ptr(), 1, self.lse2.data_ptr(),
+                             self.ent.data_ptr(), dlogp.data_ptr(), None, dent.data_ptr(), self.d2.data_ptr(), V, st)
+
+        def all(self):
+            return [self.logp, self.lse2, self.ent, self.ti, self.tl, self.rows, self.loss, self.d, self.d2]
+    cap, eager = B(), B()
+    tx.normal_()
+    sx.normal_()
+    cap.run()
+    t.cuda.synchronize()
+    g = t.cuda.CUDAGraph()
+    with t.cuda.graph(g):
+        cap.run()
+    for seed in range(4):
+        t.manual_seed(seed)
+        sx.copy_(2.5 * t.randn(N, V, device="cuda"))
+        tx.copy_(sx.float() + 0.5 * t.randn(N, V, device="cuda"))
+        for a in cap.all():
+            a.zero_()
+        g.replay()
+        t.cuda.synchronize()
+        eager.run()
+        t.cuda.synchronize()
+        for a, b in zip(cap.all(), eager.all()):
+            assert t.equal(a, b)
+    # and the chain is right: the student's loss falls along its own gradient
+    o = cap
+    assert bool((o.rows >= -1e-5).all()) and float(o.loss) > 0
+
+
+def test_calls_on_two_streams_at_once(lib):
+    """Calls with workspaces of their own on two streams at the same time."""
+    t = _t()
+    N, V, K = 3, 70000, 40
+    _, x = on_gpu(rows_of(F32, N, V))
+    _, y = on_gpu(rows_of(F32, N, V, seed=9))
+    want = [logprobs(lib, z, F32, 1.0, None, K) for z in (x, y)]
+    t.cuda.synchronize()
+    s = [t.cuda.Stream(), t.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, z in enumerate((x, y)):
+            with t.cuda.stream(s[i]):
+                got[i].append(logprobs(lib, z, F32, 1.0, None, K))
+    t.cuda.synchronize()
+    for i in (0, 1):
+        for o in got[i]:
+            assert t.equal(o.top_ids, want[i].top_ids) and t.equal(o.lse2, want[i].lse2)
+            assert t.equal(o.top_logp, want[i].top_logp) and t.equal(o.entropy, want[i].entropy)
+
+
+def test_rows_behind_four_gigabytes(lib):
+    """Row offsets beyond 32 bits of bytes: the last rows of a tall buffer."""
+    t = _t()
+    N, V, ld = 3, 5000, 1 << 30
+    buf = t.empty((N - 1) * ld + V, dtype=t.bfloat16, device="cuda")
+    x = t.as_strided(buf, (N, V), (ld, 1))
+    x.copy_(2.5 * t.randn(N, V, device="cuda"))
+    ids = some_ids(N, V, 1, 1, none=False)
+    o = logprobs(lib, x, BF16, 1.0, ids, 7)
+    check_logprobs(o, x, 1.0, ids, 7)
+    d = t.empty(N, V, dtype=t.bfloat16, device="cuda")
+    dlogp = t.randn(N, 1, device="cuda")
+    logprobs_bwd(lib, x, BF16, 1.0, ids, o.lse2, o.entropy, dlogp, None, None, d)
+    small = x.contiguous()
+    d2 = t.empty_like(d)
+    logprobs_bwd(lib, small, BF16, 1.0, ids, o.lse2, o.entropy, dlogp, None, None, d2)
+    assert t.equal(d, d2)
+    logprobs_bwd(lib, x, BF16, 1.0, ids, o.lse2, o.entropy, dlogp, None, None, x)          # and written there
+    assert t.equal(x.contiguous(), d)

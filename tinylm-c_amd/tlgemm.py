@@ -21,6 +21,10 @@ _ip = ctypes.POINTER(ctypes.c_int)
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
+_f = ctypes.c_float
+_ll = ctypes.c_longlong
+# element types of logits buffers (include/tltrain.h)
+F32, F16, BF16 = 0, 1, 2
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -110,6 +114,12 @@ SIGNATURES = {
     "tlg_dev_xent_rows": (_i, [_vp, _vp, _vp, _vp, ctypes.c_float, _i, _i, _vp]),
     "tlg_dev_gradnorm_loss": (_i, [_vp, _sz, _vp, _vp, _i, _vp, _vp]),
     "tlg_dev_adamw": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp]),
+    "tlg_logprobs_ws_bytes": (_sz, [_i, _i, _i, _i]),
+    "tlg_dev_logprobs": (_i, [_vp, _i, _ll, _i, _i, _f, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    "tlg_dev_logprobs_bwd": (_i, [_vp, _i, _ll, _i, _i, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp]),
+    "tlg_distill_ws_bytes": (_sz, [_i, _i, _i]),
+    "tlg_dev_distill": (_i, [_vp, _i, _ll, _i, _i, _vp, _vp, _i, _i, _f, _f, _vp, _f, _vp, _vp, _vp, _ll, _f, _vp,
+                             _sz, _vp]),
     # include/tldecode.h
     "tlg_dev_dec_embed": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "tlg_dev_kv_store": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
@@ -225,6 +235,26 @@ class Lib:
                                                            N, D, F, E, wr, w1, w3, w2, gwr, gw1, gw3,
                                                            gw2, stream),
                           "tlg_dev_moe_grouped_bwd")
+
+    def logprobs(self, logits, type, ld, N, V, scale, ids, M, logp, lse2, entropy, K, top_ids, top_logp, ws, ws_bytes,
+                 stream=0):
+        """Log probabilities of given tokens, entropy and top alternatives of rows of logits."""
+        return self.check(self.dll.tlg_dev_logprobs(logits, type, ld, N, V, scale, ids, M, logp, lse2, entropy, K,
+                                                    top_ids, top_logp, ws, ws_bytes, stream), "tlg_dev_logprobs")
+
+    def logprobs_bwd(self, logits, type, ld, N, V, scale, ids, M, lse2, entropy, dlogp, dlse, dentropy, dlogits, ldd,
+                     stream=0):
+        """The gradient of logprobs' outputs with respect to the logits."""
+        return self.check(self.dll.tlg_dev_logprobs_bwd(logits, type, ld, N, V, scale, ids, M, lse2, entropy, dlogp,
+                                                        dlse, dentropy, dlogits, ldd, stream),
+                          "tlg_dev_logprobs_bwd")
+
+    def distill(self, logits, type, ld, N, V, t_ids, t_logp, K, tail, temp, w_kd, tgt, w_ce, rows, loss, dlogits, ldd,
+                scale, ws, ws_bytes, stream=0):
+        """Distillation from a teacher's top log probabilities: loss and gradient."""
+        return self.check(self.dll.tlg_dev_distill(logits, type, ld, N, V, t_ids, t_logp, K, tail, temp, w_kd, tgt,
+                                                   w_ce, rows, loss, dlogits, ldd, scale, ws, ws_bytes, stream),
+                          "tlg_dev_distill")
 
     def group(self, calls, stream=0, flush=True):
         """tlg_dev_gemm_group over dicts {op, beta, C, M, K, N, A: [..], B: [..], Nseg: [..], R}."""
