@@ -5,283 +5,1086 @@
 // For one row x[0..V) and a scale s = 1 / temperature:
 //   m = max x,  S = sum_v e^(s (x_v - m)),  log p_v = s (x_v - m) - log S
 //   H = -sum_v p_v log p_v = log S - s sum_v (x_v - m) e^(s (x_v - m)) / S
-// Sums are fp32 (and fp64 where K terms cancel), outputs are rounded once.
+// All of them are bound by HBM: a logit is read once (and its gradient written
+// once) per call, and the work on it (one or two exponentials, a maximum, two or
+// three sums) fits in the time its bytes take.  Sums are fp32, joined over
+// threads in a fixed order, and fp64 where K terms cancel; outputs are rounded once.
 #include "tlg_internal.h"
 #include "../../include/tltrain.h"
+#include <float.h>
 #include <math.h>
 
 #define ST(s) ((hipStream_t)(s))
 #define LAUNCH_CHECK() TLG_HIP(hipGetLastError())
-#define VB 256
 
 // ------------------------------------------------------------- elements --
-template <int TYPE> struct El;
-template <> struct El<TLG_F32> { typedef float t; };
-template <> struct El<TLG_F16> { typedef _Float16 t; };
-template <> struct El<TLG_BF16> { typedef __bf16 t; };
+// Rows are read and written 16 bytes at a time, on the 16-byte grid of the
+// address space: a row that starts `sh` elements behind a grid point takes
+// `nv` grid vectors, of which the first and the last may hold elements of its
+// neighbours; those are loaded and stored element by element.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <int TYPE> struct El {
+    static constexpr int VE = TYPE == TLG_F32 ? 4 : 8;              // elements of a vector
+    static constexpr int SZ = TYPE == TLG_F32 ? 4 : 2;
+    static constexpr unsigned NEG = TYPE == TLG_F32 ? 0xff800000u : TYPE == TLG_F16 ? 0xfc00u : 0xff80u;  // -inf
+};
 
-__device__ __forceinline__ float vb_max(float v, float *sh)
+template <int TYPE> __device__ __forceinline__ float el_float(unsigned bits)
 {
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    if constexpr (TYPE == TLG_F32) return __uint_as_float(bits);
+    else if constexpr (TYPE == TLG_F16) return (float)__builtin_bit_cast(_Float16, (unsigned short)bits);
+    else return __uint_as_float(bits << 16);
 }
-template <typename F> __device__ __forceinline__ F vb_sum(F v, F *sh)
+// Between two uses of a vector kept in registers: without it the compiler keeps
+// the elements unpacked from the first use to the second, twice the registers.
+__device__ __forceinline__ void keep_packed(u32x4 &r) { asm volatile("" : "+v"(r)); }
+// element e of a raw vector; e is a constant where it is called
+template <int TYPE> __device__ __forceinline__ float el_at(const u32x4 &r, int e)
 {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    if constexpr (TYPE == TLG_F32) return __uint_as_float(r[e]);
+    else if constexpr (TYPE == TLG_BF16) return __uint_as_float(e & 1 ? r[e >> 1] & 0xffff0000u : r[e >> 1] << 16);
+    else return el_float<TYPE>(e & 1 ? r[e >> 1] >> 16 : r[e >> 1] & 0xffffu);
+}
+template <int TYPE> __device__ __forceinline__ unsigned el_bits(float v)      // rounded to nearest even
+{
+    if constexpr (TYPE == TLG_F32) return __float_as_uint(v);
+    else if constexpr (TYPE == TLG_F16) return __builtin_bit_cast(unsigned short, (_Float16)v);
+    else return __builtin_bit_cast(unsigned short, (__bf16)v);
+}
+template <int TYPE> __device__ __forceinline__ float el_load(const char *x, int i)
+{
+    if constexpr (TYPE == TLG_F32) return ((const float *)x)[i];
+    else return el_float<TYPE>(((const unsigned short *)x)[i]);
+}
+template <int TYPE> __device__ __forceinline__ void el_store(char *x, int i, float v)
+{
+    if constexpr (TYPE == TLG_F32) ((float *)x)[i] = v;
+    else ((unsigned short *)x)[i] = (unsigned short)el_bits<TYPE>(v);
+}
+
+template <int TYPE> struct Row {
+    static constexpr int VE = El<TYPE>::VE;
+    const char *x;              // element 0
+    const u32x4 *v;             // grid vector 0
+    int V, sh, nv, f0, f1;      // whole vectors: [f0, f1)
+    __device__ __forceinline__ Row(const void *base, long long ld, size_t r, int V_)
+    {
+        x = (const char *)base + (long long)r * ld * El<TYPE>::SZ;
+        const int a = (int)((uintptr_t)x & 15);
+        v = (const u32x4 *)(x - a);
+        V = V_;
+        sh = a / El<TYPE>::SZ;
+        nv = (V + sh + VE - 1) / VE;
+        f0 = sh ? 1 : 0;
+        f1 = (V + sh) / VE;
+    }
+    __device__ __forceinline__ u32x4 edge(int j) const
+    {
+        u32x4 r;
+        unsigned b[VE];
+#pragma unroll
+        for (int e = 0; e < VE; e++) {
+            const int i = j * VE + e - sh;
+            b[e] = El<TYPE>::NEG;
+            if (i >= 0 && i < V) {
+                if constexpr (TYPE == TLG_F32) b[e] = ((const unsigned *)x)[i];
+                else b[e] = ((const unsigned short *)x)[i];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if constexpr (TYPE == TLG_F32) r[k] = b[k];
+            else r[k] = b[2 * k] | b[2 * k + 1] << 16;
+        }
+        return r;
+    }
+    // vector j, -inf where it is no part of the row
+    __device__ __forceinline__ u32x4 any(int j) const
+    {
+        if (j >= f0 && j < f1) return v[j];
+        if (j >= nv) {
+            const unsigned n = TYPE == TLG_F32 ? El<TYPE>::NEG : El<TYPE>::NEG * 0x10001u;
+            return u32x4{n, n, n, n};
+        }
+        return edge(j);
+    }
+};
+
+// ------------------------------------------------------------ threads of a row --
+// W waves work on one row: 64 W threads, synchronised by a barrier or, for one
+// wave, by its own order.
+template <int W> __device__ __forceinline__ void row_sync()
+{
+    if constexpr (W > 1) __syncthreads();
+    else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+// Sum and maximum over a wave in a fixed order: neighbours in each row of 16
+// lanes by data-parallel moves, then the four rows; every lane of an active
+// wave must take part, and every lane gets the result.
+template <int CTRL> __device__ __forceinline__ float lane_move(float v)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row_of(float v, int r)
+{
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16 * r));
+}
+#define WAVE_REDUCE(name, OP)                                                              \
+    __device__ __forceinline__ float name(float v)                                         \
+    {                                                                                      \
+        v = OP(v, lane_move<0xB1>(v));      /* quad_perm 1,0,3,2 */                         \
+        v = OP(v, lane_move<0x4E>(v));      /* quad_perm 2,3,0,1 */                         \
+        v = OP(v, lane_move<0x141>(v));     /* row_half_mirror */                          \
+        v = OP(v, lane_move<0x140>(v));     /* row_mirror */                               \
+        return OP(OP(row_of(v, 0), row_of(v, 1)), OP(row_of(v, 2), row_of(v, 3)));         \
+    }
+__device__ __forceinline__ float add_op(float a, float b) { return a + b; }
+WAVE_REDUCE(wave_max, fmaxf)
+WAVE_REDUCE(wave_sum, add_op)
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane)
+{
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)v, lane);
+    const unsigned hi = __builtin_amdgcn_readlane((unsigned)(v >> 32), lane);
+    return (u64)hi << 32 | lo;
 }
 
 // A total order of values (equal for -0 and +0) in the high half and the lower
-// index first in the low half; 0 for -inf, which is no alternative.
-__device__ __forceinline__ unsigned long long vb_key(float x, int i)
+// position first in the low half; 0 for -inf, which is no alternative.
+__device__ __forceinline__ u64 vb_key(float x, int g)
 {
     const unsigned b = __float_as_uint(x + 0.0f);
     const unsigned o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return x == -INFINITY ? 0ull : (unsigned long long)o << 32 | (unsigned)~i;
+    return x == -INFINITY ? 0ull : (u64)o << 32 | (unsigned)~g;
 }
-__device__ __forceinline__ float vb_key_value(unsigned long long k)
+__device__ __forceinline__ float vb_key_value(u64 k)
 {
     const unsigned o = (unsigned)(k >> 32);
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// --------------------------------------------------------- log probabilities --
-// One workgroup per row.
-template <int TYPE>
-__global__ __launch_bounds__(VB) void k_logprobs(const void *__restrict__ logits, long long ld, int V, float scale,
-                                                 const int *__restrict__ ids, int M, float *__restrict__ logp,
-                                                 float *__restrict__ lse2, float *__restrict__ entropy, int K,
-                                                 int *__restrict__ top_ids, float *__restrict__ top_logp)
+// -------------------------------------------------------------- one pass --
+// Running sums of a thread's part of a row in base 2: with c = scale log2 e
+// rounded and a reference R = m c rounded, m the part's maximum so far,
+//   t_v = x_v c - R (one fused product),  s = sum 2^t,  u = sum t 2^t.
+// R is exact as the reference it is, whatever its distance from m c, so parts
+// join by the differences of their references, and
+//   rho = R - m c,  log sum e^(scale (x - m)) = ln 2 rho + log(s + kappa u),
+// with kappa = ln 2 (scale log2 e - c) / c for the rounding of c, to first order.
+// NaN and +inf make s NaN.  Exponents are clamped at -200, where 2^t is 0, in the
+// factor of the products only: 0 * -inf must not be NaN, NaN must stay.  R is kept
+// at -1e38 or above.  Where a maximum of that size, of either sign, leaves s = 0
+// although not all is masked, sums_apart forms the sums from differences.
+struct Acc { float R, s, u; };
+#define ACC0 {-1e38f, 0.f, 0.f}
+__device__ __forceinline__ float acc_ref(float m, float c) { return fmaxf(m * c, -1e38f); }
+__device__ __forceinline__ void acc_shift(Acc &a, float R)                    // to a reference R >= a.R
 {
-    typedef typename El<TYPE>::t T;
-    __shared__ float sh[4];
-    __shared__ unsigned long long shk[4];
-    const size_t r = blockIdx.x;
-    const int t = threadIdx.x;
-    const T *x = (const T *)logits + r * ld;
-    float m = -INFINITY;
-    for (int i = t; i < V; i += VB) m = fmaxf(m, (float)x[i]);
-    m = vb_max(m, sh);
-    const bool empty = m == -INFINITY;
-    float s = 0.f, u = 0.f;
-    for (int i = t; i < V; i += VB) {
-        const float d = ((float)x[i] - m) * scale, e = expf(d);
-        s += empty ? 0.f : e;
-        u += e > 0.f || e != e ? e * d : 0.f;
+    const float d = a.R - R, f = __builtin_amdgcn_exp2f(d);
+    a.u = f * fmaf(fmaxf(d, -200.f), a.s, a.u);
+    a.s *= f;
+    a.R = R;
+}
+__device__ __forceinline__ void acc_add(Acc &a, float x, float c)
+{
+    const float t = fmaf(x, c, -a.R), e = __builtin_amdgcn_exp2f(t);
+    a.s += e;
+    a.u = fmaf(e, fmaxf(t, -200.f), a.u);
+}
+// all lanes' parts in every lane, m the wave's maximum; the order of additions is fixed
+__device__ __forceinline__ Acc acc_wave(Acc a, float m, float c)
+{
+    acc_shift(a, acc_ref(m, c));
+    return Acc{a.R, wave_sum(a.s), wave_sum(a.u)};
+}
+// parts {s, u, m} relative to their own references
+__device__ __forceinline__ Acc acc_join(const f32x4 *p, int n, float c, float &m)
+{
+    m = p[0][2];
+    for (int w = 1; w < n; w++) m = fmaxf(m, p[w][2]);
+    Acc r = {acc_ref(m, c), 0.f, 0.f};
+    for (int w = 0; w < n; w++) {
+        Acc a = {acc_ref(p[w][2], c), p[w][0], p[w][1]};
+        acc_shift(a, r.R);
+        r.s += a.s;
+        r.u += a.u;
     }
-    s = vb_sum(s, sh);
-    u = vb_sum(u, sh);
-    const bool bad = s != s;
-    if (empty) u = 0.f;
-    // a row with NaN or +inf has no distribution
-    const float ls = bad ? NAN : empty ? -INFINITY : logf(s);
-    for (int j = t; j < M; j += VB) {
-        const int id = ids[r * M + j];
-        float o = 0.f;
-        if (id >= V) o = NAN;
-        else if (id >= 0) o = empty ? -INFINITY : ((float)x[id] - m) * scale - ls;
-        logp[r * M + j] = o;
-    }
-    if (t == 0) {
-        if (lse2) { lse2[2 * r] = bad ? NAN : m; lse2[2 * r + 1] = ls; }
-        if (entropy) entropy[r] = empty ? 0.f : ls - u / s;
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < K; k++) {
-        unsigned long long b = 0;
-        if (last && !bad)
-            for (int i = t; i < V; i += VB) {
-                const unsigned long long c = vb_key((float)x[i], i);
-                if (c < last && c > b) b = c;
-            }
-        for (int o = 32; o > 0; o >>= 1) {
-            const unsigned long long c = __shfl_xor(b, o);
-            if (c > b) b = c;
+    return r;
+}
+// What is asked of a row: m its maximum, ls = log sum e^(scale (x - m)), H the
+// entropy; NaN and -inf mark rows without a distribution.
+struct Sums { float m, ls, H; };
+template <int TYPE, int W>
+__device__ __noinline__ Acc sums_apart(const Row<TYPE> x, float m, float c, int t, f32x4 *part)
+{
+    constexpr int VE = El<TYPE>::VE;
+    Acc a = {0.f, 0.f, 0.f};
+    for (int j = t; j < x.nv; j += 64 * W) {
+        const u32x4 q = x.any(j);
+#pragma unroll
+        for (int e = 0; e < VE; e++) {
+            const float d = (el_at<TYPE>(q, e) - m) * c, f = __builtin_amdgcn_exp2f(d);
+            a.s += f;
+            a.u = fmaf(f, fmaxf(d, -200.f), a.u);
         }
-        __syncthreads();
-        if ((t & 63) == 0) shk[t >> 6] = b;
-        __syncthreads();
-        for (int w = 0; w < 4; w++) b = shk[w] > b ? shk[w] : b;
-        last = b;
-        if (t == 0) {
-            top_ids[r * K + k] = b ? ~(unsigned)b : -1;
-            top_logp[r * K + k] = bad ? NAN : b ? (vb_key_value(b) - m) * scale - ls : -INFINITY;
+    }
+    a.s = wave_sum(a.s);
+    a.u = wave_sum(a.u);
+    if constexpr (W > 1) {
+        row_sync<W>();
+        if (t % 64 == 0) part[t / 64] = f32x4{a.s, a.u, 0.f, 0.f};
+        row_sync<W>();
+        a.s = a.u = 0.f;
+        for (int w = 0; w < W; w++) {
+            a.s += part[w][0];
+            a.u += part[w][1];
+        }
+        row_sync<W>();
+    }
+    return a;
+}
+template <int TYPE, int W>
+__device__ __forceinline__ Sums sums_of(const Row<TYPE> &x, float m, Acc a, float c, float kappa, int t, f32x4 *part)
+{
+    float rho = -fmaf(m, c, -a.R);
+    if (a.s == 0.f && m > -INFINITY) {
+        a = sums_apart<TYPE, W>(x, m, c, t, part);
+        rho = 0.f;
+    }
+    if (a.s != a.s) return Sums{NAN, NAN, NAN};
+    if (m == -INFINITY) return Sums{-INFINITY, -INFINITY, 0.f};
+    const float ls = fmaf(0.69314718056f, rho, logf(fmaf(kappa, a.u, a.s)));
+    return Sums{m, ls, ls - 0.69314718056f * fmaf(a.u, __builtin_amdgcn_rcpf(a.s), rho)};
+}
+
+// --------------------------------------------------------- log probabilities --
+// The K largest of a row beside its sums.  Every thread keeps its own maximum v1.
+// These are different elements, so a bound T that enough of them reach (J =
+// ceil(K / waves) lanes of every wave) is reached by K elements of the row at
+// least, in a row of random order by little more.  They go to a list, which is
+// ranked by counting.  A row of one wave and U vectors a lane at most (RES) is still
+// in registers then.  Of longer rows the pass leaves line maxima in LDS, for less
+// than an operation per element: eight neighbouring lanes' vectors are a line of 128
+// bytes (2^q lines U 64 W vectors apart, in rows of more than LP_LINES lines per
+// wave); the lines that reach T are read again, by all threads evenly.  A list that
+// overflows, from many equal values or large values that lie together, raises T by
+// the same argument over what it holds, and is made again.
+struct LpArgs {
+    const void *logits;
+    long long ld;
+    int N, V, S;                 // S segments of a row, joined by k_logprobs_join
+    float scale, c, kappa;       // c = scale log2 e rounded, kappa = ln 2 (scale log2 e - c) / c
+    const int *ids;
+    int M;
+    float *logp, *lse2, *entropy;
+    int K;
+    int *top_ids;
+    float *top_logp;
+    float *part;                 // S > 1: [N][S][4]
+    u64 *keys;                   // S > 1: [N][K][S], descending over K
+};
+
+// What a row's threads share.
+#define LP_LINES 512
+template <int W, bool LINES, bool TOP> struct LpShared {
+    static constexpr int CAP = W < 4 ? 256 * W : 1024;
+    f32x4 part[W];               // a wave's sums, maximum and bound
+    u64 t[W];
+    int n, lines;
+    union {
+        alignas(16) float max[LINES ? LP_LINES * W : 1];         // until the lines are chosen
+        u64 cand[TOP ? CAP : 1];
+    };
+    unsigned short line[LINES ? LP_LINES * W : 1];
+};
+
+// A value that at least J lanes of the wave reach, and not many more; the lowest
+// finite one if there is no such value.  Pivots are lanes' values; each step drops
+// the pivot's lane at least.
+__device__ __forceinline__ float wave_bound(float v, int J)
+{
+    float T = -FLT_MAX;
+    u64 open = ~0ull;
+    while (open) {
+        const float p = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), __ffsll((long long)open) - 1));
+        const u64 reach = __ballot(v >= p);
+        const int n = __popcll(reach);
+        if (n >= J) {
+            T = fmaxf(T, p);
+            if (n <= J + J / 4 + 1) break;
+            open &= __ballot(v > p);
+        } else
+            open &= ~reach & ~(1ull << (__ffsll((long long)open) - 1));
+    }
+    return T;
+}
+// the same for the list's keys, exactly J lanes
+__device__ __forceinline__ u64 wave_bound_key(u64 v, int J)
+{
+    u64 T = 0, open = ~0ull;
+    while (open) {
+        const int l = __ffsll((long long)open) - 1;
+        const u64 p = lane_u64(v, l), reach = __ballot(v >= p);
+        if (__popcll(reach) >= J) {
+            T = p;
+            open &= __ballot(v > p);
+        } else
+            open &= ~reach;
+    }
+    return T;
+}
+
+// The lanes' elements with `take` to the wave's list, whose length is n.
+template <typename E> __device__ __forceinline__ void wave_push(bool take, E v, E *list, int &n, int cap)
+{
+    const u64 m = __ballot(take);
+    const int at = n + __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0));
+    if (take && at < cap) list[at] = v;
+    n += __popcll(m);
+}
+// all elements of a vector at place j that reach T (by value, then by key)
+template <int TYPE, int W>
+__device__ __forceinline__ void lp_list(const u32x4 &q, int j, float T, u64 Tkey, u64 *cand, int &n, int cap)
+{
+#pragma unroll
+    for (int e = 0; e < El<TYPE>::VE; e++) {
+        const float x = el_at<TYPE>(q, e);
+        if constexpr (W == 1) {                          // most vectors have none: all lanes at once
+            if (__ballot(x >= T)) {
+                const u64 key = vb_key(x, j * El<TYPE>::VE + e);
+                wave_push(x >= T && key >= Tkey, key, cand, n, cap);
+            }
+        } else if (x >= T) {
+            const u64 key = vb_key(x, j * El<TYPE>::VE + e);
+            if (key >= Tkey) {
+                const int at = atomicAdd(&n, 1);
+                if (at < cap) cand[at] = key;
+            }
         }
     }
 }
 
-// dlogits of logp, lse and entropy: dz_v = sum_j g_j (1{v = id_j} - p_v) +
-// g_lse p_v - g_H p_v (log p_v + H).  One workgroup per row; the rows of the
-// ids are written again after the others.
-#define VB_IDS 64
-template <int TYPE>
-__global__ __launch_bounds__(VB) void k_logprobs_bwd(const void *logits, long long ld, int V, float scale,
-                                                     const int *__restrict__ ids, int M,
-                                                     const float *__restrict__ lse2,
-                                                     const float *__restrict__ entropy,
-                                                     const float *__restrict__ dlogp, const float *__restrict__ dlse,
-                                                     const float *__restrict__ dent, void *dlogits, long long ldd)
+// a given token of a row and its logit, loaded ahead of the row's sums
+struct Given { int id; float x; };
+template <int TYPE> __device__ __forceinline__ Given lp_given(const LpArgs &a, size_t r, const char *x, int t)
 {
-    typedef typename El<TYPE>::t T;
-    __shared__ int si[VB_IDS];
-    __shared__ float sg[VB_IDS];
+    Given g = {-1, 0.f};
+    if (t < a.M) {
+        g.id = a.ids[r * a.M + t];
+        if (g.id >= 0 && g.id < a.V) g.x = el_load<TYPE>(x, g.id);
+    }
+    return g;
+}
+__device__ __forceinline__ void lp_finish(const LpArgs &a, size_t r, const Given &g, const Sums &s, int t)
+{
+    if (t < a.M) {
+        float o = (g.x - s.m) * a.scale - s.ls;
+        if (s.m == -INFINITY) o = -INFINITY;
+        a.logp[r * a.M + t] = g.id >= a.V ? NAN : g.id < 0 ? 0.f : o;
+    }
+    if (t == 0) {
+        if (a.lse2) {
+            a.lse2[2 * r] = s.m;
+            a.lse2[2 * r + 1] = s.ls;
+        }
+        if (a.entropy) a.entropy[r] = s.H;
+    }
+}
+
+__device__ __forceinline__ void lp_put(const LpArgs &a, size_t r, int k, u64 key, int sh, const Sums &s)
+{
+    const bool bad = s.ls != s.ls;
+    a.top_ids[r * a.K + k] = key && !bad ? (int)~(unsigned)key - sh : -1;
+    a.top_logp[r * a.K + k] = bad ? NAN : key ? (vb_key_value(key) - s.m) * a.scale - s.ls : -INFINITY;
+}
+
+// W waves on a row, or on one of its S segments (W > 1); 4 rows of one wave per
+// workgroup.  TOP: K > 0.
+template <int TYPE, int W, int U, bool RES, bool TOP>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
+{
+    constexpr int VE = El<TYPE>::VE, TPR = 64 * W;
+    constexpr bool LINES = TOP && !RES;
+    typedef LpShared<W, LINES, TOP> Sh;
+    constexpr int CAP = Sh::CAP;
+    __shared__ Sh shared[W == 1 ? 4 : 1];
+    const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, t = W == 1 ? lane : threadIdx.x;
+    Sh &sh = shared[W == 1 ? threadIdx.x >> 6 : 0];
+    size_t r;
+    int seg = 0;
+    if constexpr (W == 1) {
+        r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+        if (r >= (size_t)a.N) return;                    // whole waves: no barrier follows for W == 1
+    } else {
+        r = blockIdx.x / (unsigned)a.S;
+        seg = blockIdx.x % (unsigned)a.S;
+    }
+    const Row<TYPE> x(a.logits, a.ld, r, a.V);
+    // the segment's vectors [j0, j1)
+    const int per = a.S > 1 ? ((x.nv + a.S - 1) / a.S + TPR - 1) / TPR * TPR : x.nv;
+    const int j0 = min(seg * per, x.nv), j1 = min(j0 + per, x.nv);
+    u32x4 raw[U];
+    auto load = [&](int j) {
+        if (j >= x.f0 && j + (U - 1) * TPR < min(x.f1, j1)) {
+#pragma unroll
+            for (int k = 0; k < U; k++) raw[k] = __builtin_nontemporal_load(x.v + j + k * TPR);
+        } else {
+#pragma unroll
+            for (int k = 0; k < U; k++) raw[k] = x.any(j + k * TPR < j1 ? j + k * TPR : x.nv);
+        }
+    };
+
+    // lines are joined over 2^q rounds of the loop
+    int q = 0;
+    if constexpr (LINES)
+        while (LP_LINES * 8 * W << q < j1 - j0 + 8 * U * W) q++;
+    const Given given = lp_given<TYPE>(a, r, x.x, t);
+    Acc A = ACC0;
+    float v1 = -INFINITY, lm[U];
+    for (int j = j0 + t, i = 0; RES ? i == 0 : j - lane < j1; j += U * TPR, i++) {      // whole waves
+        load(j);
+        float gm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            float vm = el_at<TYPE>(raw[k], 0);
+#pragma unroll
+            for (int e = 1; e < VE; e++) vm = fmaxf(vm, el_at<TYPE>(raw[k], e));
+            gm = fmaxf(gm, vm);
+            if constexpr (LINES) lm[k] = i & ((1 << q) - 1) ? fmaxf(lm[k], vm) : vm;
+        }
+        if constexpr (LINES) {
+            float o[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) {               // over 8 lanes
+                o[k] = fmaxf(lm[k], lane_move<0xB1>(lm[k]));
+                o[k] = fmaxf(o[k], lane_move<0x4E>(o[k]));
+                o[k] = fmaxf(o[k], lane_move<0x141>(o[k]));
+            }
+            if (lane % 8 == 0) {
+                float *to = sh.max + (((i >> q) * W + wave) * 8 + lane / 8) * U;
+                if constexpr (U == 4) *(f32x4 *)to = f32x4{o[0], o[1], o[2], o[3]};
+                else
+#pragma unroll
+                    for (int k = 0; k < U; k++) to[k] = o[k];
+            }
+        }
+        v1 = fmaxf(v1, gm);
+        acc_shift(A, acc_ref(v1, a.c));
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            if (RES) keep_packed(raw[k]);
+#pragma unroll
+            for (int e = 0; e < VE; e++) acc_add(A, el_at<TYPE>(raw[k], e), a.c);
+            if (RES) keep_packed(raw[k]);
+        }
+    }
+
+    // the row's sums, maximum and bound
+    float m = wave_max(v1), T = -FLT_MAX;
+    A = acc_wave(A, m, a.c);
+    if constexpr (TOP) {
+        const int full = min(W, (j1 - j0) / 64);        // waves whose lanes all have a vector
+        const int J = full ? (a.K + full - 1) / full : 65;
+        T = wave >= (full ? full : 1) ? FLT_MAX : wave_bound(v1, J);
+        if (W > 1 && t == 0) sh.n = sh.lines = 0;
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) sh.part[wave] = f32x4{A.s, A.u, m, T};
+    }
+    row_sync<W>();
+    if constexpr (W > 1) {
+        A = acc_join(sh.part, W, a.c, m);
+        for (int w = 0; w < W; w++) T = fminf(T, sh.part[w][3]);
+        if (a.S > 1 && t == 0) ((f32x4 *)a.part)[r * a.S + seg] = f32x4{A.s, A.u, m, 0.f};
+    }
+    Sums sum = {0.f, 0.f, 0.f};
+    if (W == 1 || a.S == 1) {
+        sum = sums_of<TYPE, W>(x, m, A, a.c, a.kappa, t, sh.part);
+        lp_finish(a, r, given, sum, t);
+    }
+    if constexpr (!TOP) return;
+
+    // The lines that reach T, then the elements that do.  Line l is the lanes 8 o ..
+    // 8 o + 7 of wave w in load k of the rounds i 2^q ..., from l's digits.
+    int n1 = 0, lines1 = 0;                             // the lists' lengths, for one wave
+    int &n = W == 1 ? n1 : sh.n, &lines = W == 1 ? lines1 : sh.lines;
+    auto first = [&](int l) {
+        const int k = l % U, o = l / U % 8, w = l / (U * 8) % W, i = l / (U * 8 * W);
+        return j0 + (((i << q) * U + k) * W + w) * 64 + o * 8;
+    };
+    int items = 0;
+    if constexpr (LINES) {
+        const int rounds = (j1 - j0 + U * TPR - 1) / (U * TPR), all = ((rounds + (1 << q) - 1) >> q) * (U * 8 * W);
+        for (int l = t; l - lane < all; l += TPR) {
+            const bool take = l < all && first(l) < j1 && sh.max[l] >= T;
+            if constexpr (W == 1) wave_push(take, (unsigned short)l, sh.line, lines, LP_LINES);
+            else if (take) sh.line[atomicAdd(&lines, 1)] = l;
+        }
+        row_sync<W>();
+        items = lines * 8 << q;
+    }
+    auto list = [&](u64 Tkey) {
+        if constexpr (RES) {
+#pragma unroll
+            for (int k = 0; k < U; k++) lp_list<TYPE, W>(raw[k], j0 + t + k * TPR, T, Tkey, sh.cand, n, CAP);
+        } else
+            for (int i = t; i - lane < items; i += TPR) {
+                int j = x.nv;
+                if (i < items)
+                    j = first(sh.line[i >> (3 + q)]) + (i >> 3 & ((1 << q) - 1)) * (U * TPR) + i % 8;
+                lp_list<TYPE, W>(x.any(j < j1 ? j : x.nv), j, T, Tkey, sh.cand, n, CAP);
+            }
+        row_sync<W>();
+    };
+    list(0);
+    while (n > CAP) {
+        u64 b = 0;
+        for (int i = t; i < CAP; i += TPR) b = sh.cand[i] > b ? sh.cand[i] : b;
+        b = wave_bound_key(b, (a.K + W - 1) / W);
+        if constexpr (W > 1) {
+            if (lane == 0) sh.t[wave] = b;
+            row_sync<W>();
+            for (int w = 0; w < W; w++) b = sh.t[w] < b ? sh.t[w] : b;
+            if (t == 0) n = 0;
+        } else
+            n = 0;
+        row_sync<W>();
+        list(b);
+    }
+    const int got = n;
+    u64 *out = a.keys + r * a.K * a.S + seg;             // S > 1
+    for (int i = t; i < got; i += TPR) {
+        const u64 key = sh.cand[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int o = 0; o < got; o++) rank += sh.cand[o] > key;
+        if (rank < a.K) {
+            if (W > 1 && a.S > 1) out[(size_t)rank * a.S] = key;
+            else lp_put(a, r, rank, key, x.sh, sum);
+        }
+    }
+    for (int k = got + t; k < a.K; k += TPR) {
+        if (W > 1 && a.S > 1) out[(size_t)k * a.S] = 0;
+        else lp_put(a, r, k, 0, x.sh, sum);
+    }
+}
+
+// Joins the S segments of a row: one workgroup per row.  Their K largest come
+// sorted; the same bound and list pick the row's K from them, and the list can
+// hold all of them.
+#define LP_JOIN 4096                                     // S K at most
+template <int TYPE, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a)
+{
+    __shared__ f32x4 part[64];
+    __shared__ float tw[4];
+    __shared__ u64 cand[TOP ? LP_JOIN : 1];
+    __shared__ int cnt;
     const size_t r = blockIdx.x;
-    const int t = threadIdx.x;
-    const T *x = (const T *)logits + r * ld;
-    T *d = (T *)dlogits + r * ldd;
-    float xv = 0.f;
-    if (t < M) {
-        const int id = ids[r * M + t];
-        si[t] = id;
-        sg[t] = id >= V ? NAN : id >= 0 ? dlogp[r * M + t] : 0.f;
-        if (id >= 0 && id < V) xv = (float)x[id];
+    const int t = threadIdx.x, lane = t & 63, n = a.S * a.K;
+    const Row<TYPE> x(a.logits, a.ld, r, a.V);
+    const Given given = lp_given<TYPE>(a, r, x.x, t);
+    if (t < a.S) part[t] = ((const f32x4 *)a.part)[r * a.S + t];
+    float T = -FLT_MAX;
+    const u64 *keys = a.keys + r * n;
+    if constexpr (TOP) {
+        u64 b = 0;
+        for (int i = t; i < n; i += 256) b = keys[i] > b ? keys[i] : b;
+        const int full = min(4, n / 64), J = full ? (a.K + full - 1) / full : 65;
+        T = t / 64 >= (full ? full : 1) ? FLT_MAX : wave_bound(b ? vb_key_value(b) : -FLT_MAX, J);
+        if (lane == 0) tw[t >> 6] = T;
+        if (t == 0) cnt = 0;
     }
     __syncthreads();
-    float c0 = dlse ? dlse[r] : 0.f;
-    for (int j = 0; j < M; j++) c0 -= sg[j];
-    const float c1 = dent ? dent[r] : 0.f, H = dent ? entropy[r] : 0.f;
-    const float m = lse2[2 * r], ls = lse2[2 * r + 1];
-    const bool empty = m == -INFINITY, zero = empty || (c0 == 0.f && c1 == 0.f);
-    auto grad = [&](float v) -> float {
-        if (zero) return 0.f;
-        const float lp = (v - m) * scale - ls, p = expf(lp);
-        return c0 * p - (p == 0.f ? 0.f : c1 * p * (lp + H));
-    };
-    for (int i = t; i < V; i += VB) d[i] = (T)(scale * grad(zero ? 0.f : (float)x[i]));
+    float m;
+    const Acc A = acc_join(part, a.S, a.c, m);
     __syncthreads();
-    if (t < M && !empty && si[t] >= 0 && si[t] < V) {
+    const Sums sum = sums_of<TYPE, 4>(x, m, A, a.c, a.kappa, t, part);
+    lp_finish(a, r, given, sum, t);
+    if constexpr (!TOP) return;
+    for (int w = 0; w < 4; w++) T = fminf(T, tw[w]);
+    for (int i = t; i < n; i += 256)
+        if (keys[i] && vb_key_value(keys[i]) >= T) cand[atomicAdd(&cnt, 1)] = keys[i];
+    __syncthreads();
+    const int got = cnt;
+    for (int i = t; i < got; i += 256) {
+        const u64 q = cand[i];
+        int rank = 0;
+        for (int o = 0; o < got; o++) rank += cand[o] > q;
+        if (rank < a.K) lp_put(a, r, rank, q, x.sh, sum);
+    }
+    for (int k = got + t; k < a.K; k += 256) lp_put(a, r, k, 0, x.sh, sum);
+}
+
+// Writing: vector j of row x's grid, one element at a time where the row's ends
+// or a different alignment of the written row ask for it.
+template <int TYPE>
+__device__ __forceinline__ void row_store(const Row<TYPE> &x, const Row<TYPE> &d, int j, const float *g)
+{
+    constexpr int VE = El<TYPE>::VE;
+    if (j >= x.f0 && j < x.f1 && d.sh == x.sh) {
+        u32x4 q;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if constexpr (TYPE == TLG_F32) q[k] = __float_as_uint(g[k]);
+            else q[k] = el_bits<TYPE>(g[2 * k]) | el_bits<TYPE>(g[2 * k + 1]) << 16;
+        }
+        __builtin_nontemporal_store(q, const_cast<u32x4 *>(d.v) + j);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+        const int i = j * VE + e - x.sh;
+        if (i >= 0 && i < x.V) el_store<TYPE>(const_cast<char *>(d.x), i, g[e]);
+    }
+}
+
+// ------------------------------------------------- log probabilities' gradient --
+// dz_v = p_v (c0 - c1 (log p_v + H)) + the given tokens' own terms, with t_v =
+// (x_v - m) c:  p_v = 2^t_v / S and log p_v = ln 2 t_v - log S, so a logit costs one
+// exponential and two products.  One workgroup writes a segment of up to BW_SEG
+// vectors of a row, then once more the given tokens among them; their logits are
+// read before the first write, which may go to the same place.
+#define BW_SEG 2048
+struct LpBwdArgs {
+    const void *logits;
+    long long ld;
+    int V, S;
+    float scale, c;
+    const int *ids;
+    int M;
+    const float *lse2, *entropy, *dlogp, *dlse, *dent;
+    void *dlogits;
+    long long ldd;
+};
+
+template <int TYPE> __global__ __launch_bounds__(256) void k_logprobs_bwd(LpBwdArgs a)
+{
+    constexpr int VE = El<TYPE>::VE, U = 4;
+    __shared__ int si[TLG_VOCAB_IDS];
+    __shared__ float sg[TLG_VOCAB_IDS];
+    const size_t r = blockIdx.x / (unsigned)a.S;
+    const int seg = blockIdx.x % (unsigned)a.S, t = threadIdx.x;
+    const Row<TYPE> x(a.logits, a.ld, r, a.V), d(a.dlogits, a.ldd, r, a.V);
+    const int j0 = seg * BW_SEG, j1 = min(j0 + BW_SEG, x.nv);
+    float xv = 0.f;
+    bool mine = false;
+    if (t < a.M) {
+        const int id = a.ids[r * a.M + t];
+        si[t] = id;
+        sg[t] = id >= a.V ? NAN : id >= 0 ? a.dlogp[r * a.M + t] : 0.f;
+        const int j = (id + x.sh) / VE;
+        mine = id >= 0 && id < a.V && j >= j0 && j < j1;
+        if (mine) xv = el_load<TYPE>(x.x, id);
+    }
+    __syncthreads();
+    float c0 = a.dlse ? a.dlse[r] : 0.f;
+    for (int j = 0; j < a.M; j++) c0 -= sg[j];
+    const float c1 = a.dent ? a.dent[r] : 0.f, H = a.dent ? a.entropy[r] : 0.f;
+    const float m = a.lse2[2 * r], ls = a.lse2[2 * r + 1];
+    const bool empty = m == -INFINITY, zero = empty || (c0 == 0.f && c1 == 0.f);
+    const float rs = a.scale * __expf(-ls), k1 = -0.69314718056f * c1, k0 = c0 - c1 * (H - ls);
+    auto grad = [&](float v) -> float {
+        const float e = (v - m) * a.c;
+        return __builtin_amdgcn_exp2f(e) * rs * fmaf(k1, fmaxf(e, -200.f), k0);
+    };
+    for (int j = j0 + t; j < j1; j += U * 256) {
+        u32x4 raw[U];
+        float g[U][VE];
+        if (zero) {
+#pragma unroll
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) g[k][e] = 0.f;
+        } else {
+            if (j >= x.f0 && j + (U - 1) * 256 < min(x.f1, j1)) {
+#pragma unroll
+                for (int k = 0; k < U; k++) raw[k] = __builtin_nontemporal_load(x.v + j + k * 256);
+            } else {
+#pragma unroll
+                for (int k = 0; k < U; k++) raw[k] = x.any(j + k * 256 < j1 ? j + k * 256 : x.nv);
+            }
+#pragma unroll
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) g[k][e] = grad(el_at<TYPE>(raw[k], e));
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++)
+            if (j + k * 256 < j1) row_store<TYPE>(x, d, j + k * 256, g[k]);
+    }
+    __syncthreads();
+    if (mine && !empty) {
         float g = 0.f;
-        for (int j = 0; j < M; j++) g += si[j] == si[t] ? sg[j] : 0.f;
-        d[si[t]] = (T)(scale * (grad(xv) + g));
+        for (int j = 0; j < a.M; j++) g += si[j] == si[t] ? sg[j] : 0.f;
+        el_store<TYPE>(const_cast<char *>(d.x), si[t], (zero ? 0.f : grad(xv)) + a.scale * g);
     }
 }
 
 // -------------------------------------------------------------- distillation --
-struct DistillArgs {
+// With S the teacher's ids, m_o and s_o the maximum and sum over the tokens
+// outside S (over all of them when there is no remainder), M and s the whole
+// row's, every token outside S has
+//   d / dx_v = E_v (w_kd tau (Q F / s - q_r / s_o) + w_ce F / s),  E_v = 2^((x_v - m_o) c),
+//   F = 2^((m_o - M) c)
+// (one exponential; a second one where the cross-entropy has another temperature).
+// The reference m_o keeps the remainder exact however little the student gives
+// it, and summing it without the ids' terms, which a bitmap in LDS marks, keeps it
+// from being a difference.  The ids and the target are written again afterwards.
+struct KdArgs {
     const void *logits;
     long long ld;
-    int V, K, tail;
+    int N, V, S, K, tail;
     float tau, w_kd, w_ce, scale;
+    float c, kappa, inv;          // log2 e / tau rounded, ln 2 (log2 e / tau - c) / c, 1 / tau
+    int two;                      // the cross-entropy needs sums of its own: w_ce != 0 and tau != 1
     const int *t_ids;
     const float *t_logp;
     const int *tgt;
     float *rows;
     void *dlogits;
     long long ldd;
+    int words;                    // tail: 32-bit words of a row's (or segment's) bitmap
+    float *part;                  // S > 1: [N][S][4] sums, then [N][KD_XS] logits of ids and target
+};
+#define KD_XS (TLG_VOCAB_TOP + 1)
+#define KD_C1 1.44269504088896f   // log2 e, the cross-entropy's c
+
+// sums of a part: at temperature tau with entropy sum (for the rounding of c), and at 1
+struct Kd { float m, s, u, s1; };
+__device__ __forceinline__ void kd_shift(Kd &a, float m, float c, int two)
+{
+    const float d = (a.m - m) * c, f = __builtin_amdgcn_exp2f(d);
+    if (two) a.s1 *= __builtin_amdgcn_exp2f((a.m - m) * KD_C1);
+    a.u = f * fmaf(fmaxf(d, -200.f), a.s, a.u);
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ void kd_add(Kd &a, float x, float c, int two)
+{
+    const float t = (x - a.m) * c, e = __builtin_amdgcn_exp2f(t);
+    if (two) a.s1 += __builtin_amdgcn_exp2f((x - a.m) * KD_C1);
+    a.s += e;
+    a.u = fmaf(e, fmaxf(t, -200.f), a.u);
+}
+__device__ __forceinline__ Kd kd_wave(Kd a, float c, int two)
+{
+    kd_shift(a, wave_max(a.m), c, two);
+    return Kd{a.m, wave_sum(a.s), wave_sum(a.u), two ? wave_sum(a.s1) : 0.f};
+}
+__device__ __forceinline__ Kd kd_join(const float (*p)[4], int n, float c, int two)
+{
+    Kd r = {-FLT_MAX, 0.f, 0.f, 0.f};
+    for (int w = 0; w < n; w++) r.m = fmaxf(r.m, p[w][0]);
+    for (int w = 0; w < n; w++) {
+        Kd a = {p[w][0], p[w][1], p[w][2], p[w][3]};
+        kd_shift(a, r.m, c, two);
+        r.s += a.s;
+        r.u += a.u;
+        r.s1 += a.s1;
+    }
+    return r;
+}
+
+template <int W> struct KdShared {
+    float part[W][4];
+    float in[2][4];               // the ids' part, by the waves that hold them
+    int ids[TLG_VOCAB_TOP];
+    double d[2][4];
+    float f[2];
+    int flag;                     // an id or a target past the vocabulary
 };
 
-#define VB_TOP 128
-template <int TYPE> __global__ __launch_bounds__(VB) void k_distill(DistillArgs a)
+enum { KD_WHOLE = 0, KD_SUMS = 1, KD_GRAD = 2 };
+// W waves on a row (PHASE KD_WHOLE) or on one of its S segments: KD_SUMS leaves
+// the segment's sums, KD_GRAD joins them and writes the segment.  RES: a
+// thread's part, at most U vectors, stays in registers between sums and gradient.
+template <int TYPE, int W, int U, bool RES, int PHASE>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(KdArgs a)
 {
-    typedef typename El<TYPE>::t T;
-    __shared__ float sh[4];
-    __shared__ double shd[4];
-    __shared__ int si[VB_TOP];
-    __shared__ int sflag;
-    extern __shared__ unsigned bits[];              // tail: the support as a set
-    const size_t r = blockIdx.x;
-    const int t = threadIdx.x, V = a.V, K = a.K;
-    const T *x = (const T *)a.logits + r * a.ld;
-    T *d = a.dlogits ? (T *)a.dlogits + r * a.ldd : nullptr;
+    constexpr int VE = El<TYPE>::VE, TPR = 64 * W, EPT = W == 1 ? 2 : 1, EW = W == 1 ? 1 : 2;
+    __shared__ KdShared<W> shared[W == 1 ? 4 : 1];
+    extern __shared__ unsigned all_bits[];              // tail: the support, a bit for each element
+    const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, t = W == 1 ? lane : threadIdx.x;
+    const int slot = W == 1 ? threadIdx.x >> 6 : 0;
+    KdShared<W> &sh = shared[slot];
+    size_t r;
+    int seg = 0;
+    if constexpr (W == 1) {
+        r = (size_t)blockIdx.x * 4 + slot;
+        if (r >= (size_t)a.N) return;
+    } else {
+        r = blockIdx.x / (unsigned)a.S;
+        seg = blockIdx.x % (unsigned)a.S;
+    }
+    const Row<TYPE> x(a.logits, a.ld, r, a.V);
+    const int per = a.S > 1 ? ((x.nv + a.S - 1) / a.S + TPR - 1) / TPR * TPR : x.nv;
+    const int j0 = min(seg * per, x.nv), j1 = min(j0 + per, x.nv);
+    const int K = a.K;
+    const float c = a.c;
+
+    u32x4 raw[U];
+    auto load = [&](int j) {
+        if (j >= x.f0 && j + (U - 1) * TPR < min(x.f1, j1)) {
+#pragma unroll
+            for (int k = 0; k < U; k++) raw[k] = RES ? __builtin_nontemporal_load(x.v + j + k * TPR) : x.v[j + k * TPR];
+        } else {
+#pragma unroll
+            for (int k = 0; k < U; k++) raw[k] = x.any(j + k * TPR < j1 ? j + k * TPR : x.nv);
+        }
+    };
+
+    if (RES) load(j0 + t);
+
+    // the ids: a repeated one counts at its first place
+    unsigned *bits = all_bits + slot * a.words;
     const int tgt = a.w_ce != 0.f ? a.tgt[r] : -1;
-    if (t == 0) sflag = tgt >= V;
-    if (t < K) si[t] = a.t_ids[r * K + t];
-    if (a.tail)
-        for (int i = t; i < (V + 31) / 32; i += VB) bits[i] = 0;
-    __syncthreads();
-    // the teacher's entry of thread t: an id counts once, at its first place
-    int id = -1;
-    double tl = -INFINITY;
-    if (t < K) {
-        id = si[t];
-        if (id >= V) sflag = 1;
-        for (int j = 0; j < t; j++)
-            if (si[j] == id) id = -1;
-        if (id >= V) id = -1;
-        if (id >= 0) {
-            tl = a.t_logp[r * K + t];
-            if (a.tail) atomicOr(&bits[id >> 5], 1u << (id & 31));
+    if (t == 0) sh.flag = tgt >= a.V;
+    int id[EPT];
+#pragma unroll
+    for (int k = 0; k < EPT; k++) {
+        id[k] = t + 64 * k < K ? a.t_ids[r * K + t + 64 * k] : -1;
+        if (t + 64 * k < TLG_VOCAB_TOP) sh.ids[t + 64 * k] = id[k];
+    }
+    if (a.tail && PHASE != KD_GRAD)
+        for (int i = t; i < a.words; i += TPR) bits[i] = 0;
+    row_sync<W>();
+    bool any = false, hit = false;                       // entries at all; the target among them
+#pragma unroll
+    for (int k = 0; k < EPT; k++) {
+        if (id[k] >= a.V) sh.flag = 1;
+        if (id[k] >= 0)
+            for (int j = 0; j < t + 64 * k; j++)
+                if (sh.ids[j] == id[k]) id[k] = -1;
+        if (id[k] >= a.V) id[k] = -1;
+        if (a.tail && PHASE != KD_GRAD && id[k] >= 0) {
+            const int g = id[k] + x.sh - j0 * VE;
+            if (g >= 0 && g < per * VE) atomicOr(&bits[g >> 5], 1u << (g & 31));
         }
     }
-    __syncthreads();
-    const bool bad_id = sflag;
-    const int some = (int)vb_sum(id >= 0 ? 1.f : 0.f, sh);
-    if (!some && tgt < 0) {                       // nothing to learn from: the logits are not read
-        if (d)
-            for (int i = t; i < V; i += VB) d[i] = (T)0.f;
-        if (a.rows && t == 0) a.rows[r] = bad_id ? NAN : 0.f;
+    for (int j = 0; j < K; j++) {
+        const int i = sh.ids[j];
+        any |= i >= 0 && i < a.V;
+        hit |= i == tgt;
+    }
+    row_sync<W>();
+    const bool bad_id = sh.flag;
+    const bool nothing = !any && tgt < 0 && !bad_id;     // such a row's logits are not read
+
+    // the ids' logits and the teacher's side, in 64 bits: q, Q, q_r
+    float xk[EPT], xt = 0.f;
+    double q[EPT], tl[EPT];
+    const float *xs = a.part + (size_t)a.N * a.S * 4 + r * KD_XS;        // S > 1
+    Kd B = {-FLT_MAX, 0.f, 0.f, 0.f};
+    float tm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < EPT; k++) {
+        xk[k] = -INFINITY;
+        tl[k] = -INFINITY;
+        if (id[k] >= 0) {
+            xk[k] = PHASE == KD_GRAD ? xs[t + 64 * k] : el_load<TYPE>(x.x, id[k]);
+            const float l = a.t_logp[r * K + t + 64 * k];
+            tl[k] = l;
+            tm = fmaxf(tm, l);
+        }
+    }
+    if (tgt >= 0 && tgt < a.V) xt = PHASE == KD_GRAD ? xs[KD_XS - 1] : el_load<TYPE>(x.x, tgt);
+    // sums
+    Kd A = {-FLT_MAX, 0.f, 0.f, 0.f};
+    if (PHASE != KD_GRAD && !nothing) {
+        for (int j = j0 + t; RES ? j == j0 + t : j < j1; j += U * TPR) {
+            if (!RES) load(j);
+            if (a.tail)
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    const int g = (j + k * TPR - j0) * VE;           // VE divides 32
+                    unsigned b = j + k * TPR < j1 ? bits[g >> 5] >> (g & 31) & ((1u << VE) - 1) : 0;
+                    if (b)
+#pragma unroll
+                        for (int e = 0; e < VE; e++)
+                            if (b >> e & 1) {
+                                if constexpr (TYPE == TLG_F32) raw[k][e] = El<TYPE>::NEG;
+                                else raw[k][e >> 1] = e & 1 ? (raw[k][e >> 1] & 0xffffu) | El<TYPE>::NEG << 16
+                                                            : (raw[k][e >> 1] & 0xffff0000u) | El<TYPE>::NEG;
+                            }
+                }
+            float m = A.m;
+#pragma unroll
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) m = fmaxf(m, el_at<TYPE>(raw[k], e));
+            kd_shift(A, m, c, a.two);
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                if (RES) keep_packed(raw[k]);
+#pragma unroll
+                for (int e = 0; e < VE; e++) kd_add(A, el_at<TYPE>(raw[k], e), c, a.two);
+                if (RES) keep_packed(raw[k]);
+            }
+        }
+    }
+
+    if constexpr (PHASE == KD_SUMS) {
+        A = kd_wave(A, c, a.two);
+        if (lane == 0) { sh.part[wave][0] = A.m; sh.part[wave][1] = A.s; sh.part[wave][2] = A.u; sh.part[wave][3] = A.s1; }
+        row_sync<W>();
+        if (t == 0) {
+            A = kd_join(sh.part, W, c, a.two);
+            float *p = a.part + (r * a.S + seg) * 4;
+            p[0] = A.m; p[1] = A.s; p[2] = A.u; p[3] = A.s1;
+        }
+        if (seg == 0) {
+            float *o = const_cast<float *>(xs);
+            if (t < TLG_VOCAB_TOP) o[t] = xk[0];
+            if (t == 0) o[KD_XS - 1] = xt;
+        }
         return;
     }
-    const float inv = 1.0f / a.tau;
-    float xk = 0.f, xt = 0.f;
-    if (id >= 0) xk = (float)x[id];
-    if (tgt >= 0 && tgt < V) xt = (float)x[tgt];
-    float m = -INFINITY;
-    for (int i = t; i < V; i += VB) m = fmaxf(m, (float)x[i]);
-    m = vb_max(m, sh);
-    const bool empty = m == -INFINITY;
-    float s1 = 0.f, so = 0.f, si_ = 0.f;            // CE; outside and inside the support
-    for (int i = t; i < V; i += VB) {
-        const float v = empty ? -INFINITY : (float)x[i] - m, e = expf(v * inv);
-        s1 += expf(v);
-        if (a.tail && (bits[i >> 5] >> (i & 31) & 1)) si_ += e;
-        else so += e;
+    // the waves that hold entries: all of W == 1's, two of the others
+    if (wave < EW) {
+        if (a.tail) {
+#pragma unroll
+            for (int k = 0; k < EPT; k++) B.m = fmaxf(B.m, xk[k]);
+#pragma unroll
+            for (int k = 0; k < EPT; k++) kd_add(B, xk[k], c, a.two);
+            B = kd_wave(B, c, a.two);
+        }
+        tm = wave_max(tm);
+        if (W > 1 && lane == 0) {
+            sh.in[wave][0] = B.m; sh.in[wave][1] = B.s; sh.in[wave][2] = B.u; sh.in[wave][3] = B.s1;
+            sh.f[wave] = tm;
+        }
     }
-    s1 = vb_sum(s1, sh);
-    so = vb_sum(so, sh);
-    si_ = vb_sum(si_, sh);
-    const float s = so + si_;
-    // the teacher's distribution
-    double q, Q, qr = 0.0;
-    if (a.tail) {
-        q = id >= 0 ? exp(tl) : 0.0;
-        Q = vb_sum(q, shd);
-        if (some && some < V && Q < 1.0) qr = 1.0 - Q;
-        Q += qr;
+    if constexpr (PHASE == KD_WHOLE) {
+        A = kd_wave(A, c, a.two);
+        if (W > 1 && lane == 0) {
+            sh.part[wave][0] = A.m; sh.part[wave][1] = A.s; sh.part[wave][2] = A.u; sh.part[wave][3] = A.s1;
+        }
+    }
+    row_sync<W>();
+    if constexpr (W > 1) {
+        A = PHASE == KD_WHOLE ? kd_join(sh.part, W, c, a.two) : kd_join((const float (*)[4])(a.part + r * a.S * 4), a.S, c, a.two);
+        B = kd_join(sh.in, EW, c, a.two);
+        tm = fmaxf(sh.f[0], sh.f[1]);
+    }
+    // teacher
+    double sum = 0.0;
+    if (wave < EW) {
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            q[k] = id[k] < 0 ? 0.0 : tl[k] != tl[k] ? tl[k] : a.tail ? exp(tl[k]) : tm > -INFINITY ? exp(tl[k] - tm) : 0.0;
+            sum += q[k];
+        }
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        int cnt = 0;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) cnt += __popcll(__ballot(id[k] >= 0));
+        if (W > 1 && lane == 0) {
+            sh.d[wave][0] = sum;
+            sh.d[wave][1] = cnt;
+        }
+        if (W == 1) sh.d[0][1] = cnt;
+    }
+    int some;
+    if constexpr (W > 1) {
+        row_sync<W>();
+        sum = sh.d[0][0] + sh.d[1][0];
+        some = (int)(sh.d[0][1] + sh.d[1][1]);
     } else {
-        const float tm = vb_max((float)tl, sh);
-        q = id >= 0 && tm > -INFINITY ? exp(tl - tm) : 0.0;
-        if (tl != tl) q = tl;
-        Q = vb_sum(q, shd);
-        q = Q > 0.0 || Q != Q ? q / Q : 0.0;
-        Q = Q > 0.0 ? 1.0 : Q;
+        some = 0;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) some += __popcll(__ballot(id[k] >= 0));
     }
-    const double ls = log((double)s), ls1 = log((double)s1);
-    double kl = 0.0;
-    if (q > 0.0 || q != q) kl = empty ? INFINITY : q * (log(q) - ((double)(xk - m) * inv - ls));
-    kl = vb_sum(kl, shd);
-    if (qr > 0.0) kl += empty ? INFINITY : qr * (log(qr) - (log((double)so) - ls));
-    if (a.rows && t == 0) {
-        double L = (double)a.w_kd * a.tau * a.tau * kl;
-        if (a.w_kd == 0.f || !some) L = 0.0;
-        if (tgt >= 0) L += (double)a.w_ce * (empty ? INFINITY : ls1 - (double)(xt - m));
-        if (s != s) L = NAN;
-        a.rows[r] = bad_id ? NAN : (float)L;
+    double qr = 0.0, Q;
+    if (a.tail) {
+        if (some && some < a.V && sum < 1.0) qr = 1.0 - sum;
+        Q = sum + qr;
+    } else {
+        const double n = sum > 0.0 || sum != sum ? 1.0 / sum : 0.0;
+        if (wave < EW)
+#pragma unroll
+            for (int k = 0; k < EPT; k++) q[k] *= n;
+        Q = sum > 0.0 ? 1.0 : sum;
     }
-    if (!d) return;
-    const float rs = 1.0f / s, rs1 = 1.0f / s1;
-    const float ck = some ? a.w_kd * a.tau * a.scale : 0.f, cc = tgt >= 0 ? a.w_ce * a.scale : 0.f;
-    const float in = (float)Q, out = qr > 0.0 && so > 0.f ? (float)(Q - qr * s / so) : in;
-    auto grad = [&](float v, float mass) -> float {
-        if (bad_id) return NAN;
-        if (empty) return 0.f;
-        const float g = v - m;
-        return ck * mass * (expf(g * inv) * rs) + (cc != 0.f ? cc * (expf(g) * rs1) : 0.f);
+    // the row's sums
+    const float so = fmaf(a.kappa, A.u, A.s);
+    const float M = fmaxf(A.m, B.m);
+    const float F = __builtin_amdgcn_exp2f((A.m - M) * c), G = __builtin_amdgcn_exp2f((B.m - M) * c);
+    const float s = so * F + fmaf(a.kappa, B.u, B.s) * G;
+    float s1 = s;
+    if (a.two)
+        s1 = A.s1 * __builtin_amdgcn_exp2f((A.m - M) * KD_C1) + B.s1 * __builtin_amdgcn_exp2f((B.m - M) * KD_C1);
+    const bool empty = s == 0.f;
+    const float ck = any ? a.w_kd * a.tau * a.scale : 0.f, cc = tgt >= 0 ? a.w_ce * a.scale : 0.f;
+    const float rs = empty ? 0.f : 1.f / s, r1 = empty ? 0.f : 1.f / s1;
+    const float kin = ck * (float)Q * rs;                                  // inside S, reference M
+    float kout = kin * F;                                                  // outside, reference m_o
+    if (qr > 0.0 && A.s > 0.f) kout -= ck * ((float)qr / so);
+    if (!a.two) kout += cc * r1 * F;
+    const float k1 = a.two ? cc * r1 : 0.f;
+    if (bad_id) kout = NAN;
+    auto outside = [&](float v) -> float {
+        float g = kout * __builtin_amdgcn_exp2f((v - A.m) * c);
+        if (a.two) g = fmaf(k1, __builtin_amdgcn_exp2f((v - M) * KD_C1), g);
+        return g;
     };
-    __syncthreads();                              // every read of x[id] precedes the writes (in place)
-    for (int i = t; i < V; i += VB) d[i] = (T)grad((float)x[i], out);
-    __syncthreads();
-    bool hit = false;                             // is the target one of the teacher's ids?
-    for (int j = 0; j < K; j++) hit |= si[j] == tgt;
-    if (empty || bad_id) return;
-    if (id >= 0) d[id] = (T)(grad(xk, in) - ck * (float)q - (id == tgt ? cc : 0.f));
-    if (t == 0 && tgt >= 0 && tgt < V && !hit) d[tgt] = (T)(grad(xt, out) - cc);
+    char *dl = (char *)a.dlogits;
+    if (dl) {
+        const Row<TYPE> d(a.dlogits, a.ldd, r, a.V);
+        const bool zero = nothing || (empty && !bad_id);
+        for (int j = j0 + t; RES ? j == j0 + t : j < j1; j += U * TPR) {
+            if (!RES && !zero) load(j);
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                float g[VE];
+#pragma unroll
+                for (int e = 0; e < VE; e++) g[e] = zero ? 0.f : outside(el_at<TYPE>(raw[k], e));
+                if (j + k * TPR < j1) row_store<TYPE>(x, d, j + k * TPR, g);
+            }
+        }
+        row_sync<W>();
+        if (!zero && !bad_id) {
+#pragma unroll
+            for (int k = 0; k < EPT; k++) {
+                const int j = (id[k] + x.sh) / VE;
+                if (id[k] >= 0 && j >= j0 && j < j1) {
+                    const float p = __builtin_amdgcn_exp2f((xk[k] - M) * c);
+                    float p1 = p * r1;
+                    if (a.two) p1 = __builtin_amdgcn_exp2f((xk[k] - M) * KD_C1) * r1;
+                    float g = kin * p - ck * (float)q[k] + (cc != 0.f ? cc * p1 : 0.f);
+                    if (id[k] == tgt) g -= cc;
+                    el_store<TYPE>(const_cast<char *>(d.x), id[k], g);
+                }
+            }
+            const int j = (tgt + x.sh) / VE;
+            if (t == 0 && tgt >= 0 && !hit && j >= j0 && j < j1)
+                el_store<TYPE>(const_cast<char *>(d.x), tgt, outside(xt) - cc);
+        }
+    }
+    if (!a.rows || seg != 0) return;
+    // the row's loss: log p_k = (x_k - M) / tau - log s
+    const double ls = log((double)s);
+    double kl = 0.0;
+    if (wave < EW) {
+#pragma unroll
+        for (int k = 0; k < EPT; k++)
+            if (q[k] > 0.0 || q[k] != q[k]) kl += empty ? INFINITY : q[k] * (log(q[k]) - ((double)(xk[k] - M) / a.tau - ls));
+        for (int o = 32; o > 0; o >>= 1) kl += __shfl_xor(kl, o);
+        if (W > 1 && lane == 0) sh.d[wave][2] = kl;
+    }
+    if constexpr (W > 1) row_sync<W>();
+    if (t == 0) {
+        if constexpr (W > 1) kl = sh.d[0][2] + sh.d[1][2];
+        if (qr > 0.0) kl += empty ? INFINITY : qr * (log(qr) - ((double)(A.m - M) / a.tau + log((double)so) - ls));
+        double L = 0.0;
+        if (any && a.w_kd != 0.f) L = (double)a.w_kd * a.tau * a.tau * kl;
+        if (tgt >= 0) L += (double)a.w_ce * (empty ? INFINITY : log((double)s1) - (double)(xt - M));
+        if (s != s) L = NAN;
+        a.rows[r] = bad_id ? NAN : nothing ? 0.f : (float)L;
+    }
 }
 
 // the mean of the row losses, summed in double in a fixed order
@@ -323,19 +1126,81 @@ static int vb_check_out(const char *who, const void *logits, long long ld, const
         return tlg_fail(TLG_EINVAL, "%s: dlogits overlaps logits without being the same rows", who);
     return TLG_OK;
 }
+static int vb_check_ws(const char *who, const void *ws, size_t have, size_t need)
+{
+    if (need && (have < need || !ws || (uintptr_t)ws % 16))
+        return tlg_fail(TLG_EINVAL, "%s: workspace %p of %zu bytes, %zu needed", who, ws, have, need);
+    return TLG_OK;
+}
 static bool vb_positive(float s) { return s > 0.f && s <= 3.4028234e38f; }
 
-#define BY_TYPE(kernel, grid, lds, ...)                                                                          \
-    do {                                                                                                         \
-        if (type == TLG_F32) hipLaunchKernelGGL(kernel<TLG_F32>, grid, dim3(VB), lds, st, __VA_ARGS__);          \
-        else if (type == TLG_F16) hipLaunchKernelGGL(kernel<TLG_F16>, grid, dim3(VB), lds, st, __VA_ARGS__);     \
-        else hipLaunchKernelGGL(kernel<TLG_BF16>, grid, dim3(VB), lds, st, __VA_ARGS__);                         \
+static float f_of(double v) { return (float)v; }
+
+// vectors of the longest row of a call: one more where rows do not all start on
+// the 16-byte grid
+static int vb_vectors(int type, const void *logits, long long ld, int V)
+{
+    const int b = (int)vb_size(type), ve = 16 / b;
+    const bool on_grid = (uintptr_t)logits % 16 == 0 && ld * b % 16 == 0;
+    return (V + (on_grid ? 0 : ve - 1) + ve - 1) / ve;
+}
+// Segments of a row.  A workgroup alone takes 12 us for a row of 8192 vectors and
+// 19 for one of 16384 (log probabilities, 20 alternatives); from 8192 vectors on, few
+// rows are cut into pieces of 2048 until 512 workgroups work (one row of 16384: 12.5
+// us, 128 of them 27.8 -> 20.2).  Shorter rows and 512 of them are not: the second
+// launch costs more than it saves (48 rows of 4000 vectors: 11.3 us whole, 12.4 cut).
+#define VB_CUT 8192
+#define VB_PIECE 2048
+#define VB_FILL 512
+static int vb_segments(int type, int N, int V, int most)
+{
+    const int ve = type == TLG_F32 ? 4 : 8;
+    if (V / ve < VB_CUT) return 1;
+    const long long by_rows = (VB_FILL + N - 1) / N, by_size = (V / ve + VB_PIECE - 1) / VB_PIECE;
+    const long long s = by_rows < by_size ? by_rows : by_size;
+    return s > most ? most : (int)s;
+}
+
+#define BY_TYPE(grid, block, lds, a, K0, ...)                                                                       \
+    do {                                                                                                            \
+        if (type == TLG_F32) hipLaunchKernelGGL((K0<TLG_F32 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a);    \
+        else if (type == TLG_F16) hipLaunchKernelGGL((K0<TLG_F16 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a); \
+        else hipLaunchKernelGGL((K0<TLG_BF16 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a);                   \
     } while (0)
+
+static int lp_segments(int type, int N, int V, int K)
+{
+    const int most = K > 0 && LP_JOIN / K < 64 ? LP_JOIN / K : 64;
+    return vb_segments(type, N, V, most);
+}
 
 extern "C" size_t tlg_logprobs_ws_bytes(int type, int N, int V, int K)
 {
-    (void)type; (void)N; (void)V; (void)K;
-    return 0;
+    if (N <= 0 || V <= 0 || K < 0) return 0;
+    const size_t S = lp_segments(type, N, V, K);
+    return S > 1 ? (size_t)N * S * (16 + 8 * (size_t)K) : 0;
+}
+
+// One wave per row where the rows are short and many: no barriers, and a lane's
+// four (or, of fp32, eight) vectors stay in registers; 4096 rows of 2048 fp32 values
+// with 8 alternatives take 11.3 us so, 13.2 with the rows read again, 18.3 with four
+// waves each.  Four waves win for fewer rows (512 of those: 6.5 against 7.1 us) and for
+// longer ones (4096 of 16384 fp32 values: 49 against 58 us).
+template <bool TOP> static void lp_launch(const LpArgs &a, int type, int nv, hipStream_t st)
+{
+    const unsigned rows = (unsigned)a.N;
+    const bool wave = a.K <= 48 && rows >= 1024;
+    if (a.S > 1) {
+        BY_TYPE(rows * a.S, 256, 0, a, k_logprobs, , 4, 4, false, TOP);
+        BY_TYPE(rows, 256, 0, a, k_logprobs_join, , TOP);
+    } else if (wave && nv <= 256)
+        BY_TYPE((rows + 3) / 4, 256, 0, a, k_logprobs, , 1, 4, true, TOP);
+    else if (wave && nv <= 512 && type == TLG_F32)
+        hipLaunchKernelGGL((k_logprobs<TLG_F32, 1, 8, true, TOP>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
+    else if (wave && nv <= 1024 && rows >= 2 * (unsigned)nv)
+        BY_TYPE((rows + 3) / 4, 256, 0, a, k_logprobs, , 1, 4, false, TOP);
+    else
+        BY_TYPE(rows, 256, 0, a, k_logprobs, , 4, 4, false, TOP);
 }
 
 extern "C" int tlg_dev_logprobs(const void *logits, int type, long long ld, int N, int V, float scale, const int *ids,
@@ -350,12 +1215,17 @@ extern "C" int tlg_dev_logprobs(const void *logits, int type, long long ld, int 
     if (N == 0) return TLG_OK;
     if ((M && (!ids || !logp)) || (K && (!top_ids || !top_logp)))
         return tlg_fail(TLG_EINVAL, "logprobs: NULL ids, logp, top_ids or top_logp");
-    if (ws_bytes < tlg_logprobs_ws_bytes(type, N, V, K))
-        return tlg_fail(TLG_EINVAL, "logprobs: workspace of %zu bytes", ws_bytes);
-    (void)ws;
+    if ((rc = vb_check_ws("logprobs", ws, ws_bytes, tlg_logprobs_ws_bytes(type, N, V, K)))) return rc;
     if ((rc = tlg_ensure_init())) return rc;
+    const double c = (double)scale * 1.4426950408889634;
+    LpArgs a = {logits, ld, N, V, lp_segments(type, N, V, K), scale, f_of(c), 0.f, ids, M, logp, lse2, entropy, K,
+                top_ids, top_logp, (float *)ws, nullptr};
+    a.kappa = f_of(0.6931471805599453 * (c - (double)a.c) / c);
+    a.keys = (u64 *)(a.part + (size_t)N * a.S * 4);
     hipStream_t st = ST(stream);
-    BY_TYPE(k_logprobs, dim3(N), 0, logits, ld, V, scale, ids, M, logp, lse2, entropy, K, top_ids, top_logp);
+    const int nv = vb_vectors(type, logits, ld, V);
+    if (K) lp_launch<true>(a, type, nv, st);
+    else lp_launch<false>(a, type, nv, st);
     LAUNCH_CHECK();
     return TLG_OK;
 }
@@ -374,17 +1244,22 @@ extern "C" int tlg_dev_logprobs_bwd(const void *logits, int type, long long ld, 
         return tlg_fail(TLG_EINVAL, "logprobs_bwd: NULL lse2, dlogits, ids, dlogp or entropy");
     if ((rc = vb_check_out("logprobs_bwd", logits, ld, dlogits, type, ldd, N, V))) return rc;
     if ((rc = tlg_ensure_init())) return rc;
+    const int S = (vb_vectors(type, logits, ld, V) + BW_SEG - 1) / BW_SEG;
+    const LpBwdArgs a = {logits, ld, V, S, scale, f_of((double)scale * 1.4426950408889634), ids, M, lse2, entropy,
+                         dlogp, dlse, dentropy, dlogits, ldd};
     hipStream_t st = ST(stream);
-    BY_TYPE(k_logprobs_bwd, dim3(N), 0, logits, ld, V, scale, ids, M, lse2, entropy, dlogp, dlse, dentropy, dlogits,
-            ldd);
+    BY_TYPE((unsigned)N * S, 256, 0, a, k_logprobs_bwd, );
     LAUNCH_CHECK();
     return TLG_OK;
 }
 
+static int kd_segments(int type, int N, int V) { return vb_segments(type, N, V, 64); }
+
 extern "C" size_t tlg_distill_ws_bytes(int type, int N, int V)
 {
-    (void)type; (void)N; (void)V;
-    return 0;
+    if (N <= 0 || V <= 0) return 0;
+    const size_t S = kd_segments(type, N, V);
+    return S > 1 ? (size_t)N * (S * 16 + KD_XS * 4) : 0;
 }
 
 extern "C" int tlg_dev_distill(const void *logits, int type, long long ld, int N, int V, const int *t_ids,
@@ -402,13 +1277,26 @@ extern "C" int tlg_dev_distill(const void *logits, int type, long long ld, int N
         return tlg_fail(TLG_EINVAL, "distill: NULL t_ids, t_logp or tgt");
     if ((!rows && !dlogits) || (loss && !rows)) return tlg_fail(TLG_EINVAL, "distill: NULL rows");
     if (dlogits && (rc = vb_check_out("distill", logits, ld, dlogits, type, ldd, N, V))) return rc;
-    if (ws_bytes < tlg_distill_ws_bytes(type, N, V))
-        return tlg_fail(TLG_EINVAL, "distill: workspace of %zu bytes", ws_bytes);
-    (void)ws;
+    if ((rc = vb_check_ws("distill", ws, ws_bytes, tlg_distill_ws_bytes(type, N, V)))) return rc;
     if ((rc = tlg_ensure_init())) return rc;
+    const double c = 1.4426950408889634 / (double)temp;
+    const int nv = vb_vectors(type, logits, ld, V), ve = type == TLG_F32 ? 4 : 8, S = kd_segments(type, N, V);
+    KdArgs a = {logits, ld, N, V, S, K, tail ? 1 : 0, temp, w_kd, w_ce, scale, f_of(c), 0.f, 1.f / temp,
+                w_ce != 0.f && temp != 1.f, t_ids, t_logp, tgt, rows, dlogits, ldd, 0, (float *)ws};
+    a.kappa = f_of(0.6931471805599453 * (c - (double)a.c) / c);
     hipStream_t st = ST(stream);
-    const DistillArgs a = {logits, ld, V, K, tail, temp, w_kd, w_ce, scale, t_ids, t_logp, tgt, rows, dlogits, ldd};
-    BY_TYPE(k_distill, dim3(N), tail ? (size_t)(V + 31) / 32 * 4 : 0, a);
+    const unsigned r = (unsigned)N;
+    // a segment is a multiple of 256 vectors, see the kernel
+    const int per = S > 1 ? ((nv + S - 1) / S + 255) / 256 * 256 : nv;
+    a.words = tail ? (per * ve + 31) / 32 : 0;
+    const size_t lds = (size_t)a.words * 4;
+    if (S > 1) {
+        BY_TYPE(r * S, 256, lds, a, k_distill, , 4, 4, false, KD_SUMS);
+        BY_TYPE(r * S, 256, 0, a, k_distill, , 4, 4, false, KD_GRAD);
+    } else if (nv <= 512 && N >= 512)
+        BY_TYPE((r + 3) / 4, 256, 4 * lds, a, k_distill, , 1, 8, true, KD_WHOLE);
+    else
+        BY_TYPE(r, 256, lds, a, k_distill, , 4, 4, false, KD_WHOLE);
     if (loss) hipLaunchKernelGGL(k_rows_mean, dim3(1), dim3(1024), 0, st, (const float *)rows, N, loss);
     LAUNCH_CHECK();
     return TLG_OK;
