@@ -140,12 +140,13 @@ int tlg_dev_xent_rows(const float *logits, const int *tgt, float *dlogits, doubl
 /* ---- rows of logits: log probabilities and distillation ------------------
  * Operators over logits [N][V] of element type `type`, row n at logits + n * ld
  * elements (ld >= V; what lies between the rows is neither read nor written).
- * V is 1 .. TLG_VOCAB_MAX and need not be a multiple of anything; pointers
- * need the alignment of their elements only.  Sums are fp32 or wider and every
+ * V is 1 .. TLG_VOCAB_MAX and need not be a multiple of anything, N is 0 ..
+ * TLG_VOCAB_ROWS; pointers need the alignment of their elements only, scales
+ * and temperatures lie in 1e-30 .. 1e30.  Sums are fp32 or wider and every
  * output is rounded once.  Only the caller's buffers are used: calls may
  * overlap on any streams as long as their outputs and workspaces differ, and
- * any call can be captured into a graph.  Results do not depend on the number
- * of rows beside a row, except for the order of its fp32 sums.
+ * any call can be captured into a graph.  Equal calls give equal bits; the
+ * number of rows may change the order of a row's fp32 sums.
  *
  * A logit of -inf is a masked token (probability 0).  A row of nothing but
  * -inf has no distribution: its log probabilities are -inf, its entropy 0, its
@@ -155,6 +156,7 @@ int tlg_dev_xent_rows(const float *logits, const int *tgt, float *dlogits, doubl
  * zeros whatever its logits hold. */
 enum { TLG_F32 = 0, TLG_F16 = 1, TLG_BF16 = 2 };     /* element types (IEEE fp32 and fp16, bfloat16) */
 #define TLG_VOCAB_MAX (1 << 20)                       /* columns of a row */
+#define TLG_VOCAB_ROWS (1 << 21)                      /* rows of a call */
 #define TLG_VOCAB_IDS 64                              /* given tokens of a row */
 #define TLG_VOCAB_TOP 128                             /* alternatives, teacher entries of a row */
 

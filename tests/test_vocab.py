@@ -39,7 +39,7 @@ def kd(L, logits=P, type=F32, ld=8, N=2, V=8, t_ids=P, t_logp=P, K=2, tail=0, te
 
 
 @pytest.mark.parametrize("call,name", [(lp, "logprobs"), (bwd, "logprobs_bwd"), (kd, "distill")])
-@pytest.mark.parametrize("bad", [dict(type=3), dict(type=-1), dict(N=-1), dict(V=0), dict(V=-5), dict(ld=7),
+@pytest.mark.parametrize("bad", [dict(type=3), dict(type=-1), dict(N=-1), dict(N=(1 << 21) + 1), dict(V=0), dict(V=-5), dict(ld=7),
                                  dict(V=(1 << 20) + 1, ld=1 << 21), dict(logits=None), dict(logits=P + 2),
                                  dict(type=F16, logits=P + 1), dict(type=BF16, logits=P + 1)])
 def test_bad_rows_are_refused(L, call, name, bad):
@@ -47,7 +47,7 @@ def test_bad_rows_are_refused(L, call, name, bad):
 
 
 @pytest.mark.parametrize("bad", [dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-                                 dict(scale=float("inf")), dict(M=-1), dict(M=65), dict(K=-1), dict(K=129),
+                                 dict(scale=float("inf")), dict(scale=1e-31), dict(scale=1e31), dict(M=-1), dict(M=65), dict(K=-1), dict(K=129),
                                  dict(ids=None), dict(logp=None), dict(top_ids=None), dict(top_logp=None)])
 def test_bad_logprobs_are_refused(L, bad):
     refused(L, lp(L, **bad), "logprobs")
@@ -60,7 +60,7 @@ def test_bad_gradients_are_refused(L, bad):
     refused(L, bwd(L, **bad), "logprobs_bwd")
 
 
-@pytest.mark.parametrize("bad", [dict(temp=0.0), dict(temp=-2.0), dict(temp=float("nan")), dict(w_kd=float("inf")),
+@pytest.mark.parametrize("bad", [dict(temp=0.0), dict(temp=-2.0), dict(temp=1e-38), dict(temp=1e38), dict(temp=float("nan")), dict(w_kd=float("inf")),
                                  dict(w_ce=float("nan")), dict(scale=float("nan")), dict(K=-1), dict(K=129),
                                  dict(t_ids=None), dict(t_logp=None), dict(tgt=None), dict(rows=None, loss=P),
                                  dict(rows=None, loss=None, d=None), dict(ldd=7), dict(d=P + 4), dict(d=P, ldd=9)])

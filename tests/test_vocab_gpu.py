@@ -276,6 +276,25 @@ def test_logprobs(lib, ty, N, V, K):
         check_logprobs(logprobs(lib, x, ty, scale, ids, K), x, scale, ids, K)
 
 
+@pytest.mark.parametrize("ty,N,V,K,pad", [
+    (F32, 1030, 1000, 8, 0), (BF16, 1027, 2048, 48, 0), (F16, 1025, 1999, 3, 1),         # a wave a row, in registers
+    (F32, 1026, 2048, 40, 0), (F32, 1024, 1500, 1, 3),                                    # eight vectors a lane
+    (F32, 2003, 4000, 20, 0), (BF16, 1601, 6001, 48, 1), (F16, 2048, 8100, 10, 4),        # a wave a row, read again
+    (F32, 1030, 1000, 49, 0), (BF16, 600, 4096, 128, 0),                                  # four waves
+    (F32, 5, 40000, 128, 1), (F16, 40, 66000, 30, 0), (BF16, 300, 80000, 7, 1),           # rows in segments
+    (F32, 1, 400000, 128, 0), (BF16, 2, 1 << 20, 100, 0)])
+def test_logprobs_every_launch(lib, ty, N, V, K, pad):
+    """The sizes at which the launches change: one wave a row or four, parts in
+    registers or read again, rows cut into segments."""
+    print("launch", NAMES[ty], N, V, K, pad, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, 1 if pad else 0))
+    x[0] = 0.5                                           # every value the same
+    x[N // 2, : V // 2] = 7.0
+    x[N - 1, V // 3:] = -math.inf
+    ids = some_ids(N, V, 2, V)
+    check_logprobs(logprobs(lib, x, ty, 0.9, ids, K), x, 0.9, ids, K)
+
+
 @pytest.mark.parametrize("ty", [F32, F16, BF16])
 @pytest.mark.parametrize("N,V,ld,off", [(3, 1000, 1003, 1), (2, 2048, 2051, 3), (5, 333, 340, 7), (2, 40001, 40010, 5),
                                         (300, 777, 900, 2)])
@@ -309,7 +328,7 @@ def test_logprobs_optional_outputs(lib):
 
 
 @pytest.mark.parametrize("ty", [F32, F16, BF16])
-@pytest.mark.parametrize("N,V", [(4, 100), (4, 2048), (3, 40000), (260, 5000)])
+@pytest.mark.parametrize("N,V", [(4, 100), (4, 2048), (3, 40000), (260, 5000), (1030, 1000)])
 def test_ties_go_to_the_lowest_index(lib, ty, N, V):
     """Rows of equal values, of few different values, of both zeros."""
     t = _t()
@@ -606,8 +625,41 @@ def test_distill(lib, ty, N, V, K, tail, tau, w_kd, w_ce, pad, off):
     assert t.equal(o3.rows, o.rows) and t.equal(x, d)
 
 
+@pytest.mark.parametrize("ty,N,V,K,tail,tau,pad", [
+    (F32, 2050, 1000, 8, True, 2.0, 0), (BF16, 2049, 2048, 70, False, 1.0, 0), (F16, 2051, 1500, 5, True, 1.0, 3),
+    (F32, 2048, 2048, 32, True, 1.0, 0), (F32, 2050, 2000, 32, False, 2.0, 1),
+    (F32, 20, 3000, 20, True, 2.0, 0), (BF16, 20, 8000, 20, True, 1.0, 1),
+    (F32, 20, 8000, 128, True, 1.0, 0), (F16, 20, 16000, 20, False, 2.0, 1),
+    (F32, 20, 16000, 20, True, 2.0, 1), (BF16, 20, 30000, 65, True, 1.0, 0),
+    (F32, 130, 32000, 20, True, 1.0, 0), (F32, 200, 50000, 20, True, 1.0, 1), (F32, 260, 40000, 9, False, 1.0, 0),
+    (F32, 140, 33000, 20, True, 2.0, 0), (BF16, 135, 66000, 20, True, 1.0, 1), (F16, 200, 40000, 20, True, 2.0, 0),
+    (F32, 3, 50000, 128, True, 2.0, 1), (BF16, 10, 131000, 64, True, 1.0, 0), (F32, 1, 1 << 20, 100, True, 1.0, 0)])
+def test_distill_every_launch(lib, ty, N, V, K, tail, tau, pad):
+    """The sizes at which the launches change: one to sixteen waves a row, rows
+    in registers or read twice, rows cut into segments."""
+    t = _t()
+    print("distill launch", NAMES[ty], N, V, K, tail, tau, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, 1 if pad else 0))
+    ids, tl = teacher(x, K, tau)
+    ids[N // 2, K // 2] = ids[N // 2, 0]                 # a repeated id
+    tgt = t.randint(0, V, (N,), generator=t.Generator().manual_seed(2), dtype=t.int32).cuda()
+    tgt[0] = ids[0, K - 1]
+    buf, d = like_rows(x, ty)
+    o = distill(lib, x, ty, ids, tl, tail, tau, 1.0, tgt, 0.5, d, 0.25)
+    pick = sorted(set(list(range(0, N, max(1, N // 60))) + [N // 2, N - 1]))
+    o.rows, dd = o.rows[pick], d[pick]
+    whole = o.loss.clone()
+    o.loss = o.rows.double().mean().float().reshape(1)
+    check_distill(o, dd, ty, x[pick], ids[pick], tl[pick], tail, tau, 1.0, tgt[pick], 0.5, 0.25)
+    o2 = distill(lib, x, ty, ids, tl, tail, tau, 1.0, tgt, 0.5, x, 0.25)          # in place
+    assert t.equal(x, d) and t.equal(o2.loss, whole)
+    assert abs(float(whole) - float(o2.rows.double().mean())) <= 2 * EPS * abs(float(whole))
+    t.as_strided(buf, tuple(d.shape), (d.stride(0), 1), d.storage_offset()).fill_(float("nan"))
+    assert bool(t.isnan(buf).all()), "wrote outside its rows"
+
+
 @pytest.mark.parametrize("tail", [False, True])
-@pytest.mark.parametrize("N,V", [(12, 300), (12, 50003), (530, 2048)])
+@pytest.mark.parametrize("N,V", [(12, 300), (12, 50003), (530, 2048), (2060, 1200)])
 def test_distill_special_rows(lib, tail, N, V):
     """Repeated ids, entries without mass, a support that is all the student
     has, padding over NaN, masked and NaN rows, ids past the vocabulary."""
@@ -645,6 +697,21 @@ def test_distill_special_rows(lib, tail, N, V):
     o.rows, dd = o.rows[good], d[good]
     o.loss = o.rows.mean().reshape(1)
     check_distill(o, dd, F32, sub, ids[good], tl[good], tail, 1.0, 1.0, tgt[good], 0.5, 1.0)
+
+
+def test_distill_largest_vocabulary_in_one_piece(lib):
+    """Rows of 2^20 columns that are not cut: the largest bitmap of the ids."""
+    t = _t()
+    N, V, K = 520, 1 << 20, 64
+    x = (2.5 * t.randn(N, V, device="cuda", generator=t.Generator("cuda").manual_seed(1))).bfloat16()
+    ids = t.randint(0, V, (N, K), generator=t.Generator().manual_seed(1), dtype=t.int32).cuda()
+    tl = (-5.0 - t.rand(N, K, generator=t.Generator().manual_seed(2))).cuda()
+    d = t.full((N, V), float("nan"), dtype=t.bfloat16, device="cuda")
+    o = distill(lib, x, BF16, ids, tl, True, 1.0, 1.0, None, 0.0, d)
+    assert bool(d.isfinite().all())
+    pick = [0, 255, N - 1]
+    o.rows, o.loss = o.rows[pick], o.rows[pick].mean().reshape(1)
+    check_distill(o, d[pick], BF16, x[pick], ids[pick], tl[pick], True, 1.0, 1.0, None, 0.0, 1.0)
 
 
 def test_distill_targets_past_the_vocabulary(lib):

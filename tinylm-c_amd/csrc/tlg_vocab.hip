@@ -734,12 +734,14 @@ template <int TYPE> __global__ __launch_bounds__(256) void k_logprobs_bwd(LpBwdA
 // The reference m_o keeps the remainder exact however little the student gives
 // it, and summing it without the ids' terms, which a bitmap in LDS marks, keeps it
 // from being a difference.  The ids and the target are written again afterwards.
+// The teacher's side and the logarithms are in 64 bits, by one wave.
 struct KdArgs {
     const void *logits;
     long long ld;
     int N, V, S, K, tail;
     float tau, w_kd, w_ce, scale;
-    float c, kappa, inv;          // log2 e / tau rounded, ln 2 (log2 e / tau - c) / c, 1 / tau
+    float c, c_lo;                // log2 e / tau = c + c_lo, c_lo > 0
+    double inv;                   // 1 / tau
     int two;                      // the cross-entropy needs sums of its own: w_ce != 0 and tau != 1
     const int *t_ids;
     const float *t_logp;
@@ -751,61 +753,92 @@ struct KdArgs {
     float *part;                  // S > 1: [N][S][4] sums, then [N][KD_XS] logits of ids and target
 };
 #define KD_XS (TLG_VOCAB_TOP + 1)
-#define KD_C1 1.44269504088896f   // log2 e, the cross-entropy's c
+#define KD_C1 1.44269502162933349609375f       // log2 e = KD_C1 + KD_C1_LO
+#define KD_C1_LO 1.925963033500e-8f
 
-// sums of a part: at temperature tau with entropy sum (for the rounding of c), and at 1
-struct Kd { float m, s, u, s1; };
-__device__ __forceinline__ void kd_shift(Kd &a, float m, float c, int two)
+// 2^((x - m) (c + lo)): with the constant in two parts the only roundings are the
+// difference's, the product's and the exponential's.  lo > 0, so that -inf stays -inf.
+__device__ __forceinline__ float kd_exp(float d, float c, float lo)
 {
-    const float d = (a.m - m) * c, f = __builtin_amdgcn_exp2f(d);
-    if (two) a.s1 *= __builtin_amdgcn_exp2f((a.m - m) * KD_C1);
-    a.u = f * fmaf(fmaxf(d, -200.f), a.s, a.u);
-    a.s *= f;
+    return __builtin_amdgcn_exp2f(fmaf(d, lo, d * c));
+}
+// sums of a part at temperature tau and, with TWO, at the cross-entropy's 1
+struct Kd { float m, s, s1; };
+#define KD0 {-FLT_MAX, 0.f, 0.f}
+template <bool TWO> __device__ __forceinline__ void kd_shift(Kd &a, float m, const KdArgs &k)
+{
+    const float d = a.m - m;
+    a.s *= kd_exp(d, k.c, k.c_lo);
+    if (TWO) a.s1 *= kd_exp(d, KD_C1, KD_C1_LO);
     a.m = m;
 }
-__device__ __forceinline__ void kd_add(Kd &a, float x, float c, int two)
+template <bool TWO> __device__ __forceinline__ Kd kd_wave(Kd a, const KdArgs &k)
 {
-    const float t = (x - a.m) * c, e = __builtin_amdgcn_exp2f(t);
-    if (two) a.s1 += __builtin_amdgcn_exp2f((x - a.m) * KD_C1);
-    a.s += e;
-    a.u = fmaf(e, fmaxf(t, -200.f), a.u);
+    kd_shift<TWO>(a, wave_max(a.m), k);
+    return Kd{a.m, wave_sum(a.s), TWO ? wave_sum(a.s1) : 0.f};
 }
-__device__ __forceinline__ Kd kd_wave(Kd a, float c, int two)
+template <bool TWO> __device__ __forceinline__ Kd kd_join(const f32x4 *p, int n, const KdArgs &k)
 {
-    kd_shift(a, wave_max(a.m), c, two);
-    return Kd{a.m, wave_sum(a.s), wave_sum(a.u), two ? wave_sum(a.s1) : 0.f};
-}
-__device__ __forceinline__ Kd kd_join(const float (*p)[4], int n, float c, int two)
-{
-    Kd r = {-FLT_MAX, 0.f, 0.f, 0.f};
-    for (int w = 0; w < n; w++) r.m = fmaxf(r.m, p[w][0]);
+    Kd r = {p[0][0], 0.f, 0.f};
+#pragma unroll 4
+    for (int w = 1; w < n; w++) r.m = fmaxf(r.m, p[w][0]);
+#pragma unroll 4
     for (int w = 0; w < n; w++) {
-        Kd a = {p[w][0], p[w][1], p[w][2], p[w][3]};
-        kd_shift(a, r.m, c, two);
+        Kd a = {p[w][0], p[w][1], p[w][2]};
+        kd_shift<TWO>(a, r.m, k);
         r.s += a.s;
-        r.u += a.u;
         r.s1 += a.s1;
     }
     return r;
 }
+__device__ __forceinline__ double lane_double(double v, int lane)
+{
+    return __builtin_bit_cast(double, lane_u64(__builtin_bit_cast(u64, v), lane));
+}
+template <int CTRL> __device__ __forceinline__ double lane_move64(double v)
+{
+    const u64 b = __builtin_bit_cast(u64, v);
+    const unsigned lo = __float_as_uint(lane_move<CTRL>(__uint_as_float((unsigned)b)));
+    const unsigned hi = __float_as_uint(lane_move<CTRL>(__uint_as_float((unsigned)(b >> 32))));
+    return __builtin_bit_cast(double, (u64)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v)          // as wave_sum
+{
+    v += lane_move64<0xB1>(v);
+    v += lane_move64<0x4E>(v);
+    v += lane_move64<0x141>(v);
+    v += lane_move64<0x140>(v);
+    return (lane_double(v, 0) + lane_double(v, 16)) + (lane_double(v, 32) + lane_double(v, 48));
+}
 
+// What a row's threads share: the waves' sums, the ids' sums, and the teacher's
+// entries (id, logit, q, log q before normalising) between the first wave's two turns.
+#define KD_HASH 128
 template <int W> struct KdShared {
-    float part[W][4];
-    float in[2][4];               // the ids' part, by the waves that hold them
-    int ids[TLG_VOCAB_TOP];
-    double d[2][4];
-    float f[2];
-    int flag;                     // an id or a target past the vocabulary
+    f32x4 part[W], in;
+    double Q, qr, lq0;            // sum q + q_r, q_r, what log q subtracts
+    int flags, tgt;
+    float xt;
+    double q[TLG_VOCAB_TOP];
+    float x[TLG_VOCAB_TOP], l[TLG_VOCAB_TOP];
+    union {
+        int id[TLG_VOCAB_TOP];
+        unsigned seen[KD_HASH];
+    };
 };
+// entries at all; the target among them; an id or target past V; a target
+enum { KD_ANY = 1, KD_HIT = 2, KD_BAD = 4, KD_CE = 8 };
 
 enum { KD_WHOLE = 0, KD_SUMS = 1, KD_GRAD = 2 };
 // W waves on a row (PHASE KD_WHOLE) or on one of its S segments: KD_SUMS leaves
-// the segment's sums, KD_GRAD joins them and writes the segment.  RES: a
-// thread's part, at most U vectors, stays in registers between sums and gradient.
-template <int TYPE, int W, int U, bool RES, int PHASE>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(KdArgs a)
+// the segment's sums, KD_GRAD joins them and writes the segment.  RES: a thread's
+// part, at most U vectors, stays in registers, as exponentials, from the sums to
+// the gradient; longer rows are read twice.  TWO: a cross-entropy at another
+// temperature than the teacher's.
+template <int TYPE, int W, int U, bool RES, bool TWO, int PHASE>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8) void k_distill(KdArgs a)
 {
-    constexpr int VE = El<TYPE>::VE, TPR = 64 * W, EPT = W == 1 ? 2 : 1, EW = W == 1 ? 1 : 2;
+    constexpr int VE = El<TYPE>::VE, TPR = 64 * W;
     __shared__ KdShared<W> shared[W == 1 ? 4 : 1];
     extern __shared__ unsigned all_bits[];              // tail: the support, a bit for each element
     const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, t = W == 1 ? lane : threadIdx.x;
@@ -816,87 +849,162 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(KdArgs a)
     if constexpr (W == 1) {
         r = (size_t)blockIdx.x * 4 + slot;
         if (r >= (size_t)a.N) return;
-    } else {
+    } else if constexpr (PHASE == KD_WHOLE)
+        r = blockIdx.x;
+    else {
         r = blockIdx.x / (unsigned)a.S;
         seg = blockIdx.x % (unsigned)a.S;
     }
     const Row<TYPE> x(a.logits, a.ld, r, a.V);
-    const int per = a.S > 1 ? ((x.nv + a.S - 1) / a.S + TPR - 1) / TPR * TPR : x.nv;
-    const int j0 = min(seg * per, x.nv), j1 = min(j0 + per, x.nv);
-    const int K = a.K;
+    const int per = PHASE == KD_WHOLE ? x.nv : ((x.nv + a.S - 1) / a.S + TPR - 1) / TPR * TPR;
+    const int j0 = PHASE == KD_WHOLE ? 0 : min(seg * per, x.nv), j1 = PHASE == KD_WHOLE ? x.nv : min(j0 + per, x.nv);
     const float c = a.c;
 
     u32x4 raw[U];
-    auto load = [&](int j) {
+    auto load = [&](int j, bool last) {
         if (j >= x.f0 && j + (U - 1) * TPR < min(x.f1, j1)) {
 #pragma unroll
-            for (int k = 0; k < U; k++) raw[k] = RES ? __builtin_nontemporal_load(x.v + j + k * TPR) : x.v[j + k * TPR];
+            for (int k = 0; k < U; k++) raw[k] = last ? __builtin_nontemporal_load(x.v + j + k * TPR) : x.v[j + k * TPR];
         } else {
 #pragma unroll
             for (int k = 0; k < U; k++) raw[k] = x.any(j + k * TPR < j1 ? j + k * TPR : x.nv);
         }
     };
+    // The first wave's loads of the teacher's entries, lane and lane + 64, go ahead of
+    // the row's, so that the entries' logits are on their way while the row arrives.
+    const int K = a.K;
+    int id[2] = {-1, -1}, tgt = -1;
+    float tl[2] = {-INFINITY, -INFINITY};
+    if (wave == 0) {
+        if (lane < K) {
+            id[0] = a.t_ids[r * K + lane];
+            tl[0] = a.t_logp[r * K + lane];
+        }
+        if (lane + 64 < K) {
+            id[1] = a.t_ids[r * K + lane + 64];
+            tl[1] = a.t_logp[r * K + lane + 64];
+        }
+        if (a.w_ce != 0.f) tgt = a.tgt[r];
+    }
+    if (PHASE != KD_GRAD) load(j0 + t, RES);
 
-    if (RES) load(j0 + t);
-
-    // the ids: a repeated one counts at its first place
     unsigned *bits = all_bits + slot * a.words;
-    const int tgt = a.w_ce != 0.f ? a.tgt[r] : -1;
-    if (t == 0) sh.flag = tgt >= a.V;
-    int id[EPT];
-#pragma unroll
-    for (int k = 0; k < EPT; k++) {
-        id[k] = t + 64 * k < K ? a.t_ids[r * K + t + 64 * k] : -1;
-        if (t + 64 * k < TLG_VOCAB_TOP) sh.ids[t + 64 * k] = id[k];
-    }
-    if (a.tail && PHASE != KD_GRAD)
+    float *xs = a.part + (size_t)a.N * a.S * 4 + r * KD_XS;              // S > 1
+    if (PHASE != KD_GRAD && a.tail)
         for (int i = t; i < a.words; i += TPR) bits[i] = 0;
-    row_sync<W>();
-    bool any = false, hit = false;                       // entries at all; the target among them
+    if (wave == 0) {
+        float xk[2] = {-INFINITY, -INFINITY}, xt = 0.f;
+        for (int i = lane; i < KD_HASH; i += 64) sh.seen[i] = 0;
+        int flags = __ballot(tgt >= a.V || id[0] >= a.V || id[1] >= a.V) ? KD_BAD : 0;
+        if (tgt >= 0) flags |= KD_CE;
+        if (__ballot(tgt >= 0 && (id[0] == tgt || id[1] == tgt))) flags |= KD_HIT;
+        if (id[0] >= a.V) id[0] = -1;
+        if (id[1] >= a.V) id[1] = -1;
 #pragma unroll
-    for (int k = 0; k < EPT; k++) {
-        if (id[k] >= a.V) sh.flag = 1;
-        if (id[k] >= 0)
-            for (int j = 0; j < t + 64 * k; j++)
-                if (sh.ids[j] == id[k]) id[k] = -1;
-        if (id[k] >= a.V) id[k] = -1;
-        if (a.tail && PHASE != KD_GRAD && id[k] >= 0) {
-            const int g = id[k] + x.sh - j0 * VE;
-            if (g >= 0 && g < per * VE) atomicOr(&bits[g >> 5], 1u << (g & 31));
+        for (int k = 0; k < 2; k++)
+            if (id[k] >= 0) xk[k] = PHASE == KD_GRAD ? xs[lane + 64 * k] : el_load<TYPE>(x.x, id[k]);
+        if (tgt >= 0 && tgt < a.V) xt = PHASE == KD_GRAD ? xs[KD_XS - 1] : el_load<TYPE>(x.x, tgt);
+        // A repeated id counts at its first place: looked for only where a set of
+        // 32 KD_HASH bits says that there may be one.
+        row_sync<1>();
+        bool twice = false;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (id[k] >= 0) {
+                const unsigned h = (unsigned)id[k] % (32 * KD_HASH);
+                twice |= atomicOr(&sh.seen[h / 32], 1u << h % 32) >> h % 32 & 1;
+            }
+        if (__ballot(twice)) {
+            const int was[2] = {id[0], id[1]};
+            for (int j = 0; j < K; j++) {
+                const int o = __builtin_amdgcn_readlane(j < 64 ? was[0] : was[1], j % 64);
+                if (o == was[0] && j < lane) id[0] = -1;
+                if (o == was[1] && j < lane + 64) id[1] = -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (id[k] < 0) xk[k] = -INFINITY;
         }
+        const int some = __popcll(__ballot(id[0] >= 0)) + __popcll(__ballot(id[1] >= 0));
+        if (some) flags |= KD_ANY;
+        row_sync<1>();
+        if constexpr (PHASE == KD_SUMS) {
+            if (seg == 0) {
+                xs[lane] = xk[0];
+                xs[lane + 64] = xk[1];
+                if (lane == 0) xs[KD_XS - 1] = xt;
+            }
+        } else {
+            // q, its sum and the remainder; the ids' part of the sums, which the bitmap leaves out
+            if (id[0] < 0) tl[0] = -INFINITY;
+            if (id[1] < 0) tl[1] = -INFINITY;
+            const float tm = a.tail ? 0.f : wave_max(fmaxf(tl[0], tl[1]));
+            double q[2] = {0.0, 0.0};
+            if (tm > -INFINITY) {
+                q[0] = exp((double)tl[0] - tm);
+                if (K > 64) q[1] = exp((double)tl[1] - tm);
+            }
+            double Q = wave_sum64(q[0] + q[1]), qr = 0.0, lq0 = 0.0;
+            if (a.tail) {
+                if (some && some < a.V && Q < 1.0) qr = 1.0 - Q;
+                Q += qr;
+            } else if (Q > 0.0) {
+                const double n = 1.0 / Q;
+                q[0] *= n;
+                q[1] *= n;
+                lq0 = Q;
+                Q = 1.0;
+            }
+            Kd B = KD0;
+            if (a.tail) {
+                B.m = fmaxf(fmaxf(xk[0], xk[1]), -FLT_MAX);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    B.s += kd_exp(xk[k] - B.m, c, a.c_lo);
+                    if (TWO) B.s1 += kd_exp(xk[k] - B.m, KD_C1, KD_C1_LO);
+                }
+                B = kd_wave<TWO>(B, a);
+            }
+            if (lane == 0) {
+                sh.Q = Q;
+                sh.qr = qr;
+                sh.lq0 = lq0;
+                sh.in = f32x4{B.m, B.s, B.s1, 0.f};
+                sh.xt = xt;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (lane + 64 * k < K) {
+                    sh.q[lane + 64 * k] = q[k];
+                    sh.x[lane + 64 * k] = xk[k];
+                    sh.l[lane + 64 * k] = tl[k] - tm;
+                }
+        }
+        if (lane == 0) {
+            sh.flags = flags;
+            sh.tgt = tgt;
+        }
+        if (lane < K) sh.id[lane] = id[0];
+        if (lane + 64 < K) sh.id[lane + 64] = id[1];
     }
-    for (int j = 0; j < K; j++) {
-        const int i = sh.ids[j];
-        any |= i >= 0 && i < a.V;
-        hit |= i == tgt;
+    if (PHASE != KD_GRAD && a.tail) {
+        row_sync<W>();
+        for (int k = t; k < a.K; k += TPR) {
+            const int g = sh.id[k] + x.sh - j0 * VE;
+            if (sh.id[k] >= 0 && g >= 0 && g < a.words * 32) atomicOr(&bits[g >> 5], 1u << (g & 31));
+        }
+        row_sync<W>();
     }
-    row_sync<W>();
-    const bool bad_id = sh.flag;
-    const bool nothing = !any && tgt < 0 && !bad_id;     // such a row's logits are not read
 
-    // the ids' logits and the teacher's side, in 64 bits: q, Q, q_r
-    float xk[EPT], xt = 0.f;
-    double q[EPT], tl[EPT];
-    const float *xs = a.part + (size_t)a.N * a.S * 4 + r * KD_XS;        // S > 1
-    Kd B = {-FLT_MAX, 0.f, 0.f, 0.f};
-    float tm = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < EPT; k++) {
-        xk[k] = -INFINITY;
-        tl[k] = -INFINITY;
-        if (id[k] >= 0) {
-            xk[k] = PHASE == KD_GRAD ? xs[t + 64 * k] : el_load<TYPE>(x.x, id[k]);
-            const float l = a.t_logp[r * K + t + 64 * k];
-            tl[k] = l;
-            tm = fmaxf(tm, l);
-        }
-    }
-    if (tgt >= 0 && tgt < a.V) xt = PHASE == KD_GRAD ? xs[KD_XS - 1] : el_load<TYPE>(x.x, tgt);
     // sums
-    Kd A = {-FLT_MAX, 0.f, 0.f, 0.f};
-    if (PHASE != KD_GRAD && !nothing) {
+    Kd A = KD0;
+    constexpr bool EXP = RES && U * VE <= 32 * (VE == 4 ? 2 : 1);      // kept as exponentials, else as they came
+    float ex[EXP ? U * VE : 1], ex1[EXP && TWO ? U * VE : 1];
+    int jl = j0 + t;                                    // the last round's vector
+    if constexpr (PHASE != KD_GRAD) {
         for (int j = j0 + t; RES ? j == j0 + t : j < j1; j += U * TPR) {
-            if (!RES) load(j);
+            if (!RES && j != j0 + t) load(j, false);
+            jl = j;
             if (a.tail)
 #pragma unroll
                 for (int k = 0; k < U; k++) {
@@ -916,175 +1024,127 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_distill(KdArgs a)
             for (int k = 0; k < U; k++)
 #pragma unroll
                 for (int e = 0; e < VE; e++) m = fmaxf(m, el_at<TYPE>(raw[k], e));
-            kd_shift(A, m, c, a.two);
+            kd_shift<TWO>(A, m, a);
+            if constexpr (RES && !EXP)
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                if (RES) keep_packed(raw[k]);
+                for (int k = 0; k < U; k++) keep_packed(raw[k]);
 #pragma unroll
-                for (int e = 0; e < VE; e++) kd_add(A, el_at<TYPE>(raw[k], e), c, a.two);
-                if (RES) keep_packed(raw[k]);
-            }
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) {
+                    const float d = el_at<TYPE>(raw[k], e) - A.m, v = kd_exp(d, c, a.c_lo);
+                    const float v1 = TWO ? kd_exp(d, KD_C1, KD_C1_LO) : 0.f;
+                    A.s += v;
+                    if (TWO) A.s1 += v1;
+                    if constexpr (EXP) ex[k * VE + e] = v;
+                    if constexpr (EXP && TWO) ex1[k * VE + e] = v1;
+                    if constexpr (RES && !EXP)
+                        if (e == VE - 1) keep_packed(raw[k]);
+                }
         }
     }
-
-    if constexpr (PHASE == KD_SUMS) {
-        A = kd_wave(A, c, a.two);
-        if (lane == 0) { sh.part[wave][0] = A.m; sh.part[wave][1] = A.s; sh.part[wave][2] = A.u; sh.part[wave][3] = A.s1; }
-        row_sync<W>();
-        if (t == 0) {
-            A = kd_join(sh.part, W, c, a.two);
-            float *p = a.part + (r * a.S + seg) * 4;
-            p[0] = A.m; p[1] = A.s; p[2] = A.u; p[3] = A.s1;
-        }
-        if (seg == 0) {
-            float *o = const_cast<float *>(xs);
-            if (t < TLG_VOCAB_TOP) o[t] = xk[0];
-            if (t == 0) o[KD_XS - 1] = xt;
-        }
-        return;
-    }
-    // the waves that hold entries: all of W == 1's, two of the others
-    if (wave < EW) {
-        if (a.tail) {
-#pragma unroll
-            for (int k = 0; k < EPT; k++) B.m = fmaxf(B.m, xk[k]);
-#pragma unroll
-            for (int k = 0; k < EPT; k++) kd_add(B, xk[k], c, a.two);
-            B = kd_wave(B, c, a.two);
-        }
-        tm = wave_max(tm);
-        if (W > 1 && lane == 0) {
-            sh.in[wave][0] = B.m; sh.in[wave][1] = B.s; sh.in[wave][2] = B.u; sh.in[wave][3] = B.s1;
-            sh.f[wave] = tm;
-        }
-    }
-    if constexpr (PHASE == KD_WHOLE) {
-        A = kd_wave(A, c, a.two);
-        if (W > 1 && lane == 0) {
-            sh.part[wave][0] = A.m; sh.part[wave][1] = A.s; sh.part[wave][2] = A.u; sh.part[wave][3] = A.s1;
-        }
+    const float mine = A.m;                             // the reference of ex, ex1
+    if constexpr (PHASE != KD_GRAD) {
+        A = kd_wave<TWO>(A, a);
+        if (W > 1 && lane == 0) sh.part[wave] = f32x4{A.m, A.s, A.s1, 0.f};
     }
     row_sync<W>();
     if constexpr (W > 1) {
-        A = PHASE == KD_WHOLE ? kd_join(sh.part, W, c, a.two) : kd_join((const float (*)[4])(a.part + r * a.S * 4), a.S, c, a.two);
-        B = kd_join(sh.in, EW, c, a.two);
-        tm = fmaxf(sh.f[0], sh.f[1]);
+        if constexpr (PHASE == KD_GRAD) A = kd_join<TWO>((const f32x4 *)a.part + r * a.S, a.S, a);
+        else A = kd_join<TWO>(sh.part, W, a);
     }
-    // teacher
-    double sum = 0.0;
-    if (wave < EW) {
-#pragma unroll
-        for (int k = 0; k < EPT; k++) {
-            q[k] = id[k] < 0 ? 0.0 : tl[k] != tl[k] ? tl[k] : a.tail ? exp(tl[k]) : tm > -INFINITY ? exp(tl[k] - tm) : 0.0;
-            sum += q[k];
-        }
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        int cnt = 0;
-#pragma unroll
-        for (int k = 0; k < EPT; k++) cnt += __popcll(__ballot(id[k] >= 0));
-        if (W > 1 && lane == 0) {
-            sh.d[wave][0] = sum;
-            sh.d[wave][1] = cnt;
-        }
-        if (W == 1) sh.d[0][1] = cnt;
+    if constexpr (PHASE == KD_SUMS) {
+        if (t == 0) ((f32x4 *)a.part)[r * a.S + seg] = f32x4{A.m, A.s, A.s1, 0.f};
+        return;
     }
-    int some;
-    if constexpr (W > 1) {
-        row_sync<W>();
-        sum = sh.d[0][0] + sh.d[1][0];
-        some = (int)(sh.d[0][1] + sh.d[1][1]);
-    } else {
-        some = 0;
-#pragma unroll
-        for (int k = 0; k < EPT; k++) some += __popcll(__ballot(id[k] >= 0));
-    }
-    double qr = 0.0, Q;
-    if (a.tail) {
-        if (some && some < a.V && sum < 1.0) qr = 1.0 - sum;
-        Q = sum + qr;
-    } else {
-        const double n = sum > 0.0 || sum != sum ? 1.0 / sum : 0.0;
-        if (wave < EW)
-#pragma unroll
-            for (int k = 0; k < EPT; k++) q[k] *= n;
-        Q = sum > 0.0 ? 1.0 : sum;
-    }
-    // the row's sums
-    const float so = fmaf(a.kappa, A.u, A.s);
+
+    // the row's sums and coefficients
+    const Kd B = {sh.in[0], sh.in[1], sh.in[2]};
+    const float Q = (float)sh.Q, qr = (float)sh.qr;
+    const int flags = sh.flags;
+    const bool any = flags & KD_ANY, bad_id = flags & KD_BAD, ce = flags & KD_CE;
     const float M = fmaxf(A.m, B.m);
-    const float F = __builtin_amdgcn_exp2f((A.m - M) * c), G = __builtin_amdgcn_exp2f((B.m - M) * c);
-    const float s = so * F + fmaf(a.kappa, B.u, B.s) * G;
+    const float F = kd_exp(A.m - M, c, a.c_lo), s = A.s * F + B.s * kd_exp(B.m - M, c, a.c_lo);
     float s1 = s;
-    if (a.two)
-        s1 = A.s1 * __builtin_amdgcn_exp2f((A.m - M) * KD_C1) + B.s1 * __builtin_amdgcn_exp2f((B.m - M) * KD_C1);
-    const bool empty = s == 0.f;
-    const float ck = any ? a.w_kd * a.tau * a.scale : 0.f, cc = tgt >= 0 ? a.w_ce * a.scale : 0.f;
-    const float rs = empty ? 0.f : 1.f / s, r1 = empty ? 0.f : 1.f / s1;
-    const float kin = ck * (float)Q * rs;                                  // inside S, reference M
+    if (TWO) s1 = A.s1 * kd_exp(A.m - M, KD_C1, KD_C1_LO) + B.s1 * kd_exp(B.m - M, KD_C1, KD_C1_LO);
+    const bool empty = s == 0.f, nothing = !any && !ce && !bad_id;
+    const float ck = any ? a.w_kd * a.tau * a.scale : 0.f, cc = ce ? a.w_ce * a.scale : 0.f;
+    const float rs = empty ? 0.f : __builtin_amdgcn_rcpf(s), r1 = empty ? 0.f : __builtin_amdgcn_rcpf(s1);
+    const float kin = ck * Q * rs;                                         // inside S, reference M
     float kout = kin * F;                                                  // outside, reference m_o
-    if (qr > 0.0 && A.s > 0.f) kout -= ck * ((float)qr / so);
-    if (!a.two) kout += cc * r1 * F;
-    const float k1 = a.two ? cc * r1 : 0.f;
+    if (qr > 0.f && A.s > 0.f) kout -= ck * qr * __builtin_amdgcn_rcpf(A.s);
+    if (!TWO) kout += cc * r1 * F;
+    const float k1 = TWO ? cc * r1 : 0.f;                                  // of the second exponential, reference M
     if (bad_id) kout = NAN;
     auto outside = [&](float v) -> float {
         float g = kout * __builtin_amdgcn_exp2f((v - A.m) * c);
-        if (a.two) g = fmaf(k1, __builtin_amdgcn_exp2f((v - M) * KD_C1), g);
+        if (TWO) g = fmaf(k1, __builtin_amdgcn_exp2f((v - M) * KD_C1), g);
         return g;
     };
-    char *dl = (char *)a.dlogits;
-    if (dl) {
+    if (a.dlogits) {
         const Row<TYPE> d(a.dlogits, a.ldd, r, a.V);
         const bool zero = nothing || (empty && !bad_id);
-        for (int j = j0 + t; RES ? j == j0 + t : j < j1; j += U * TPR) {
-            if (!RES && !zero) load(j);
+        // of exponentials with a thread's own reference
+        const float fk = kout * kd_exp(mine - A.m, c, a.c_lo), f1 = TWO ? k1 * kd_exp(mine - M, KD_C1, KD_C1_LO) : 0.f;
+        // backwards: the sums' last rounds are the likeliest to be in the caches still
+        if (PHASE == KD_GRAD) jl = j0 + t + (max(j1 - j0 - t, 1) - 1) / (U * TPR) * (U * TPR);
+        for (int j = jl; j >= j0; j -= U * TPR) {
+            if (!RES && !zero) load(j, true);
 #pragma unroll
             for (int k = 0; k < U; k++) {
                 float g[VE];
 #pragma unroll
-                for (int e = 0; e < VE; e++) g[e] = zero ? 0.f : outside(el_at<TYPE>(raw[k], e));
+                for (int e = 0; e < VE; e++) {
+                    if constexpr (EXP) {
+                        g[e] = fk * ex[k * VE + e];
+                        if constexpr (TWO) g[e] = fmaf(f1, ex1[k * VE + e], g[e]);
+                    } else
+                        g[e] = outside(el_at<TYPE>(raw[k], e));
+                    if (zero) g[e] = 0.f;
+                }
                 if (j + k * TPR < j1) row_store<TYPE>(x, d, j + k * TPR, g);
             }
+            if (RES) break;
         }
         row_sync<W>();
-        if (!zero && !bad_id) {
-#pragma unroll
-            for (int k = 0; k < EPT; k++) {
-                const int j = (id[k] + x.sh) / VE;
-                if (id[k] >= 0 && j >= j0 && j < j1) {
-                    const float p = __builtin_amdgcn_exp2f((xk[k] - M) * c);
-                    float p1 = p * r1;
-                    if (a.two) p1 = __builtin_amdgcn_exp2f((xk[k] - M) * KD_C1) * r1;
-                    float g = kin * p - ck * (float)q[k] + (cc != 0.f ? cc * p1 : 0.f);
-                    if (id[k] == tgt) g -= cc;
-                    el_store<TYPE>(const_cast<char *>(d.x), id[k], g);
+        if (wave == 0 && !zero && !bad_id) {
+            const int tgt = sh.tgt;
+            for (int k = lane; k < K; k += 64) {
+                const int id = sh.id[k], j = (id + x.sh) / VE;
+                if (id >= 0 && j >= j0 && j < j1) {
+                    const float p = kd_exp(sh.x[k] - M, c, a.c_lo);
+                    const float p1 = TWO ? kd_exp(sh.x[k] - M, KD_C1, KD_C1_LO) : p;
+                    float g = kin * p - ck * (float)sh.q[k] + (ce ? cc * (p1 * r1) : 0.f);
+                    if (id == tgt) g -= cc;
+                    el_store<TYPE>(const_cast<char *>(d.x), id, g);
                 }
             }
             const int j = (tgt + x.sh) / VE;
-            if (t == 0 && tgt >= 0 && !hit && j >= j0 && j < j1)
-                el_store<TYPE>(const_cast<char *>(d.x), tgt, outside(xt) - cc);
+            if (lane == 0 && ce && !(flags & KD_HIT) && j >= j0 && j < j1)
+                el_store<TYPE>(const_cast<char *>(d.x), tgt, outside(sh.xt) - cc);
         }
     }
-    if (!a.rows || seg != 0) return;
-    // the row's loss: log p_k = (x_k - M) / tau - log s
-    const double ls = log((double)s);
+    if (!a.rows || seg != 0 || wave != 0) return;
+    // The row's loss: log p_k = (x_k - M) / tau - log s, log q_k = l_k - log of their
+    // sum.  One logarithm, of s, s_o, s1, q_r and that sum in lanes of their own.
+    const double arg = lane == 0 ? (double)s : lane == 1 ? (double)A.s : lane == 2 ? (double)s1
+                     : lane == 3 ? sh.qr : sh.lq0 > 0.0 ? sh.lq0 : 1.0;
+    const double logs = log(arg), ls = lane_double(logs, 0), lo = lane_double(logs, 1), ls1 = lane_double(logs, 2),
+                 lr = lane_double(logs, 3), lq = lane_double(logs, 4);
     double kl = 0.0;
-    if (wave < EW) {
-#pragma unroll
-        for (int k = 0; k < EPT; k++)
-            if (q[k] > 0.0 || q[k] != q[k]) kl += empty ? INFINITY : q[k] * (log(q[k]) - ((double)(xk[k] - M) / a.tau - ls));
-        for (int o = 32; o > 0; o >>= 1) kl += __shfl_xor(kl, o);
-        if (W > 1 && lane == 0) sh.d[wave][2] = kl;
+    for (int k = lane; k < a.K; k += 64) {
+        const double q = sh.q[k];
+        if (q > 0.0 || q != q)
+            kl += empty ? INFINITY : q * (((double)sh.l[k] - lq) - ((double)(sh.x[k] - M) * a.inv - ls));
     }
-    if constexpr (W > 1) row_sync<W>();
-    if (t == 0) {
-        if constexpr (W > 1) kl = sh.d[0][2] + sh.d[1][2];
-        if (qr > 0.0) kl += empty ? INFINITY : qr * (log(qr) - ((double)(A.m - M) / a.tau + log((double)so) - ls));
-        double L = 0.0;
-        if (any && a.w_kd != 0.f) L = (double)a.w_kd * a.tau * a.tau * kl;
-        if (tgt >= 0) L += (double)a.w_ce * (empty ? INFINITY : log((double)s1) - (double)(xt - M));
-        if (s != s) L = NAN;
-        a.rows[r] = bad_id ? NAN : nothing ? 0.f : (float)L;
-    }
+    kl = wave_sum64(kl);
+    if (lane != 0) return;
+    if (sh.qr > 0.0) kl += empty ? INFINITY : sh.qr * (lr - ((double)(A.m - M) * a.inv + lo - ls));
+    double L = 0.0;
+    if (any && a.w_kd != 0.f) L = (double)a.w_kd * a.tau * a.tau * kl;
+    if (ce) L += (double)a.w_ce * (empty ? INFINITY : ls1 - (double)(sh.xt - M));
+    if (s != s) L = NAN;
+    a.rows[r] = bad_id ? NAN : nothing ? 0.f : (float)L;
 }
 
 // the mean of the row losses, summed in double in a fixed order
@@ -1109,7 +1169,7 @@ static size_t vb_size(int type) { return type == TLG_F32 ? 4 : 2; }
 static int vb_check(const char *who, const void *logits, int type, long long ld, int N, int V)
 {
     if (type != TLG_F32 && type != TLG_F16 && type != TLG_BF16) return tlg_fail(TLG_EINVAL, "%s: type %d", who, type);
-    if (N < 0 || V <= 0 || V > TLG_VOCAB_MAX || ld < V)
+    if (N < 0 || N > TLG_VOCAB_ROWS || V <= 0 || V > TLG_VOCAB_MAX || ld < V)
         return tlg_fail(TLG_EINVAL, "%s: N=%d V=%d ld=%lld", who, N, V, ld);
     if (N > 0 && (!logits || (uintptr_t)logits % vb_size(type)))
         return tlg_fail(TLG_EINVAL, "%s: logits %p", who, logits);
@@ -1132,7 +1192,8 @@ static int vb_check_ws(const char *who, const void *ws, size_t have, size_t need
         return tlg_fail(TLG_EINVAL, "%s: workspace %p of %zu bytes, %zu needed", who, ws, have, need);
     return TLG_OK;
 }
-static bool vb_positive(float s) { return s > 0.f && s <= 3.4028234e38f; }
+// a scale or temperature: its multiples by log2 e and back must be finite and normal
+static bool vb_positive(float s) { return s >= 1e-30f && s <= 1e30f; }
 
 static float f_of(double v) { return (float)v; }
 
@@ -1165,6 +1226,12 @@ static int vb_segments(int type, int N, int V, int most)
     do {                                                                                                            \
         if (type == TLG_F32) hipLaunchKernelGGL((K0<TLG_F32 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a);    \
         else if (type == TLG_F16) hipLaunchKernelGGL((K0<TLG_F16 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a); \
+        else hipLaunchKernelGGL((K0<TLG_BF16 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a);                   \
+    } while (0)
+
+#define BY_16(grid, block, lds, a, K0, ...)                                                                         \
+    do {                                                                                                            \
+        if (type == TLG_F16) hipLaunchKernelGGL((K0<TLG_F16 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a);    \
         else hipLaunchKernelGGL((K0<TLG_BF16 __VA_ARGS__>), dim3(grid), dim3(block), lds, st, a);                   \
     } while (0)
 
@@ -1253,7 +1320,54 @@ extern "C" int tlg_dev_logprobs_bwd(const void *logits, int type, long long ld, 
     return TLG_OK;
 }
 
-static int kd_segments(int type, int N, int V) { return vb_segments(type, N, V, 64); }
+// Distillation's uncut rows have up to sixteen waves each, so that only fewer or
+// longer rows gain by a second launch: 16384 vectors take 12.8 us cut and 17.6 whole for
+// one row, 19.1 and 20.6 for 64, 24.4 and 23.0 for 128.
+static int kd_segments(int type, int N, int V)
+{
+    return (long long)N * 256 <= V / (type == TLG_F32 ? 4 : 8) ? vb_segments(type, N, V, 64) : 1;
+}
+
+// Rows of up to 16384 vectors of fp32 and 4096 of 16 bits stay in registers between
+// sums and gradient, on as few waves as hold them: 4096 rows of 2048 fp32 values take
+// 19.7 us on one wave and 25.0 read twice by four, of 16384 101 against 120, of 65536
+// 404 against 465.  The longer 16-bit ones leave a workgroup no second one on its CU
+// to work while it waits (4096 rows of 131072: 516 us); they are read twice, by sixteen
+// waves, so that the rows in work (two on a CU) fit the last-level cache: 468 us, with
+// eight waves 502, with four 583.  Two exponentials need registers: eight waves then
+// (527 against 551 us), and fp32 stays in registers up to 4096 vectors only (586 against
+// 463 us at 16384).  Beyond 8192 vectors a row in registers has a CU to itself, which
+// pays where the rows fill three quarters of their rounds over the 256 CUs (301 rows of
+// 50021: 46.5 us in registers, 38.2 read twice).
+template <bool TWO> static void kd_launch(const KdArgs &a, int type, int nv, size_t lds, hipStream_t st)
+{
+    const unsigned rows = a.N;
+    const bool f32 = type == TLG_F32;
+    if (a.S > 1) {
+        BY_TYPE(rows * a.S, 256, lds, a, k_distill, , 4, 4, false, TWO, KD_SUMS);
+        BY_TYPE(rows * a.S, 256, 0, a, k_distill, , 4, 4, false, TWO, KD_GRAD);
+    } else if (nv <= 256 && rows >= 2048)
+        BY_TYPE((rows + 3) / 4, 256, 4 * lds, a, k_distill, , 1, 4, true, TWO, KD_WHOLE);
+    else if (nv <= 512 && f32 && rows >= 2048)
+        hipLaunchKernelGGL((k_distill<TLG_F32, 1, 8, true, TWO, KD_WHOLE>), dim3((rows + 3) / 4), dim3(256), 4 * lds,
+                           st, a);
+    else if (nv <= 512)
+        BY_TYPE(rows, 256, lds, a, k_distill, , 4, 2, true, TWO, KD_WHOLE);
+    else if (nv <= 1024)
+        BY_TYPE(rows, 256, lds, a, k_distill, , 4, 4, true, TWO, KD_WHOLE);
+    else if (nv <= 2048)
+        BY_TYPE(rows, 256, lds, a, k_distill, , 4, 8, true, TWO, KD_WHOLE);
+    else if (nv <= 4096)
+        BY_TYPE(rows, 512, lds, a, k_distill, , 8, 8, true, TWO, KD_WHOLE);
+    else if (nv <= 8192 && f32 && !TWO)
+        hipLaunchKernelGGL((k_distill<TLG_F32, 16, 8, true, false, KD_WHOLE>), dim3(rows), dim3(1024), lds, st, a);
+    else if (nv <= 16384 && f32 && !TWO && 4 * rows >= 3 * ((rows + 255) / 256 * 256))
+        hipLaunchKernelGGL((k_distill<TLG_F32, 16, 16, true, false, KD_WHOLE>), dim3(rows), dim3(1024), lds, st, a);
+    else if (TWO && !f32)
+        BY_16(rows, 512, lds, a, k_distill, , 8, 2, false, TWO, KD_WHOLE);
+    else
+        BY_TYPE(rows, 1024, lds, a, k_distill, , 16, 2, false, TWO, KD_WHOLE);
+}
 
 extern "C" size_t tlg_distill_ws_bytes(int type, int N, int V)
 {
@@ -1281,22 +1395,18 @@ extern "C" int tlg_dev_distill(const void *logits, int type, long long ld, int N
     if ((rc = tlg_ensure_init())) return rc;
     const double c = 1.4426950408889634 / (double)temp;
     const int nv = vb_vectors(type, logits, ld, V), ve = type == TLG_F32 ? 4 : 8, S = kd_segments(type, N, V);
-    KdArgs a = {logits, ld, N, V, S, K, tail ? 1 : 0, temp, w_kd, w_ce, scale, f_of(c), 0.f, 1.f / temp,
-                w_ce != 0.f && temp != 1.f, t_ids, t_logp, tgt, rows, dlogits, ldd, 0, (float *)ws};
-    a.kappa = f_of(0.6931471805599453 * (c - (double)a.c) / c);
+    float hi = f_of(c);                                  // below c, so that what is left is positive
+    if ((double)hi >= c) hi = nextafterf(hi, 0.f);
+    KdArgs a = {logits, ld, N, V, S, K, tail ? 1 : 0, temp, w_kd, w_ce, scale, hi, f_of(c - (double)hi),
+                1.0 / (double)temp, w_ce != 0.f && temp != 1.f, t_ids, t_logp, tgt, rows, dlogits, ldd, 0,
+                (float *)ws};
     hipStream_t st = ST(stream);
-    const unsigned r = (unsigned)N;
     // a segment is a multiple of 256 vectors, see the kernel
     const int per = S > 1 ? ((nv + S - 1) / S + 255) / 256 * 256 : nv;
     a.words = tail ? (per * ve + 31) / 32 : 0;
     const size_t lds = (size_t)a.words * 4;
-    if (S > 1) {
-        BY_TYPE(r * S, 256, lds, a, k_distill, , 4, 4, false, KD_SUMS);
-        BY_TYPE(r * S, 256, 0, a, k_distill, , 4, 4, false, KD_GRAD);
-    } else if (nv <= 512 && N >= 512)
-        BY_TYPE((r + 3) / 4, 256, 4 * lds, a, k_distill, , 1, 8, true, KD_WHOLE);
-    else
-        BY_TYPE(r, 256, lds, a, k_distill, , 4, 4, false, KD_WHOLE);
+    if (a.two) kd_launch<true>(a, type, nv, lds, st);
+    else kd_launch<false>(a, type, nv, lds, st);
     if (loss) hipLaunchKernelGGL(k_rows_mean, dim3(1), dim3(1024), 0, st, (const float *)rows, N, loss);
     LAUNCH_CHECK();
     return TLG_OK;
