@@ -756,11 +756,12 @@ struct KdArgs {
 #define KD_C1 1.44269502162933349609375f       // log2 e = KD_C1 + KD_C1_LO
 #define KD_C1_LO 1.925963033500e-8f
 
-// 2^((x - m) (c + lo)): with the constant in two parts the only roundings are the
-// difference's, the product's and the exponential's.  lo > 0, so that -inf stays -inf.
+// 2^((x - m) (c + lo)): the small product first, so that the fused one rounds the
+// whole exponent once (added to a rounded d c it would always be lost, and sums be off
+// by the rounding of c in one direction).  lo > 0, so that -inf stays -inf.
 __device__ __forceinline__ float kd_exp(float d, float c, float lo)
 {
-    return __builtin_amdgcn_exp2f(fmaf(d, lo, d * c));
+    return __builtin_amdgcn_exp2f(fmaf(d, c, d * lo));
 }
 // sums of a part at temperature tau and, with TWO, at the cross-entropy's 1
 struct Kd { float m, s, s1; };
