@@ -759,6 +759,19 @@ def test_cross_entropy_alone_is_xent(lib):
     assert float((d - d2).abs().max()) <= (2 * rho(V) + 100 * EPS) / N
 
 
+@pytest.mark.parametrize("ty,N,V", [(F32, 8192, 2048), (BF16, 2048, 30000), (F32, 1024, 16384)])
+def test_log_sums_lean_to_neither_side(lib, ty, N, V):
+    """The mean signed error of log S over many rows: each row's is random with
+    a deviation below 2e-7 (a few eps), so that the mean's is below 2e-7 /
+    sqrt(N); the hardware exponential leans by 3.5e-9 (measured)."""
+    t = _t()
+    x = (2.5 * t.randn(N, V, device="cuda", generator=t.Generator("cuda").manual_seed(V))).to(dtype(ty))
+    o = distill(lib, x, ty, None, None, False, 1.0, 1.0, x.argmax(1).int(), 1.0, None)
+    z = x.double()
+    err = o.rows.double() - t.log(t.exp(z - z.amax(1, keepdim=True)).sum(1))
+    assert abs(float(err.mean())) <= 5 * 2e-7 / math.sqrt(N) + 5e-9, float(err.mean())
+
+
 # ------------------------------------------------- graphs, streams, repeats --
 @pytest.mark.parametrize("N,V", [(2, 60000), (40, 2048), (600, 3001)])
 def test_same_bits_every_time(lib, N, V):

@@ -35,6 +35,8 @@ struct TlDecode {
     int unfused;                 /* 1: the glue as separate launches (tl_decode_set_fused) */
     /* a prompt's leading rows, up to `bulk` at a time (run_bulk); 0: none */
     int bulk, *bpos, *btok;
+    void *score;                 /* tl_decode_score's buffers, grown on demand */
+    size_t score_bytes;
     float *bx, *by, *bn, *bq, *bk, *bv, *bctx, *bact;
 };
 
@@ -158,6 +160,7 @@ void tl_decode_free(TlDecode *d)
 {
     if (!d) return;
     for (int c = 0; c < TLD_MAXPOOL; c++) if (d->graph[c]) tlg_graph_destroy(d->graph[c]);
+    if (d->score) tlg_dev_free(d->score);
     if (d->arena) tlg_dev_free(d->arena);
     free(d->Kc);
     free(d->Vc);
@@ -409,10 +412,12 @@ static int run_chunk(TlDecode *d, int m, int use_state, int start, int copy, voi
  * projections as MFMA GEMMs over all rows instead of one weight stream per
  * chunk.  Rows below W take ring slots of their own, so a row sees the same
  * keys however the prompt is cut.  The last `tail` rows go on to the logits,
- * as the last chunk's; the others end with the last layer's ring.  A 250-token
- * prompt of the 8-layer, D = 384 model took 32 chunks of 0.42 ms. */
-static int run_bulk(TlDecode *d, const int *tok, int m, int start, int tail, void *st)
+ * as the last chunk's; the others end with the last layer's ring.  With `all`
+ * ([m][V]) every row goes on, to logits there.  A 250-token prompt of the
+ * 8-layer, D = 384 model took 32 chunks of 0.42 ms. */
+static int run_bulk(TlDecode *d, const int *tok, int m, int start, int tail, float *all, void *st)
 {
+    if (all) tail = m;
     const TlModel *md = &d->m;
     const int D = md->D, H = md->H, KV = md->KV, KD = d->KD, F = md->F, hd = d->hd;
     const float *P = d->P[0];
@@ -445,8 +450,16 @@ static int run_bulk(TlDecode *d, const int *tok, int m, int start, int tail, voi
         fc.R = y + o;
         CK(tlg_dev_gemm_group(&fc, 1, st));
     }
-    CK(tlg_memcpy_d2d(d->x, x + (size_t)(m - tail) * D, 4 * (size_t)tail * D, st));
     dmap(d, 0, &w);
+    if (all) {
+        CK(tlg_dev_rmsnorm_fwd(x, P + w.nf, d->bn, NULL, m, D, st));
+        TlgGemmCall head = MMc(all, d->bn, P + w.emb, m, md->V, D);
+        head.op = 1;                                 /* memset + mm_bt, as run_chunk's */
+        head.beta = 0;
+        CK(tlg_dev_gemm_group(&head, 1, st));
+        return tlg_dev_gemm_flush(st);
+    }
+    CK(tlg_memcpy_d2d(d->x, x + (size_t)(m - tail) * D, 4 * (size_t)tail * D, st));
     DGEMV(st, DG(1, 0, d->logits, tail, md->V, D, d->x, P + w.emb, 1, P + w.nf, NULL));
     return 0;
 }
@@ -478,7 +491,7 @@ static int prime_bulk(TlDecode *d, const int *prompt, int n, int *done, int *las
     /* pieces before the last are whole chunks (bulk is), so none cuts the tail */
     for (int i = 0, m; i < rows; i += m) {
         m = rows - i < d->bulk ? rows - i : d->bulk;
-        CK(run_bulk(d, prompt + i, m, i, rows == n && i + m == n ? tail : 0, st));
+        CK(run_bulk(d, prompt + i, m, i, rows == n && i + m == n ? tail : 0, NULL, st));
     }
     *done = rows;
     if (rows == n) *last = tail;
@@ -498,6 +511,64 @@ int tl_decode_prime(TlDecode *d, const int *prompt, int n, void *st)
     const int s[3] = {n - m, m, 0};                   /* the last chunk; argmax advances it */
     CK(tlg_memcpy_h2d(d->state, s, sizeof s, st));    /* state[3] (exchange sequence) is kept */
     CK(tlg_dev_dec_argmax(d->logits, d->m.V, m, d->state, d->tok, st));
+    return tlg_stream_sync(st);
+}
+
+int tl_decode_score(TlDecode *d, const int *tok, int n, float temp, float *logp, float *entropy, int K, int *top_ids,
+                    float *top_logp, void *st)
+{
+    if (!d || !tok || n <= 0 || n > d->maxpos || !logp || K < 0 || K > TLG_VOCAB_TOP || (K && (!top_ids || !top_logp)) ||
+        !(temp >= 1e-30f && temp <= 1e30f))
+        return TLG_EINVAL;
+    for (int j = 0; j < n; j++) if (tok[j] < 0 || tok[j] >= d->m.V) return TLG_EINVAL;
+    const int V = d->m.V;
+    /* rows at once: the bulk pass takes what fits the ring, chunks of mmax the rest */
+    const int bulk = !d->unfused && d->bulk && n >= 2 * TLD_MAXM ? (n <= d->W ? n : d->W / d->mmax * d->mmax) : 0;
+    const int piece = bulk < d->bulk ? bulk : d->bulk;
+    const size_t pad = 255, b1 = (4 * (size_t)n + pad) & ~pad, bk = (4 * (size_t)n * K + pad) & ~pad,
+                 bl = (4 * (size_t)piece * V + pad) & ~pad;
+    size_t ws_b = 0;                                 /* no piece has fewer rows than 1 nor more than these */
+    for (int m = 1; m <= (piece > d->mmax ? piece : d->mmax); m++) {
+        const size_t b = tlg_logprobs_ws_bytes(TLG_F32, m, V, K);
+        if (b > ws_b) ws_b = b;
+    }
+    const size_t bytes = 3 * b1 + 2 * bk + bl + ws_b;
+    if (bytes > d->score_bytes) {
+        CK(tlg_stream_sync(st));
+        void *mem = tlg_dev_malloc(bytes);
+        if (!mem) return TLG_ENOMEM;
+        if (d->score) tlg_dev_free(d->score);
+        d->score = mem;
+        d->score_bytes = bytes;
+    }
+    char *p = d->score;
+    int *next = (int *)p, *ti = (int *)(p + 3 * b1);
+    float *lp = (float *)(p + b1), *en = (float *)(p + 2 * b1), *tl = (float *)(p + 3 * b1 + bk),
+          *all = (float *)(p + 3 * b1 + 2 * bk);
+    void *ws = p + 3 * b1 + 2 * bk + bl;
+    const int none = -1;
+    if (n > 1) CK(tlg_memcpy_h2d(next, tok + 1, 4 * (size_t)(n - 1), st));
+    CK(tlg_memcpy_h2d(next + n - 1, &none, 4, st));
+    CK(tlg_stream_sync(st));
+    for (int i = 0, m; i < n; i += m) {
+        const float *rows = d->logits;
+        if (i < bulk) {
+            m = bulk - i < piece ? bulk - i : piece;
+            CK(run_bulk(d, tok + i, m, i, 0, all, st));
+            rows = all;
+        } else {
+            m = n - i < d->mmax ? n - i : d->mmax;
+            CK(tl_decode_chunk(d, tok + i, m, i, st));
+        }
+        CK(tlg_dev_logprobs(rows, TLG_F32, V, m, V, 1.0f / temp, next + i, 1, lp + i, NULL, entropy ? en + i : NULL, K,
+                            ti + (size_t)i * K, tl + (size_t)i * K, ws, ws_b, st));
+    }
+    CK(tlg_memcpy_d2h(logp, lp, 4 * (size_t)n, st));
+    if (entropy) CK(tlg_memcpy_d2h(entropy, en, 4 * (size_t)n, st));
+    if (K) {
+        CK(tlg_memcpy_d2h(top_ids, ti, 4 * (size_t)n * K, st));
+        CK(tlg_memcpy_d2h(top_logp, tl, 4 * (size_t)n * K, st));
+    }
     return tlg_stream_sync(st);
 }
 

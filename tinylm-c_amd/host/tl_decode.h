@@ -64,6 +64,17 @@ int tl_decode_chunk(TlDecode *d, const int *tok, int m, int start, void *stream)
 /* Prefill a prompt in chunks of <= mmax (positions 0..n-1), then take the
  * greedy token: the state now holds position n and that token. */
 int tl_decode_prime(TlDecode *d, const int *prompt, int n, void *stream);
+/* Score a text (the reference's `score` and `nll` commands, within
+ * tinylm.c:3844-4687): feed n host tokens at positions 0..n-1, as
+ * tl_decode_prime does, and for every row i, with the next-token distribution
+ * softmax(logits_i / temp), give logp[i] = log p(tok[i + 1]) (0 for the last
+ * row), entropy[i] (if not NULL) and the K <= TLG_VOCAB_TOP likeliest tokens
+ * top_ids[i][] with top_logp[i][] (tlg_dev_logprobs, include/tltrain.h; host arrays).
+ * top_ids and top_logp are what tl_train_set_teacher takes.  Synchronous; the
+ * ring then holds the text, the greedy state is left alone, and what
+ * tl_decode_mtp_draft reads is undefined.  Weights copy 0. */
+int tl_decode_score(TlDecode *d, const int *tok, int n, float temp, float *logp, float *entropy, int K, int *top_ids,
+                    float *top_logp, void *stream);
 /* One greedy token step from the device state (weights copy `copy`). */
 int tl_decode_greedy_step(TlDecode *d, int copy, void *stream);
 /* MTP head k's greedy draft (mtp_argmax, tinylm.c:3930-3936) from row `row`

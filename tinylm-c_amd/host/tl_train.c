@@ -44,6 +44,13 @@ struct TlTrain {
      * read by its backward instead of a recompute */
     char *moe_keep;
     size_t moe_keep_b;
+    /* distillation (tl_train_set_teacher): K entries a row, 0 without a teacher */
+    struct { int K, tail; float temp, w_kd, w_ce; } kd;
+    void *kd_mem;                       /* ids, log probabilities, row losses, workspace */
+    size_t kd_bytes, kd_ws_b;
+    int *kd_ids;
+    float *kd_logp, *kd_rows;
+    void *kd_ws;
     float hyper_host[8];
     void *graph;
     /* per grouped GEMM launch of a step, in call order: tile configuration + 1
@@ -167,6 +174,7 @@ void tl_train_free(TlTrain *t)
 {
     if (!t) return;
     if (t->graph) tlg_graph_destroy(t->graph);
+    if (t->kd_mem) tlg_dev_free(t->kd_mem);
     if (t->arena) tlg_dev_free(t->arena);
     free(t);
 }
@@ -200,6 +208,8 @@ float *tl_train_act(TlTrain *t, const char *name, int layer)
     return NULL;
 }
 
+#define CK(x) do { int rc_ = (x); if (rc_) return rc_; } while (0)
+
 /* ---- host <-> device at step boundaries ------------------------------------ */
 int tl_train_upload(TlTrain *t, const float *P, void *st)
 {
@@ -222,6 +232,44 @@ int tl_train_set_batch(TlTrain *t, const int *tok, const int *tgt, const int *tg
     if (!rc && nm) rc = tlg_memcpy_h2d(t->tgt_mtp, tgt_mtp, 4 * (size_t)N * nm, st);
     if (!rc) rc = tlg_stream_sync(st);
     return rc;
+}
+
+int tl_train_set_teacher(TlTrain *t, const int *ids, const float *logp, int K, int tail, float temp, float w_kd,
+                         float w_ce, void *st)
+{
+    if (!t || K < 0 || K > TLG_VOCAB_TOP || (K && (!ids || !logp)) || !(temp >= 1e-30f && temp <= 1e30f) ||
+        !isfinite(w_kd) || !isfinite(w_ce))
+        return TLG_EINVAL;
+    const size_t N = t->N, n = N * (size_t)K, pad = 255;
+    for (size_t i = 0; i < n; i++)
+        if (ids[i] >= t->m.V) return TLG_EINVAL;
+    const size_t b_ids = (4 * n + pad) & ~pad, b_rows = (4 * N + pad) & ~pad,
+                 b_ws = K ? tlg_distill_ws_bytes(TLG_F32, t->N, t->m.V) : 0, bytes = 2 * b_ids + b_rows + b_ws;
+    const int same = K == t->kd.K && !!tail == t->kd.tail && temp == t->kd.temp && w_kd == t->kd.w_kd &&
+                     w_ce == t->kd.w_ce && bytes <= t->kd_bytes;
+    if (K && bytes > t->kd_bytes) {
+        CK(tlg_stream_sync(st));                     /* a step in flight may read the old ones */
+        void *mem = tlg_dev_malloc(bytes);
+        if (!mem) return TLG_ENOMEM;
+        if (t->kd_mem) tlg_dev_free(t->kd_mem);
+        t->kd_mem = mem;
+        t->kd_bytes = bytes;
+    }
+    if (!same && (K || t->kd.K) && t->graph) {       /* the captured step is stale */
+        tlg_graph_destroy(t->graph);
+        t->graph = NULL;
+    }
+    t->kd.K = K; t->kd.tail = !!tail; t->kd.temp = temp; t->kd.w_kd = w_kd; t->kd.w_ce = w_ce;
+    if (!K) return TLG_OK;
+    char *p = t->kd_mem;
+    t->kd_ids = (int *)p;
+    t->kd_logp = (float *)(p + b_ids);
+    t->kd_rows = (float *)(p + 2 * b_ids);
+    t->kd_ws = p + 2 * b_ids + b_rows;
+    t->kd_ws_b = b_ws;
+    CK(tlg_memcpy_h2d(t->kd_ids, ids, 4 * n, st));
+    CK(tlg_memcpy_h2d(t->kd_logp, logp, 4 * n, st));
+    return tlg_stream_sync(st);
 }
 
 int tl_train_set_hyper(TlTrain *t, float lr, float b1, float b2, float wd, int step, void *st)
@@ -281,7 +329,6 @@ static TlgGemmCall BTN(float *dX, int beta, int M, int K, int n, const float *co
     return c;
 }
 
-#define CK(x) do { int rc_ = (x); if (rc_) return rc_; } while (0)
 
 /* One grouped GEMM launch, the step's k-th: pinned to its tile configuration
  * when the step has a table, bracketed by events while autotuning. */
@@ -371,8 +418,13 @@ static int forward_impl(TlTrain *t, int clear_g, void *st)
     } else {
         GROUP(st, BT(t->logits, 0, t->fn, P + w.emb, N, V, D));
     }
-    /* softmax-CE, with backward's dlogits (:1076-1082) from the same pass */
-    if (clear_g)
+    /* softmax-CE, or the distillation loss in its place, with backward's
+     * dlogits (:1076-1082) from the same pass */
+    if (t->kd.K)
+        CK(tlg_dev_distill(t->logits, TLG_F32, V, N, V, t->kd_ids, t->kd_logp, t->kd.K, t->kd.tail, t->kd.temp,
+                           t->kd.w_kd, t->tgt, t->kd.w_ce, t->kd_rows, t->loss, t->dl, V, 1.0f / N, t->kd_ws,
+                           t->kd_ws_b, st));
+    else if (clear_g)
         CK(tlg_dev_xent_rows(t->logits, t->tgt, t->dl, t->lrows, 1.0f / N, N, V, st));
     else
         CK(tlg_dev_xent(t->logits, t->tgt, t->dl, t->loss, 1.0f / N, N, V, st));
@@ -483,7 +535,7 @@ int tl_train_step(TlTrain *t, void *st)
     const int fold = t->np <= (size_t)INT_MAX;         /* the clear item's extent is an int */
     CK(forward_impl(t, fold, st));
     CK(backward_impl(t, fold, st));
-    return optimize_impl(t, fold, st);
+    return optimize_impl(t, fold && !t->kd.K, st);     /* distillation leaves its loss averaged */
 }
 
 int tl_train_graph_build(TlTrain *t, void *st)

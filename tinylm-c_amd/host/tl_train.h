@@ -51,6 +51,17 @@ int  tl_train_upload(TlTrain *t, const float *P, void *stream);
 /* Copy one batch of host tokens in: tok and tgt are N ints, tgt_mtp is
  * n_mtp x N ints (NULL when n_mtp = 0).  Tokens must lie in [0, V). */
 int  tl_train_set_batch(TlTrain *t, const int *tok, const int *tgt, const int *tgt_mtp, void *stream);
+/* Distil from a teacher (no counterpart in the reference): the following
+ * steps' loss and head gradient are tlg_dev_distill's (include/tltrain.h), with
+ * the batch's targets as its hard ones, in place of the softmax cross-entropy
+ * (tinylm.c:1019-1028, :1076-1082); MTP heads keep theirs.  ids and logp are host
+ * arrays [N][K] (K <= TLG_VOCAB_TOP) of each row's teacher tokens and their log
+ * probabilities at temperature temp, as tl_decode_score gives them; a negative
+ * id is no entry, one from V on is refused.  K = 0 goes back to the
+ * cross-entropy (ids and logp may be NULL).  A captured step stays valid while
+ * only the arrays' contents change, and is dropped otherwise. */
+int  tl_train_set_teacher(TlTrain *t, const int *ids, const float *logp, int K, int tail, float temp, float w_kd,
+                          float w_ce, void *stream);
 /* AdamW hyper-parameters for step `step` (1-based, adamw's t): copied to the
  * device, so captured steps replay with the current values. */
 int  tl_train_set_hyper(TlTrain *t, float lr, float b1, float b2, float wd, int step, void *stream);

@@ -388,6 +388,18 @@ class Train:
                                                   None if tm is None else tm.ctypes.data, stream),
                  "tl_train_set_batch")
 
+    def set_teacher(self, ids, logp, stream, tail=False, temp=1.0, w_kd=1.0, w_ce=0.0):
+        """Distil from a teacher's top log probabilities: ids and logp [N][K]
+        (tl_train_set_teacher); ids None goes back to the cross-entropy."""
+        import numpy as np
+        fn = self.host.dll.tl_train_set_teacher
+        if ids is None:
+            return self._ck(fn(self.h, None, None, 0, 0, 1.0, 0.0, 0.0, stream), "tl_train_set_teacher")
+        ids, logp = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(logp, np.float32)
+        assert ids.shape == logp.shape and ids.ndim == 2 and ids.shape[0] == self.N
+        return self._ck(fn(self.h, ids.ctypes.data, logp.ctypes.data, ids.shape[1], int(tail), temp, w_kd, w_ce, stream),
+                        "tl_train_set_teacher")
+
     def set_hyper(self, lr, b1, b2, wd, step, stream):
         return self._ck(self.host.dll.tl_train_set_hyper(self.h, lr, b1, b2, wd, step, stream), "tl_train_set_hyper")
 
@@ -522,6 +534,19 @@ class Decode:
         import numpy as np
         p = np.ascontiguousarray(prompt, np.int32)
         return self._ck(self.host.dll.tl_decode_prime(self.h, p.ctypes.data, p.size, stream), "tl_decode_prime")
+
+    def score(self, tok, stream, K=0, temp=1.0):
+        """Log probability of every token's successor in a text, the entropy of
+        its distribution and its K likeliest tokens (tl_decode_score):
+        (logp [n], entropy [n], top_ids [n][K], top_logp [n][K])."""
+        import numpy as np
+        tok = np.ascontiguousarray(tok, np.int32)
+        n = tok.size
+        lp, en = np.empty(n, np.float32), np.empty(n, np.float32)
+        ti, tl = np.empty((n, K), np.int32), np.empty((n, K), np.float32)
+        self._ck(self.host.dll.tl_decode_score(self.h, tok.ctypes.data, n, temp, lp.ctypes.data, en.ctypes.data, K,
+                                               ti.ctypes.data, tl.ctypes.data, stream), "tl_decode_score")
+        return lp, en, ti, tl
 
     def greedy_step(self, stream, copy=0):
         return self._ck(self.host.dll.tl_decode_greedy_step(self.h, copy, stream), "tl_decode_greedy_step")
@@ -718,6 +743,8 @@ class Host:
         d.tl_train_act.restype = _vp
         d.tl_train_upload.argtypes = [_vp, _vp, _vp]
         d.tl_train_set_batch.argtypes = [_vp, _vp, _vp, _vp, _vp]
+        d.tl_train_set_teacher.argtypes = [_vp, _vp, _vp, _i, _i, _f, _f, _f, _vp]
+        d.tl_train_set_teacher.restype = _i
         d.tl_train_set_hyper.argtypes = [_vp, ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float, _i, _vp]
         for n in ("tl_train_forward", "tl_train_backward", "tl_train_optimize", "tl_train_step",
                   "tl_train_graph_build", "tl_train_graph_step"):
@@ -754,6 +781,8 @@ class Host:
             getattr(d, n).restype = _i
         d.tl_decode_chunk.argtypes = [_vp, _vp, _i, _i, _vp]
         d.tl_decode_prime.argtypes = [_vp, _vp, _i, _vp]
+        d.tl_decode_score.argtypes = [_vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _vp]
+        d.tl_decode_score.restype = _i
         d.tl_decode_greedy_step.argtypes = [_vp, _i, _vp]
         d.tl_decode_persist.argtypes = [_vp, _i, _vp, _vp]
         d.tl_decode_persist.restype = _i
