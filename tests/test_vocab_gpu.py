@@ -395,6 +395,39 @@ def test_masked_rows_infinities_and_nan(lib, ty, V, N):
     check_logprobs(logprobs(lib, x, ty, 1.0, ids, 12), x, 1.0, ids, 12)
 
 
+@pytest.mark.parametrize("N,V", [(9, 300), (9, 9000), (3, 50000), (1100, 2048), (9, 2048)])
+def test_large_finite_masks_and_values(lib, N, V):
+    """Masks of -1e5 .. -1e38 over parts of a row (whole lanes, waves and
+    segments of it), over all of it, and logits as large as that."""
+    t = _t()
+    print("large", N, V, flush=True)
+    g = t.Generator().manual_seed(V)
+    base = 2 * t.randn(N, V, generator=g)
+    for far in (1e5, 1e6, 1e7, 1e9, 1e10, 1e20, 3e38):
+        x = base.clone()
+        x[0] = -far
+        x[1, 7:] = -far
+        x[2, : V - 1] = -far
+        if N > 3:
+            x[3, t.rand(V, generator=g) < 0.9] = -far
+            x[4] = far
+            x[5, V // 2] = far
+            x[6, V // 3] = -far
+            x[7, :: 2] = -far
+            x[8, V // 4: V // 2] = -far
+        for ty in (F32, BF16):
+            y = x.to(dtype(ty)).cuda()
+            ids = some_ids(N, V, 2, 1)
+            check_logprobs(logprobs(lib, y, ty, 1.0, ids, 5), y, 1.0, ids, 5)
+            tgt = ids[:, 1].contiguous()
+            _, d = like_rows(y, ty)
+            o = distill(lib, y, ty, None, None, False, 1.0, 1.0, tgt, 1.0, d)
+            rows, grad = ref_distill(f64(y), np.zeros((N, 0), int), np.zeros((N, 0)), False, 1.0, 1.0, tgt.cpu().numpy(), 1.0)
+            # differences of values this large are exact or off by half a step of theirs
+            close(f64(o.rows), rows, 3 * rho(V) + 8 * EPS * (60 + np.abs(rows)), "rows")
+            close(f64(d), grad, (half_step(ty) * 1.01 + 8 * EPS) * np.abs(grad) + 2 * rho(V) + 200 * EPS, "dlogits")
+
+
 def test_extreme_temperatures(lib):
     """Almost greedy and almost uniform distributions."""
     _, x = on_gpu(rows_of(F32, 5, 3000))

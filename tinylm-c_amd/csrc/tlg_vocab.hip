@@ -177,11 +177,14 @@ __device__ __forceinline__ float vb_key_value(u64 k)
 // with kappa = ln 2 (scale log2 e - c) / c for the rounding of c, to first order.
 // NaN and +inf make s NaN.  Exponents are clamped at -200, where 2^t is 0, in the
 // factor of the products only: 0 * -inf must not be NaN, NaN must stay.  R is kept
-// at -1e38 or above.  Where a maximum of that size, of either sign, leaves s = 0
-// although not all is masked, sums_apart forms the sums from differences.
+// at -ACC_FAR or above, so that a part of nothing but masked values, -inf or large
+// finite ones, has s = 0 or one of its size; a row whose maximum is farther than
+// that from 0, where the rounding of m c would reach the exponents, has its sums
+// formed from differences (sums_apart).
+#define ACC_FAR 1e6f
 struct Acc { float R, s, u; };
-#define ACC0 {-1e38f, 0.f, 0.f}
-__device__ __forceinline__ float acc_ref(float m, float c) { return fmaxf(m * c, -1e38f); }
+#define ACC0 {-ACC_FAR, 0.f, 0.f}
+__device__ __forceinline__ float acc_ref(float m, float c) { return fmaxf(m * c, -ACC_FAR); }
 __device__ __forceinline__ void acc_shift(Acc &a, float R)                    // to a reference R >= a.R
 {
     const float d = a.R - R, f = __builtin_amdgcn_exp2f(d);
@@ -215,6 +218,7 @@ __device__ __forceinline__ Acc acc_join(const f32x4 *p, int n, float c, float &m
     }
     return r;
 }
+__device__ __forceinline__ bool acc_far(float m, float c) { return fabsf(m * c) > ACC_FAR && m > -INFINITY; }
 // What is asked of a row: m its maximum, ls = log sum e^(scale (x - m)), H the
 // entropy; NaN and -inf mark rows without a distribution.
 struct Sums { float m, ls, H; };
@@ -222,7 +226,7 @@ template <int TYPE, int W>
 __device__ __noinline__ Acc sums_apart(const Row<TYPE> x, float m, float c, int t, f32x4 *part)
 {
     constexpr int VE = El<TYPE>::VE;
-    Acc a = {0.f, 0.f, 0.f};
+    Acc a = {0.f, 0.f, 0.f};                            // R is not used: rho = 0
     for (int j = t; j < x.nv; j += 64 * W) {
         const u32x4 q = x.any(j);
 #pragma unroll
@@ -247,17 +251,11 @@ __device__ __noinline__ Acc sums_apart(const Row<TYPE> x, float m, float c, int 
     }
     return a;
 }
-template <int TYPE, int W>
-__device__ __forceinline__ Sums sums_of(const Row<TYPE> &x, float m, Acc a, float c, float kappa, int t, f32x4 *part)
+__device__ __forceinline__ Sums sums_of(float m, const Acc &a, float c, float kappa)
 {
-    float rho = -fmaf(m, c, -a.R);
-    if (a.s == 0.f && m > -INFINITY) {
-        a = sums_apart<TYPE, W>(x, m, c, t, part);
-        rho = 0.f;
-    }
     if (a.s != a.s) return Sums{NAN, NAN, NAN};
     if (m == -INFINITY) return Sums{-INFINITY, -INFINITY, 0.f};
-    const float ls = fmaf(0.69314718056f, rho, logf(fmaf(kappa, a.u, a.s)));
+    const float rho = acc_far(m, c) ? 0.f : -fmaf(m, c, -a.R), ls = fmaf(0.69314718056f, rho, logf(fmaf(kappa, a.u, a.s)));
     return Sums{m, ls, ls - 0.69314718056f * fmaf(a.u, __builtin_amdgcn_rcpf(a.s), rho)};
 }
 
@@ -346,20 +344,35 @@ template <typename E> __device__ __forceinline__ void wave_push(bool take, E v, 
     if (take && at < cap) list[at] = v;
     n += __popcll(m);
 }
+// element e, any e, of a raw vector
+template <int TYPE> __device__ __forceinline__ float el_any(const u32x4 &r, int e)
+{
+    constexpr int P = El<TYPE>::VE / 4;                  // elements of a register
+    const int k = e / P;
+    const unsigned a = k & 1 ? r[1] : r[0], b = k & 1 ? r[3] : r[2], w = k & 2 ? b : a;
+    return el_float<TYPE>(P == 1 ? w : w >> (e & 1) * 16 & 0xffffu);
+}
 // all elements of a vector at place j that reach T (by value, then by key)
 template <int TYPE, int W>
 __device__ __forceinline__ void lp_list(const u32x4 &q, int j, float T, u64 Tkey, u64 *cand, int &n, int cap)
 {
+    if constexpr (W == 1) {                              // all lanes at once: most elements reach T in none
 #pragma unroll
-    for (int e = 0; e < El<TYPE>::VE; e++) {
-        const float x = el_at<TYPE>(q, e);
-        if constexpr (W == 1) {                          // most vectors have none: all lanes at once
+        for (int e = 0; e < El<TYPE>::VE; e++) {
+            const float x = el_at<TYPE>(q, e);
             if (__ballot(x >= T)) {
                 const u64 key = vb_key(x, j * El<TYPE>::VE + e);
                 wave_push(x >= T && key >= Tkey, key, cand, n, cap);
             }
-        } else if (x >= T) {
-            const u64 key = vb_key(x, j * El<TYPE>::VE + e);
+        }
+    } else {
+        unsigned hit = 0;
+#pragma unroll
+        for (int e = El<TYPE>::VE - 1; e >= 0; e--) hit = hit * 2 + (el_at<TYPE>(q, e) >= T);
+        while (hit) {
+            const int e = __ffs(hit) - 1;
+            hit &= hit - 1;
+            const u64 key = vb_key(el_any<TYPE>(q, e), j * El<TYPE>::VE + e);
             if (key >= Tkey) {
                 const int at = atomicAdd(&n, 1);
                 if (at < cap) cand[at] = key;
@@ -438,49 +451,50 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
         }
     };
 
-    // lines are joined over 2^q rounds of the loop
+    // lines are joined over 2^q rounds; every wave takes part in every round, so that
+    // all lines up to the last round's are written
     int q = 0;
     if constexpr (LINES)
         while (LP_LINES * 8 * W << q < j1 - j0 + 8 * U * W) q++;
     const Given given = lp_given<TYPE>(a, r, x.x, t);
     Acc A = ACC0;
-    float v1 = -INFINITY, lm[U];
-    for (int j = j0 + t, i = 0; RES ? i == 0 : j - lane < j1; j += U * TPR, i++) {      // whole waves
-        load(j);
-        float gm = -INFINITY;
+    float v1 = -INFINITY;
+    float *to = LINES ? sh.max + (wave * 8 + lane / 8) * U : nullptr;
+    for (int j = j0 + t; RES || j - t < j1; to += U * 8 * W) {
+        float lm[U];
 #pragma unroll
-        for (int k = 0; k < U; k++) {
-            float vm = el_at<TYPE>(raw[k], 0);
+        for (int k = 0; k < U; k++) lm[k] = -INFINITY;
+        for (int i = 0; i < 1 << q && (RES || j - t < j1); i++, j += U * TPR) {
+            load(j);
+            float gm = -INFINITY;
 #pragma unroll
-            for (int e = 1; e < VE; e++) vm = fmaxf(vm, el_at<TYPE>(raw[k], e));
-            gm = fmaxf(gm, vm);
-            if constexpr (LINES) lm[k] = i & ((1 << q) - 1) ? fmaxf(lm[k], vm) : vm;
+            for (int k = 0; k < U; k++) {
+                float vm = el_at<TYPE>(raw[k], 0);
+#pragma unroll
+                for (int e = 1; e < VE; e++) vm = fmaxf(vm, el_at<TYPE>(raw[k], e));
+                gm = fmaxf(gm, vm);
+                if constexpr (LINES) lm[k] = fmaxf(lm[k], vm);
+            }
+            v1 = fmaxf(v1, gm);
+            acc_shift(A, acc_ref(v1, a.c));
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                if (RES) keep_packed(raw[k]);
+#pragma unroll
+                for (int e = 0; e < VE; e++) acc_add(A, el_at<TYPE>(raw[k], e), a.c);
+                if (RES) keep_packed(raw[k]);
+            }
         }
         if constexpr (LINES) {
-            float o[U];
 #pragma unroll
             for (int k = 0; k < U; k++) {               // over 8 lanes
-                o[k] = fmaxf(lm[k], lane_move<0xB1>(lm[k]));
-                o[k] = fmaxf(o[k], lane_move<0x4E>(o[k]));
-                o[k] = fmaxf(o[k], lane_move<0x141>(o[k]));
+                lm[k] = fmaxf(lm[k], lane_move<0xB1>(lm[k]));
+                lm[k] = fmaxf(lm[k], lane_move<0x4E>(lm[k]));
+                lm[k] = fmaxf(lm[k], lane_move<0x141>(lm[k]));
             }
-            if (lane % 8 == 0) {
-                float *to = sh.max + (((i >> q) * W + wave) * 8 + lane / 8) * U;
-                if constexpr (U == 4) *(f32x4 *)to = f32x4{o[0], o[1], o[2], o[3]};
-                else
-#pragma unroll
-                    for (int k = 0; k < U; k++) to[k] = o[k];
-            }
+            if (lane % 8 == 0) *(f32x4 *)to = f32x4{lm[0], lm[1], lm[2], lm[3]};
         }
-        v1 = fmaxf(v1, gm);
-        acc_shift(A, acc_ref(v1, a.c));
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            if (RES) keep_packed(raw[k]);
-#pragma unroll
-            for (int e = 0; e < VE; e++) acc_add(A, el_at<TYPE>(raw[k], e), a.c);
-            if (RES) keep_packed(raw[k]);
-        }
+        if (RES) break;
     }
 
     // the row's sums, maximum and bound
@@ -501,12 +515,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
         for (int w = 0; w < W; w++) T = fminf(T, sh.part[w][3]);
         if (a.S > 1 && t == 0) ((f32x4 *)a.part)[r * a.S + seg] = f32x4{A.s, A.u, m, 0.f};
     }
-    Sums sum = {0.f, 0.f, 0.f};
-    if (W == 1 || a.S == 1) {
-        sum = sums_of<TYPE, W>(x, m, A, a.c, a.kappa, t, sh.part);
-        lp_finish(a, r, given, sum, t);
+    const bool whole = W == 1 || a.S == 1;
+    if (whole && acc_far(m, a.c)) A = sums_apart<TYPE, W>(x, m, a.c, t, sh.part);
+    if constexpr (!TOP) {
+        if (whole && wave == 0) lp_finish(a, r, given, sums_of(m, A, a.c, a.kappa), t);
+        return;
     }
-    if constexpr (!TOP) return;
 
     // The lines that reach T, then the elements that do.  Line l is the lanes 8 o ..
     // 8 o + 7 of wave w in load k of the rounds i 2^q ..., from l's digits.
@@ -519,10 +533,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
     int items = 0;
     if constexpr (LINES) {
         const int rounds = (j1 - j0 + U * TPR - 1) / (U * TPR), all = ((rounds + (1 << q) - 1) >> q) * (U * 8 * W);
-        for (int l = t; l - lane < all; l += TPR) {
-            const bool take = l < all && first(l) < j1 && sh.max[l] >= T;
-            if constexpr (W == 1) wave_push(take, (unsigned short)l, sh.line, lines, LP_LINES);
-            else if (take) sh.line[atomicAdd(&lines, 1)] = l;
+        for (int l = 4 * t; l - 4 * lane < all; l += 4 * TPR) {          // all is a multiple of 32
+            const f32x4 v = l < all ? *(const f32x4 *)(sh.max + l) : f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (W == 1) wave_push(v[e] >= T, (unsigned short)(l + e), sh.line, lines, LP_LINES);
+                else if (v[e] >= T) sh.line[atomicAdd(&lines, 1)] = l + e;
+            }
         }
         row_sync<W>();
         items = lines * 8 << q;
@@ -557,6 +574,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
     }
     const int got = n;
     u64 *out = a.keys + r * a.K * a.S + seg;             // S > 1
+    if (wave > 0 && 64 * wave >= max(got, a.K)) return;  // nothing of the rest is this wave's
+    Sums sum = {0.f, 0.f, 0.f};
+    if (whole) {
+        sum = sums_of(m, A, a.c, a.kappa);
+        if (wave == 0) lp_finish(a, r, given, sum, t);
+    }
     for (int i = t; i < got; i += TPR) {
         const u64 key = sh.cand[i];
         int rank = 0;
@@ -600,9 +623,10 @@ template <int TYPE, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_
     }
     __syncthreads();
     float m;
-    const Acc A = acc_join(part, a.S, a.c, m);
+    Acc A = acc_join(part, a.S, a.c, m);
     __syncthreads();
-    const Sums sum = sums_of<TYPE, 4>(x, m, A, a.c, a.kappa, t, part);
+    if (acc_far(m, a.c)) A = sums_apart<TYPE, 4>(x, m, a.c, t, part);
+    const Sums sum = sums_of(m, A, a.c, a.kappa);
     lp_finish(a, r, given, sum, t);
     if constexpr (!TOP) return;
     for (int w = 0; w < 4; w++) T = fminf(T, tw[w]);
