@@ -264,9 +264,9 @@ __device__ __forceinline__ Sums sums_of(float m, const Acc &a, float c, float ka
 // These are different elements, so a bound T that enough of them reach (J =
 // ceil(K / waves) lanes of every wave) is reached by K elements of the row at
 // least, in a row of random order by little more.  They go to a list, which is
-// ranked by counting.  A row of one wave and U vectors a lane at most (RES) is still
-// in registers then.  Of longer rows the pass leaves line maxima in LDS, for less
-// than an operation per element: eight neighbouring lanes' vectors are a line of 128
+// ranked by counting.  A row of at most U vectors a thread (RES) is still in
+// registers then.  Of longer rows the pass leaves line maxima in LDS, for less than
+// an operation per element: eight neighbouring lanes' vectors are a line of 128
 // bytes (2^q lines U 64 W vectors apart, in rows of more than LP_LINES lines per
 // wave); the lines that reach T are read again, by all threads evenly.  A list that
 // overflows, from many equal values or large values that lie together, raises T by
@@ -613,9 +613,15 @@ template <int TYPE, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_
     if (t < a.S) part[t] = ((const f32x4 *)a.part)[r * a.S + t];
     float T = -FLT_MAX;
     const u64 *keys = a.keys + r * n;
+    u64 held[2] = {0, 0};
     if constexpr (TOP) {
         u64 b = 0;
-        for (int i = t; i < n; i += 256) b = keys[i] > b ? keys[i] : b;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {                    // most are held from the first reading
+            held[k] = t + 256 * k < n ? keys[t + 256 * k] : 0;
+            b = held[k] > b ? held[k] : b;
+        }
+        for (int i = t + 512; i < n; i += 256) b = keys[i] > b ? keys[i] : b;
         const int full = min(4, n / 64), J = full ? (a.K + full - 1) / full : 65;
         T = t / 64 >= (full ? full : 1) ? FLT_MAX : wave_bound(b ? vb_key_value(b) : -FLT_MAX, J);
         if (lane == 0) tw[t >> 6] = T;
@@ -630,8 +636,12 @@ template <int TYPE, bool TOP> __global__ __launch_bounds__(256) void k_logprobs_
     lp_finish(a, r, given, sum, t);
     if constexpr (!TOP) return;
     for (int w = 0; w < 4; w++) T = fminf(T, tw[w]);
-    for (int i = t; i < n; i += 256)
-        if (keys[i] && vb_key_value(keys[i]) >= T) cand[atomicAdd(&cnt, 1)] = keys[i];
+    auto put = [&](u64 key) {
+        if (key && vb_key_value(key) >= T) cand[atomicAdd(&cnt, 1)] = key;
+    };
+    put(held[0]);
+    put(held[1]);
+    for (int i = t + 512; i < n; i += 256) put(keys[i]);
     __syncthreads();
     const int got = cnt;
     for (int i = t; i < got; i += 256) {
@@ -1275,9 +1285,10 @@ extern "C" size_t tlg_logprobs_ws_bytes(int type, int N, int V, int K)
 
 // One wave per row where the rows are short and many: no barriers, and a lane's
 // four (or, of fp32, eight) vectors stay in registers; 4096 rows of 2048 fp32 values
-// with 8 alternatives take 11.3 us so, 13.2 with the rows read again, 18.3 with four
+// with 8 alternatives take 11.2 us so, 13.2 with the rows read again, 18.3 with four
 // waves each.  Four waves win for fewer rows (512 of those: 6.5 against 7.1 us) and for
-// longer ones (4096 of 16384 fp32 values: 49 against 58 us).
+// longer ones (4096 of 16384 fp32 values: 49 against 58 us); they too keep four vectors
+// a thread (900 rows of 4000 fp32 values: 8.2 us, 9.1 read again).
 template <bool TOP> static void lp_launch(const LpArgs &a, int type, int nv, hipStream_t st)
 {
     const unsigned rows = (unsigned)a.N;
@@ -1291,6 +1302,8 @@ template <bool TOP> static void lp_launch(const LpArgs &a, int type, int nv, hip
         hipLaunchKernelGGL((k_logprobs<TLG_F32, 1, 8, true, TOP>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
     else if (wave && nv <= 1024 && rows >= 2 * (unsigned)nv)
         BY_TYPE((rows + 3) / 4, 256, 0, a, k_logprobs, , 1, 4, false, TOP);
+    else if (nv <= 1024)
+        BY_TYPE(rows, 256, 0, a, k_logprobs, , 4, 4, true, TOP);
     else
         BY_TYPE(rows, 256, 0, a, k_logprobs, , 4, 4, false, TOP);
 }
