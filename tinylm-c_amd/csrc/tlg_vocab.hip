@@ -1182,19 +1182,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
     a.rows[r] = bad_id ? NAN : nothing ? 0.f : (float)L;
 }
 
-// the mean of the row losses, summed in double in a fixed order
+// The mean of the row losses, summed in double in a fixed order by one workgroup:
+// eight loads in flight a thread, one barrier.
 __global__ __launch_bounds__(1024) void k_rows_mean(const float *__restrict__ rows, int n, float *__restrict__ out)
 {
-    __shared__ double s[1024];
+    __shared__ double s[16];
+    const int t = threadIdx.x;
     double a = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) a += (double)rows[i];
-    s[threadIdx.x] = a;
-    __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
-        __syncthreads();
+    for (int i = t; i < n; i += 8 * 1024) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = i + 1024 * k < n ? rows[i + 1024 * k] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) a += (double)v[k];
     }
-    if (threadIdx.x == 0) out[0] = (float)(s[0] / n);
+    a = wave_sum64(a);
+    if (t % 64 == 0) s[t / 64] = a;
+    __syncthreads();
+    if (t >= 64) return;
+    a = wave_sum64(t < 16 ? s[t] : 0.0);
+    if (t == 0) out[0] = (float)(a / n);
 }
 
 // -------------------------------------------------------------------- entries --
