@@ -526,16 +526,18 @@ def test_logprobs_bwd_special_rows(lib):
         ids[0] = t.tensor([0, 3])
         ids[2] = -1
         ids[4, 1] = V
+        x[7] = -math.inf
+        ids[7, 0] = V                                    # a bad id in a row that is masked
         f = logprobs(lib, x, F32, 1.0, ids, 0)
         dlogp, dent = t.randn(N, 2, device="cuda"), t.randn(N, device="cuda")
         dent[2] = 0.0
         _, d = like_rows(x, F32)
         logprobs_bwd(lib, x, F32, 1.0, ids, f.lse2, f.entropy, dlogp, None, dent, d)
         assert bool((d[0] == 0).all()) and bool((d[2] == 0).all())
-        assert bool(t.isnan(d[1]).all()) and bool(t.isnan(d[4]).all())
+        assert bool(t.isnan(d[1]).all()) and bool(t.isnan(d[4]).all()) and bool(t.isnan(d[7]).all())
         part = ids[3, 0] >= V // 2
         assert bool((d[3, : V // 2][t.arange(V // 2, device="cuda") != ids[3, 0]][:100].isfinite()).all()) or part
-        assert bool(d[5:].isfinite().all())
+        assert bool(d[5:7].isfinite().all()) and bool(d[8:].isfinite().all())
 
 
 def test_logprobs_gradient_against_differences(lib):

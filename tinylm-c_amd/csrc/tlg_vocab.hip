@@ -455,12 +455,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
     // all lines up to the last round's are written
     int q = 0;
     if constexpr (LINES)
-        while (LP_LINES * 8 * W << q < j1 - j0 + 8 * U * W) q++;
+        while (LP_LINES * 8 * W << q < j1 - j0) q++;
     const Given given = lp_given<TYPE>(a, r, x.x, t);
     Acc A = ACC0;
     float v1 = -INFINITY;
-    float *to = LINES ? sh.max + (wave * 8 + lane / 8) * U : nullptr;
-    for (int j = j0 + t; RES || j - t < j1; to += U * 8 * W) {
+    for (int j = j0 + t, l = (wave * 8 + lane / 8) * U; RES || j - t < j1; l += U * 8 * W) {
         float lm[U];
 #pragma unroll
         for (int k = 0; k < U; k++) lm[k] = -INFINITY;
@@ -492,7 +491,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void k_logprobs(LpArgs a)
                 lm[k] = fmaxf(lm[k], lane_move<0x4E>(lm[k]));
                 lm[k] = fmaxf(lm[k], lane_move<0x141>(lm[k]));
             }
-            if (lane % 8 == 0) *(f32x4 *)to = f32x4{lm[0], lm[1], lm[2], lm[3]};
+            if (lane % 8 == 0) *(f32x4 *)(sh.max + l) = f32x4{lm[0], lm[1], lm[2], lm[3]};
         }
         if (RES) break;
     }
@@ -719,7 +718,7 @@ template <int TYPE> __global__ __launch_bounds__(256) void k_logprobs_bwd(LpBwdA
     for (int j = 0; j < a.M; j++) c0 -= sg[j];
     const float c1 = a.dent ? a.dent[r] : 0.f, H = a.dent ? a.entropy[r] : 0.f;
     const float m = a.lse2[2 * r], ls = a.lse2[2 * r + 1];
-    const bool empty = m == -INFINITY, zero = empty || (c0 == 0.f && c1 == 0.f);
+    const bool empty = m == -INFINITY && c0 == c0, zero = empty || (c0 == 0.f && c1 == 0.f);
     const float rs = a.scale * __expf(-ls), k1 = -0.69314718056f * c1, k0 = c0 - c1 * (H - ls);
     auto grad = [&](float v) -> float {
         const float e = (v - m) * a.c;

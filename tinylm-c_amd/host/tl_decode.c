@@ -518,7 +518,7 @@ int tl_decode_score(TlDecode *d, const int *tok, int n, float temp, float *logp,
                     float *top_logp, void *st)
 {
     if (!d || !tok || n <= 0 || n > d->maxpos || !logp || K < 0 || K > TLG_VOCAB_TOP || (K && (!top_ids || !top_logp)) ||
-        !(temp >= 1e-30f && temp <= 1e30f))
+        !(temp >= 1e-29f && temp <= 1e29f))
         return TLG_EINVAL;
     for (int j = 0; j < n; j++) if (tok[j] < 0 || tok[j] >= d->m.V) return TLG_EINVAL;
     const int V = d->m.V;
