@@ -863,6 +863,10 @@ template <int W> struct KdShared {
 // entries at all; the target among them; an id or target past V; a target
 enum { KD_ANY = 1, KD_HIT = 2, KD_BAD = 4, KD_CE = 8 };
 
+// Rounds before the last one that a row read twice keeps in registers between its
+// reads (4096 rows of 131072 in bf16: 468 us with none, 444 with 1, 436 with 2; a
+// third takes the kernel past 64 registers, 457).
+#define KD_HOLD 2
 enum { KD_WHOLE = 0, KD_SUMS = 1, KD_GRAD = 2 };
 // W waves on a row (PHASE KD_WHOLE) or on one of its S segments: KD_SUMS leaves
 // the segment's sums, KD_GRAD joins them and writes the segment.  RES: a thread's
@@ -1035,10 +1039,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
     constexpr bool EXP = RES && U * VE <= 32 * (VE == 4 ? 2 : 1);      // kept as exponentials, else as they came
     float ex[EXP ? U * VE : 1], ex1[EXP && TWO ? U * VE : 1];
     int jl = j0 + t;                                    // the last round's vector
+    // rounds before the last whose vectors stay, as far as registers reach
+    constexpr int HOLD = RES || PHASE != KD_WHOLE ? 0 : KD_HOLD;
+    u32x4 hold[HOLD ? HOLD : 1][U];
+    if constexpr (HOLD > 0)
+#pragma unroll
+        for (int h = 0; h < HOLD; h++)
+#pragma unroll
+            for (int k = 0; k < U; k++) hold[h][k] = raw[k];
     if constexpr (PHASE != KD_GRAD) {
         for (int j = j0 + t; RES ? j == j0 + t : j < j1; j += U * TPR) {
-            if (!RES && j != j0 + t) load(j, false);
-            jl = j;
+            if (!RES && j != j0 + t) {
+                if constexpr (HOLD > 0)
+#pragma unroll
+                    for (int k = 0; k < U; k++) {
+#pragma unroll
+                        for (int h = HOLD - 1; h > 0; h--) hold[h][k] = hold[h - 1][k];
+                        hold[0][k] = raw[k];
+                    }
+                load(j, false);
+            }
             if (a.tail)
 #pragma unroll
                 for (int k = 0; k < U; k++) {
@@ -1053,6 +1073,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
                                                             : (raw[k][e >> 1] & 0xffff0000u) | El<TYPE>::NEG;
                             }
                 }
+            if constexpr (HOLD > 0) jl = j;
             float m = A.m;
 #pragma unroll
             for (int k = 0; k < U; k++)
@@ -1120,10 +1141,19 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
         const bool zero = nothing || (empty && !bad_id);
         // of exponentials with a thread's own reference
         const float fk = kout * kd_exp(mine - A.m, c, a.c_lo), f1 = TWO ? k1 * kd_exp(mine - M, KD_C1, KD_C1_LO) : 0.f;
-        // backwards: the sums' last rounds are the likeliest to be in the caches still
+        // backwards: the sums' last rounds are here or the likeliest to be in the caches still
         if (PHASE == KD_GRAD) jl = j0 + t + (max(j1 - j0 - t, 1) - 1) / (U * TPR) * (U * TPR);
-        for (int j = jl; j >= j0; j -= U * TPR) {
-            if (!RES && !zero) load(j, true);
+        for (int j = jl, i = 0; j >= j0; j -= U * TPR, i++) {
+            if (!RES && !zero) {
+                if (!HOLD || i > HOLD) load(j, true);
+                else if (i > 0)
+#pragma unroll
+                    for (int k = 0; k < U; k++) {
+                        raw[k] = hold[0][k];
+#pragma unroll
+                        for (int h = 0; h + 1 < HOLD; h++) hold[h][k] = hold[h + 1][k];
+                    }
+            }
 #pragma unroll
             for (int k = 0; k < U; k++) {
                 float g[VE];
@@ -1377,8 +1407,8 @@ static int kd_segments(int type, int N, int V)
 // 19.7 us on one wave and 25.0 read twice by four, of 16384 101 against 120, of 65536
 // 404 against 465.  The longer 16-bit ones leave a workgroup no second one on its CU
 // to work while it waits (4096 rows of 131072: 516 us); they are read twice, by sixteen
-// waves, so that the rows in work (two on a CU) fit the last-level cache: 468 us, with
-// eight waves 502, with four 583.  Two exponentials need registers: eight waves then
+// waves, so that the rows in work (two on a CU) fit the last-level cache (468 us,
+// with eight waves 502, with four 583), the last rounds in registers: 436.  Two exponentials need registers: eight waves then
 // (527 against 551 us), and fp32 stays in registers up to 4096 vectors only (586 against
 // 463 us at 16384).  Beyond 8192 vectors a row in registers has a CU to itself, which
 // pays where the rows fill three quarters of their rounds over the 256 CUs (301 rows of
