@@ -693,6 +693,36 @@ def test_distill_every_launch(lib, ty, N, V, K, tail, tau, pad):
     assert bool(t.isnan(buf).all()), "wrote outside its rows"
 
 
+@pytest.mark.parametrize("ty,N,V,tau,pad", [
+    (F32, 20, 16388, 2.0, 0), (F32, 33, 24577, 1.0, 3), (F32, 35, 32771, 1.0, 0), (F32, 45, 41001, 2.0, 1),
+    (F32, 60, 57350, 1.0, 0), (F32, 130, 131077, 2.0, 0), (F32, 260, 262144, 1.0, 0),
+    (F16, 20, 20000, 2.0, 0), (BF16, 20, 32769, 1.0, 7), (F16, 21, 33001, 2.0, 1), (BF16, 22, 41001, 2.0, 0),
+    (BF16, 25, 49153, 1.0, 0), (F16, 40, 65530, 1.0, 5), (BF16, 44, 90001, 1.0, 0), (F16, 70, 131072, 1.0, 0),
+    (BF16, 140, 262147, 1.0, 1)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_rows_read_twice(lib, ty, N, V, tau, pad, tail):
+    """Every number of rounds: all of a row's kept in registers, the first ones in
+    LDS, the rest read again; the last round full, partly full or one vector."""
+    t = _t()
+    print("distill twice", NAMES[ty], N, V, tau, pad, tail, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, 1 if pad else 0))
+    ids, tl = teacher(x, 40, tau)
+    ids[:, 1] = V - 1                                    # an id in each row's last round
+    ids[:, 2] = t.arange(N, dtype=t.int32, device="cuda") * 257 % V
+    tgt = t.randint(0, V, (N,), generator=t.Generator().manual_seed(2), dtype=t.int32).cuda()
+    buf, d = like_rows(x, ty)
+    o = distill(lib, x, ty, ids, tl, tail, tau, 1.0, tgt, 0.5, d, 0.25)
+    pick = [0, 1, N // 2, N - 2, N - 1]
+    o.rows, dd = o.rows[pick], d[pick]
+    whole = o.loss.clone()
+    o.loss = o.rows.double().mean().float().reshape(1)
+    check_distill(o, dd, ty, x[pick], ids[pick], tl[pick], tail, tau, 1.0, tgt[pick], 0.5, 0.25)
+    o2 = distill(lib, x, ty, ids, tl, tail, tau, 1.0, tgt, 0.5, x, 0.25)          # in place
+    assert t.equal(x, d) and t.equal(o2.loss, whole)
+    t.as_strided(buf, tuple(d.shape), (d.stride(0), 1), d.storage_offset()).fill_(float("nan"))
+    assert bool(t.isnan(buf).all()), "wrote outside its rows"
+
+
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("N,V", [(12, 300), (12, 50003), (530, 2048), (2060, 1200)])
 def test_distill_special_rows(lib, tail, N, V):

@@ -782,7 +782,8 @@ struct KdArgs {
     float *rows;
     void *dlogits;
     long long ldd;
-    int words;                    // tail: 32-bit words of a row's (or segment's) bitmap
+    int words;                    // tail: 32-bit words of a row's (or segment's) bitmap, a multiple of 4
+    int keep;                     // first rounds of a row read twice that stay in LDS, behind the bitmap
     float *part;                  // S > 1: [N][S][4] sums, then [N][KD_XS] logits of ids and target
 };
 #define KD_XS (TLG_VOCAB_TOP + 1)
@@ -874,11 +875,12 @@ enum { KD_WHOLE = 0, KD_SUMS = 1, KD_GRAD = 2 };
 // the gradient; longer rows are read twice.  TWO: a cross-entropy at another
 // temperature than the teacher's.
 template <int TYPE, int W, int U, bool RES, bool TWO, int PHASE>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8) void k_distill(KdArgs a)
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES ? 4 : 8) void k_distill(KdArgs a)
 {
     constexpr int VE = El<TYPE>::VE, TPR = 64 * W;
     __shared__ KdShared<W> shared[W == 1 ? 4 : 1];
-    extern __shared__ unsigned all_bits[];              // tail: the support, a bit for each element
+    // tail: the support, a bit for each element; then the rounds kept
+    extern __shared__ __attribute__((aligned(16))) unsigned all_bits[];
     const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6, t = W == 1 ? lane : threadIdx.x;
     const int slot = W == 1 ? threadIdx.x >> 6 : 0;
     KdShared<W> &sh = shared[slot];
@@ -1038,7 +1040,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
     Kd A = KD0;
     constexpr bool EXP = RES && U * VE <= 32 * (VE == 4 ? 2 : 1);      // kept as exponentials, else as they came
     float ex[EXP ? U * VE : 1], ex1[EXP && TWO ? U * VE : 1];
-    int jl = j0 + t;                                    // the last round's vector
+    int jl = j0 + t, round = 0;                         // the last round's vector; rounds
+    u32x4 *kept = (u32x4 *)(all_bits + a.words);
     // rounds before the last whose vectors stay, as far as registers reach
     constexpr int HOLD = RES || PHASE != KD_WHOLE ? 0 : KD_HOLD;
     u32x4 hold[HOLD ? HOLD : 1][U];
@@ -1073,7 +1076,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
                                                             : (raw[k][e >> 1] & 0xffff0000u) | El<TYPE>::NEG;
                             }
                 }
-            if constexpr (HOLD > 0) jl = j;
+            if constexpr (HOLD > 0) {
+                jl = j;
+                if (round < a.keep)
+#pragma unroll
+                    for (int k = 0; k < U; k++) kept[(round * U + k) * TPR + t] = raw[k];
+                round++;
+            }
             float m = A.m;
 #pragma unroll
             for (int k = 0; k < U; k++)
@@ -1145,7 +1154,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES && U * W != 128 ? 4 : 8)
         if (PHASE == KD_GRAD) jl = j0 + t + (max(j1 - j0 - t, 1) - 1) / (U * TPR) * (U * TPR);
         for (int j = jl, i = 0; j >= j0; j -= U * TPR, i++) {
             if (!RES && !zero) {
-                if (!HOLD || i > HOLD) load(j, true);
+                if (HOLD && i > HOLD && round - 1 - i < a.keep)
+#pragma unroll
+                    for (int k = 0; k < U; k++) raw[k] = kept[((round - 1 - i) * U + k) * TPR + t];
+                else if (!HOLD || i > HOLD) load(j, true);
                 else if (i > 0)
 #pragma unroll
                     for (int k = 0; k < U; k++) {
@@ -1402,18 +1414,28 @@ static int kd_segments(int type, int N, int V)
     return (long long)N * 256 <= V / (type == TLG_F32 ? 4 : 8) ? vb_segments(type, N, V, 64) : 1;
 }
 
-// Rows of up to 16384 vectors of fp32 and 4096 of 16 bits stay in registers between
-// sums and gradient, on as few waves as hold them: 4096 rows of 2048 fp32 values take
-// 19.7 us on one wave and 25.0 read twice by four, of 16384 101 against 120, of 65536
-// 404 against 465.  The longer 16-bit ones leave a workgroup no second one on its CU
-// to work while it waits (4096 rows of 131072: 516 us); they are read twice, by sixteen
-// waves, so that the rows in work (two on a CU) fit the last-level cache (468 us,
-// with eight waves 502, with four 583), the last rounds in registers: 436.  Two exponentials need registers: eight waves then
-// (527 against 551 us), and fp32 stays in registers up to 4096 vectors only (586 against
-// 463 us at 16384).  Beyond 8192 vectors a row in registers has a CU to itself, which
-// pays where the rows fill three quarters of their rounds over the 256 CUs (301 rows of
-// 50021: 46.5 us in registers, 38.2 read twice).
-template <bool TWO> static void kd_launch(const KdArgs &a, int type, int nv, size_t lds, hipStream_t st)
+// The first rounds (of U vectors a thread) of a row read twice that fit a workgroup's
+// share of the LDS, 2048 threads on a CU of 160 KB, beside the bitmap and the shared rest
+// (4096 rows of 65536 fp32 values, two temperatures: 428 us without, 406; 301 rows of
+// 50021: 37.6, 35.9; of 65536 in bf16, where the caches hold them too, 221, 226).
+static int kd_keep(int threads, int U, size_t bits)
+{
+    static_assert(sizeof(KdShared<16>) <= 4096 && sizeof(KdShared<8>) <= 4096, "the shared rest");
+    const size_t share = 160 * 1024 / (2048 / threads), rest = bits + 4096;
+    return rest < share ? (int)((share - rest) / ((size_t)threads * U * 16)) : 0;
+}
+
+// Rows of up to 4096 vectors (of 2048, with 16-bit types and two temperatures) stay in
+// registers between sums and gradient, on as few waves as hold them: 4096 rows of 2048
+// fp32 values take 19.7 us on one wave and 25.0 read twice by four, of 16384 101 against
+// 110, of 32768 in bf16 107 against 131, but of 20000 in bf16 with two temperatures 115
+// against 104.  In longer ones a row's waves wait for each other with nothing else to
+// work on their CU (256 rows of 50021 fp32 values: 30.9 us, 26.5 read twice).  These
+// are read twice, by sixteen waves, so that the rows in work (two on a CU) fit the
+// last-level cache (4096 rows of 131072 in bf16: 468 us, with eight waves 502, with four
+// 583), the last rounds in registers (436) and the first in LDS (430).  With two
+// temperatures and 16-bit types eight waves are faster (501 against 521 us).
+template <bool TWO> static void kd_launch(KdArgs a, int type, int nv, size_t lds, hipStream_t st)
 {
     const unsigned rows = a.N;
     const bool f32 = type == TLG_F32;
@@ -1431,16 +1453,21 @@ template <bool TWO> static void kd_launch(const KdArgs &a, int type, int nv, siz
         BY_TYPE(rows, 256, lds, a, k_distill, , 4, 4, true, TWO, KD_WHOLE);
     else if (nv <= 2048)
         BY_TYPE(rows, 256, lds, a, k_distill, , 4, 8, true, TWO, KD_WHOLE);
-    else if (nv <= 4096)
-        BY_TYPE(rows, 512, lds, a, k_distill, , 8, 8, true, TWO, KD_WHOLE);
-    else if (nv <= 8192 && f32 && !TWO)
-        hipLaunchKernelGGL((k_distill<TLG_F32, 16, 8, true, false, KD_WHOLE>), dim3(rows), dim3(1024), lds, st, a);
-    else if (nv <= 16384 && f32 && !TWO && 4 * rows >= 3 * ((rows + 255) / 256 * 256))
-        hipLaunchKernelGGL((k_distill<TLG_F32, 16, 16, true, false, KD_WHOLE>), dim3(rows), dim3(1024), lds, st, a);
-    else if (TWO && !f32)
-        BY_16(rows, 512, lds, a, k_distill, , 8, 2, false, TWO, KD_WHOLE);
-    else
-        BY_TYPE(rows, 1024, lds, a, k_distill, , 16, 2, false, TWO, KD_WHOLE);
+    else if (nv <= 4096 && f32)
+        hipLaunchKernelGGL((k_distill<TLG_F32, 8, 8, true, TWO, KD_WHOLE>), dim3(rows), dim3(512), lds, st, a);
+    else if (nv <= 4096 && !TWO)
+        BY_16(rows, 512, lds, a, k_distill, , 8, 8, true, false, KD_WHOLE);
+    else if (TWO && !f32) {
+        a.keep = kd_keep(512, 2, lds);
+        BY_16(rows, 512, lds + a.keep * 16384, a, k_distill, , 8, 2, false, TWO, KD_WHOLE);
+    } else {
+        a.keep = kd_keep(1024, 2, lds);
+        if (f32)
+            hipLaunchKernelGGL((k_distill<TLG_F32, 16, 2, false, TWO, KD_WHOLE>), dim3(rows), dim3(1024),
+                               lds + a.keep * 32768, st, a);
+        else
+            BY_16(rows, 1024, lds + a.keep * 32768, a, k_distill, , 16, 2, false, false, KD_WHOLE);
+    }
 }
 
 extern "C" size_t tlg_distill_ws_bytes(int type, int N, int V)
@@ -1472,12 +1499,12 @@ extern "C" int tlg_dev_distill(const void *logits, int type, long long ld, int N
     float hi = f_of(c);                                  // below c, so that what is left is positive
     if ((double)hi >= c) hi = nextafterf(hi, 0.f);
     KdArgs a = {logits, ld, N, V, S, K, tail ? 1 : 0, temp, w_kd, w_ce, scale, hi, f_of(c - (double)hi),
-                1.0 / (double)temp, w_ce != 0.f && temp != 1.f, t_ids, t_logp, tgt, rows, dlogits, ldd, 0,
+                1.0 / (double)temp, w_ce != 0.f && temp != 1.f, t_ids, t_logp, tgt, rows, dlogits, ldd, 0, 0,
                 (float *)ws};
     hipStream_t st = ST(stream);
     // a segment is a multiple of 256 vectors, see the kernel
     const int per = S > 1 ? ((nv + S - 1) / S + 255) / 256 * 256 : nv;
-    a.words = tail ? (per * ve + 31) / 32 : 0;
+    a.words = tail ? ((per * ve + 31) / 32 + 3) & ~3 : 0;
     const size_t lds = (size_t)a.words * 4;
     if (a.two) kd_launch<true>(a, type, nv, lds, st);
     else kd_launch<false>(a, type, nv, lds, st);
