@@ -256,6 +256,7 @@ int tl_train_set_teacher(TlTrain *t, const int *ids, const float *logp, int K, i
         t->kd_bytes = bytes;
     }
     if (!same && (K || t->kd.K) && t->graph) {       /* the captured step is stale */
+        CK(tlg_stream_sync(st));
         tlg_graph_destroy(t->graph);
         t->graph = NULL;
     }
