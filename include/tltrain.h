@@ -146,7 +146,8 @@ int tlg_dev_xent_rows(const float *logits, const int *tgt, float *dlogits, doubl
  * output is rounded once.  Only the caller's buffers are used: calls may
  * overlap on any streams as long as their outputs and workspaces differ, and
  * any call can be captured into a graph (after tlg_init).  Equal calls give
- * equal bits; the number of rows may change the order of a row's fp32 sums.
+ * equal bits; the number of rows, and where a row lies on the grid of 16 bytes,
+ * may change the order of its fp32 sums.
  *
  * A logit of -inf is a masked token (probability 0).  A row of nothing but
  * -inf has no distribution: its log probabilities are -inf, its entropy 0, its
