@@ -540,6 +540,42 @@ def test_logprobs_bwd_special_rows(lib):
         assert bool(d[5:7].isfinite().all()) and bool(d[8:].isfinite().all())
 
 
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V", [(8, 300), (8, 70001), (600, 2048)])
+@pytest.mark.parametrize("how", ["pair", "lse", "same token"])
+def test_logprobs_bwd_coefficients_that_cancel(lib, ty, N, V, how):
+    """Coefficients that cancel in their sum are no padding: the gradient of a
+    finite row is theirs at the given tokens alone, that of a NaN or +inf row NaN."""
+    t = _t()
+    print("cancel", NAMES[ty], N, V, how, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V))
+    x[1, 5], x[2, 7], x[4] = math.nan, math.inf, math.nan
+    x[3] = -math.inf
+    x[5, 9] = math.nan
+    ids = t.tensor([[11, V - 2]], dtype=t.int32, device="cuda").repeat(N, 1)
+    dlogp = t.tensor([[0.75, -0.75]], device="cuda").repeat(N, 1)
+    dlse = None
+    if how == "lse":
+        dlogp[:, 1] = 0.5
+        dlse = dlogp.sum(1)                              # 1.25: exact
+        dlse[4] = 0.0
+    elif how == "same token":
+        ids[:, 1] = ids[:, 0]
+    ids[4] = -1                                          # a padded row over NaN
+    dlogp[5] = 0.0                                       # one whose coefficients are all 0
+    if dlse is not None:
+        dlse[5] = 0.0
+    f = logprobs(lib, x, ty, 1.0, ids, 0)
+    _, d = like_rows(x, ty)
+    logprobs_bwd(lib, x, ty, 1.0, ids, f.lse2, None, dlogp, dlse, None, d)
+    assert bool(t.isnan(d[1]).all()) and bool(t.isnan(d[2]).all()), "a NaN row"
+    assert not bool(d[3:6].any()), "a masked row, a padded one and one without coefficients"
+    want = t.zeros(N, V, device="cuda")
+    want.scatter_add_(1, ids.clamp(min=0).long(), dlogp)
+    good = [0] + list(range(6, N))
+    assert t.equal(d[good].float(), want[good])          # 0.75 and 0.5 are exact in every type
+
+
 def test_logprobs_gradient_against_differences(lib):
     """Directional central differences of the kernel's own forward."""
     t = _t()

@@ -722,10 +722,15 @@ template <int TYPE> __global__ __launch_bounds__(256) void k_logprobs_bwd(LpBwdA
     }
     __syncthreads();
     float c0 = a.dlse ? a.dlse[r] : 0.f;
-    for (int j = 0; j < a.M; j++) c0 -= sg[j];
+    bool some = c0 != 0.f;                               // any coefficient: those that cancel are no padding
+    for (int j = 0; j < a.M; j++) {
+        c0 -= sg[j];
+        some |= sg[j] != 0.f;
+    }
     const float c1 = a.dent ? a.dent[r] : 0.f, H = a.dent ? a.entropy[r] : 0.f;
     const float m = a.lse2[2 * r], ls = a.lse2[2 * r + 1];
-    const bool empty = m == -INFINITY && c0 == c0, zero = empty || (c0 == 0.f && c1 == 0.f);
+    const bool empty = m == -INFINITY && c0 == c0;
+    const bool zero = empty || (c0 == 0.f && c1 == 0.f && !(some && ls != ls));
     const float rs = a.scale * __expf(-ls), k1 = -0.69314718056f * c1, k0 = c0 - c1 * (H - ls);
     auto grad = [&](float v) -> float {
         const float e = (v - m) * a.c;
