@@ -199,8 +199,12 @@ int tlg_dev_logprobs_bwd(const void *logits, int type, long long ld, int N, int 
  * cross-entropy, loss and gradient in one call (as tlg_dev_xent is for the
  * latter alone).  The teacher gives row n K tokens t_ids[n][] and their log
  * probabilities t_logp[n][] at temperature temp, as tlg_dev_logprobs(scale =
- * 1 / temp) writes them; a negative id is no entry, an id given twice counts at
- * its first place.  With S the row's ids, p = softmax(x / temp):
+ * 1 / temp) writes them; a negative id is no entry (whatever its log
+ * probability), an id given twice counts at its first place.  An entry whose log
+ * probability is NaN or +inf makes its row's results NaN; a row of NaN logits
+ * comes from tlg_dev_logprobs without ids and is a row without an entry here, so
+ * a teacher's own lse2 or entropy has to be looked at for those.  With S the
+ * row's ids, p = softmax(x / temp):
  *   rows[n] = w_kd temp^2 KL_n + w_ce CE_n,  CE_n = -log softmax(x)[tgt[n]]
  *   tail 0: q = the entries' e^t_logp normalised to sum 1,
  *           KL = sum_{k in S} q_k (log q_k - log p_k)

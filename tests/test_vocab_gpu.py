@@ -800,6 +800,36 @@ def test_distill_special_rows(lib, tail, N, V):
     check_distill(o, dd, F32, sub, ids[good], tl[good], tail, 1.0, 1.0, tgt[good], 0.5, 1.0)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("N,V,w_kd,w_ce", [(9, 300, 1.0, 0.5), (9, 300, 0.0, 0.5), (9, 70000, 1.0, 0.5), (300, 50003, 1.0, 0.0),
+                                           (530, 2048, 1.0, 0.5), (2060, 1200, 1.0, 0.5)])
+def test_distill_broken_teachers(lib, tail, N, V, w_kd, w_ce):
+    """An entry whose log probability is NaN or +inf makes its row's loss and
+    gradient NaN, whatever stands beside it; beside a negative id, or at an id's
+    second place, it is no entry."""
+    t = _t()
+    print("broken teacher", tail, N, V, w_kd, w_ce, flush=True)
+    _, x = on_gpu(rows_of(F32, N, V))
+    K = 70
+    ids, tl = teacher(x, K, 2.0)
+    ids[3, 4], ids[4, 9], ids[5] = -1, ids[4, 2], -1
+    tgt = t.randint(0, V, (N,), generator=t.Generator().manual_seed(2), dtype=t.int32).cuda()
+    _, d0 = like_rows(x, F32)
+    clean = distill(lib, x, F32, ids, tl, tail, 2.0, w_kd, tgt, w_ce, d0)
+    assert bool(clean.rows.isfinite().all()) and bool(d0.isfinite().all())
+    tl = tl.clone()
+    tl[0] = math.nan                                     # every entry
+    tl[1, 3] = math.nan                                  # one of many
+    tl[2, 66] = math.inf
+    tl[3, 4] = tl[4, 9] = math.nan                       # no entries
+    tl[5] = math.nan
+    _, d = like_rows(x, F32)
+    o = distill(lib, x, F32, ids, tl, tail, 2.0, w_kd, tgt, w_ce, d)
+    assert np.isnan(f64(o.rows[:3])).all() and np.isnan(f64(o.loss)).all()
+    assert bool(t.isnan(d[:3]).all())
+    assert t.equal(o.rows[3:], clean.rows[3:]) and t.equal(d[3:], d0[3:])
+
+
 def test_distill_largest_vocabulary_in_one_piece(lib):
     """Rows of 2^20 columns that are not cut: the largest bitmap of the ids."""
     t = _t()

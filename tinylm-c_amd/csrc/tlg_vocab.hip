@@ -873,7 +873,8 @@ template <int W> struct KdShared {
         unsigned seen[KD_HASH];
     };
 };
-// entries at all; the target among them; an id or target past V; a target
+// entries at all; the target among them; an id or target past V, an entry of NaN
+// or +inf (which a maximum would not show); a target
 enum { KD_ANY = 1, KD_HIT = 2, KD_BAD = 4, KD_CE = 8 };
 
 // Rounds before the last one that a row read twice keeps in registers between its
@@ -979,6 +980,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES ? 4 : 8) void k_distill(
         }
         const int some = __popcll(__ballot(id[0] >= 0)) + __popcll(__ballot(id[1] >= 0));
         if (some) flags |= KD_ANY;
+        if (__ballot((id[0] >= 0 && !(tl[0] < INFINITY)) || (id[1] >= 0 && !(tl[1] < INFINITY)))) flags |= KD_BAD;
         row_sync<1>();
         if constexpr (PHASE == KD_SUMS) {
             if (seg == 0) {
