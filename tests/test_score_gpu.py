@@ -224,3 +224,42 @@ def test_set_teacher_refuses(host, lib, stream):
     tr.set_teacher(ids, lp, stream, w_ce=1.0)
     tr.step(stream)
     assert math.isfinite(tr.loss(stream))
+
+
+def test_broken_teachers_are_refused(host, lib, stream):
+    """Log probabilities of NaN or +inf never train: set_teacher refuses them at
+    entries, and rows as a decoder with NaN weights scores them; the teacher that
+    was there stays.  Padding may hold anything else."""
+    import tlgemm
+    tr, tok, tgt, start = train_state(host, lib, stream)
+    ids, lp = np.zeros((tr.N, 3), np.int32), np.full((tr.N, 3), -1.5)
+    ids[:, 1], ids[:, 2] = 1, 2
+    tr.set_teacher(ids, lp, stream)
+    tr.step(stream)
+    loss = tr.loss(stream)
+    for v in (math.nan, math.inf):
+        bad = lp.copy()
+        bad[7, 2] = v
+        with pytest.raises(tlgemm.TlgError):
+            tr.set_teacher(ids, bad, stream)
+    P = weights(KW, 11)
+    P[5 * KW["D"]] = math.nan                            # token 5's embedding: every row's logits
+    broken = host.decode(KW, KW["T"], kv_f16=0, exact_exp=1, maxpos=256)
+    broken.upload(P, stream)
+    got = [broken.score(s, stream, K=3) for s in tok.reshape(-1, KW["T"])]
+    bids, blp = np.concatenate([g[2] for g in got]), np.concatenate([g[3] for g in got])
+    assert (bids == -1).all() and np.isnan(blp).all()
+    with pytest.raises(tlgemm.TlgError):
+        tr.set_teacher(bids, blp, stream)
+    one = np.where(np.arange(tr.N)[:, None] == 3, bids, ids), np.where(np.arange(tr.N)[:, None] == 3, blp, lp)
+    with pytest.raises(tlgemm.TlgError):
+        tr.set_teacher(one[0], one[1], stream)
+    start()
+    tr.step(stream)
+    assert tr.loss(stream) == loss
+    ids[3], lp[3, 0], lp[3, 1:] = -1, -math.inf, math.nan                # padding
+    ids[4, 2], lp[4, 2] = -1, math.nan
+    tr.set_teacher(ids, lp, stream)
+    start()
+    tr.step(stream)
+    assert math.isfinite(tr.loss(stream))

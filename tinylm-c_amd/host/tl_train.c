@@ -241,8 +241,14 @@ int tl_train_set_teacher(TlTrain *t, const int *ids, const float *logp, int K, i
         !isfinite(w_kd) || !isfinite(w_ce))
         return TLG_EINVAL;
     const size_t N = t->N, n = N * (size_t)K, pad = 255;
-    for (size_t i = 0; i < n; i++)
-        if (ids[i] >= t->m.V) return TLG_EINVAL;
+    for (size_t r = 0; r < N; r++) {
+        int broken = K > 0;                          /* a row as a decoder scores NaN logits */
+        for (size_t i = r * K; i < (r + 1) * K; i++) {
+            if (ids[i] >= t->m.V || (ids[i] >= 0 && !(logp[i] < INFINITY))) return TLG_EINVAL;
+            if (ids[i] >= 0 || !isnan(logp[i])) broken = 0;
+        }
+        if (broken) return TLG_EINVAL;
+    }
     const size_t b_ids = (4 * n + pad) & ~pad, b_rows = (4 * N + pad) & ~pad,
                  b_ws = K ? tlg_distill_ws_bytes(TLG_F32, t->N, t->m.V) : 0, bytes = 2 * b_ids + b_rows + b_ws;
     const int same = K == t->kd.K && !!tail == t->kd.tail && temp == t->kd.temp && w_kd == t->kd.w_kd &&

@@ -57,9 +57,12 @@ int  tl_train_set_batch(TlTrain *t, const int *tok, const int *tgt, const int *t
  * (tinylm.c:1019-1028, :1076-1082); MTP heads keep theirs.  ids and logp are host
  * arrays [N][K] (K <= TLG_VOCAB_TOP) of each row's teacher tokens and their log
  * probabilities at temperature temp, as tl_decode_score gives them; a negative
- * id is no entry, one from V on is refused.  K = 0 goes back to the
- * cross-entropy (ids and logp may be NULL).  A captured step stays valid while
- * only the arrays' contents change, and is dropped otherwise. */
+ * id is no entry, one from V on is refused.  So is a broken teacher: an entry
+ * whose log probability is NaN or +inf, or a row of nothing but negative ids
+ * and NaN, which is what tl_decode_score gives for NaN logits (padding may hold
+ * anything else).  What is refused leaves the teacher as it was.  K = 0 goes
+ * back to the cross-entropy (ids and logp may be NULL).  A captured step stays
+ * valid while only the arrays' contents change, and is dropped otherwise. */
 int  tl_train_set_teacher(TlTrain *t, const int *ids, const float *logp, int K, int tail, float temp, float w_kd,
                           float w_ce, void *stream);
 /* AdamW hyper-parameters for step `step` (1-based, adamw's t): copied to the
