@@ -83,6 +83,44 @@ def test_score(host, stream, cut, opt):
     assert np.abs(lp2 - lp).max() <= 2 * tol
 
 
+@pytest.mark.parametrize("opt", [dict(), dict(n_exp=2), dict(unfused=1)], ids=str)
+@pytest.mark.parametrize("n", [1, 7, 16, 40, 64, 90])
+def test_score_leaves_the_greedy_state(host, stream, n, opt):
+    """Greedy decoding goes on after a score of the same text as if there had been
+    none, eagerly and from a step captured before it: the next position and
+    the token chosen for it are kept."""
+    opt = dict(opt)
+    unfused = opt.pop("unfused", 0)
+    kw = dict(KW, **opt)
+    tok = np.random.default_rng(n).integers(0, KW["V"], n).astype(np.int32)
+    a, b = (host.decode(kw, 64, kv_f16=0, exact_exp=1, maxpos=256, mmax=8, pool=1) for _ in range(2))
+    for d in (a, b):
+        if unfused:
+            d.set_fused(0)
+        d.upload(weights(kw, 3), stream)
+        d.prime(tok, stream)
+    b.graph_build(stream)
+    before = list(a.state(stream))
+    assert list(b.state(stream)) == before
+    for d in (a, b):
+        d.score(tok, stream, K=3)
+        assert list(d.state(stream)) == before
+    want = host.decode(kw, 64, kv_f16=0, exact_exp=1, maxpos=256, mmax=8, pool=1)
+    if unfused:
+        want.set_fused(0)
+    want.upload(weights(kw, 3), stream)
+    want.prime(tok, stream)
+    for _ in range(3):
+        a.greedy_step(stream)
+        b.graph_step(stream)
+        want.greedy_step(stream)
+        z = want.logits(1, stream)
+        for d in (a, b):
+            assert list(d.state(stream)) == list(want.state(stream))
+            # the ring holds the same text, by passes whose sums differ in their order
+            assert np.abs(d.logits(1, stream) - z).max() <= 1e-5 * np.abs(z).mean()
+
+
 def test_score_refuses(host, stream):
     import tlgemm
     d = host.decode(KW, 64, maxpos=128)

@@ -532,7 +532,7 @@ int tl_decode_score(TlDecode *d, const int *tok, int n, float temp, float *logp,
         const size_t b = tlg_logprobs_ws_bytes(TLG_F32, m, V, K);
         if (b > ws_b) ws_b = b;
     }
-    const size_t bytes = 3 * b1 + 2 * bk + bl + ws_b;
+    const size_t bt = (4 * (size_t)d->mmax + pad) & ~pad, bytes = 3 * b1 + 2 * bk + bl + bt + ws_b;
     if (bytes > d->score_bytes) {
         CK(tlg_stream_sync(st));
         void *mem = tlg_dev_malloc(bytes);
@@ -545,23 +545,32 @@ int tl_decode_score(TlDecode *d, const int *tok, int n, float temp, float *logp,
     int *next = (int *)p, *ti = (int *)(p + 3 * b1);
     float *lp = (float *)(p + b1), *en = (float *)(p + 2 * b1), *tl = (float *)(p + 3 * b1 + bk),
           *all = (float *)(p + 3 * b1 + 2 * bk);
-    void *ws = p + 3 * b1 + 2 * bk + bl;
+    void *held = p + 3 * b1 + 2 * bk + bl, *ws = p + 3 * b1 + 2 * bk + bl + bt;
     const int none = -1;
     if (n > 1) CK(tlg_memcpy_h2d(next, tok + 1, 4 * (size_t)(n - 1), st));
     CK(tlg_memcpy_h2d(next + n - 1, &none, 4, st));
+    /* the greedy state's token lies where chunks put theirs */
+    CK(tlg_memcpy_d2d(held, d->tok, 4 * (size_t)d->mmax, st));
     CK(tlg_stream_sync(st));
-    for (int i = 0, m; i < n; i += m) {
+    int rc = 0;
+    for (int i = 0, m; !rc && i < n; i += m) {
         const float *rows = d->logits;
         if (i < bulk) {
             m = bulk - i < piece ? bulk - i : piece;
-            CK(run_bulk(d, tok + i, m, i, 0, all, st));
+            rc = run_bulk(d, tok + i, m, i, 0, all, st);
             rows = all;
         } else {
             m = n - i < d->mmax ? n - i : d->mmax;
-            CK(tl_decode_chunk(d, tok + i, m, i, st));
+            rc = tl_decode_chunk(d, tok + i, m, i, st);
         }
-        CK(tlg_dev_logprobs(rows, TLG_F32, V, m, V, 1.0f / temp, next + i, 1, lp + i, NULL, entropy ? en + i : NULL, K,
-                            ti + (size_t)i * K, tl + (size_t)i * K, ws, ws_b, st));
+        if (!rc)
+            rc = tlg_dev_logprobs(rows, TLG_F32, V, m, V, 1.0f / temp, next + i, 1, lp + i, NULL, entropy ? en + i : NULL,
+                                  K, ti + (size_t)i * K, tl + (size_t)i * K, ws, ws_b, st);
+    }
+    CK(tlg_memcpy_d2d(d->tok, held, 4 * (size_t)d->mmax, st));
+    if (rc) {
+        tlg_stream_sync(st);                         /* copies from the caller's text */
+        return rc;
     }
     CK(tlg_memcpy_d2h(logp, lp, 4 * (size_t)n, st));
     if (entropy) CK(tlg_memcpy_d2h(entropy, en, 4 * (size_t)n, st));

@@ -71,8 +71,9 @@ int tl_decode_prime(TlDecode *d, const int *prompt, int n, void *stream);
  * row), entropy[i] (if not NULL) and the K <= TLG_VOCAB_TOP likeliest tokens
  * top_ids[i][] with top_logp[i][] (tlg_dev_logprobs, include/tltrain.h; host arrays).
  * top_ids and top_logp are what tl_train_set_teacher takes.  Synchronous; the
- * ring then holds the text, the greedy state is left alone, and what
- * tl_decode_mtp_draft reads is undefined.  Weights copy 0. */
+ * ring then holds the text, the greedy state (position and token) is left
+ * alone, and tl_decode_logits and what tl_decode_mtp_draft reads are undefined.
+ * Weights copy 0. */
 int tl_decode_score(TlDecode *d, const int *tok, int n, float temp, float *logp, float *entropy, int K, int *top_ids,
                     float *top_logp, void *stream);
 /* One greedy token step from the device state (weights copy `copy`). */
