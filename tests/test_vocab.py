@@ -96,3 +96,19 @@ def test_workspace_is_needed_and_checked(L, type):
         for V in (1, 100, 2048, 50021, 131072, 1 << 20):
             assert 0 <= L.tlg_logprobs_ws_bytes(type, N, V, 128) <= 16 << 20
             assert 0 <= L.tlg_distill_ws_bytes(type, N, V) <= 16 << 20
+
+
+@pytest.mark.parametrize("ids,logp", [((5, 3), (4, 3)), ((5, 3), (4, 2)), ((4, 3), (4, 4)), ((4,), (4,)), ((3, 3), (3, 3))])
+def test_teachers_of_another_shape_are_refused(ids, logp):
+    """Before the arrays reach the library, with or without assertions (-O)."""
+    from types import SimpleNamespace as NS
+
+    import numpy as np
+    tr = object.__new__(tlgemm.Train)
+    tr.N, tr.h = 4, None
+
+    def call(*args):
+        raise RuntimeError("read past an array")
+    tr.host = NS(dll=NS(tl_train_set_teacher=call))
+    with pytest.raises(ValueError):
+        tr.set_teacher(np.zeros(ids, np.int32), np.zeros(logp, np.float32), None)

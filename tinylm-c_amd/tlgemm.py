@@ -396,7 +396,8 @@ class Train:
         if ids is None:
             return self._ck(fn(self.h, None, None, 0, 0, 1.0, 0.0, 0.0, stream), "tl_train_set_teacher")
         ids, logp = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(logp, np.float32)
-        assert ids.shape == logp.shape and ids.ndim == 2 and ids.shape[0] == self.N
+        if ids.ndim != 2 or ids.shape != logp.shape or ids.shape[0] != self.N:
+            raise ValueError(f"ids {ids.shape} and logp {logp.shape} must be [{self.N}][K]")
         return self._ck(fn(self.h, ids.ctypes.data, logp.ctypes.data, ids.shape[1], int(tail), temp, w_kd, w_ce, stream),
                         "tl_train_set_teacher")
 
