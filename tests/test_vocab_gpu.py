@@ -428,6 +428,46 @@ def test_large_finite_masks_and_values(lib, N, V):
             close(f64(d), grad, (half_step(ty) * 1.01 + 8 * EPS) * np.abs(grad) + 2 * rho(V) + 200 * EPS, "dlogits")
 
 
+@pytest.mark.parametrize("ty", [F32, BF16])
+@pytest.mark.parametrize("N,V", [(3, 40), (5, 300), (2, 70001), (1030, 1000)])
+def test_differences_beyond_the_type(lib, ty, N, V):
+    """Logits farther apart than fp32 reaches: scaled, their log probabilities
+    and a weighted loss are ordinary numbers."""
+    t = _t()
+    print("beyond", NAMES[ty], N, V, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V))
+    x[0, 3], x[0, 7:20], x[0, 30] = 3e38, -3e38, -math.inf
+    x[1, V - 1], x[1, 5] = 2e38, -2.5e38
+    ids = some_ids(N, V, 3, 1, none=False)
+    ids[:2, 0], ids[:2, 1], ids[0, 2] = 7, 5, 30
+    K = 40 if N > 1000 else 128
+    for scale in (float(np.float32(1e-30)), 0.25):
+        check_logprobs(logprobs(lib, x, ty, scale, ids, K), x, scale, ids, K)
+    X = f64(x)
+    tids = t.tensor([[3, 7, 9]], dtype=t.int32, device="cuda").repeat(N, 1)
+    tids[1, 1] = 5
+    tl = t.full((N, 3), math.log(0.25), device="cuda")
+    tgt = tids[:, 1].contiguous()
+    for tail in (False, True):
+        o = distill(lib, x, ty, tids, tl, tail, 1.0, 1e-6, tgt, 1e-6, None)
+        # q is 1/4 each, and 1/4 remains, or 1/3 each; log p_r in the logarithms' domain (e^-3e38 is 0)
+        lp, I = ref_logp(X, 1.0)[0], tids.cpu().numpy().astype(np.int64)
+        q = math.exp(float(tl[0, 0])) if tail else 1.0 / 3.0
+        qr = 1.0 - 3.0 * q if tail else 0.0
+        rest = lp.copy()
+        np.put_along_axis(rest, I, -np.inf, 1)
+        top = rest.max(1)
+        with np.errstate(divide="ignore"):
+            lpr = top + np.log(np.exp(rest - top[:, None]).sum(1))
+        kl = (q * (math.log(q) - np.take_along_axis(lp, I, 1))).sum(1)
+        if tail:
+            kl += qr * (math.log(qr) - lpr)
+        rows = 1e-6 * (kl - lp[np.arange(N), I[:, 1]])
+        # weights as rounded to fp32, the remainder's parts and the last rounding: a half step
+        # each; ordinary rows as elsewhere
+        close(f64(o.rows), rows, 6 * EPS * np.abs(rows) + 1e-6 * (6 * rho(V) + 12 * EPS * 60), "rows")
+
+
 def test_extreme_temperatures(lib):
     """Almost greedy and almost uniform distributions."""
     _, x = on_gpu(rows_of(F32, 5, 3000))

@@ -392,10 +392,17 @@ template <int TYPE> __device__ __forceinline__ Given lp_given(const LpArgs &a, s
     }
     return g;
 }
+// scale (x - m); halves where the difference of finite values passes fp32 and
+// its product need not
+__device__ __forceinline__ float lp_scaled(float x, float m, float scale)
+{
+    const float d = x - m;
+    return d > -INFINITY || x == -INFINITY ? d * scale : (0.5f * x - 0.5f * m) * scale * 2.f;
+}
 __device__ __forceinline__ void lp_finish(const LpArgs &a, size_t r, const Given &g, const Sums &s, int t)
 {
     if (t < a.M) {
-        float o = (g.x - s.m) * a.scale - s.ls;
+        float o = lp_scaled(g.x, s.m, a.scale) - s.ls;
         if (s.m == -INFINITY) o = -INFINITY;
         a.logp[r * a.M + t] = g.id >= a.V ? NAN : g.id < 0 ? 0.f : o;
     }
@@ -412,7 +419,7 @@ __device__ __forceinline__ void lp_put(const LpArgs &a, size_t r, int k, u64 key
 {
     const bool bad = s.ls != s.ls;
     a.top_ids[r * a.K + k] = key && !bad ? (int)~(unsigned)key - sh : -1;
-    a.top_logp[r * a.K + k] = bad ? NAN : key ? (vb_key_value(key) - s.m) * a.scale - s.ls : -INFINITY;
+    a.top_logp[r * a.K + k] = bad ? NAN : key ? lp_scaled(vb_key_value(key), s.m, a.scale) - s.ls : -INFINITY;
 }
 
 // W waves on a row, or on one of its S segments (W > 1); 4 rows of one wave per
@@ -1225,14 +1232,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, RES ? 4 : 8) void k_distill(
     for (int k = lane; k < a.K; k += 64) {
         const double q = sh.q[k];
         if (q > 0.0 || q != q)
-            kl += empty ? INFINITY : q * (((double)sh.l[k] - lq) - ((double)(sh.x[k] - M) * a.inv - ls));
+            kl += empty ? INFINITY : q * (((double)sh.l[k] - lq) - (((double)sh.x[k] - M) * a.inv - ls));
     }
     kl = wave_sum64(kl);
     if (lane != 0) return;
-    if (sh.qr > 0.0) kl += empty ? INFINITY : sh.qr * (lr - ((double)(A.m - M) * a.inv + lo - ls));
+    if (sh.qr > 0.0) kl += empty ? INFINITY : sh.qr * (lr - (((double)A.m - M) * a.inv + lo - ls));
     double L = 0.0;
     if (any && a.w_kd != 0.f) L = (double)a.w_kd * a.tau * a.tau * kl;
-    if (ce) L += (double)a.w_ce * (empty ? INFINITY : ls1 - (double)(sh.xt - M));
+    if (ce) L += (double)a.w_ce * (empty ? INFINITY : ls1 - ((double)sh.xt - M));
     if (s != s) L = NAN;
     a.rows[r] = bad_id ? NAN : nothing ? 0.f : (float)L;
 }
