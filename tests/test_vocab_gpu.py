@@ -943,6 +943,43 @@ def test_log_sums_lean_to_neither_side(lib, ty, N, V):
     assert abs(float(err.mean())) <= 5 * 2e-7 / math.sqrt(N) + 5e-9, float(err.mean())
 
 
+@pytest.mark.parametrize("scale", [1.0, 0.9, 1.0 / 0.7])
+@pytest.mark.parametrize("ty,N,V", [(F32, 16384, 2048), (BF16, 8192, 30000), (BF16, 2048, 131072), (F32, 256, 1 << 20)])
+def test_log_probabilities_lean_to_neither_side(lib, ty, N, V, scale):
+    """The mean signed error of log S: its constant, which k_logprobs puts right
+    through the entropy sum, and the many small terms of long rows.  Against the fp32 logarithm of the exact S, so that what the
+    logarithm's own last bit leans by does not count: a row's error is random
+    with a deviation below 6e-7 (two roundings of a number below 16), the mean's
+    below that / sqrt(N); the hardware exponential leans by 3.5e-9 (measured).
+    One rounding is not random: s + kappa u, where s is a fp32 number and kappa u
+    (-5.5e-8 s at scale 1) less than a step of it, 2^-24 s to 2^-23 s: it always
+    vanishes or always counts a whole step, depending on s, and is off by half a
+    step at most, 2^-24 of s, in one direction.  (Without kappa the mean is off by
+    1.7e-7 at scale 0.9; summed an element at a time, by 1.1e-7, 5e-7 and 4e-6 at
+    scale 1 / 0.7 in rows of 30000, 131072 and 2^20.)"""
+    t = _t()
+    x = (2.5 * t.randn(N, V, device="cuda", generator=t.Generator("cuda").manual_seed(V))).to(dtype(ty))
+    s = float(np.float32(scale))
+    o = logprobs(lib, x, ty, s, None, 0)
+    S = t.cat([t.exp((z - z.amax(1, keepdim=True)) * s).sum(1) for z in (c.double() for c in x.split(512))])
+    err = o.lse2[:, 1].double() - t.log(S.float()).double()
+    print("lean", NAMES[ty], N, V, scale, float(err.mean()), float(err.std()), flush=True)
+    assert abs(float(err.mean())) <= 5 * 6e-7 / math.sqrt(N) + 5e-9 + EPS, float(err.mean())
+
+
+@pytest.mark.parametrize("ty,N,V", [(BF16, 2048, 30000), (BF16, 2048, 131072), (F32, 520, 1 << 20)])
+def test_log_sums_of_long_rows_lean_to_neither_side(lib, ty, N, V):
+    """As test_log_sums_lean_to_neither_side, for rows whose sums are made of few
+    large and very many small terms."""
+    t = _t()
+    x = (2.5 / 0.7 * t.randn(N, V, device="cuda", generator=t.Generator("cuda").manual_seed(V))).to(dtype(ty))
+    o = distill(lib, x, ty, None, None, False, 1.0, 1.0, x.argmax(1).int(), 1.0, None)
+    S = t.cat([t.exp(z - z.amax(1, keepdim=True)).sum(1) for z in (c.double() for c in x.split(256))])
+    err = o.rows.double() - t.log(S)
+    print("lean", NAMES[ty], N, V, float(err.mean()), float(err.std()), flush=True)
+    assert abs(float(err.mean())) <= 5 * 2e-7 / math.sqrt(N) + 5e-9, float(err.mean())
+
+
 # ------------------------------------------------- graphs, streams, repeats --
 @pytest.mark.parametrize("N,V", [(2, 60000), (40, 2048), (600, 3001)])
 def test_same_bits_every_time(lib, N, V):
