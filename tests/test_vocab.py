@@ -112,3 +112,17 @@ def test_teachers_of_another_shape_are_refused(ids, logp):
     tr.host = NS(dll=NS(tl_train_set_teacher=call))
     with pytest.raises(ValueError):
         tr.set_teacher(np.zeros(ids, np.int32), np.zeros(logp, np.float32), None)
+
+
+@pytest.mark.parametrize("type", [F32, F16, BF16])
+def test_cut_rows_need_their_workspace(L, type):
+    """One row of 131072 columns is cut for every type and both operators, and
+    refused without the workspace or with a smaller or unaligned one."""
+    V = 131072
+    need = L.tlg_logprobs_ws_bytes(type, 1, V, 20)
+    assert need > 0 and L.tlg_distill_ws_bytes(type, 1, V) > 0
+    for bad in (dict(ws_bytes=need - 1), dict(ws_bytes=need, ws=None), dict(ws_bytes=need, ws=P + 8)):
+        refused(L, lp(L, type=type, N=1, V=V, ld=V, K=20, **bad), "logprobs: workspace")
+    need = L.tlg_distill_ws_bytes(type, 1, V)
+    for bad in (dict(ws_bytes=need - 1), dict(ws_bytes=need, ws=None), dict(ws_bytes=need, ws=P + 8)):
+        refused(L, kd(L, type=type, N=1, V=V, ld=V, ldd=V, d=1 << 40, **bad), "distill: workspace")

@@ -476,6 +476,46 @@ def test_extreme_temperatures(lib):
         check_logprobs(logprobs(lib, x, F32, scale, ids, 6), x, scale, ids, 6)
 
 
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V", [(3, 300), (2, 70001), (1030, 1000), (41, 40003)])
+def test_smallest_and_largest_temperatures(lib, ty, N, V):
+    """Scales and temperatures at both ends of their range, over masked tokens
+    and logits whose scaled values pass fp32."""
+    t = _t()
+    print("temperatures", NAMES[ty], N, V, flush=True)
+    lo, hi = float(np.float32(1e-30)), float(np.float32(1e30))
+    _, x = on_gpu(rows_of(ty, N, V))
+    x[0, ::3] = -math.inf
+    ids = some_ids(N, V, 2, 1)
+    for scale in (lo, hi):
+        check_logprobs(logprobs(lib, x, ty, scale, ids, 20), x, scale, ids, 20)
+    if ty != F16:
+        y = x.clone()
+        y[1, 11], y[1, 40:50], y[0, 20:] = 3e38, -3e38, -3e38
+        check_logprobs(logprobs(lib, y, ty, hi, None, 0), y, hi, None, 0)
+    tids, tl = teacher(x, 8, 1.0)
+    x[1] = 0.25
+    X, I, q = f64(x), tids.cpu().numpy().astype(np.int64), np.exp(f64(tl))
+    for tau in (lo, hi):
+        p = np.exp(ref_logp(X, 1.0 / tau)[0])
+        Xo = X.copy()
+        np.put_along_axis(Xo, I, -np.inf, 1)
+        po = np.exp(ref_logp(Xo, 1.0 / tau)[0])          # among the tokens the teacher does not name
+        for tail in (False, True):
+            _, d = like_rows(x, ty)
+            scale = float(np.float32(1.0 / tau))         # so that the gradient is an ordinary number
+            distill(lib, x, ty, tids, tl, tail, tau, 1.0, None, 0.0, d, scale)
+            Q = q.sum(1, keepdims=True)
+            want = p.copy()
+            np.put_along_axis(want, I, np.take_along_axis(p, I, 1) - (q if tail else q / Q), 1)
+            if tail:
+                want -= (1.0 - Q) * po
+            # p and po: sums and exponentials; q in 64 bits; a few roundings of the factors
+            # tau, scale and their product; the output's half step
+            bar = (p + tail * po) * (4 * rho(V) + 40 * EPS) + (half_step(ty) * 1.01 + 20 * EPS) * np.abs(want) + 8 * EPS
+            close(f64(d), want, bar, ("dlogits", tau, tail))
+
+
 # ---------------------------------------------------------------- gradient --
 def grad_tol(ty, X, scale, want, c0, c1, H, factor):
     """|d p| <= p eps (4 |z'| + 2 |log S| + 8) for the recomputed probabilities,
@@ -978,6 +1018,153 @@ def test_log_sums_of_long_rows_lean_to_neither_side(lib, ty, N, V):
     err = o.rows.double() - t.log(S)
     print("lean", NAMES[ty], N, V, float(err.mean()), float(err.std()), flush=True)
     assert abs(float(err.mean())) <= 5 * 2e-7 / math.sqrt(N) + 5e-9, float(err.mean())
+
+
+def other_rows(N, V, ld, off, ty):
+    t = _t()
+    b = t.full((off + N * ld + 16,), float("nan"), dtype=dtype(ty), device="cuda")
+    return b, t.as_strided(b, (N, V), (ld, 1), off)
+
+
+def written_elsewhere(run, x, ty, ld, off):
+    """run(d) into rows of a layout of their own: the bits that rows like the
+    logits' get, and nothing around them."""
+    t = _t()
+    _, like = like_rows(x, ty)
+    run(like)
+    buf, d = other_rows(*x.shape, ld, off, ty)
+    run(d)
+    assert t.equal(d, like) and bool(like.isfinite().all())
+    d.fill_(float("nan"))
+    assert bool(t.isnan(buf).all()), "wrote outside its rows"
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+@pytest.mark.parametrize("N,V,pad,off,ld,doff", [
+    (5, 333, 3, 1, 333, 0), (5, 333, 0, 0, 341, 3), (300, 2049, 7, 2, 2049, 5), (1030, 1001, 0, 0, 1008, 8), (2100, 1001, 7, 1, 1003, 0),
+    (9, 8191, 1, 3, 8192, 0), (9, 16001, 0, 1, 16004, 4), (45, 40001, 6, 0, 40001, 1), (2, 131070, 2, 0, 131071, 3)])
+def test_gradients_of_another_layout(lib, ty, N, V, pad, off, ld, doff):
+    """Padded logits with a dense gradient and the reverse, in every launch: rows
+    in registers, read twice, cut."""
+    t = _t()
+    print("layout", NAMES[ty], N, V, pad, off, ld, doff, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, off))
+    ids = some_ids(N, V, 2, V)
+    f = logprobs(lib, x, ty, 1.0, ids, 0)
+    dlogp, dent = t.randn(N, 2, device="cuda"), t.randn(N, device="cuda")
+    written_elsewhere(lambda d: logprobs_bwd(lib, x, ty, 1.0, ids, f.lse2, f.entropy, dlogp, None, dent, d), x, ty, ld, doff)
+    tids, tl = teacher(x, 8, 2.0)
+    tgt = ids[:, 1].contiguous()
+    for tail, w_ce in ((False, 0.0), (True, 0.5)):
+        written_elsewhere(lambda d: distill(lib, x, ty, tids, tl, tail, 2.0, 1.0, tgt, w_ce, d), x, ty, ld, doff)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_gradients_at_every_pair_of_alignments(lib, ty):
+    t = _t()
+    VE, N, V = 4 if ty == F32 else 8, 3, 61
+    for off in range(VE):
+        _, x = on_gpu(rows_of(ty, N, V, V + 3, off))
+        ids = some_ids(N, V, 2, V)
+        f = logprobs(lib, x, ty, 1.0, ids, 0)
+        dlogp = t.randn(N, 2, device="cuda")
+        tids, tl = teacher(x, 5, 1.0)
+        for doff in range(VE):
+            written_elsewhere(lambda d: logprobs_bwd(lib, x, ty, 1.0, ids, f.lse2, None, dlogp, None, None, d), x, ty, V + 5, doff)
+            written_elsewhere(lambda d: distill(lib, x, ty, tids, tl, True, 1.0, 1.0, None, 0.0, d), x, ty, V + 5, doff)
+
+
+@pytest.mark.parametrize("ty", [F32, F16, BF16])
+def test_logprobs_bwd_without_given_tokens(lib, ty):
+    """M = 0: the gradient of the entropy or of the log-sum-exp alone."""
+    t = _t()
+    for N, V in ((5, 300), (2, 40001), (130, 2048)):
+        print("no tokens", NAMES[ty], N, V, flush=True)
+        _, x = on_gpu(rows_of(ty, N, V))
+        X = f64(x)
+        _, m, ls, H = ref_logp(X, 0.8)
+        lse2 = t.tensor(np.stack([m, ls], 1), dtype=t.float32, device="cuda")
+        ent = t.tensor(H, dtype=t.float32, device="cuda")
+        g = t.Generator().manual_seed(V)
+        a, b = (t.randn(N, generator=g).cuda() for _ in range(2))
+        for dlse, dent in ((a, None), (None, b), (a, b)):
+            _, d = like_rows(x, ty)
+            logprobs_bwd(lib, x, ty, 0.8, None, lse2, ent, None, dlse, dent, d)
+            c0, c1 = (np.zeros(N) if v is None else f64(v) for v in (dlse, dent))
+            want = ref_bwd(X, 0.8, np.zeros((N, 0), int), np.zeros((N, 0)), c0, c1)
+            close(f64(d), want, grad_tol(ty, X, 0.8, want, np.abs(c0), c1, H, 0.8), "dlogits")
+
+
+def test_logprobs_bwd_masked_tokens(lib):
+    """A masked token that is not given has gradient 0 exactly."""
+    t = _t()
+    for ty in (F32, F16, BF16):
+        for N, V in ((4, 300), (4, 70001), (600, 2048)):
+            _, x = on_gpu(rows_of(ty, N, V))
+            x[:, : V // 2] = -math.inf
+            ids = some_ids(N, V, 2, 4, none=False)
+            f = logprobs(lib, x, ty, 1.0, ids, 0)
+            dlogp, dent = t.randn(N, 2, device="cuda"), t.randn(N, device="cuda")
+            _, d = like_rows(x, ty)
+            logprobs_bwd(lib, x, ty, 1.0, ids, f.lse2, f.entropy, dlogp, None, dent, d)
+            assert bool(d.isfinite().all())
+            d.scatter_(1, ids.long(), 0.0)
+            assert not bool(d[:, : V // 2].any()) and bool(d[:, V // 2:].any(1).all())
+
+
+@pytest.mark.parametrize("ty,N,V", [(F32, 70, 2048), (BF16, 9, 5003), (F32, 2, 70000), (F16, 45, 60001)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_gradient_without_losses(lib, ty, N, V, tail):
+    """rows and loss NULL: the same gradient."""
+    t = _t()
+    print("no losses", NAMES[ty], N, V, tail, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V))
+    ids, tl = teacher(x, 20, 2.0)
+    tgt = some_ids(N, V, 1, 5)
+    _, d = like_rows(x, ty)
+    distill(lib, x, ty, ids, tl, tail, 2.0, 1.0, tgt, 0.5, d)
+    _, d2 = like_rows(x, ty)
+    nb = lib.tlg_distill_ws_bytes(ty, N, V)
+    ws = t.full((nb + 16,), 255, device="cuda", dtype=t.uint8)
+    lib.distill(x.data_ptr(), ty, V, N, V, ids.data_ptr(), tl.data_ptr(), 20, int(tail), 2.0, 1.0, tgt.data_ptr(), 0.5,
+                None, None, d2.data_ptr(), V, 1.0, ws.data_ptr(), nb, stream())
+    assert t.equal(d, d2)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("N,V,tau", [(9, 300, 1.0), (70, 2048, 2.0), (2100, 1000, 2.0), (45, 50003, 1.0)])
+def test_distill_weights_of_either_sign(lib, N, V, tau, tail):
+    """Zero and negative weights: negating both negates every bit of the results,
+    and each term alone counts as it does beside the other."""
+    t = _t()
+    print("weights", N, V, tau, tail, flush=True)
+    _, x = on_gpu(rows_of(F32, N, V))
+    ids, tl = teacher(x, 12, tau)
+    tgt = t.randint(0, V, (N,), generator=t.Generator().manual_seed(2), dtype=t.int32).cuda()
+    tgt[0] = ids[0, 3]
+
+    def run(w_kd, w_ce):
+        _, d = like_rows(x, F32)
+        o = distill(lib, x, F32, ids, tl, tail, tau, w_kd, tgt, w_ce, d)
+        return o, d
+    o, d = run(0.75, 0.5)
+    n, e = run(-0.75, -0.5)
+    assert t.equal(o.rows, -n.rows) and t.equal(o.loss, -n.loss) and t.equal(d, -e)
+    X, G, I = f64(x), tgt.cpu().numpy(), ids.cpu().numpy()
+    p, p1 = np.exp(ref_logp(X, 1.0 / tau)[0]), np.exp(ref_logp(X, 1.0)[0])
+    hot = np.zeros((N, V))
+    np.put_along_axis(hot, I.astype(np.int64), 1.0, 1)
+    np.put_along_axis(hot, G[:, None].astype(np.int64), 1.0, 1)
+    for w_kd, w_ce in ((0.0, 0.5), (-0.75, 0.5), (0.75, -0.5), (0.75, 0.0), (0.0, 0.0)):
+        o, d = run(w_kd, w_ce)
+        rows, grad = ref_distill(X, I, f64(tl), tail, tau, w_kd, G, w_ce)
+        a, b = abs(w_kd), abs(w_ce)
+        # |log p| <= 60 here; sums rho-close each, the remainder's three times
+        close(f64(o.rows), rows, (a * tau * tau + b) * (3 * rho(V) + 6 * EPS * 120) + 2 * EPS * np.abs(rows), "rows")
+        out = 1.0 - np.take_along_axis(p, I.astype(np.int64), 1).sum(1)
+        ratio = 2.0 + (1.0 / out if tail else 0.0 * out)
+        bar = (a * tau * p * ratio[:, None] + b * p1) * (EPS * (4 * 120 + 12) + 4 * rho(V)) + 8 * EPS * (a * tau + b) * hot
+        close(f64(d), grad, bar + 8 * EPS * np.abs(grad) + tiny(F32), "dlogits")
 
 
 # ------------------------------------------------- graphs, streams, repeats --
