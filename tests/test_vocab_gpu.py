@@ -29,6 +29,13 @@ def _t():
     return torch
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    """The same inputs on every run and in every selection of tests: torch seeds
+    the GPU's generator by chance."""
+    _t().manual_seed(0)
+
+
 def dtype(ty):
     t = _t()
     return {F32: t.float32, F16: t.float16, BF16: t.bfloat16}[ty]
