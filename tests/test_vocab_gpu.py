@@ -302,6 +302,21 @@ def test_logprobs_every_launch(lib, ty, N, V, K, pad):
     check_logprobs(logprobs(lib, x, ty, 0.9, ids, K), x, 0.9, ids, K)
 
 
+@pytest.mark.parametrize("ty,N,V,K,pad", [
+    (F32, 2560, 2048, 40, 0), (BF16, 2559, 2048, 40, 0), (F16, 2050, 2047, 32, 1), (BF16, 2047, 1000, 32, 0),     # in registers
+    (F32, 4100, 2048, 41, 0), (F16, 1280, 999, 20, 3),
+    (F32, 3840, 2800, 20, 0), (BF16, 3839, 4801, 20, 1), (F16, 6150, 2100, 32, 0), (F32, 2048, 4096, 10, 0)])     # read again
+def test_logprobs_launches_by_alternatives(lib, ty, N, V, K, pad):
+    """Where the number of alternatives decides between one wave a row and four."""
+    print("launch", NAMES[ty], N, V, K, pad, flush=True)
+    _, x = on_gpu(rows_of(ty, N, V, V + pad, 1 if pad else 0))
+    x[0] = 0.5
+    x[N // 2, : V // 2] = 7.0
+    x[N - 1, V // 3:] = -math.inf
+    ids = some_ids(N, V, 2, V)
+    check_logprobs(logprobs(lib, x, ty, 0.9, ids, K), x, 0.9, ids, K)
+
+
 @pytest.mark.parametrize("ty", [F32, F16, BF16])
 @pytest.mark.parametrize("N,V,ld,off", [(3, 1000, 1003, 1), (2, 2048, 2051, 3), (5, 333, 340, 7), (2, 40001, 40010, 5),
                                         (300, 777, 900, 2)])

@@ -1377,14 +1377,21 @@ extern "C" size_t tlg_logprobs_ws_bytes(int type, int N, int V, int K)
 
 // One wave per row where the rows are short and many: no barriers, and a lane's
 // four (or, of fp32, eight) vectors stay in registers; 4096 rows of 2048 fp32 values
-// with 8 alternatives take 11.2 us so, 13.2 with the rows read again, 18.3 with four
-// waves each.  Four waves win for fewer rows (512 of those: 6.5 against 7.1 us) and for
-// longer ones (4096 of 16384 fp32 values: 49 against 58 us); they too keep four vectors
-// a thread (900 rows of 4000 fp32 values: 8.2 us, 9.1 read again).
+// with 8 alternatives take 11.2 us so, 13.2 with the rows read again, 16.5 with four
+// waves each.  Four waves win for fewer rows (2048 columns, 8 alternatives, fp32: 512
+// rows 5.8 against 7.1 us, 1024 equal at 7.5, 2048 11.0 against 8.7; bf16: 6.7 equal at
+// 512, 8.4 against 7.3 at 1024) and for many alternatives, whose bound one wave finds
+// lane by lane and whose list overflows near 48 (fp32: 20 of 1024 rows 7.9 against 8.4,
+// of 1536 9.5 against 9.2; 32 of 1024 8.3 against 10.1, of 2048 12.0 against 11.5; 40
+// of 2048 12.7 against 13.9, of 4096 19.5 against 17.9; 48 of 4096 20.4 against 26.9).
+// Rows that one wave reads again need more of all that (4096 rows of 2800 fp32 values: 8
+// alternatives 16.0 us, four waves 17.9; 20: 18.3, 18.8; 32: 22.0, 20.5; 2048 such
+// rows with 20: 14.0, 12.4; 4096 of 16384 fp32 values: 58, 49).  Four waves too keep four
+// vectors a thread (900 rows of 4000 fp32 values: 8.2 us, 9.1 read again).
 template <bool TOP> static void lp_launch(const LpArgs &a, int type, int nv, hipStream_t st)
 {
     const unsigned rows = (unsigned)a.N;
-    const bool wave = a.K <= 48 && rows >= 1024;
+    const bool wave = a.K <= 40 && rows >= 1024 && rows >= 64u * a.K;
     if (a.S > 1) {
         BY_TYPE(rows * a.S, 256, 0, a, k_logprobs, , 4, 4, false, TOP);
         BY_TYPE(rows, 256, 0, a, k_logprobs_join, , TOP);
@@ -1392,7 +1399,7 @@ template <bool TOP> static void lp_launch(const LpArgs &a, int type, int nv, hip
         BY_TYPE((rows + 3) / 4, 256, 0, a, k_logprobs, , 1, 4, true, TOP);
     else if (wave && nv <= 512 && type == TLG_F32)
         hipLaunchKernelGGL((k_logprobs<TLG_F32, 1, 8, true, TOP>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
-    else if (wave && nv <= 1024 && rows >= 2 * (unsigned)nv)
+    else if (wave && nv <= 1024 && rows >= 2 * (unsigned)nv && rows >= 192u * a.K)
         BY_TYPE((rows + 3) / 4, 256, 0, a, k_logprobs, , 1, 4, false, TOP);
     else if (nv <= 1024)
         BY_TYPE(rows, 256, 0, a, k_logprobs, , 4, 4, true, TOP);
