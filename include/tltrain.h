@@ -141,13 +141,14 @@ int tlg_dev_xent_rows(const float *logits, const int *tgt, float *dlogits, doubl
  * Operators over logits [N][V] of element type `type`, row n at logits + n * ld
  * elements (ld >= V; what lies between the rows is neither read nor written).
  * V is 1 .. TLG_VOCAB_MAX and need not be a multiple of anything, N is 0 ..
- * TLG_VOCAB_ROWS; pointers need the alignment of their elements only, scales
- * and temperatures lie in 1e-30 .. 1e30.  Sums are fp32 or wider and every
- * output is rounded once.  Only the caller's buffers are used: calls may
- * overlap on any streams as long as their outputs and workspaces differ, and
- * any call can be captured into a graph (after tlg_init).  Equal calls give
- * equal bits; the number of rows, and where a row lies on the grid of 16 bytes,
- * may change the order of its fp32 sums.
+ * TLG_VOCAB_ROWS (a call with N = 0 writes nothing, no loss either); pointers
+ * need the alignment of their elements only, scales and temperatures lie in
+ * 1e-30 .. 1e30.  Sums are fp32 or wider, gradients in 16 bits are rounded once.
+ * Only the caller's buffers are used: calls may overlap on any streams as long
+ * as their outputs and workspaces differ, and any call can be captured into a
+ * graph (after tlg_init).  Equal calls give equal bits; the numbers of rows and
+ * of alternatives, and where a row lies on the grid of 16 bytes, may change the
+ * order of its fp32 sums.
  *
  * A logit of -inf is a masked token (probability 0).  A row of nothing but
  * -inf has no distribution: its log probabilities are -inf, its entropy 0, its
@@ -188,9 +189,11 @@ int tlg_dev_logprobs(const void *logits, int type, long long ld, int N, int V, f
  *   dz_v = sum_j dlogp_j (1{v = ids_j} - p_v) + dlse p_v
  *          - dentropy p_v (log p_v + entropy)
  * and dlogits = scale * dz, of the logits' type, rows ldd elements apart; it
- * may be the logits themselves (same address and ld), else it must not overlap
- * them.  lse2 and entropy (with dentropy) are the forward's.  An id given twice
- * counts twice. */
+ * may be the logits themselves (same address and ld), else the memory from its
+ * first to its last element must not overlap theirs.  Rows that start at the
+ * logits' offset from the grid of 16 bytes are written 16 bytes at a time,
+ * others an element at a time.  lse2 and entropy (with dentropy) are the
+ * forward's.  An id given twice counts twice. */
 int tlg_dev_logprobs_bwd(const void *logits, int type, long long ld, int N, int V, float scale, const int *ids, int M,
                          const float *lse2, const float *entropy, const float *dlogp, const float *dlse,
                          const float *dentropy, void *dlogits, long long ldd, void *stream);
@@ -214,7 +217,8 @@ int tlg_dev_logprobs_bwd(const void *logits, int type, long long ld, int N, int 
  *   dlogits_v = scale d rows[n] / d x_v
  *         = scale (w_kd temp (Q p_v - q_v) + w_ce (softmax(x)_v - 1{v = tgt}))
  *           with Q = sum q (+ q_r), outside S Q - q_r / p_r (tail 1)
- * and loss[0] = the mean of rows over the N rows (summed in double).  Rows
+ * and loss[0] = the mean of rows over the N rows (summed in double).  A row's
+ * loss is off by what its log sums are (a few 1e-7) times w_kd temp^2.  Rows
  * without an entry have KL 0, with a negative target CE 0.  rows may be NULL
  * (then loss too) if dlogits is given, and dlogits if rows is; dlogits as in
  * tlg_dev_logprobs_bwd.  t_ids and t_logp may be NULL with K = 0, tgt with
