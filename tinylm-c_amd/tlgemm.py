@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libtlgemm.so")
 HEADER = os.path.join(REPO, "include", "tlgemm.h")
 TRAIN_HEADER = os.path.join(REPO, "include", "tltrain.h")
 DECODE_HEADER = os.path.join(REPO, "include", "tldecode.h")
+SERVE_HEADER = os.path.join(REPO, "include", "tlserve.h")
 
 _fp = ctypes.POINTER(ctypes.c_float)
 _ip = ctypes.POINTER(ctypes.c_int)
@@ -137,14 +138,21 @@ SIGNATURES = {
     "tlg_dev_dec_persist": (_i, [_vp, _i, _vp]),
     "tlg_dev_dec_chunks": (_i, [_vp, _i, _vp, _i, _vp]),
     "tlg_dec_persist_status": (_i, [_vp, _vp]),
+    # include/tlserve.h
+    "tlg_dev_paged_store": (_i, [_vp, _vp, _vp, _ll, _vp, _ll, _i, _vp, _ll, _vp, _ll, _i, _vp, _vp, _i, _vp]),
+    "tlg_paged_attn_ws_bytes": (_sz, [_vp, _vp, _i, _i]),
+    "tlg_dev_paged_attn": (_i, [_vp, _vp, _vp, _i, _ll, _i, _f, _i, _i, _vp, _ll, _vp, _vp, _sz, _vp]),
+    "tlg_spec_verify_ws_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "tlg_dev_spec_verify": (_i, [_vp, _i, _ll, _f, _vp, _ll, _f, _i, _i, _vp, _i, _vp, _vp, _vp, _ll, _vp, _vp, _vp,
+                                 _vp, _sz, _vp]),
 }
 
 
 def header_symbols(path=None):
     """Function names declared in a C header (tlg_*/tl_* prototypes); by
-    default the library's two public headers."""
+    default the library's public headers."""
     names = set()
-    for p in ([path] if path else [HEADER, TRAIN_HEADER, DECODE_HEADER]):
+    for p in ([path] if path else [HEADER, TRAIN_HEADER, DECODE_HEADER, SERVE_HEADER]):
         text = open(p).read()
         text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
         names |= set(re.findall(r"\b(tlg?_[a-z0-9_]+)\s*\(", text))
@@ -169,6 +177,31 @@ class TlgDecGemv(ctypes.Structure):
                 ("M", ctypes.c_int), ("K", ctypes.c_int), ("N", ctypes.c_int), ("A", _vp), ("B", _vp),
                 ("pro", ctypes.c_int), ("gain", _vp), ("A2", _vp), ("bsel", _vp), ("bstride", ctypes.c_longlong),
                 ("cgate", _vp)]
+
+
+class TlgPages(ctypes.Structure):
+    """include/tlserve.h TlgPages: one layer's paged KV cache."""
+    _fields_ = [("K", _vp), ("V", _vp), ("type", ctypes.c_int), ("KV", ctypes.c_int), ("hd", ctypes.c_int),
+                ("page", ctypes.c_int), ("n_pages", ctypes.c_int), ("page_ld", ctypes.c_longlong),
+                ("tok_ld", ctypes.c_longlong), ("head_ld", ctypes.c_longlong)]
+
+
+class TlgBatch(ctypes.Structure):
+    """include/tlserve.h TlgBatch: rows, lengths and page tables of the sequences."""
+    _fields_ = [("B", ctypes.c_int), ("N", ctypes.c_int), ("row0", _vp), ("len", _vp), ("table", _vp),
+                ("ldt", ctypes.c_int), ("max_rows", ctypes.c_int), ("max_len", ctypes.c_int)]
+
+
+def pages(K, V, type, KV, hd, page, n_pages, page_ld=None, tok_ld=None, head_ld=None):
+    """A paged cache at device addresses K and V; [n_pages][page][KV][hd] unless
+    other distances (in elements) are given."""
+    return TlgPages(K, V, type, KV, hd, page, n_pages, page * KV * hd if page_ld is None else page_ld,
+                    KV * hd if tok_ld is None else tok_ld, hd if head_ld is None else head_ld)
+
+
+def batch(B, N, row0, len, table, ldt, max_rows=0, max_len=0):
+    """B sequences over N rows; row0, len and table are device addresses."""
+    return TlgBatch(B, N, row0, len, table, ldt, max_rows, max_len)
 
 
 class Lib:
@@ -255,6 +288,28 @@ class Lib:
         return self.check(self.dll.tlg_dev_distill(logits, type, ld, N, V, t_ids, t_logp, K, tail, temp, w_kd, tgt,
                                                    w_ce, rows, loss, dlogits, ldd, scale, ws, ws_bytes, stream),
                           "tlg_dev_distill")
+
+    def paged_store(self, pages, batch, q, ldq, q_out, ldqo, H, k, ldk, v, ldv, type, cos_t, sin_t, maxpos, stream=0):
+        """New rows of keys and values into a paged cache, with RoPE of keys and queries."""
+        return self.check(self.dll.tlg_dev_paged_store(ctypes.byref(pages), ctypes.byref(batch), q, ldq, q_out, ldqo, H,
+                                                       k, ldk, v, ldv, type, cos_t, sin_t, maxpos, stream),
+                          "tlg_dev_paged_store")
+
+    def paged_attn_ws_bytes(self, pages, batch, type, H):
+        return self.dll.tlg_paged_attn_ws_bytes(ctypes.byref(pages), ctypes.byref(batch), type, H)
+
+    def paged_attn(self, pages, batch, q, type, ldq, H, scale, win, sinks, out, ldo, lse, ws, ws_bytes, stream=0):
+        """Attention of every sequence's new rows over its pages."""
+        return self.check(self.dll.tlg_dev_paged_attn(ctypes.byref(pages), ctypes.byref(batch), q, type, ldq, H, scale,
+                                                      win, sinks, out, ldo, lse, ws, ws_bytes, stream),
+                          "tlg_dev_paged_attn")
+
+    def spec_verify(self, logits, type, ld, scale, draft_logits, ldd, dscale, N, V, row0, B, draft, u, noise, ldn, tokens,
+                    logp, accepted, ws, ws_bytes, stream=0):
+        """Verification of drafted tokens by sampling from given random numbers."""
+        return self.check(self.dll.tlg_dev_spec_verify(logits, type, ld, scale, draft_logits, ldd, dscale, N, V, row0, B,
+                                                       draft, u, noise, ldn, tokens, logp, accepted, ws, ws_bytes,
+                                                       stream), "tlg_dev_spec_verify")
 
     def group(self, calls, stream=0, flush=True):
         """tlg_dev_gemm_group over dicts {op, beta, C, M, K, N, A: [..], B: [..], Nseg: [..], R}."""
