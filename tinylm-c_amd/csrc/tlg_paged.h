@@ -1,0 +1,288 @@
+// tlg_paged.h -- batches of sequences over a paged KV cache, as the kernels of
+// tlg_paged.hip and tlg_paged_tile.hip see them.
+#pragma once
+#include "tlg_internal.h"
+#include "../../include/tlserve.h"
+#include <math.h>
+#include <limits.h>
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16;
+typedef __bf16 b16;
+
+template <int T> struct ElT;
+template <> struct ElT<TLG_F32> { typedef float E; };
+template <> struct ElT<TLG_F16> { typedef h16 E; };
+template <> struct ElT<TLG_BF16> { typedef b16 E; };
+
+// ----------------------------------------------------------------- batches --
+// What the kernels know of a batch and its cache.  Page numbers, rows and lengths
+// come from device memory and are cut to what the buffers hold where they are read.
+struct PgBatch {
+    const int *row0, *len, *table;
+    int B, N, ldt;
+    int page, n_pages;
+    unsigned magic;              // ceil(2^32 / page)
+    long long page_ld, tok_ld, head_ld;
+};
+// t / page for 0 <= t < 2^31: the product is t / page or one more (its error is below t / 2^32)
+__device__ __forceinline__ int pg_of(const PgBatch &b, int t)
+{
+    if (b.page == 1) return t;
+    int g = (int)__umulhi((unsigned)t, b.magic);
+    return g - (g * b.page > t);
+}
+__device__ __forceinline__ int pg_row0(const PgBatch &b, int i) { return min(max(b.row0[i], 0), b.N); }
+
+// The last i in [0, n) with start(i) <= x (0 if there is none), all lanes of a wave
+// at once: 64 probes a step; start must not decrease.
+template <typename F> __device__ __forceinline__ int pg_search(int n, long long x, F start)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const bool in = i < n && (i == 0 || start(lo + i) <= x);
+        const int k = __popcll(__ballot(in));            // probes at or below x are the first ones
+        lo += (k - 1) * step;
+        n = min(step, n - (k - 1) * step);
+    }
+    return lo;
+}
+
+// --------------------------------------------------------------- attention --
+struct AttnArgs {
+    PgBatch b;
+    const char *K, *V, *q;
+    char *out;
+    float *lse;
+    long long ldq, ldo;
+    int H, KV, G, win, sinks;
+    int S;                       // workgroups that share a tile's tokens, at most
+    int few, many;               // sequences of at most `few` rows times heads are left out, of more than `many` too
+    float c;                     // scale log2 e
+    float *po, *pm;              // S > 1: [S][N][H][hd] sums and [S][N][H][2] references and weights
+};
+
+// Base-2 scores against a reference: with R the largest c (q . k) of a row so far,
+// rounded once, a weight is 2^(c (q . k) - R), one fused product, and whatever R is
+// exactly, it is the same for all of a row's tokens.  R stays while no score passes it by
+// more than PG_SLACK (weights up to 2^8 lose nothing in fp16, bf16 or fp32), so that
+// the sums are rarely rescaled.
+#define PG_SLACK 8.0f
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+template <int T> struct Vec8 { typedef typename ElT<T>::E E; typedef E e8 __attribute__((ext_vector_type(8))); };
+template <int T> __device__ __forceinline__ f32x16 pg_mfma(u32x4 a, u32x4 b, f32x16 c)
+{
+    typedef typename Vec8<T>::e8 e8;
+    if constexpr (T == TLG_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(e8, a), __builtin_bit_cast(e8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(e8, a), __builtin_bit_cast(e8, b), c, 0, 0, 0);
+}
+template <int T> __device__ __forceinline__ unsigned pg_pack(float lo, float hi)      // rounded to nearest even
+{
+    typedef typename ElT<T>::E e2 __attribute__((ext_vector_type(2)));
+    const e2 v = {(typename ElT<T>::E)lo, (typename ElT<T>::E)hi};
+    return __builtin_bit_cast(unsigned, v);
+}
+// both halves' values of a wave, in every lane
+__device__ __forceinline__ void pg_halves(float v, float &lo, float &hi)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    lo = __uint_as_float(r[0]);
+    hi = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float pg_both_max(float v)
+{
+    float a, b;
+    pg_halves(v, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float pg_both_sum(float v)
+{
+    float a, b;
+    pg_halves(v, a, b);
+    return a + b;
+}
+// element (row) of register i of a 32 x 32 product in lane half h
+__device__ __forceinline__ int pg_at(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// A sequence of the batch, and the column of a tile that a lane has: the row i and
+// query head g of its KV head, rh = i G + g of n G.
+struct Seq { int lo, n, len; };
+__device__ __forceinline__ Seq pg_seq(const PgBatch &b, int s)
+{
+    Seq q;
+    q.lo = pg_row0(b, s);
+    q.n = max(pg_row0(b, s + 1) - q.lo, 0);
+    q.len = max(b.len[s], 0);
+    return q;
+}
+// Positions are cut to `cap`, the first token that no table has a column for: it
+// stands for all of them, as a token without a page.
+__device__ __forceinline__ int pg_pos(const AttnArgs &a, const Seq &q, int i)
+{
+    return min(q.len - q.n + i, a.b.ldt * a.b.page);
+}
+__device__ __forceinline__ int pg_from(const AttnArgs &a, int p) { return a.win ? max(0, p - a.win + 1) : 0; }
+
+// The tokens that columns [rh0, rh1) of a sequence see, in tiles of TT: `sink` tiles
+// from 0 on, then those from tile `first` on, `total` in all.
+struct Range { int pmin, pmax, lomax, sink, first, total; };
+template <int TT> __device__ __forceinline__ Range pg_range(const AttnArgs &a, const Seq &q, int rh0, int rh1)
+{
+    Range r;
+    r.pmin = pg_pos(a, q, rh0 / a.G);
+    r.pmax = pg_pos(a, q, (rh1 - 1) / a.G);
+    r.lomax = pg_from(a, r.pmax);
+    r.first = pg_from(a, r.pmin) / TT;
+    r.sink = min((a.sinks + TT - 1) / TT, r.first);
+    r.total = r.pmax < 0 ? 0 : r.sink + r.pmax / TT - r.first + 1;
+    return r;
+}
+template <int TT> __device__ __forceinline__ int pg_tile(const Range &r, int j)
+{
+    return (j < r.sink ? j : r.first + j - r.sink) * TT;
+}
+// Of the S workgroups of a tile those take part that get PG_MIN tokens.
+#define PG_MIN 256
+template <int TT> __device__ __forceinline__ int pg_parts(int S, int total)
+{
+    return max(1, min(S, total / (PG_MIN / TT)));
+}
+
+// A token's elements in the cache, -1 without a page.  Loads of such a token go to the
+// first page, and a key of it is made NaN, which its scores then are.
+__device__ __forceinline__ long long pg_token(const PgBatch &b, const int *table, int t)
+{
+    const int g = pg_of(b, t), n = g < b.ldt ? table[g] : -1;
+    return n >= 0 && n < b.n_pages ? n * b.page_ld + (t - g * b.page) * b.tok_ld : -1;
+}
+
+// What is not finite in a register of cache elements becomes 0; true if anything was.
+template <int C> __device__ __forceinline__ bool pg_clean(unsigned &w)
+{
+    bool hit = false;
+    if constexpr (C == TLG_F32) {
+        hit = (w & 0x7f800000u) == 0x7f800000u;
+        w = hit ? 0u : w;
+    } else {
+        constexpr unsigned X = C == TLG_F16 ? 0x7c00u : 0x7f80u;
+        const bool l = (w & X) == X, h = (w & X << 16) == X << 16;
+        w &= (l ? 0xffff0000u : ~0u) & (h ? 0x0000ffffu : ~0u);
+        hit = l || h;
+    }
+    return hit;
+}
+__device__ __forceinline__ bool pg_finite(float v) { return fabsf(v) < INFINITY; }
+
+__device__ __forceinline__ bool pg_sees(const AttnArgs &a, int t, int p, int from)
+{
+    return t <= p && (t >= from || t < a.sinks);
+}
+// Values that are not finite would reach, through products with a weight of 0, columns
+// that do not see their tokens.  In tiles that some column sees in part they are 0 in
+// the products, and come here, from the cache, to the columns that do see them: one
+// token at a time, for it is rare.  e: the weights of the 32 tokens from t0 on in the
+// product's layout; off(i): token i's elements of V, the same in all lanes; at(b, m): the
+// element that row m of block b stands for.
+template <int C, int NB, typename OFF, typename AT>
+__device__ __forceinline__ void pg_special(const AttnArgs &a, f32x16 (&o)[NB], const float *e, int t0, int pmax, int p,
+                                           int from, OFF off, AT at)
+{
+    typedef typename ElT<C>::E E;
+    const int h = threadIdx.x >> 5 & 1;
+#pragma unroll 1
+    for (int k = 0; k < 32; k++) {
+        const int t = t0 + k, hk = k >> 2 & 1, i = (k >> 3) * 4 + (k & 3);      // pg_at(i, hk) = k
+        const long long w = off(k);
+        if (t > pmax || w < 0) continue;
+        float own = e[0], lo, hi;
+#pragma unroll
+        for (int j = 1; j < 16; j++) own = j == i ? e[j] : own;
+        pg_halves(own, lo, hi);
+        const float f = hk ? hi : lo;
+        const bool see = pg_sees(a, t, p, from);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float v = (float)((const E *)a.V)[w + at(b, pg_at(j, h))];
+                if (see && !pg_finite(v)) o[b][j] = fmaf(f, v, o[b][j]);
+            }
+    }
+}
+// Orders a wave's own reads and writes of LDS.
+__device__ __forceinline__ void pg_wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The running maximum of a column and what it does to its sums: z the scores of N
+// registers (hidden ones -inf), which become weights.
+template <int N, int NB>
+__device__ __forceinline__ void pg_weights(float (&z)[N], float c, float &R, float &l, f32x16 (&o)[NB])
+{
+    float m[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+    for (int i = 4; i < N; i++) m[i & 3] = fmaxf(m[i & 3], z[i]);
+    const float mx = pg_both_max(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * c;
+    if (__any(mx > R + PG_SLACK)) {
+        const float n = fmaxf(R, mx), f = __builtin_amdgcn_exp2f(R - (n == -INFINITY ? 0.f : n));
+        R = n;
+        l *= f;
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[b] *= f;
+    }
+    const float ref = R == -INFINITY ? 0.f : R;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        z[i] = __builtin_amdgcn_exp2f(fmaf(z[i], c, -ref));
+        s[i & 3] += z[i];
+    }
+    l += (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// K consecutive elements of a row of out (final: weighted by 1 / l) or of the sums of
+// workgroup s of several.
+__device__ __forceinline__ float pg_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+template <int T, int K> __device__ __forceinline__ void pg_put(char *p, const float *x)
+{
+    typedef typename ElT<T>::E E;
+    E v[K];
+#pragma unroll
+    for (int i = 0; i < K; i++) v[i] = (E)x[i];
+    __builtin_memcpy(__builtin_assume_aligned(p, K * sizeof(E) % 16 == 0 ? 16 : K * sizeof(E) % 8 == 0 ? 8 : 4), v, sizeof v);
+}
+template <int T, int K>
+__device__ __forceinline__ void pg_out(const AttnArgs &a, int hd, int s, int parts, int r, int head, int d, float l, float *x)
+{
+    if (parts > 1) {
+        pg_put<TLG_F32, K>((char *)(a.po + (((long long)s * a.b.N + r) * a.H + head) * hd + d), x);
+        return;
+    }
+    const float f = pg_inverse(l);
+#pragma unroll
+    for (int i = 0; i < K; i++) x[i] = l == 0.f ? 0.f : x[i] * f;
+    pg_put<T, K>(a.out + ((long long)r * a.ldo + (long long)head * hd + d) * (T == TLG_F32 ? 4 : 2), x);
+}
+__device__ __forceinline__ float pg_lse(float R, float l)
+{
+    return l == 0.f ? -INFINITY : ((R == -INFINITY ? 0.f : R) + __builtin_amdgcn_logf(l)) * 0.69314718056f;
+}
+__device__ __forceinline__ void pg_out_sums(const AttnArgs &a, int s, int parts, int r, int head, float R, float l)
+{
+    if (parts > 1) *(float2 *)(a.pm + (((long long)s * a.b.N + r) * a.H + head) * 2) = float2{R, l};
+    else if (a.lse) a.lse[(long long)r * a.H + head] = pg_lse(R, l);
+}
+
+// What the launches of tlg_paged_tile.hip take (tlg_paged.hip decides).
+#define PGT_ROWS 128                 /* columns (rows times heads) of a workgroup */
+#define PGT_TOKENS(hd) ((hd) == 256 ? 32 : 64)
+void pg_tile_launch(const AttnArgs &a, int type, int hd, unsigned slots, hipStream_t st);
