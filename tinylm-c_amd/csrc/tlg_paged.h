@@ -23,15 +23,14 @@ struct PgBatch {
     const int *row0, *len, *table;
     int B, N, ldt;
     int page, n_pages;
-    unsigned magic;              // ceil(2^32 / page)
+    unsigned magic;              // floor((2^32 - 1) / page)
     long long page_ld, tok_ld, head_ld;
 };
-// t / page for 0 <= t < 2^31: the product is t / page or one more (its error is below t / 2^32)
+// t / page for 0 <= t < 2^31: the product is t / page or one less (its error is below t / 2^32 + 1)
 __device__ __forceinline__ int pg_of(const PgBatch &b, int t)
 {
-    if (b.page == 1) return t;
-    int g = (int)__umulhi((unsigned)t, b.magic);
-    return g - (g * b.page > t);
+    const int g = (int)__umulhi((unsigned)t, b.magic);
+    return g + (t - g * b.page >= b.page);
 }
 __device__ __forceinline__ int pg_row0(const PgBatch &b, int i) { return min(max(b.row0[i], 0), b.N); }
 
@@ -59,7 +58,7 @@ struct AttnArgs {
     float *lse;
     long long ldq, ldo;
     int H, KV, G, win, sinks;
-    int S;                       // workgroups that share a tile's tokens, at most
+    int S, per;                  // workgroups that share a tile's tokens, at most, and how much each takes
     int few, many;               // sequences of at most `few` rows times heads are left out, of more than `many` too
     float c;                     // scale log2 e
     float *po, *pm;              // S > 1: [S][N][H][hd] sums and [S][N][H][2] references and weights
@@ -74,14 +73,30 @@ struct AttnArgs {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
 template <int T> struct Vec8 { typedef typename ElT<T>::E E; typedef E e8 __attribute__((ext_vector_type(8))); };
-template <int T> __device__ __forceinline__ f32x16 pg_mfma(u32x4 a, u32x4 b, f32x16 c)
+// Products of W x W blocks (W 32 or 16): the lane's column is lane % W, its group lane
+// / W; register i of a result is row pg_at<W>(i, group).  16-bit operands have eight
+// reduction elements a lane, fp32 ones one.
+template <int W> struct AccT;
+template <> struct AccT<32> { typedef f32x16 A; };
+template <> struct AccT<16> { typedef f32x4 A; };
+template <int W> __device__ __forceinline__ int pg_at(int i, int group) { return 256 / W * (i >> 2) + 4 * group + (i & 3); }
+template <int T, int W>
+__device__ __forceinline__ typename AccT<W>::A pg_mfma(u32x4 a, u32x4 b, typename AccT<W>::A c)
 {
     typedef typename Vec8<T>::e8 e8;
-    if constexpr (T == TLG_F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(e8, a), __builtin_bit_cast(e8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(e8, a), __builtin_bit_cast(e8, b), c, 0, 0, 0);
+    const e8 x = __builtin_bit_cast(e8, a), y = __builtin_bit_cast(e8, b);
+    if constexpr (T == TLG_F16 && W == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+    else if constexpr (T == TLG_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+    else if constexpr (W == 32) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+}
+template <int W> __device__ __forceinline__ typename AccT<W>::A pg_mfma32(float a, float b, typename AccT<W>::A c)
+{
+    if constexpr (W == 32) return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 template <int T> __device__ __forceinline__ unsigned pg_pack(float lo, float hi)      // rounded to nearest even
 {
@@ -89,27 +104,25 @@ template <int T> __device__ __forceinline__ unsigned pg_pack(float lo, float hi)
     const e2 v = {(typename ElT<T>::E)lo, (typename ElT<T>::E)hi};
     return __builtin_bit_cast(unsigned, v);
 }
-// both halves' values of a wave, in every lane
-__device__ __forceinline__ void pg_halves(float v, float &lo, float &hi)
+// Sum and maximum over the groups of lanes that share a column, in every lane.
+template <int W, typename OP> __device__ __forceinline__ float pg_groups(float v, OP op)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    lo = __uint_as_float(r[0]);
-    hi = __uint_as_float(r[1]);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    if constexpr (W == 16) {
+        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+    }
+    return v;
 }
-__device__ __forceinline__ float pg_both_max(float v)
+template <int W> __device__ __forceinline__ float pg_gmax(float v)
 {
-    float a, b;
-    pg_halves(v, a, b);
-    return fmaxf(a, b);
+    return pg_groups<W>(v, [](float a, float b) { return fmaxf(a, b); });
 }
-__device__ __forceinline__ float pg_both_sum(float v)
+template <int W> __device__ __forceinline__ float pg_gsum(float v)
 {
-    float a, b;
-    pg_halves(v, a, b);
-    return a + b;
+    return pg_groups<W>(v, [](float a, float b) { return a + b; });
 }
-// element (row) of register i of a 32 x 32 product in lane half h
-__device__ __forceinline__ int pg_at(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // A sequence of the batch, and the column of a tile that a lane has: the row i and
 // query head g of its KV head, rh = i G + g of n G.
@@ -148,11 +161,11 @@ template <int TT> __device__ __forceinline__ int pg_tile(const Range &r, int j)
 {
     return (j < r.sink ? j : r.first + j - r.sink) * TT;
 }
-// Of the S workgroups of a tile those take part that get PG_MIN tokens.
-#define PG_MIN 256
-template <int TT> __device__ __forceinline__ int pg_parts(int S, int total)
+// The workgroups that share a tile's tokens: one for every `per` tiles of 32 tokens, S at most.
+template <int TT> __device__ __forceinline__ int pg_parts(const AttnArgs &a, int total)
 {
-    return max(1, min(S, total / (PG_MIN / TT)));
+    const int per = a.per * 32 / TT;
+    return max(1, min(a.S, (total + per - 1) / per));
 }
 
 // A token's elements in the cache, -1 without a page.  Loads of such a token go to the
@@ -182,39 +195,7 @@ __device__ __forceinline__ bool pg_finite(float v) { return fabsf(v) < INFINITY;
 
 __device__ __forceinline__ bool pg_sees(const AttnArgs &a, int t, int p, int from)
 {
-    return t <= p && (t >= from || t < a.sinks);
-}
-// Values that are not finite would reach, through products with a weight of 0, columns
-// that do not see their tokens.  In tiles that some column sees in part they are 0 in
-// the products, and come here, from the cache, to the columns that do see them: one
-// token at a time, for it is rare.  e: the weights of the 32 tokens from t0 on in the
-// product's layout; off(i): token i's elements of V, the same in all lanes; at(b, m): the
-// element that row m of block b stands for.
-template <int C, int NB, typename OFF, typename AT>
-__device__ __forceinline__ void pg_special(const AttnArgs &a, f32x16 (&o)[NB], const float *e, int t0, int pmax, int p,
-                                           int from, OFF off, AT at)
-{
-    typedef typename ElT<C>::E E;
-    const int h = threadIdx.x >> 5 & 1;
-#pragma unroll 1
-    for (int k = 0; k < 32; k++) {
-        const int t = t0 + k, hk = k >> 2 & 1, i = (k >> 3) * 4 + (k & 3);      // pg_at(i, hk) = k
-        const long long w = off(k);
-        if (t > pmax || w < 0) continue;
-        float own = e[0], lo, hi;
-#pragma unroll
-        for (int j = 1; j < 16; j++) own = j == i ? e[j] : own;
-        pg_halves(own, lo, hi);
-        const float f = hk ? hi : lo;
-        const bool see = pg_sees(a, t, p, from);
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float v = (float)((const E *)a.V)[w + at(b, pg_at(j, h))];
-                if (see && !pg_finite(v)) o[b][j] = fmaf(f, v, o[b][j]);
-            }
-    }
+    return (t <= p) & ((t >= from) | (t < a.sinks));
 }
 // Orders a wave's own reads and writes of LDS.
 __device__ __forceinline__ void pg_wave_sync()
@@ -223,15 +204,52 @@ __device__ __forceinline__ void pg_wave_sync()
     __builtin_amdgcn_wave_barrier();
 }
 
+// Values that are not finite would reach, through products with a weight of 0, columns
+// that do not see their tokens.  In tiles that some column sees in part they are 0 in
+// the products, and come here, from the cache, to the columns that do see them: one
+// token at a time, for it is rare.  e: the weights of the 32 tokens from t0 on in the
+// product's layout, w: 1 KB of LDS of the wave's own; off(i): token i's elements of V, the
+// same in all lanes; at(b, m): the element that row m of block b stands for.
+template <int C, int W, int NB, typename OFF, typename AT>
+__device__ __forceinline__ void pg_special(const AttnArgs &a, typename AccT<W>::A (&o)[NB], const float *e, float *w,
+                                           const char *V, int t0, int pmax, int p, int from, OFF off, AT at)
+{
+    typedef typename ElT<C>::E E;
+    const int lane = threadIdx.x & 63, col = lane % W, g = lane / W;
+#pragma unroll
+    for (int i = 0; i < W / 2; i += 4) {
+        const int tb = pg_at<W>(i, 0);                   // the 256 / W tokens of four registers
+        pg_wave_sync();
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[(4 * g + j) * W + col] = e[i + j];
+        pg_wave_sync();
+#pragma unroll 1
+        for (int k = 0; k < 256 / W && t0 + tb + k <= pmax; k++) {
+            const long long at0 = off(tb + k);
+            if (at0 < 0) continue;
+            const float f = w[k * W + col];
+            const bool see = pg_sees(a, t0 + tb + k, p, from);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int j = 0; j < W * W / 64; j++) {
+                    const float v = (float)((const E *)V)[at0 + at(b, pg_at<W>(j, g))];
+                    if (see && !pg_finite(v)) o[b][j] = fmaf(f, v, o[b][j]);
+                }
+        }
+    }
+    pg_wave_sync();
+}
+
 // The running maximum of a column and what it does to its sums: z the scores of N
 // registers (hidden ones -inf), which become weights.
-template <int N, int NB>
-__device__ __forceinline__ void pg_weights(float (&z)[N], float c, float &R, float &l, f32x16 (&o)[NB])
+template <int W, int N, int NB>
+__device__ __forceinline__ void pg_weights(float (&z)[N], float c, float &R, float &l, typename AccT<W>::A (&o)[NB])
 {
     float m[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
     for (int i = 4; i < N; i++) m[i & 3] = fmaxf(m[i & 3], z[i]);
-    const float mx = pg_both_max(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * c;
+    const float mx = pg_gmax<W>(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * c;
     if (__any(mx > R + PG_SLACK)) {
         const float n = fmaxf(R, mx), f = __builtin_amdgcn_exp2f(R - (n == -INFINITY ? 0.f : n));
         R = n;
@@ -285,4 +303,4 @@ __device__ __forceinline__ void pg_out_sums(const AttnArgs &a, int s, int parts,
 // What the launches of tlg_paged_tile.hip take (tlg_paged.hip decides).
 #define PGT_ROWS 128                 /* columns (rows times heads) of a workgroup */
 #define PGT_TOKENS(hd) ((hd) == 256 ? 32 : 64)
-void pg_tile_launch(const AttnArgs &a, int type, int hd, unsigned slots, hipStream_t st);
+void pg_tile_launch(const AttnArgs &a, int type, int hd, unsigned grid, hipStream_t st);

@@ -115,39 +115,45 @@ template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(Sto
 }
 
 // --------------------------------------------------------------- attention --
-// Scores are formed transposed, S^T = K Q^T, 32 tokens by 32 columns (rows times query
-// heads of one KV head, so that a key is read once for all heads that share it): a lane
-// then has 16 of a column's 32 scores, its softmax needs one exchange between the halves
-// of the wave, and the weights are already the operand of O^T = V^T P^T, whose sums
-// the lane rescales by its own column's factor.  Which token stands at which place of
-// an operand's reduction is free as long as both operands agree, so nothing moves
-// between lanes.
+// Scores are formed transposed, S^T = K Q^T, tokens by columns (rows times query heads
+// of one KV head, so that a key is read once for all heads that share it): a lane then
+// has a share of one column's scores, its softmax needs exchanges between the two or
+// four lanes of a column only, and the weights are already the operand of O^T = V^T
+// P^T, whose sums the lane rescales by its own column's factor.  Which token stands at
+// which place of an operand's reduction is free as long as both operands agree, so
+// nothing moves between lanes.
 //
-// k_paged_direct works from global memory: a lane reads its token's key (one row of the
-// first operand) in pieces of 16 bytes.  For 16-bit rows the values go through LDS, each
-// wave's own 32 tokens, and are read back transposed; fp32 products (two tokens at a
-// time) take them as they are, element 32 m.. of lane m being whatever is contiguous.
+// k_paged_direct works from global memory, on 32 tokens at a time: a lane reads its
+// tokens' keys (rows of the first operand) in pieces of 16 bytes.  For 16-bit rows the values
+// go through LDS, each wave's own tokens, and are read back transposed; fp32 products
+// take them as they are, rows of V^T being dealt out so that a lane's are contiguous.
 // !ROWS: few columns (a decoded token, a drafted chunk), bound by the cache's bytes: the
 // four waves of a workgroup take every fourth tile of the tokens and join their sums,
-// and S workgroups share a long sequence.  ROWS (fp32): every wave 32 columns of its
-// own, whose keys the waves of a workgroup find in the CU's cache.
-template <int T, int C, int HD, bool ROWS>
-__global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 : 2) void k_paged_direct(AttnArgs a)
+// and S workgroups share a long sequence.  Blocks of W = 16 columns where there are no
+// more: half the registers of 32.  ROWS (fp32): every wave 32 columns of its own,
+// whose keys the waves of a workgroup find in the CU's cache.
+template <int T, int C, int HD, int W, bool ROWS>
+__global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128 && W == 32) || HD == 256 ? 1 : 2) void k_paged_direct(AttnArgs a)
 {
-    constexpr bool F = T == TLG_F32;
-    constexpr int NB = HD / 32, ts = F ? 4 : 2, cs = C == TLG_F32 ? 4 : 2;
-    constexpr int NK = F ? HD / 8 : HD / 16, KW = F ? cs : 4;           // pieces of a key and their registers
-    constexpr int NV = F ? 16 : HD / 16, VW = F ? (NB * cs + 3) / 4 : 4;
-    constexpr int VST = (HD / 2) % 64 == 16 || (HD / 2) % 64 == 48 ? HD : HD + 32;   // elements between tokens in LDS
-    constexpr int VB = F ? 0 : 4 * 32 * VST * 2, MB = ROWS ? 0 : 4 * 32 * 36 * 4;
     typedef typename ElT<C>::E E;
-    __shared__ __align__(16) char mem[VB > MB ? VB : MB ? MB : 16];
+    typedef typename AccT<W>::A Acc;
+    constexpr bool F = T == TLG_F32;
+    constexpr int G = 64 / W, TB = 32 / W;                              // groups of lanes, blocks of tokens
+    constexpr int NB = HD / W, NR = W * W / 64, NE = W / 2;             // blocks of a value, registers of a block, weights
+    constexpr int ts = F ? 4 : 2, cs = C == TLG_F32 ? 4 : 2;
+    constexpr int PE = F ? 4 : 8, NQ = HD / (PE * G), NK = NQ * TB, KW = PE * cs / 4;  // a key's pieces: elements, number, registers
+    constexpr int NV = F ? NE : HD / 16, VW = F ? (NB * cs + 3) / 4 : 4;
+    constexpr int VST = (HD / 2) % 64 == 16 || (HD / 2) % 64 == 48 ? HD : HD + 32;     // elements between tokens in LDS
+    constexpr int MS = W + 4, BS = NB % 4 ? 2 : 4, MB = W == 32 ? 1 : BS;              // the sums' blocks joined at once
+    constexpr int V1 = F ? 0 : 32 * VST * 2, M1 = MB * W * MS * 4, P1 = 1024;
+    constexpr int PW = V1 > M1 ? (V1 > P1 ? V1 : P1) : (M1 > P1 ? M1 : P1);            // LDS of a wave
+    __shared__ __align__(16) char mem[4 * PW];
     __shared__ long long toff[4][2][32];
-    __shared__ float red[4][2][32];
+    __shared__ float red[4][2][W];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane % W, g = lane / W;
     const int kvh = blockIdx.x % a.KV, s = blockIdx.x / a.KV % a.S, y = blockIdx.x / a.KV / a.S;
-    int b = y, base = blockIdx.y * 32;
+    int b = y, base = blockIdx.y * W;
     if (ROWS) {
         auto start = [&](int i) { return (long long)pg_row0(a.b, i) * a.G / 128 + i; };
         b = pg_search(a.b.B, y, start);
@@ -157,16 +163,13 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
     const int cols = q.n * a.G;
     if (base < 0 || base >= cols || cols <= a.few || cols > a.many) return;
     const int *table = a.b.table + (long long)b * a.b.ldt;
-    const long long head = kvh * a.b.head_ld;
-    const E *Kc = (const E *)a.K + head, *Vc = (const E *)a.V + head;
-    AttnArgs av = a;                                                    // pg_special reads V from the head on
-    av.V = (const char *)Vc;
-    auto at = [](int blk, int m) { return F ? NB * m + blk : 32 * blk + m; };
-    E *vs = (E *)mem + wave * 32 * VST;
+    const E *Kc = (const E *)a.K + kvh * a.b.head_ld, *Vc = (const E *)a.V + kvh * a.b.head_ld;
+    auto at = [](int blk, int m) { return F ? NB * m + blk : W * blk + m; };
+    E *vs = (E *)(mem + wave * PW);
 
-    for (int rh0 = base; rh0 < cols; rh0 += 32 * gridDim.y) {
-        const Range rg = pg_range<32>(a, q, rh0, min(rh0 + 32, cols));
-        const int parts = pg_parts<32>(a.S, rg.total);
+    for (int rh0 = base; rh0 < cols; rh0 += W * gridDim.y) {
+        const Range rg = pg_range<32>(a, q, rh0, min(rh0 + W, cols));
+        const int parts = pg_parts<32>(a, rg.total);
         if (s >= parts) {
             if (ROWS) return;
             continue;
@@ -174,47 +177,55 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
         const int j0 = (int)((long long)rg.total * s / parts), j1 = (int)((long long)rg.total * (s + 1) / parts);
         const int step = ROWS ? 1 : 4;
         // the lane's column
-        const int rh = rh0 + col, ci = min(rh, cols - 1) / a.G, g = min(rh, cols - 1) - ci * a.G;
+        const int rh = rh0 + col, ci = min(rh, cols - 1) / a.G, gq = min(rh, cols - 1) - ci * a.G;
         const bool live = rh < cols;
         const int r = q.lo + ci, p = live ? pg_pos(a, q, ci) : -1, from = pg_from(a, p);
-        u32x4 qf[NK];
+        u32x4 qf[NQ];
         {
-            const char *qp = a.q + ((long long)r * a.ldq + (kvh * a.G + g) * HD + (F ? 4 : 8) * h) * ts;
+            const char *qp = a.q + ((long long)r * a.ldq + (kvh * a.G + gq) * HD + PE * g) * ts;
 #pragma unroll
-            for (int i = 0; i < NK; i++) {
-                qf[i] = *(const u32x4 *)(qp + i * (F ? 8 : 16) * ts);
+            for (int i = 0; i < NQ; i++) {
+                qf[i] = *(const u32x4 *)(qp + i * PE * G * ts);
                 if (!live) qf[i] = u32x4{0, 0, 0, 0};
             }
         }
-        f32x16 o[NB];
+        Acc o[NB];
 #pragma unroll
         for (int i = 0; i < NB; i++)
 #pragma unroll
-            for (int k = 0; k < 16; k++) o[i][k] = 0.f;
+            for (int k = 0; k < NR; k++) o[i][k] = 0.f;
         float R = -INFINITY, l = 0.f;
 
         unsigned kr[NK][KW], vr[NV][VW];
-        // the page of the lane's token of tile j, then its elements
+        // the page of token lane % 32 of tile j, then its elements
         auto page = [&](int j) {
-            const int t = pg_tile<32>(rg, j) + col, n = pg_of(a.b, t);
+            const int t = pg_tile<32>(rg, j) + (lane & 31), n = pg_of(a.b, t);
             return j < j1 && t <= rg.pmax && n < a.b.ldt ? table[n] : -1;
         };
         auto elems = [&](int j, int n) {
-            const int t = pg_tile<32>(rg, j) + col;
+            const int t = pg_tile<32>(rg, j) + (lane & 31);
             return n >= 0 && n < a.b.n_pages ? n * a.b.page_ld + (t - pg_of(a.b, t) * a.b.page) * a.b.tok_ld : -1ll;
         };
-        auto loadK = [&](long long off) {
-            const E *k = Kc + max(off, 0ll) + (F ? 4 : 8) * h;
-#pragma unroll
-            for (int i = 0; i < NK; i++) __builtin_memcpy(kr[i], __builtin_assume_aligned(k + i * (F ? 8 : 16), 4 * KW), 4 * KW);
-        };
-        auto loadV = [&](int buf, long long off) {
-            if (h == 0) toff[wave][buf][col] = off;
+        // a key that has no page is NaN in its first element of the lane's, and so are its scores
+        bool lost[TB];
+        auto loadK = [&](int buf, long long off) {
+            if (lane < 32) toff[wave][buf][lane] = off;
             pg_wave_sync();
+#pragma unroll
+            for (int t = 0; t < TB; t++) {
+                const long long k0 = toff[wave][buf][W * t + col];
+                lost[t] = k0 < 0;
+                const E *k = Kc + max(k0, 0ll) + PE * g;
+#pragma unroll
+                for (int i = 0; i < NQ; i++)
+                    __builtin_memcpy(kr[t * NQ + i], __builtin_assume_aligned(k + i * PE * G, 4 * KW), 4 * KW);
+            }
+        };
+        auto loadV = [&](int buf) {
             if constexpr (F) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const E *v = Vc + max(toff[wave][buf][pg_at(i, h)], 0ll) + NB * col;
+                for (int i = 0; i < NV; i++) {
+                    const E *v = Vc + max(toff[wave][buf][pg_at<W>(i, g)], 0ll) + NB * col;
                     vr[i][VW - 1] = 0;
                     __builtin_memcpy(vr[i], v, NB * cs);
                 }
@@ -227,10 +238,9 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
             }
         };
         int j = j0 + (ROWS ? 0 : wave), buf = 0, ahead = page(j + step);
-        long long off = elems(j, page(j));
         if (j < j1) {
-            loadK(off);
-            loadV(0, off);
+            loadK(0, elems(j, page(j)));
+            loadV(0);
         }
         for (; j < j1; j += step, buf ^= 1) {
             const int t0 = pg_tile<32>(rg, j);
@@ -238,31 +248,38 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
             const long long next = elems(j + step, ahead);
             ahead = page(j + 2 * step);
             // scores
-            f32x16 z;
+            float e[NE];
 #pragma unroll
-            for (int i = 0; i < 16; i++) z[i] = 0.f;
-            if (off < 0) kr[0][0] = ~0u;
-            if constexpr (F) {
+            for (int t = 0; t < TB; t++) {
+                Acc z;
 #pragma unroll
-                for (int i = 0; i < NK; i++)
+                for (int i = 0; i < NR; i++) z[i] = 0.f;
+                if (lost[t]) kr[t * NQ][0] = ~0u;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float k;
-                        if constexpr (C == TLG_F32) k = __uint_as_float(kr[i][e]);
-                        else k = (float)__builtin_bit_cast(E, (unsigned short)(kr[i][e / 2] >> (e & 1) * 16));
-                        z = __builtin_amdgcn_mfma_f32_32x32x2f32(k, __uint_as_float(qf[i][e]), z, 0, 0, 0);
+                for (int i = 0; i < NQ; i++) {
+                    unsigned *k = kr[t * NQ + i];
+                    if constexpr (!F) z = pg_mfma<T, W>(u32x4{k[0], k[1], k[2], k[3]}, qf[i], z);
+                    else {
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            float f;
+                            if constexpr (C == TLG_F32) f = __uint_as_float(k[x]);
+                            else f = (float)__builtin_bit_cast(E, (unsigned short)(k[x / 2] >> (x & 1) * 16));
+                            z = pg_mfma32<W>(f, __uint_as_float(qf[i][x]), z);
+                        }
                     }
-            } else {
+                }
 #pragma unroll
-                for (int i = 0; i < NK; i++) z = pg_mfma<T>(u32x4{kr[i][0], kr[i][1], kr[i][2], kr[i][3]}, qf[i], z);
+                for (int i = 0; i < NR; i++) e[t * NR + i] = z[i];
             }
-            if (more) loadK(next);
+            if (more) loadK(buf ^ 1, next);
             // weights
             const bool full = t0 + 31 <= rg.pmin && (rg.lomax <= t0 || t0 + 31 < a.sinks);
-            float e[16];
+            if (!full) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) e[i] = full || pg_sees(a, t0 + pg_at(i, h), p, from) ? z[i] : -INFINITY;
-            pg_weights<16, NB>(e, a.c, R, l, o);
+                for (int i = 0; i < NE; i++) e[i] = pg_sees(a, t0 + pg_at<W>(i, g), p, from) ? e[i] : -INFINITY;
+            }
+            pg_weights<W, NE, NB>(e, a.c, R, l, o);
             bool odd = false;
             if (!full) {
 #pragma unroll
@@ -270,7 +287,7 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
                     bool hit = false;
 #pragma unroll
                     for (int k = 0; k < VW; k++) hit |= pg_clean<C>(vr[i][k]);
-                    const int t = F ? pg_at(i, h) : (lane + 64 * i) / (HD / 8);
+                    const int t = F ? pg_at<W>(i, g) : (lane + 64 * i) / (HD / 8);
                     odd |= hit && t0 + t <= rg.pmax;
                 }
                 odd = __any(odd);
@@ -278,15 +295,15 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
             // values
             if constexpr (F) {
 #pragma unroll
-                for (int i = 0; i < 16; i++)
+                for (int i = 0; i < NV; i++)
 #pragma unroll
                     for (int k = 0; k < NB; k++) {
                         float v;
                         if constexpr (C == TLG_F32) v = __uint_as_float(vr[i][k]);
                         else v = (float)__builtin_bit_cast(E, (unsigned short)(vr[i][k / 2] >> (k & 1) * 16));
-                        o[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, e[i], o[k], 0, 0, 0);
+                        o[k] = pg_mfma32<W>(v, e[i], o[k]);
                     }
-                if (more) loadV(buf ^ 1, next);
+                if (more) loadV(buf ^ 1);
             } else {
                 pg_wave_sync();
 #pragma unroll
@@ -294,108 +311,101 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128) || HD == 256 ? 1 :
                     const int ch = lane + 64 * i, t = ch / (HD / 8), d = ch % (HD / 8) * 8;
                     *(u32x4 *)(vs + t * VST + d) = u32x4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
                 }
-                if (more) loadV(buf ^ 1, next);
+                if (more) loadV(buf ^ 1);
                 pg_wave_sync();
-                u32x4 pf[2];
+                u32x4 pf[NE / 8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) pf[i / 4][i & 3] = pg_pack<T>(e[2 * i], e[2 * i + 1]);
-                typedef short s16x4 __attribute__((ext_vector_type(4)));
-                typedef __attribute__((address_space(3))) s16x4 *lds;
-                const E *vt = vs + (4 * h + (lane >> 2 & 3)) * VST + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+                for (int i = 0; i < NE / 2; i++) pf[i / 4][i & 3] = pg_pack<T>(e[2 * i], e[2 * i + 1]);
+                // sixteen lanes read four tokens of sixteen elements and get a column of them each
+                const E *vt = vs + (4 * g + (lane >> 2 & 3)) * VST + (W == 32 ? 16 * (lane >> 4 & 1) : 0) + 4 * (lane & 3);
 #pragma unroll
                 for (int k = 0; k < NB; k++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(vt + 16 * i * VST + 32 * k)));
-                        const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(vt + (16 * i + 8) * VST + 32 * k)));
-                        o[k] = pg_mfma<T>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[i], o[k]);
+                    for (int i = 0; i < NE / 8; i++) {
+                        const E *v = vt + 16 * i * VST + W * k;
+                        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v));
+                        const u32x2 v1 =
+                            __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + 4 * G * VST)));
+                        o[k] = pg_mfma<T, W>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[i], o[k]);
                     }
             }
-            if (odd) pg_special<C, NB>(av, o, e, t0, rg.pmax, p, from, [&](int k) { return toff[wave][buf][k]; }, at);
-            off = next;
+            if (odd)
+                pg_special<C, W, NB>(a, o, e, (float *)(mem + wave * PW), (const char *)Vc, t0, rg.pmax, p, from,
+                                     [&](int k) { return toff[wave][buf][k]; }, at);
         }
-        l = pg_both_sum(l);
+        l = pg_gsum<W>(l);
         if constexpr (ROWS) {
             if (!live) return;
-            if constexpr (F) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float x[NB];
+            for (int i = 0; i < NR; i++) {
+                float x[NB];
 #pragma unroll
-                    for (int k = 0; k < NB; k++) x[k] = o[k][i];
-                    pg_out<T, NB>(a, HD, s, parts, r, kvh * a.G + g, NB * pg_at(i, h), l, x);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < NB; k++)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        float x[4] = {o[k][i], o[k][i + 1], o[k][i + 2], o[k][i + 3]};
-                        pg_out<T, 4>(a, HD, s, parts, r, kvh * a.G + g, 32 * k + pg_at(i, h), l, x);
-                    }
+                for (int k = 0; k < NB; k++) x[k] = o[k][i];
+                pg_out<T, NB>(a, HD, s, parts, r, kvh * a.G + gq, NB * pg_at<W>(i, g), l, x);
             }
-            if (h == 0) pg_out_sums(a, s, parts, r, kvh * a.G + g, R, l);
+            if (g == 0) pg_out_sums(a, s, parts, r, kvh * a.G + gq, R, l);
             return;
         } else {
             // the waves' sums against the largest of their references
-            if (h == 0) {
+            if (g == 0) {
                 red[wave][0][col] = R;
                 red[wave][1][col] = l;
             }
             __syncthreads();
             auto top = [&](int c) { return fmaxf(fmaxf(red[0][0][c], red[1][0][c]), fmaxf(red[2][0][c], red[3][0][c])); };
             const float mine = top(col), f = __builtin_amdgcn_exp2f(R - (mine == -INFINITY ? 0.f : mine));
-            const int oc = threadIdx.x >> 3, om = threadIdx.x & 7;     // the thread's column and four rows of each block
+            // the thread's column, four rows of a block, and which of MB blocks
+            const int ob = threadIdx.x / (W * W / 4), oc = threadIdx.x / (W / 4) % W, om = threadIdx.x % (W / 4) * 4;
             const float Rt = top(oc);
-            float lt = 0.f, x[4 * NB];
+            float lt = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; w++)
                 lt += red[w][1][oc] * __builtin_amdgcn_exp2f(red[w][0][oc] - (Rt == -INFINITY ? 0.f : Rt));
+            const int orh = rh0 + oc, oi = min(orh, cols - 1) / a.G, hq = kvh * a.G + min(orh, cols - 1) - oi * a.G;
             float *mg = (float *)mem;
 #pragma unroll
-            for (int k = 0; k < NB; k++) {
+            for (int k0 = 0; k0 < NB; k0 += MB) {
+                if (k0) __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *(f32x4 *)(mg + (wave * 32 + col) * 36 + 8 * i + 4 * h) =
-                        f32x4{o[k][4 * i], o[k][4 * i + 1], o[k][4 * i + 2], o[k][4 * i + 3]} * f;
+                for (int k = 0; k < MB; k++)
+#pragma unroll
+                    for (int i = 0; i < NR; i += 4)
+                        *(f32x4 *)(mg + ((wave * MB + k) * W + col) * MS + pg_at<W>(i, g)) =
+                            f32x4{o[k0 + k][i], o[k0 + k][i + 1], o[k0 + k][i + 2], o[k0 + k][i + 3]} * f;
                 __syncthreads();
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (ob < MB && orh < cols) {
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < 4; w++) v += *(const f32x4 *)(mg + (w * 32 + oc) * 36 + 4 * om);
+                    for (int w = 0; w < 4; w++) v += *(const f32x4 *)(mg + ((w * MB + ob) * W + oc) * MS + om);
+                    float x[4] = {v[0], v[1], v[2], v[3]};
+                    if constexpr (F) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[F ? i * NB + k : 4 * k + i] = v[i];
-                __syncthreads();
-            }
-            const int orh = rh0 + oc;
-            if (orh < cols) {
-                const int oi = orh / a.G, hq = kvh * a.G + orh - oi * a.G;
-                if constexpr (F) pg_out<T, 4 * NB>(a, HD, s, parts, q.lo + oi, hq, 4 * om * NB, lt, x);
-                else {
-#pragma unroll
-                    for (int k = 0; k < NB; k++) pg_out<T, 4>(a, HD, s, parts, q.lo + oi, hq, 32 * k + 4 * om, lt, x + 4 * k);
+                        for (int i = 0; i < 4; i++) pg_out<T, 1>(a, HD, s, parts, q.lo + oi, hq, at(k0 + ob, om + i), lt, x + i);
+                    } else pg_out<T, 4>(a, HD, s, parts, q.lo + oi, hq, at(k0 + ob, om), lt, x);
                 }
-                if (om == 0) pg_out_sums(a, s, parts, q.lo + oi, hq, Rt, lt);
             }
+            if (ob == 0 && om == 0 && orh < cols) pg_out_sums(a, s, parts, q.lo + oi, hq, Rt, lt);
+            __syncthreads();                             // before another tile's waves write here
         }
     }
 }
 
 // The sums of the workgroups that shared a row's tokens: one wave a row and head.  Tiles
-// of sequences of at most `few` columns had 32 of them, others `big` (their tokens in
+// of sequences of at most `few` columns had `small` of them, others `big` (their tokens in
 // tiles of 32 or, with the flag, 64).
-template <int T> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int few, int big, int by64)
+template <int T, int U> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int few, int small, int big, int by64)
 {
     const int lane = threadIdx.x & 63;
     const long long rhd = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int r = (int)(rhd / a.H), head = (int)(rhd - (long long)r * a.H);
+    const int r = __builtin_amdgcn_readfirstlane((int)(rhd / a.H)), head = __builtin_amdgcn_readfirstlane((int)(rhd % a.H));
     if (r >= a.b.N) return;
     const int b = pg_search(a.b.B, r, [&](int i) { return pg_row0(a.b, i); });
     const Seq q = pg_seq(a.b, b);
     if (r < q.lo || r >= q.lo + q.n) return;
-    const int cols = q.n * a.G, rh = (r - q.lo) * a.G + head % a.G, w = cols <= few ? 32 : big;
+    const int cols = q.n * a.G, rh = (r - q.lo) * a.G + head % a.G, w = cols <= few ? small : big;
     const int rh0 = rh / w * w, rh1 = min(rh0 + w, cols);
-    const int parts = cols > few && by64 ? pg_parts<64>(a.S, pg_range<64>(a, q, rh0, rh1).total)
-                                         : pg_parts<32>(a.S, pg_range<32>(a, q, rh0, rh1).total);
+    const int parts = cols > few && by64 ? pg_parts<64>(a, pg_range<64>(a, q, rh0, rh1).total)
+                                         : pg_parts<32>(a, pg_range<32>(a, q, rh0, rh1).total);
     if (parts < 2) return;
     const long long row = (long long)r * a.H + head, all = (long long)a.b.N * a.H;
     float R = -INFINITY, l = 0.f;
@@ -404,6 +414,12 @@ template <int T> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a,
         R = m.x;
         l = m.y;
     }
+    // U workgroups' sums in flight at a time, four elements a lane (lanes beyond hd: none)
+    const float *po = a.po + row * hd + 4 * lane;
+    const bool in = 4 * lane < hd;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, v[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) v[i] = in ? *(const f32x4 *)(po + min(i, parts - 1) * all * hd) : x;
     float top = R;
 #pragma unroll
     for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
@@ -411,20 +427,18 @@ template <int T> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a,
     l *= f;
 #pragma unroll
     for (int o = 32; o; o /= 2) l += __shfl_xor(l, o);
-    const float *po = a.po + row * hd;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < parts; s++) {
-        const float fs = __shfl(f, s);
+    for (int s = 0; s < parts; s += U) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i * 64 + lane < hd) x[i] = fmaf(fs, po[s * all * hd + i * 64 + lane], x[i]);
+        for (int i = 0; i < U; i++) {
+            const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(s + i, 63)));
+            if (s + i < parts) x += fs * v[i];
+            if (s + U < parts) v[i] = in ? *(const f32x4 *)(po + min(s + U + i, parts - 1) * all * hd) : x;
+        }
     }
-    const float inv = pg_inverse(l);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (i * 64 + lane < hd)
-            ((typename ElT<T>::E *)a.out)[(long long)r * a.ldo + (long long)head * hd + i * 64 + lane] =
-                (typename ElT<T>::E)(l == 0.f ? 0.f : x[i] * inv);
+    float y[4] = {x[0], x[1], x[2], x[3]};
+    AttnArgs one = a;
+    one.lse = nullptr;
+    if (in) pg_out<T, 4>(one, hd, 0, 1, r, head, 4 * lane, l, y);
     if (a.lse && lane == 0) a.lse[row] = pg_lse(top, l);
 }
 
@@ -459,7 +473,7 @@ static int pg_check(const char *who, const TlgPages *c, const TlgBatch *b, int t
         return tlg_fail(TLG_EINVAL, "%s: row0 %p len %p table %p", who, (const void *)b->row0, (const void *)b->len,
                         (const void *)b->table);
     *o = PgBatch{b->row0, b->len, b->table, b->B, b->N, b->ldt, c->page, c->n_pages,
-                 (unsigned)(((1ull << 32) + c->page - 1) / c->page), c->page_ld, c->tok_ld, c->head_ld};
+                 0xffffffffu / (unsigned)c->page, c->page_ld, c->tok_ld, c->head_ld};
     *work = 1;
     return TLG_OK;
 }
@@ -518,10 +532,12 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 // and, where the numbers of rows differ, the former for the sequences of few.
 #define PG_FEW 32
 #define PG_FILL 1024                 /* workgroups wanted */
+#define PG_MIN 8                     /* tiles of 32 tokens of a workgroup, at least */
 struct Plan {
     bool few, both;
-    unsigned tiles, slots;           // of 32 columns of a sequence, of 128 of all
-    int S;
+    int W;                           // columns of a workgroup of few
+    unsigned tiles, slots;           // of W columns of a sequence, of 128 of all
+    int S, per;
     size_t sums;                     // bytes of the partial sums, before their references
 };
 static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int H)
@@ -531,15 +547,19 @@ static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int H)
     const long long cols = (long long)rows * G, room = (long long)b->ldt * c->page,
                     len = b->max_len && b->max_len < room ? b->max_len : room;
     p.few = cols <= PG_FEW;
-    p.tiles = p.few ? (unsigned)((cols + 31) / 32) : 1;
+    p.W = cols <= 16 ? 16 : 32;
+    p.tiles = p.few ? (unsigned)((cols + p.W - 1) / p.W) : 1;
     p.slots = (unsigned)((long long)b->N * G / 128 + b->B);
     p.both = !p.few && (long long)b->B * rows > b->N;
     const long long groups = p.few ? (long long)b->B * p.tiles * c->KV : (long long)p.slots * c->KV,
-                    row = (long long)b->N * H * (c->hd + 2) * 4;
+                    row = (long long)b->N * H * (c->hd + 2) * 4, tiles = (len + 31) / 32;
     long long S = PG_FILL / groups;
-    if (S > len / PG_MIN) S = len / PG_MIN;
+    if (S > tiles / PG_MIN) S = tiles / PG_MIN;
     if (S > (128ll << 20) / row) S = (128ll << 20) / row;
     p.S = S < 1 ? 1 : S > 64 ? 64 : (int)S;
+    p.per = (int)((tiles + p.S - 1) / p.S);
+    if (p.per < PG_MIN) p.per = PG_MIN;
+    p.per += p.per & 1;
     p.sums = p.S > 1 ? (size_t)p.S * b->N * H * c->hd * 4 : 0;
     return p;
 }
@@ -554,21 +574,32 @@ extern "C" size_t tlg_paged_attn_ws_bytes(const TlgPages *c, const TlgBatch *b, 
     return p.sums ? p.sums + (size_t)p.S * b->N * H * 8 : 0;
 }
 
-template <int T, int C, bool ROWS> static void pg_direct(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
+template <int T, int C, int W, bool ROWS> static void pg_direct(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
 {
-    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<T, C, 32, ROWS>), grid, dim3(256), 0, st, a);
-    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<T, C, 64, ROWS>), grid, dim3(256), 0, st, a);
-    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<T, C, 96, ROWS>), grid, dim3(256), 0, st, a);
-    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<T, C, 128, ROWS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_paged_direct<T, C, 256, ROWS>), grid, dim3(256), 0, st, a);
+    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<T, C, 32, W, ROWS>), grid, dim3(256), 0, st, a);
+    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<T, C, 64, W, ROWS>), grid, dim3(256), 0, st, a);
+    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<T, C, 96, W, ROWS>), grid, dim3(256), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<T, C, 128, W, ROWS>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_direct<T, C, 256, W, ROWS>), grid, dim3(256), 0, st, a);
 }
-template <bool ROWS> static void pg_direct(const AttnArgs &a, int type, int kv, int hd, dim3 grid, hipStream_t st)
+template <int W> static void pg_few(const AttnArgs &a, int type, int kv, int hd, dim3 grid, hipStream_t st)
 {
-    if (type == TLG_F16) pg_direct<TLG_F16, TLG_F16, ROWS>(a, hd, grid, st);
-    else if (type == TLG_BF16) pg_direct<TLG_BF16, TLG_BF16, ROWS>(a, hd, grid, st);
-    else if (kv == TLG_F32) pg_direct<TLG_F32, TLG_F32, ROWS>(a, hd, grid, st);
-    else if (kv == TLG_F16) pg_direct<TLG_F32, TLG_F16, ROWS>(a, hd, grid, st);
-    else pg_direct<TLG_F32, TLG_BF16, ROWS>(a, hd, grid, st);
+    if (type == TLG_F16) pg_direct<TLG_F16, TLG_F16, W, false>(a, hd, grid, st);
+    else if (type == TLG_BF16) pg_direct<TLG_BF16, TLG_BF16, W, false>(a, hd, grid, st);
+    else if (kv == TLG_F32) pg_direct<TLG_F32, TLG_F32, W, false>(a, hd, grid, st);
+    else if (kv == TLG_F16) pg_direct<TLG_F32, TLG_F16, W, false>(a, hd, grid, st);
+    else pg_direct<TLG_F32, TLG_BF16, W, false>(a, hd, grid, st);
+}
+template <int T> static void pg_join(const AttnArgs &a, int hd, int few, int small, int big, int by64, dim3 grid, hipStream_t st)
+{
+    if (a.S <= 4) hipLaunchKernelGGL((k_paged_join<T, 4>), grid, dim3(256), 0, st, a, hd, few, small, big, by64);
+    else hipLaunchKernelGGL((k_paged_join<T, 16>), grid, dim3(256), 0, st, a, hd, few, small, big, by64);
+}
+static void pg_rows32(const AttnArgs &a, int kv, int hd, dim3 grid, hipStream_t st)
+{
+    if (kv == TLG_F32) pg_direct<TLG_F32, TLG_F32, 32, true>(a, hd, grid, st);
+    else if (kv == TLG_F16) pg_direct<TLG_F32, TLG_F16, 32, true>(a, hd, grid, st);
+    else pg_direct<TLG_F32, TLG_BF16, 32, true>(a, hd, grid, st);
 }
 
 extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const void *q, int type, long long ldq, int H,
@@ -610,25 +641,31 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
     }
     const Plan p = pg_plan(c, b, H);
     a.S = p.S;
+    a.per = p.per;
     a.few = 0;
     a.many = p.few ? INT_MAX : PG_FEW;
     a.po = (float *)ws;
     a.pm = (float *)((char *)ws + p.sums);
     hipStream_t st = ST(stream);
-    if (p.few || p.both)
-        pg_direct<false>(a, type, c->type, c->hd, dim3((unsigned)b->B * c->KV * p.S, p.tiles), st);
+    if (p.few || p.both) {
+        const dim3 grid((unsigned)b->B * c->KV * p.S, p.tiles);
+        if (p.W == 16) pg_few<16>(a, type, c->type, c->hd, grid, st);
+        else pg_few<32>(a, type, c->type, c->hd, grid, st);
+    }
     if (!p.few) {
         a.few = p.both ? PG_FEW : 0;
         a.many = INT_MAX;
-        pg_direct<true>(a, type, c->type, c->hd, dim3(p.slots * c->KV * p.S), st);
+        if (type == TLG_F32) pg_rows32(a, c->type, c->hd, dim3(p.slots * c->KV * p.S), st);
+        else pg_tile_launch(a, type, c->hd, p.slots * c->KV * p.S, st);
     }
     if (p.S > 1) {
-        const int big = 32, by64 = 0;
+        // few: every tile's columns were p.W, else those of the rows' kernel
+        const int few = p.few ? INT_MAX : a.few, big = type == TLG_F32 ? 32 : PGT_ROWS,
+                  by64 = type != TLG_F32 && PGT_TOKENS(c->hd) == 64;
         const dim3 grid((unsigned)(((long long)b->N * H + 3) / 4));
-        if (type == TLG_F32) hipLaunchKernelGGL((k_paged_join<TLG_F32>), grid, dim3(256), 0, st, a, c->hd, a.few, big, by64);
-        else if (type == TLG_F16)
-            hipLaunchKernelGGL((k_paged_join<TLG_F16>), grid, dim3(256), 0, st, a, c->hd, a.few, big, by64);
-        else hipLaunchKernelGGL((k_paged_join<TLG_BF16>), grid, dim3(256), 0, st, a, c->hd, a.few, big, by64);
+        if (type == TLG_F32) pg_join<TLG_F32>(a, c->hd, few, p.W, big, by64, grid, st);
+        else if (type == TLG_F16) pg_join<TLG_F16>(a, c->hd, few, p.W, big, by64, grid, st);
+        else pg_join<TLG_BF16>(a, c->hd, few, p.W, big, by64, grid, st);
     }
     LAUNCH_CHECK();
     return TLG_OK;

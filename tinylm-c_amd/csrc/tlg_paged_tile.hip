@@ -1,0 +1,190 @@
+// tlg_paged_tile.hip -- attention of many rows over a paged KV cache, 16-bit
+// (include/tlserve.h): prompts and long chunks, bound by the matrix cores.
+//
+// A workgroup has 128 columns (rows times query heads of one KV head), 32 a wave, and
+// walks over the tokens that any of them sees in tiles of 64, which its threads
+// bring from the pages into LDS, rows as they lie in the cache, while the waves work on
+// the tile before: two buffers, one barrier a tile.  The products are those of
+// k_paged_direct (scores transposed, weights staying in their lanes).  Rows in LDS are
+// apart by what makes the reads free of bank conflicts: keys are read 16 bytes a lane
+// down 16 tokens (row lengths 4 modulo 64 banks), values four tokens by 32 elements
+// (16 modulo 32 banks).
+#include "tlg_paged.h"
+
+template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_tile(AttnArgs a)
+{
+    typedef typename ElT<T>::E E;
+    constexpr int TT = PGT_TOKENS(HD), NB = HD / 32, NT = TT / 32, CH = HD / 8, NL = TT * CH / 256;
+    constexpr int KST = HD + 8, VST = (HD / 2) % 64 == 16 || (HD / 2) % 64 == 48 ? HD : HD + 32;
+    __shared__ __align__(16) E ks[2][TT * KST], vs[2][TT * VST];
+    __shared__ float scratch[4][256];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x % a.KV, s = blockIdx.x / a.KV % a.S, y = blockIdx.x / a.KV / a.S;
+    auto start = [&](int i) { return (long long)pg_row0(a.b, i) * a.G / PGT_ROWS + i; };
+    const int b = pg_search(a.b.B, y, start), base = (int)(y - start(b)) * PGT_ROWS;
+    const Seq q = pg_seq(a.b, b);
+    const int cols = q.n * a.G;
+    if (base < 0 || base >= cols || cols <= a.few) return;
+    const Range rg = pg_range<TT>(a, q, base, min(base + PGT_ROWS, cols));
+    const int parts = pg_parts<TT>(a, rg.total);
+    if (s >= parts) return;
+    const int j0 = (int)((long long)rg.total * s / parts), j1 = (int)((long long)rg.total * (s + 1) / parts);
+    const int *table = a.b.table + (long long)b * a.b.ldt;
+    const E *Kc = (const E *)a.K + kvh * a.b.head_ld, *Vc = (const E *)a.V + kvh * a.b.head_ld;
+
+    // the wave's and the lane's columns
+    const int rh0 = min(base + 32 * wave, cols - 1), rh = base + 32 * wave + col;
+    const bool some = base + 32 * wave < cols, live = rh < cols;
+    const Range rw = pg_range<TT>(a, q, rh0, min(rh0 + 32, cols));
+    const int lomin = pg_from(a, rw.pmin);
+    const int ci = min(rh, cols - 1) / a.G, g = min(rh, cols - 1) - ci * a.G;
+    const int r = q.lo + ci, p = live ? pg_pos(a, q, ci) : -1, from = pg_from(a, p);
+    u32x4 qf[HD / 16];
+    {
+        const E *qp = (const E *)a.q + (long long)r * a.ldq + (kvh * a.G + g) * HD + 8 * h;
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) {
+            qf[i] = *(const u32x4 *)(qp + 16 * i);
+            if (!live) qf[i] = u32x4{0, 0, 0, 0};
+        }
+    }
+    f32x16 o[NB];
+#pragma unroll
+    for (int k = 0; k < NB; k++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[k][i] = 0.f;
+    float R = -INFINITY, l = 0.f;
+
+    // the thread's pieces of a tile: token (tid + 256 i) / CH, elements 8 ((tid + 256 i) % CH)
+    int pg[NL];
+    u32x4 kr[NL], vr[NL];
+    bool lost[NL];
+    auto page = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int t = pg_tile<TT>(rg, j) + (tid + 256 * i) / CH, n = pg_of(a.b, t);
+            pg[i] = j < j1 && t <= rg.pmax && n < a.b.ldt ? table[n] : -1;
+        }
+    };
+    auto load = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int ch = tid + 256 * i, t = pg_tile<TT>(rg, j) + ch / CH, n = pg[i];
+            lost[i] = n < 0 || n >= a.b.n_pages;
+            const long long off = (lost[i] ? 0ll : n * a.b.page_ld + (t - pg_of(a.b, t) * a.b.page) * a.b.tok_ld) + ch % CH * 8;
+            kr[i] = *(const u32x4 *)(Kc + off);
+            vr[i] = *(const u32x4 *)(Vc + off);
+        }
+    };
+    auto whole = [&](const Range &x, int t0) { return t0 + TT - 1 <= x.pmin && (x.lomax <= t0 || t0 + TT - 1 < a.sinks); };
+    // to LDS; true if values of a tile that some column sees in part had to be cleaned
+    auto put = [&](int j, int buf) {
+        bool odd = false;
+        const int t0 = pg_tile<TT>(rg, j);
+        if (!whole(rg, t0)) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                bool hit = false;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    unsigned w = vr[i][k];
+                    hit |= pg_clean<T>(w);
+                    vr[i][k] = w;
+                }
+                odd |= hit && t0 + (tid + 256 * i) / CH <= rg.pmax;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int ch = tid + 256 * i, t = ch / CH, d = ch % CH * 8;
+            if (lost[i]) kr[i][0] = ~0u;
+            *(u32x4 *)(ks[buf] + t * KST + d) = kr[i];
+            *(u32x4 *)(vs[buf] + t * VST + d) = vr[i];
+        }
+        return odd;
+    };
+    bool odd = false;
+    if (j0 < j1) {
+        page(j0);
+        load(j0);
+        page(j0 + 1);
+        odd = __syncthreads_or(put(j0, 0));
+    }
+    for (int j = j0, buf = 0; j < j1; j++, buf ^= 1) {
+        const bool more = j + 1 < j1;
+        if (more) {
+            load(j + 1);
+            page(j + 2);
+        }
+        const int t0 = pg_tile<TT>(rg, j);
+        if (some && t0 <= rw.pmax && (t0 + TT > lomin || t0 < a.sinks)) {
+            float e[16 * NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                f32x16 z;
+#pragma unroll
+                for (int i = 0; i < 16; i++) z[i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++)
+                    z = pg_mfma<T, 32>(*(const u32x4 *)(ks[buf] + (32 * t + col) * KST + 16 * i + 8 * h), qf[i], z);
+#pragma unroll
+                for (int i = 0; i < 16; i++) e[16 * t + i] = z[i];
+            }
+            const bool full = whole(rw, t0);
+            if (!full) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        e[16 * t + i] = pg_sees(a, t0 + 32 * t + pg_at<32>(i, h), p, from) ? e[16 * t + i] : -INFINITY;
+            }
+            pg_weights<32, 16 * NT, NB>(e, a.c, R, l, o);
+            u32x4 pf[2 * NT];
+#pragma unroll
+            for (int i = 0; i < 8 * NT; i++) pf[i / 4][i & 3] = pg_pack<T>(e[2 * i], e[2 * i + 1]);
+            const E *vt = vs[buf] + (4 * h + (lane >> 2 & 3)) * VST + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+#pragma unroll
+            for (int i = 0; i < 2 * NT; i++)
+#pragma unroll
+                for (int k = 0; k < NB; k++) {
+                    const E *v = vt + 16 * i * VST + 32 * k;
+                    const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v));
+                    const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + 8 * VST)));
+                    o[k] = pg_mfma<T, 32>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[i], o[k]);
+                }
+            if (odd && !full) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    pg_special<T, 32, NB>(a, o, e + 16 * t, scratch[wave], (const char *)Vc, t0 + 32 * t, rg.pmax, p, from,
+                                          [&](int k) { return pg_token(a.b, table, t0 + 32 * t + k); },
+                                          [](int blk, int m) { return 32 * blk + m; });
+            }
+        }
+        if (more) odd = __syncthreads_or(put(j + 1, buf ^ 1));
+    }
+    l = pg_gsum<32>(l);
+    if (!live) return;
+#pragma unroll
+    for (int k = 0; k < NB; k++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float x[4] = {o[k][i], o[k][i + 1], o[k][i + 2], o[k][i + 3]};
+            pg_out<T, 4>(a, HD, s, parts, r, kvh * a.G + g, 32 * k + pg_at<32>(i, h), l, x);
+        }
+    if (h == 0) pg_out_sums(a, s, parts, r, kvh * a.G + g, R, l);
+}
+
+template <int T> static void launch(const AttnArgs &a, int hd, unsigned grid, hipStream_t st)
+{
+    if (hd == 32) hipLaunchKernelGGL((k_paged_tile<T, 32>), dim3(grid), dim3(256), 0, st, a);
+    else if (hd == 64) hipLaunchKernelGGL((k_paged_tile<T, 64>), dim3(grid), dim3(256), 0, st, a);
+    else if (hd == 96) hipLaunchKernelGGL((k_paged_tile<T, 96>), dim3(grid), dim3(256), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((k_paged_tile<T, 128>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_tile<T, 256>), dim3(grid), dim3(256), 0, st, a);
+}
+void pg_tile_launch(const AttnArgs &a, int type, int hd, unsigned grid, hipStream_t st)
+{
+    if (type == TLG_F16) launch<TLG_F16>(a, hd, grid, st);
+    else launch<TLG_BF16>(a, hd, grid, st);
+}
