@@ -58,10 +58,18 @@ struct AttnArgs {
     float *lse;
     long long ldq, ldo;
     int H, KV, G, win, sinks;
-    int S, per;                  // workgroups that share a tile's tokens, at most, and how much each takes
-    int few, many;               // sequences of at most `few` rows times heads are left out, of more than `many` too
+    int few, many;               // columns (rows times heads of a KV head) of the sequences that a launch takes: more than few, many at most
     float c;                     // scale log2 e
-    float *po, *pm;              // S > 1: [S][N][H][hd] sums and [S][N][H][2] references and weights
+    // rows' kernels: S workgroups share a tile's tokens, `per` tiles of 32 tokens each; S > 1:
+    // their sums [S][N][H][hd] and references and weights [S][N][H][2]
+    int S, per;
+    float *po, *pm;
+    // k_paged_direct: P workgroups of a KV head share the tokens of all sequences evenly (0: one a
+    // sequence), with the place of each sequence [B + 1], the number that took part, and the
+    // sums of tiles that are not one workgroup's, [P][KV][2][W][hd] and [..][2]
+    int P;
+    long long *place;
+    float *eo, *em;
 };
 
 // Base-2 scores against a reference: with R the largest c (q . k) of a row so far,
@@ -267,8 +275,7 @@ __device__ __forceinline__ void pg_weights(float (&z)[N], float c, float &R, flo
     l += (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// K consecutive elements of a row of out (final: weighted by 1 / l) or of the sums of
-// workgroup s of several.
+// K consecutive elements of a row of out, weighted by 1 / l.
 __device__ __forceinline__ float pg_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 template <int T, int K> __device__ __forceinline__ void pg_put(char *p, const float *x)
 {
@@ -278,11 +285,16 @@ template <int T, int K> __device__ __forceinline__ void pg_put(char *p, const fl
     for (int i = 0; i < K; i++) v[i] = (E)x[i];
     __builtin_memcpy(__builtin_assume_aligned(p, K * sizeof(E) % 16 == 0 ? 16 : K * sizeof(E) % 8 == 0 ? 8 : 4), v, sizeof v);
 }
-template <int T, int K>
-__device__ __forceinline__ void pg_out(const AttnArgs &a, int hd, int s, int parts, int r, int head, int d, float l, float *x)
+__device__ __forceinline__ float pg_lse(float R, float l)
 {
-    if (parts > 1) {
-        pg_put<TLG_F32, K>((char *)(a.po + (((long long)s * a.b.N + r) * a.H + head) * hd + d), x);
+    return l == 0.f ? -INFINITY : ((R == -INFINITY ? 0.f : R) + __builtin_amdgcn_logf(l)) * 0.69314718056f;
+}
+// (sums: where they go if they are not the row's only ones)
+template <int T, int K>
+__device__ __forceinline__ void pg_out(const AttnArgs &a, int hd, float *sums, int r, int head, int d, float l, float *x)
+{
+    if (sums) {
+        pg_put<TLG_F32, K>((char *)(sums + d), x);
         return;
     }
     const float f = pg_inverse(l);
@@ -290,14 +302,15 @@ __device__ __forceinline__ void pg_out(const AttnArgs &a, int hd, int s, int par
     for (int i = 0; i < K; i++) x[i] = l == 0.f ? 0.f : x[i] * f;
     pg_put<T, K>(a.out + ((long long)r * a.ldo + (long long)head * hd + d) * (T == TLG_F32 ? 4 : 2), x);
 }
-__device__ __forceinline__ float pg_lse(float R, float l)
+__device__ __forceinline__ void pg_out_sums(const AttnArgs &a, float *sums, int r, int head, float R, float l)
 {
-    return l == 0.f ? -INFINITY : ((R == -INFINITY ? 0.f : R) + __builtin_amdgcn_logf(l)) * 0.69314718056f;
-}
-__device__ __forceinline__ void pg_out_sums(const AttnArgs &a, int s, int parts, int r, int head, float R, float l)
-{
-    if (parts > 1) *(float2 *)(a.pm + (((long long)s * a.b.N + r) * a.H + head) * 2) = float2{R, l};
+    if (sums) *(float2 *)sums = float2{R, l};
     else if (a.lse) a.lse[(long long)r * a.H + head] = pg_lse(R, l);
+}
+// the rows' kernels' sums of workgroup s of several
+__device__ __forceinline__ float *pg_part(const AttnArgs &a, float *p, int w, int s, int parts, int r, int head)
+{
+    return parts > 1 ? p + (((long long)s * a.b.N + r) * a.H + head) * w : nullptr;
 }
 
 // What the launches of tlg_paged_tile.hip take (tlg_paged.hip decides).

@@ -115,6 +115,56 @@ template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(Sto
 }
 
 // --------------------------------------------------------------- attention --
+// Units of a sequence's tiles of W columns (of each of them), 0 where a launch leaves it out.
+template <int W> __device__ __forceinline__ long long pg_units(const AttnArgs &a, const Seq &q)
+{
+    const int cols = q.n * a.G;
+    if (cols <= a.few || cols > a.many) return 0;
+    return max(1, pg_range<32>(a, q, 0, cols).total);
+}
+// Where each sequence's units start, [B + 1] in LDS; the workgroups that take part, each
+// with PG_UNITS at least.  B <= PG_EVEN, 256 threads.
+#define PG_EVEN 1024
+#define PG_UNITS 8
+template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, long long *place)
+{
+    __shared__ long long part[4];
+    const int t = threadIdx.x, per = (a.b.B + 255) / 256, lane = t & 63;
+    long long n[PG_EVEN / 256], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PG_EVEN / 256; i++) {
+        n[i] = 0;
+        if (i < per && t * per + i < a.b.B) {
+            const Seq q = pg_seq(a.b, t * per + i);
+            n[i] = pg_units<W>(a, q) * ((q.n * a.G + W - 1) / W);
+        }
+        sum += n[i];
+    }
+    long long upto = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const long long v = __shfl_up(upto, o);
+        upto += lane >= o ? v : 0;
+    }
+    if (lane == 63) part[t >> 6] = upto;
+    __syncthreads();
+    long long all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        if (w == t >> 6) upto += all;
+        all += part[w];
+    }
+    upto -= sum;
+#pragma unroll
+    for (int i = 0; i < PG_EVEN / 256; i++) {
+        if (i < per && t * per + i < a.b.B) place[t * per + i] = upto;
+        upto += n[i];
+    }
+    if (t == 0) place[a.b.B] = all;
+    __syncthreads();
+    return (int)min((long long)a.P, max(all / PG_UNITS, all > 0 ? 1ll : 0ll));
+}
+
 // Scores are formed transposed, S^T = K Q^T, tokens by columns (rows times query heads
 // of one KV head, so that a key is read once for all heads that share it): a lane then
 // has a share of one column's scores, its softmax needs exchanges between the two or
@@ -127,13 +177,18 @@ template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(Sto
 // tokens' keys (rows of the first operand) in pieces of 16 bytes.  For 16-bit rows the values
 // go through LDS, each wave's own tokens, and are read back transposed; fp32 products
 // take them as they are, rows of V^T being dealt out so that a lane's are contiguous.
-// !ROWS: few columns (a decoded token, a drafted chunk), bound by the cache's bytes: the
-// four waves of a workgroup take every fourth tile of the tokens and join their sums,
-// and S workgroups share a long sequence.  Blocks of W = 16 columns where there are no
-// more: half the registers of 32.  ROWS (fp32): every wave 32 columns of its own,
-// whose keys the waves of a workgroup find in the CU's cache.
+// !ROWS: few columns (a decoded token, a drafted chunk), bound by the cache's bytes.  The
+// tokens of all sequences, tile after tile, are dealt out evenly to the workgroups of a
+// KV head, so that ragged lengths leave none idle; the four waves of a workgroup take
+// every fourth of its tiles and join their sums.  Blocks of W = 16 columns where there
+// are no more: half the registers of 32.  ROWS (fp32): every wave 32 columns of its
+// own, whose keys the waves of a workgroup find in the CU's cache.
+#ifndef PGBX
+#define PGBX 2
+#endif
+#define PGB (T != TLG_F32 && W == 16 && HD == 128 ? PGBX : (T == TLG_F32 && HD >= 128 && W == 32) || HD == 256 ? 1 : 2)
 template <int T, int C, int HD, int W, bool ROWS>
-__global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128 && W == 32) || HD == 256 ? 1 : 2) void k_paged_direct(AttnArgs a)
+__global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
 {
     typedef typename ElT<C>::E E;
     typedef typename AccT<W>::A Acc;
@@ -150,32 +205,68 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128 && W == 32) || HD =
     __shared__ __align__(16) char mem[4 * PW];
     __shared__ long long toff[4][2][32];
     __shared__ float red[4][2][W];
+    __shared__ long long place[ROWS ? 1 : PG_EVEN + 1];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane % W, g = lane / W;
-    const int kvh = blockIdx.x % a.KV, s = blockIdx.x / a.KV % a.S, y = blockIdx.x / a.KV / a.S;
-    int b = y, base = blockIdx.y * W;
-    if (ROWS) {
-        auto start = [&](int i) { return (long long)pg_row0(a.b, i) * a.G / 128 + i; };
-        b = pg_search(a.b.B, y, start);
-        base = (int)(y - start(b)) * 128 + 32 * wave;
-    }
-    const Seq q = pg_seq(a.b, b);
-    const int cols = q.n * a.G;
-    if (base < 0 || base >= cols || cols <= a.few || cols > a.many) return;
-    const int *table = a.b.table + (long long)b * a.b.ldt;
+    const int kvh = blockIdx.x % a.KV, y = blockIdx.x / a.KV;
     const E *Kc = (const E *)a.K + kvh * a.b.head_ld, *Vc = (const E *)a.V + kvh * a.b.head_ld;
     auto at = [](int blk, int m) { return F ? NB * m + blk : W * blk + m; };
     E *vs = (E *)(mem + wave * PW);
 
-    for (int rh0 = base; rh0 < cols; rh0 += W * gridDim.y) {
-        const Range rg = pg_range<32>(a, q, rh0, min(rh0 + W, cols));
-        const int parts = pg_parts<32>(a, rg.total);
-        if (s >= parts) {
-            if (ROWS) return;
-            continue;
+    // the workgroup's share: units [u, u1) of the sequences' tiles of W columns by 32 tokens
+    int b = y;
+    long long u = 0, u1 = 0;
+    if constexpr (ROWS) {
+        auto start = [&](int i) { return (long long)pg_row0(a.b, i) * a.G / 128 + i; };
+        b = pg_search(a.b.B, y / a.S, start);
+        u = y / a.S - start(b);
+    } else if (a.P) {
+        const int P = pg_places<W>(a, place);
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i <= a.b.B + 1; i += 256) a.place[i] = i <= a.b.B ? place[i] : P;
+        if (y >= P) return;
+        u = place[a.b.B] * y / P;
+        u1 = place[a.b.B] * (y + 1) / P;
+        b = pg_search(a.b.B, u, [&](int i) { return place[i]; });       // the last that starts there: it has units
+    }
+    const int s = ROWS ? y % a.S : 0;
+    for (bool first = true; first || (!ROWS && u < u1); first = false) {
+        const Seq q = pg_seq(a.b, b);
+        const int cols = q.n * a.G;
+        int rh0, t0seg = 0, t1seg = INT_MAX;
+        bool only = true;
+        if constexpr (ROWS) {
+            rh0 = (int)u * 128 + 32 * wave;
+            if (u < 0 || rh0 >= cols || cols <= a.few || cols > a.many) return;
+        } else {
+            const long long tot = pg_units<W>(a, q);
+            if (tot == 0) return;                        // without places only: a sequence of no rows, or not this launch's
+            long long in = u - (a.P ? place[b] : 0);
+            rh0 = (int)(in / tot) * W;
+            if (rh0 >= cols) return;
+            if (a.P) {
+                t0seg = (int)(in % tot);
+                t1seg = (int)min(tot, t0seg + u1 - u);
+                only = t0seg == 0 && t1seg == tot;
+                u += t1seg - t0seg;
+            } else {
+                u += tot;
+                u1 = tot * ((cols + W - 1) / W);
+            }
         }
-        const int j0 = (int)((long long)rg.total * s / parts), j1 = (int)((long long)rg.total * (s + 1) / parts);
-        const int step = ROWS ? 1 : 4;
+        const Range rg = pg_range<32>(a, q, rh0, min(rh0 + W, cols));
+        int parts = 1, j0, j1;
+        if constexpr (ROWS) {
+            parts = pg_parts<32>(a, rg.total);
+            if (s >= parts) return;
+            j0 = (int)((long long)rg.total * s / parts);
+            j1 = (int)((long long)rg.total * (s + 1) / parts);
+        } else {
+            j0 = min(t0seg, rg.total);
+            j1 = min(t1seg, rg.total);
+        }
+        constexpr int step = ROWS ? 1 : 4;
+        const int *table = a.b.table + (long long)b * a.b.ldt;
         // the lane's column
         const int rh = rh0 + col, ci = min(rh, cols - 1) / a.G, gq = min(rh, cols - 1) - ci * a.G;
         const bool live = rh < cols;
@@ -341,9 +432,10 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128 && W == 32) || HD =
                 float x[NB];
 #pragma unroll
                 for (int k = 0; k < NB; k++) x[k] = o[k][i];
-                pg_out<T, NB>(a, HD, s, parts, r, kvh * a.G + gq, NB * pg_at<W>(i, g), l, x);
+                pg_out<T, NB>(a, HD, pg_part(a, a.po, HD, s, parts, r, kvh * a.G + gq), r, kvh * a.G + gq, NB * pg_at<W>(i, g), l,
+                              x);
             }
-            if (g == 0) pg_out_sums(a, s, parts, r, kvh * a.G + gq, R, l);
+            if (g == 0) pg_out_sums(a, pg_part(a, a.pm, 2, s, parts, r, kvh * a.G + gq), r, kvh * a.G + gq, R, l);
             return;
         } else {
             // the waves' sums against the largest of their references
@@ -362,6 +454,9 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128 && W == 32) || HD =
             for (int w = 0; w < 4; w++)
                 lt += red[w][1][oc] * __builtin_amdgcn_exp2f(red[w][0][oc] - (Rt == -INFINITY ? 0.f : Rt));
             const int orh = rh0 + oc, oi = min(orh, cols - 1) / a.G, hq = kvh * a.G + min(orh, cols - 1) - oi * a.G;
+            // a tile that goes on from another workgroup's, and one that another goes on with, have places of their own
+            const long long slot = (((long long)y * a.KV + kvh) * 2 + (t0seg == 0)) * W + oc;
+            float *eo = only ? nullptr : a.eo + slot * HD, *em = only ? nullptr : a.em + slot * 2;
             float *mg = (float *)mem;
 #pragma unroll
             for (int k0 = 0; k0 < NB; k0 += MB) {
@@ -380,21 +475,24 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD >= 128 && W == 32) || HD =
                     float x[4] = {v[0], v[1], v[2], v[3]};
                     if constexpr (F) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) pg_out<T, 1>(a, HD, s, parts, q.lo + oi, hq, at(k0 + ob, om + i), lt, x + i);
-                    } else pg_out<T, 4>(a, HD, s, parts, q.lo + oi, hq, at(k0 + ob, om), lt, x);
+                        for (int i = 0; i < 4; i++) pg_out<T, 1>(a, HD, eo, q.lo + oi, hq, at(k0 + ob, om + i), lt, x + i);
+                    } else pg_out<T, 4>(a, HD, eo, q.lo + oi, hq, at(k0 + ob, om), lt, x);
                 }
             }
-            if (ob == 0 && om == 0 && orh < cols) pg_out_sums(a, s, parts, q.lo + oi, hq, Rt, lt);
+            if (ob == 0 && om == 0 && orh < cols) pg_out_sums(a, em, q.lo + oi, hq, Rt, lt);
             __syncthreads();                             // before another tile's waves write here
+            if (a.P)
+                while (u < u1 && place[b + 1] <= u) b++;
         }
     }
 }
 
-// The sums of the workgroups that shared a row's tokens: one wave a row and head.  Tiles
-// of sequences of at most `few` columns had `small` of them, others `big` (their tokens in
-// tiles of 32 or, with the flag, 64).
-template <int T, int U> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int few, int small, int big, int by64)
+// The sums of the workgroups that shared a row's tokens, one wave a row and head.  EVEN:
+// those of k_paged_direct in tiles of `w` columns; else of the rows' kernels, whose tiles of `w`
+// columns had their tokens in tiles of 32 or, with the flag, 64.
+template <int T, bool EVEN> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int w, int by64)
 {
+    constexpr int U = 16;
     const int lane = threadIdx.x & 63;
     const long long rhd = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int r = __builtin_amdgcn_readfirstlane((int)(rhd / a.H)), head = __builtin_amdgcn_readfirstlane((int)(rhd % a.H));
@@ -402,44 +500,63 @@ template <int T, int U> __global__ __launch_bounds__(256) void k_paged_join(Attn
     const int b = pg_search(a.b.B, r, [&](int i) { return pg_row0(a.b, i); });
     const Seq q = pg_seq(a.b, b);
     if (r < q.lo || r >= q.lo + q.n) return;
-    const int cols = q.n * a.G, rh = (r - q.lo) * a.G + head % a.G, w = cols <= few ? small : big;
-    const int rh0 = rh / w * w, rh1 = min(rh0 + w, cols);
-    const int parts = cols > few && by64 ? pg_parts<64>(a, pg_range<64>(a, q, rh0, rh1).total)
-                                         : pg_parts<32>(a, pg_range<32>(a, q, rh0, rh1).total);
-    if (parts < 2) return;
-    const long long row = (long long)r * a.H + head, all = (long long)a.b.N * a.H;
-    float R = -INFINITY, l = 0.f;
-    if (lane < parts) {
-        const float2 m = *(const float2 *)(a.pm + (row + lane * all) * 2);
-        R = m.x;
-        l = m.y;
+    const int cols = q.n * a.G, rh = (r - q.lo) * a.G + head % a.G, kvh = head / a.G;
+    if (cols <= a.few || cols > a.many) return;
+    int parts;
+    long long first, second, apart;                      // places (columns) of the first sums, the second, and from one to the next
+    const float *po, *pm;
+    if constexpr (EVEN) {
+        const long long T0 = a.place[a.b.B], P = a.place[a.b.B + 1], tiles = (cols + w - 1) / w,
+                        tot = (a.place[b + 1] - a.place[b]) / tiles, u = a.place[b] + rh / w * tot;
+        // the workgroup of unit x: the last i with T0 i / P <= x
+        const long long i0 = ((u + 1) * P - 1) / T0, i1 = ((u + tot) * P - 1) / T0;
+        parts = (int)(i1 - i0 + 1);
+        first = ((i0 * a.KV + kvh) * 2 + 1) * w + rh % w;
+        second = ((i0 + 1) * a.KV + kvh) * 2 * w + rh % w;
+        apart = 2ll * a.KV * w;
+        po = a.eo;
+        pm = a.em;
+    } else {
+        const int rh0 = rh / w * w, rh1 = min(rh0 + w, cols);
+        parts = by64 ? pg_parts<64>(a, pg_range<64>(a, q, rh0, rh1).total) : pg_parts<32>(a, pg_range<32>(a, q, rh0, rh1).total);
+        first = (long long)r * a.H + head;
+        apart = (long long)a.b.N * a.H;
+        second = first + apart;
+        po = a.po;
+        pm = a.pm;
     }
-    // U workgroups' sums in flight at a time, four elements a lane (lanes beyond hd: none)
-    const float *po = a.po + row * hd + 4 * lane;
-    const bool in = 4 * lane < hd;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f}, v[U];
-#pragma unroll
-    for (int i = 0; i < U; i++) v[i] = in ? *(const f32x4 *)(po + min(i, parts - 1) * all * hd) : x;
-    float top = R;
+    if (parts < 2) return;
+    auto where = [&](int p) { return p == 0 ? first : second + (p - 1) * apart; };
+    float top = -INFINITY;
+    for (int p = lane; p < parts; p += 64) top = fmaxf(top, pm[where(p) * 2]);
 #pragma unroll
     for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
-    const float f = __builtin_amdgcn_exp2f(R - (top == -INFINITY ? 0.f : top));
-    l *= f;
+    // U workgroups' sums in flight at a time, four elements a lane (lanes beyond hd: none)
+    const bool in = 4 * lane < hd;
+    const float *e = po + 4 * lane;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int p0 = 0; p0 < parts; p0 += U) {
+        f32x4 v[U];
+        float f = 0.f;
 #pragma unroll
-    for (int o = 32; o; o /= 2) l += __shfl_xor(l, o);
-    for (int s = 0; s < parts; s += U) {
+        for (int i = 0; i < U; i++) v[i] = in ? *(const f32x4 *)(e + where(min(p0 + i, parts - 1)) * hd) : f32x4{0.f, 0.f, 0.f, 0.f};
+        if (lane < U && p0 + lane < parts) {
+            const float2 m = *(const float2 *)(pm + where(p0 + lane) * 2);
+            f = __builtin_amdgcn_exp2f(m.x - (top == -INFINITY ? 0.f : top));
+            l += f * m.y;
+        }
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(s + i, 63)));
-            if (s + i < parts) x += fs * v[i];
-            if (s + U < parts) v[i] = in ? *(const f32x4 *)(po + min(s + U + i, parts - 1) * all * hd) : x;
+            const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
+            if (p0 + i < parts) x += fi * v[i];
         }
     }
+#pragma unroll
+    for (int o = 32; o; o /= 2) l += __shfl_xor(l, o);
     float y[4] = {x[0], x[1], x[2], x[3]};
-    AttnArgs one = a;
-    one.lse = nullptr;
-    if (in) pg_out<T, 4>(one, hd, 0, 1, r, head, 4 * lane, l, y);
-    if (a.lse && lane == 0) a.lse[row] = pg_lse(top, l);
+    if (in) pg_out<T, 4>(a, hd, nullptr, r, head, 4 * lane, l, y);
+    if (lane == 0) pg_out_sums(a, nullptr, r, head, top, l);
 }
 
 // -------------------------------------------------------------------- entries --
@@ -528,39 +645,56 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 }
 
 // How a call is launched: the columns (rows times heads of a KV head) of a sequence
-// decide.  few: only k_paged_direct with workgroups of 32 columns; else the rows' kernel,
-// and, where the numbers of rows differ, the former for the sequences of few.
+// decide.  few: only k_paged_direct; else the rows' kernel, and, where the numbers of
+// rows differ, the former for the sequences of few.
 #define PG_FEW 32
-#define PG_FILL 1024                 /* workgroups wanted */
-#define PG_MIN 8                     /* tiles of 32 tokens of a workgroup, at least */
+#define PG_FILL 256                  /* workgroups wanted of k_paged_direct */
+#define PG_FILL_ROWS 1024            /* of the rows' kernels                */
+#define PG_MANY 2048                 /* sequences times KV heads that need no sharing */
 struct Plan {
     bool few, both;
     int W;                           // columns of a workgroup of few
-    unsigned tiles, slots;           // of W columns of a sequence, of 128 of all
-    int S, per;
-    size_t sums;                     // bytes of the partial sums, before their references
+    unsigned slots;                  // tiles of 128 columns
+    int P, S, per;
+    size_t po, pm, place, eo, em, bytes;
 };
-static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int H)
+static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int H, int win, int sinks)
 {
     Plan p = {};
     const int G = H / c->KV, rows = b->max_rows && b->max_rows < b->N ? b->max_rows : b->N;
     const long long cols = (long long)rows * G, room = (long long)b->ldt * c->page,
-                    len = b->max_len && b->max_len < room ? b->max_len : room;
+                    most = b->max_len && b->max_len < room ? b->max_len : room,
+                    seen = win ? (long long)win + rows + (sinks < most ? sinks : most) + 64 : most,
+                    tiles = ((seen < most ? seen : most) + 31) / 32;
     p.few = cols <= PG_FEW;
     p.W = cols <= 16 ? 16 : 32;
-    p.tiles = p.few ? (unsigned)((cols + p.W - 1) / p.W) : 1;
-    p.slots = (unsigned)((long long)b->N * G / 128 + b->B);
     p.both = !p.few && (long long)b->B * rows > b->N;
-    const long long groups = p.few ? (long long)b->B * p.tiles * c->KV : (long long)p.slots * c->KV,
-                    row = (long long)b->N * H * (c->hd + 2) * 4, tiles = (len + 31) / 32;
-    long long S = PG_FILL / groups;
-    if (S > tiles / PG_MIN) S = tiles / PG_MIN;
-    if (S > (128ll << 20) / row) S = (128ll << 20) / row;
-    p.S = S < 1 ? 1 : S > 64 ? 64 : (int)S;
+    p.slots = (unsigned)((long long)b->N * G / 128 + b->B);
+    if ((p.few || p.both) && b->B <= PG_EVEN && (long long)b->B * c->KV < PG_MANY) {
+        long long P = PG_FILL / c->KV;
+        if (P < b->B) P = b->B;
+        const long long all = ((cols < PG_FEW ? cols : PG_FEW) + p.W - 1) / p.W * tiles * b->B / PG_UNITS;
+        p.P = (int)(P < all ? P : all);
+        if (p.P < b->B && b->B > 1) p.P = b->B;          // one sequence that nobody shares needs no places
+        if (p.P < 2) p.P = 0;
+    }
+    p.S = 1;
+    if (!p.few) {
+        long long S = PG_FILL_ROWS / ((long long)p.slots * c->KV);
+        const long long row = (long long)b->N * H * (c->hd + 2) * 4;
+        if (S > tiles / 8) S = tiles / 8;
+        if (S > (128ll << 20) / row) S = (128ll << 20) / row;
+        p.S = S < 1 ? 1 : S > 64 ? 64 : (int)S;
+    }
     p.per = (int)((tiles + p.S - 1) / p.S);
-    if (p.per < PG_MIN) p.per = PG_MIN;
+    if (p.per < 8) p.per = 8;
     p.per += p.per & 1;
-    p.sums = p.S > 1 ? (size_t)p.S * b->N * H * c->hd * 4 : 0;
+    const size_t parts = p.S > 1 ? (size_t)p.S * b->N * H : 0, even = (size_t)p.P * c->KV * 2 * p.W;
+    p.pm = parts * c->hd * 4;
+    p.place = (p.pm + parts * 8 + 15) & ~(size_t)15;
+    p.eo = (p.place + (p.P ? (b->B + 2) * 8 : 0) + 15) & ~(size_t)15;
+    p.em = p.eo + even * c->hd * 4;
+    p.bytes = p.em + even * 8;
     return p;
 }
 
@@ -570,8 +704,7 @@ extern "C" size_t tlg_paged_attn_ws_bytes(const TlgPages *c, const TlgBatch *b, 
     if (!c || !b || c->KV <= 0 || H < c->KV || b->N <= 0 || b->B <= 0 || c->hd <= 0 || c->page <= 0 || b->ldt < 0 ||
         b->max_rows < 0 || b->max_len < 0)
         return 0;
-    const Plan p = pg_plan(c, b, H);
-    return p.sums ? p.sums + (size_t)p.S * b->N * H * 8 : 0;
+    return pg_plan(c, b, H, 0, 0).bytes;
 }
 
 template <int T, int C, int W, bool ROWS> static void pg_direct(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
@@ -590,10 +723,12 @@ template <int W> static void pg_few(const AttnArgs &a, int type, int kv, int hd,
     else if (kv == TLG_F16) pg_direct<TLG_F32, TLG_F16, W, false>(a, hd, grid, st);
     else pg_direct<TLG_F32, TLG_BF16, W, false>(a, hd, grid, st);
 }
-template <int T> static void pg_join(const AttnArgs &a, int hd, int few, int small, int big, int by64, dim3 grid, hipStream_t st)
+template <bool EVEN> static void pg_join(const AttnArgs &a, int type, int hd, int w, int by64, hipStream_t st)
 {
-    if (a.S <= 4) hipLaunchKernelGGL((k_paged_join<T, 4>), grid, dim3(256), 0, st, a, hd, few, small, big, by64);
-    else hipLaunchKernelGGL((k_paged_join<T, 16>), grid, dim3(256), 0, st, a, hd, few, small, big, by64);
+    const dim3 grid((unsigned)(((long long)a.b.N * a.H + 3) / 4));
+    if (type == TLG_F32) hipLaunchKernelGGL((k_paged_join<TLG_F32, EVEN>), grid, dim3(256), 0, st, a, hd, w, by64);
+    else if (type == TLG_F16) hipLaunchKernelGGL((k_paged_join<TLG_F16, EVEN>), grid, dim3(256), 0, st, a, hd, w, by64);
+    else hipLaunchKernelGGL((k_paged_join<TLG_BF16, EVEN>), grid, dim3(256), 0, st, a, hd, w, by64);
 }
 static void pg_rows32(const AttnArgs &a, int kv, int hd, dim3 grid, hipStream_t st)
 {
@@ -639,33 +774,31 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
         a.K = a.V = a.q;
         a.b.head_ld = 0;
     }
-    const Plan p = pg_plan(c, b, H);
+    const Plan p = pg_plan(c, b, H, a.win, a.sinks);
     a.S = p.S;
     a.per = p.per;
-    a.few = 0;
-    a.many = p.few ? INT_MAX : PG_FEW;
+    a.P = p.P;
     a.po = (float *)ws;
-    a.pm = (float *)((char *)ws + p.sums);
+    a.pm = (float *)((char *)ws + p.pm);
+    a.place = (long long *)((char *)ws + p.place);
+    a.eo = (float *)((char *)ws + p.eo);
+    a.em = (float *)((char *)ws + p.em);
     hipStream_t st = ST(stream);
     if (p.few || p.both) {
-        const dim3 grid((unsigned)b->B * c->KV * p.S, p.tiles);
+        a.few = 0;
+        a.many = p.few ? INT_MAX : PG_FEW;
+        const dim3 grid((unsigned)(p.P ? p.P : b->B) * c->KV);
         if (p.W == 16) pg_few<16>(a, type, c->type, c->hd, grid, st);
         else pg_few<32>(a, type, c->type, c->hd, grid, st);
+        if (p.P) pg_join<true>(a, type, c->hd, p.W, 0, st);
     }
     if (!p.few) {
         a.few = p.both ? PG_FEW : 0;
         a.many = INT_MAX;
-        if (type == TLG_F32) pg_rows32(a, c->type, c->hd, dim3(p.slots * c->KV * p.S), st);
-        else pg_tile_launch(a, type, c->hd, p.slots * c->KV * p.S, st);
-    }
-    if (p.S > 1) {
-        // few: every tile's columns were p.W, else those of the rows' kernel
-        const int few = p.few ? INT_MAX : a.few, big = type == TLG_F32 ? 32 : PGT_ROWS,
-                  by64 = type != TLG_F32 && PGT_TOKENS(c->hd) == 64;
-        const dim3 grid((unsigned)(((long long)b->N * H + 3) / 4));
-        if (type == TLG_F32) pg_join<TLG_F32>(a, c->hd, few, p.W, big, by64, grid, st);
-        else if (type == TLG_F16) pg_join<TLG_F16>(a, c->hd, few, p.W, big, by64, grid, st);
-        else pg_join<TLG_BF16>(a, c->hd, few, p.W, big, by64, grid, st);
+        const dim3 grid(p.slots * c->KV * p.S);
+        if (type == TLG_F32) pg_rows32(a, c->type, c->hd, grid, st);
+        else pg_tile_launch(a, type, c->hd, grid.x, st);
+        if (p.S > 1) pg_join<false>(a, type, c->hd, type == TLG_F32 ? 32 : PGT_ROWS, type != TLG_F32 && PGT_TOKENS(c->hd) == 64, st);
     }
     LAUNCH_CHECK();
     return TLG_OK;

@@ -165,14 +165,16 @@ template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) vo
     }
     l = pg_gsum<32>(l);
     if (!live) return;
+    const int head = kvh * a.G + g;
+    float *sums = pg_part(a, a.po, HD, s, parts, r, head);
 #pragma unroll
     for (int k = 0; k < NB; k++)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             float x[4] = {o[k][i], o[k][i + 1], o[k][i + 2], o[k][i + 3]};
-            pg_out<T, 4>(a, HD, s, parts, r, kvh * a.G + g, 32 * k + pg_at<32>(i, h), l, x);
+            pg_out<T, 4>(a, HD, sums, r, head, 32 * k + pg_at<32>(i, h), l, x);
         }
-    if (h == 0) pg_out_sums(a, s, parts, r, kvh * a.G + g, R, l);
+    if (h == 0) pg_out_sums(a, pg_part(a, a.pm, 2, s, parts, r, head), r, head, R, l);
 }
 
 template <int T> static void launch(const AttnArgs &a, int hd, unsigned grid, hipStream_t st)
