@@ -310,10 +310,11 @@ def run_attn(lib, s, q, H, type, scale, win=0, sinks=0, ldq=None, ldo=None, lse=
     out = t.full((s.N, ldo), fill, dtype=dtype(type), device="cuda")
     ls = t.full((s.N, H), fill, device="cuda")
     nb = lib.paged_attn_ws_bytes(s.pages, s.batch, type, H)
-    ws = t.full((max(nb, 16),), 255, dtype=t.uint8, device="cuda")
+    ws = t.full((nb + 4096,), 255, dtype=t.uint8, device="cuda")
     lib.paged_attn(s.pages, s.batch, dq.data_ptr(), type, ldq, H, scale, win, sinks, out.data_ptr(), ldo,
                    ls.data_ptr() if lse else None, ws.data_ptr() if nb else None, nb, stream() if st is None else st)
     t.cuda.synchronize()
+    assert (ws[nb:] == 255).all(), "wrote behind its workspace"
     return out, ls
 
 

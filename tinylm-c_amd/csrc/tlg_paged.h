@@ -60,15 +60,15 @@ struct AttnArgs {
     int H, KV, G, win, sinks;
     int few, many;               // columns (rows times heads of a KV head) of the sequences that a launch takes: more than few, many at most
     float c;                     // scale log2 e
-    // rows' kernels: S workgroups share a tile's tokens, `per` tiles of 32 tokens each; S > 1:
-    // their sums [S][N][H][hd] and references and weights [S][N][H][2]
+    // S workgroups share a tile's tokens, `per` tiles of 32 tokens each; S > 1: their sums
+    // [S][N][H][hd] and references and weights [S][N][H][2]
     int S, per;
     float *po, *pm;
-    // k_paged_direct: P workgroups of a KV head share the tokens of all sequences evenly (0: one a
-    // sequence), with the place of each sequence [B + 1], the number that took part, and the
-    // sums of tiles that are not one workgroup's, [P][KV][2][W][hd] and [..][2]
+    // k_paged_direct, P > 0: P workgroups of a KV head share the tokens of all sequences evenly
+    // instead, with the place of each sequence [B + 1] and the number that took part, and
+    // the sums of tiles that are not one workgroup's, [P][KV][2][W][hd] and [..][2]
     int P;
-    long long *place;
+    int *place;
     float *eo, *em;
 };
 

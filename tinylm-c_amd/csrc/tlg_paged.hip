@@ -116,39 +116,43 @@ template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(Sto
 
 // --------------------------------------------------------------- attention --
 // Units of a sequence's tiles of W columns (of each of them), 0 where a launch leaves it out.
-template <int W> __device__ __forceinline__ long long pg_units(const AttnArgs &a, const Seq &q)
+__device__ __forceinline__ int pg_units(const AttnArgs &a, const Seq &q)
 {
     const int cols = q.n * a.G;
-    if (cols <= a.few || cols > a.many) return 0;
-    return max(1, pg_range<32>(a, q, 0, cols).total);
+    return cols > a.few && cols <= a.many ? max(1, pg_range<32>(a, q, 0, cols).total) : 0;
 }
-// Where each sequence's units start, [B + 1] in LDS; the workgroups that take part, each
-// with PG_UNITS at least.  B <= PG_EVEN, 256 threads.
+// Where each sequence's units start, [B + 1] in LDS (their number stays below 2^31, the
+// host sees to it); the workgroups that take part, each with PG_UNITS at least.  B <=
+// PG_EVEN, 256 threads.
 #define PG_EVEN 1024
-#define PG_UNITS 8
-template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, long long *place)
+#define PG_UNITS 4
+template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, int *place)
 {
-    __shared__ long long part[4];
+    __shared__ int part[4], with[4];
     const int t = threadIdx.x, per = (a.b.B + 255) / 256, lane = t & 63;
-    long long n[PG_EVEN / 256], sum = 0;
+    int n[PG_EVEN / 256], sum = 0, some = 0;
 #pragma unroll
     for (int i = 0; i < PG_EVEN / 256; i++) {
         n[i] = 0;
         if (i < per && t * per + i < a.b.B) {
             const Seq q = pg_seq(a.b, t * per + i);
-            n[i] = pg_units<W>(a, q) * ((q.n * a.G + W - 1) / W);
+            n[i] = pg_units(a, q) * ((q.n * a.G + W - 1) / W);
         }
         sum += n[i];
+        some += __popcll(__ballot(n[i] > 0));
     }
-    long long upto = sum;
+    int upto = sum;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-        const long long v = __shfl_up(upto, o);
+        const int v = __shfl_up(upto, o);
         upto += lane >= o ? v : 0;
     }
-    if (lane == 63) part[t >> 6] = upto;
+    if (lane == 63) {
+        part[t >> 6] = upto;
+        with[t >> 6] = some;
+    }
     __syncthreads();
-    long long all = 0;
+    int all = 0;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         if (w == t >> 6) upto += all;
@@ -162,7 +166,17 @@ template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, lon
     }
     if (t == 0) place[a.b.B] = all;
     __syncthreads();
-    return (int)min((long long)a.P, max(all / PG_UNITS, all > 0 ? 1ll : 0ll));
+    // Small shares of equal sequences are cut alike: a second sequence in a share costs its
+    // workgroup about 4 us, as much as 8 tiles or more.
+    const int seqs = with[0] + with[1] + with[2] + with[3], P = min(a.P, max(all / PG_UNITS, all > 0));
+    return P > seqs && all < 32 * P ? P / seqs * seqs : P;
+}
+// Share y of T units over P: the first T % P have one more.
+__device__ __forceinline__ int pg_share(int T, int P, int y) { return T / P * y + min(y, T % P); }
+__device__ __forceinline__ int pg_share_of(int T, int P, int u)
+{
+    const int n = T / P, more = T % P, k = u / (n + 1);
+    return k < more ? k : more + (u - more * (n + 1)) / n;
 }
 
 // Scores are formed transposed, S^T = K Q^T, tokens by columns (rows times query heads
@@ -181,14 +195,11 @@ template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, lon
 // tokens of all sequences, tile after tile, are dealt out evenly to the workgroups of a
 // KV head, so that ragged lengths leave none idle; the four waves of a workgroup take
 // every fourth of its tiles and join their sums.  Blocks of W = 16 columns where there
-// are no more: half the registers of 32.  ROWS (fp32): every wave 32 columns of its
+// are no more: half the registers of 32.  ROWS (fp32): every wave a block of columns of its
 // own, whose keys the waves of a workgroup find in the CU's cache.
-#ifndef PGBX
-#define PGBX 2
-#endif
-#define PGB (T != TLG_F32 && W == 16 && HD == 128 ? PGBX : (T == TLG_F32 && HD >= 128 && W == 32) || HD == 256 ? 1 : 2)
+// One workgroup a CU where two would spill (fp32 rows of 96 elements on, 256 elements).
 template <int T, int C, int HD, int W, bool ROWS>
-__global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
+__global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32 ? 4 : 3) >= 384) || HD == 256 ? 1 : 2) void k_paged_direct(AttnArgs a)
 {
     typedef typename ElT<C>::E E;
     typedef typename AccT<W>::A Acc;
@@ -199,13 +210,14 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
     constexpr int PE = F ? 4 : 8, NQ = HD / (PE * G), NK = NQ * TB, KW = PE * cs / 4;  // a key's pieces: elements, number, registers
     constexpr int NV = F ? NE : HD / 16, VW = F ? (NB * cs + 3) / 4 : 4;
     constexpr int VST = (HD / 2) % 64 == 16 || (HD / 2) % 64 == 48 ? HD : HD + 32;     // elements between tokens in LDS
+    constexpr bool LATE = F && HD == 256;                               // keys and values do not fit the registers at once
     constexpr int MS = W + 4, BS = NB % 4 ? 2 : 4, MB = W == 32 ? 1 : BS;              // the sums' blocks joined at once
     constexpr int V1 = F ? 0 : 32 * VST * 2, M1 = MB * W * MS * 4, P1 = 1024;
     constexpr int PW = V1 > M1 ? (V1 > P1 ? V1 : P1) : (M1 > P1 ? M1 : P1);            // LDS of a wave
     __shared__ __align__(16) char mem[4 * PW];
     __shared__ long long toff[4][2][32];
     __shared__ float red[4][2][W];
-    __shared__ long long place[ROWS ? 1 : PG_EVEN + 1];
+    __shared__ int place[ROWS ? 1 : PG_EVEN + 1];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane % W, g = lane / W;
     const int kvh = blockIdx.x % a.KV, y = blockIdx.x / a.KV;
@@ -215,50 +227,53 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
 
     // the workgroup's share: units [u, u1) of the sequences' tiles of W columns by 32 tokens
     int b = y;
-    long long u = 0, u1 = 0;
+    int u = 0, u1 = 0;
     if constexpr (ROWS) {
-        auto start = [&](int i) { return (long long)pg_row0(a.b, i) * a.G / 128 + i; };
+        auto start = [&](int i) { return (long long)pg_row0(a.b, i) * a.G / (4 * W) + i; };
         b = pg_search(a.b.B, y / a.S, start);
-        u = y / a.S - start(b);
+        u = (int)(y / a.S - start(b));
     } else if (a.P) {
         const int P = pg_places<W>(a, place);
         if (blockIdx.x == 0)
             for (int i = threadIdx.x; i <= a.b.B + 1; i += 256) a.place[i] = i <= a.b.B ? place[i] : P;
         if (y >= P) return;
-        u = place[a.b.B] * y / P;
-        u1 = place[a.b.B] * (y + 1) / P;
+        u = pg_share(place[a.b.B], P, y);
+        u1 = pg_share(place[a.b.B], P, y + 1);
         b = pg_search(a.b.B, u, [&](int i) { return place[i]; });       // the last that starts there: it has units
-    }
-    const int s = ROWS ? y % a.S : 0;
-    for (bool first = true; first || (!ROWS && u < u1); first = false) {
+    } else b = y / a.S;
+    const int s = ROWS || !a.P ? y % a.S : 0;
+    for (bool first = true; first || (!ROWS && u < u1); first = false) {   // `continue` below: !P, u counts on
         const Seq q = pg_seq(a.b, b);
         const int cols = q.n * a.G;
-        int rh0, t0seg = 0, t1seg = INT_MAX;
+        int rh0, t0seg = 0, t1seg = 0;
         bool only = true;
         if constexpr (ROWS) {
-            rh0 = (int)u * 128 + 32 * wave;
+            rh0 = (4 * u + wave) * W;
             if (u < 0 || rh0 >= cols || cols <= a.few || cols > a.many) return;
         } else {
-            const long long tot = pg_units<W>(a, q);
+            const int tot = pg_units(a, q);
             if (tot == 0) return;                        // without places only: a sequence of no rows, or not this launch's
-            long long in = u - (a.P ? place[b] : 0);
-            rh0 = (int)(in / tot) * W;
-            if (rh0 >= cols) return;
             if (a.P) {
-                t0seg = (int)(in % tot);
-                t1seg = (int)min(tot, t0seg + u1 - u);
+                const int in = u - place[b], k = in / tot;
+                rh0 = k * W;
+                t0seg = in - k * tot;
+                t1seg = min(tot, t0seg + u1 - u);
                 only = t0seg == 0 && t1seg == tot;
                 u += t1seg - t0seg;
-            } else {
-                u += tot;
-                u1 = tot * ((cols + W - 1) / W);
+            } else {                                     // its tiles of columns one after the other
+                rh0 = u * W;
+                u++;
+                u1 = (cols + W - 1) / W;
             }
         }
         const Range rg = pg_range<32>(a, q, rh0, min(rh0 + W, cols));
         int parts = 1, j0, j1;
-        if constexpr (ROWS) {
+        if (ROWS || !a.P) {
             parts = pg_parts<32>(a, rg.total);
-            if (s >= parts) return;
+            if (s >= parts) {
+                if (ROWS) return;
+                continue;
+            }
             j0 = (int)((long long)rg.total * s / parts);
             j1 = (int)((long long)rg.total * (s + 1) / parts);
         } else {
@@ -331,7 +346,7 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
         int j = j0 + (ROWS ? 0 : wave), buf = 0, ahead = page(j + step);
         if (j < j1) {
             loadK(0, elems(j, page(j)));
-            loadV(0);
+            if (!LATE) loadV(0);
         }
         for (; j < j1; j += step, buf ^= 1) {
             const int t0 = pg_tile<32>(rg, j);
@@ -363,7 +378,8 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < NR; i++) e[t * NR + i] = z[i];
             }
-            if (more) loadK(buf ^ 1, next);
+            if (LATE) loadV(buf);
+            else if (more) loadK(buf ^ 1, next);
             // weights
             const bool full = t0 + 31 <= rg.pmin && (rg.lomax <= t0 || t0 + 31 < a.sinks);
             if (!full) {
@@ -394,7 +410,8 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
                         else v = (float)__builtin_bit_cast(E, (unsigned short)(vr[i][k / 2] >> (k & 1) * 16));
                         o[k] = pg_mfma32<W>(v, e[i], o[k]);
                     }
-                if (more) loadV(buf ^ 1);
+                if (more && LATE) loadK(buf ^ 1, next);
+                if (more && !LATE) loadV(buf ^ 1);
             } else {
                 pg_wave_sync();
 #pragma unroll
@@ -457,6 +474,10 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
             // a tile that goes on from another workgroup's, and one that another goes on with, have places of their own
             const long long slot = (((long long)y * a.KV + kvh) * 2 + (t0seg == 0)) * W + oc;
             float *eo = only ? nullptr : a.eo + slot * HD, *em = only ? nullptr : a.em + slot * 2;
+            if (!a.P) {
+                eo = pg_part(a, a.po, HD, s, parts, q.lo + oi, hq);
+                em = pg_part(a, a.pm, 2, s, parts, q.lo + oi, hq);
+            }
             float *mg = (float *)mem;
 #pragma unroll
             for (int k0 = 0; k0 < NB; k0 += MB) {
@@ -487,15 +508,17 @@ __global__ __launch_bounds__(256, PGB) void k_paged_direct(AttnArgs a)
     }
 }
 
-// The sums of the workgroups that shared a row's tokens, one wave a row and head.  EVEN:
+// The sums of the workgroups that shared a row's tokens: one wave a row and head, or, for
+// few rows, four that take a quarter of the sums each (64 sums of 128 elements: 6.7 us
+// against 21; 1792 rows with four sums: 8.5 against 5).  EVEN:
 // those of k_paged_direct in tiles of `w` columns; else of the rows' kernels, whose tiles of `w`
 // columns had their tokens in tiles of 32 or, with the flag, 64.
-template <int T, bool EVEN> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int w, int by64)
+template <int T, bool EVEN, int WV> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int w, int by64)
 {
-    constexpr int U = 16;
-    const int lane = threadIdx.x & 63;
-    const long long rhd = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int r = __builtin_amdgcn_readfirstlane((int)(rhd / a.H)), head = __builtin_amdgcn_readfirstlane((int)(rhd % a.H));
+    constexpr int U = 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rhd = __builtin_amdgcn_readfirstlane(WV == 4 ? blockIdx.x : blockIdx.x * 4 + wave), part = WV == 4 ? wave : 0;
+    const int r = rhd / a.H, head = rhd - r * a.H;
     if (r >= a.b.N) return;
     const int b = pg_search(a.b.B, r, [&](int i) { return pg_row0(a.b, i); });
     const Seq q = pg_seq(a.b, b);
@@ -506,10 +529,9 @@ template <int T, bool EVEN> __global__ __launch_bounds__(256) void k_paged_join(
     long long first, second, apart;                      // places (columns) of the first sums, the second, and from one to the next
     const float *po, *pm;
     if constexpr (EVEN) {
-        const long long T0 = a.place[a.b.B], P = a.place[a.b.B + 1], tiles = (cols + w - 1) / w,
-                        tot = (a.place[b + 1] - a.place[b]) / tiles, u = a.place[b] + rh / w * tot;
-        // the workgroup of unit x: the last i with T0 i / P <= x
-        const long long i0 = ((u + 1) * P - 1) / T0, i1 = ((u + tot) * P - 1) / T0;
+        const int all = a.place[a.b.B], P = a.place[a.b.B + 1], from = a.place[b], tiles = (cols + w - 1) / w,
+                  tot = (a.place[b + 1] - from) / tiles, u = from + rh / w * tot;
+        const long long i0 = pg_share_of(all, P, u), i1 = pg_share_of(all, P, u + tot - 1);
         parts = (int)(i1 - i0 + 1);
         first = ((i0 * a.KV + kvh) * 2 + 1) * w + rh % w;
         second = ((i0 + 1) * a.KV + kvh) * 2 * w + rh % w;
@@ -536,7 +558,7 @@ template <int T, bool EVEN> __global__ __launch_bounds__(256) void k_paged_join(
     const float *e = po + 4 * lane;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += U) {
+    for (int p0 = U * part; p0 < parts; p0 += WV * U) {
         f32x4 v[U];
         float f = 0.f;
 #pragma unroll
@@ -554,6 +576,16 @@ template <int T, bool EVEN> __global__ __launch_bounds__(256) void k_paged_join(
     }
 #pragma unroll
     for (int o = 32; o; o /= 2) l += __shfl_xor(l, o);
+    if constexpr (WV == 4) {
+        __shared__ f32x4 xs[4][64];
+        __shared__ float ls[4];
+        xs[wave][lane] = x;
+        if (lane == 0) ls[wave] = l;
+        __syncthreads();
+        if (wave) return;
+        x = (xs[0][lane] + xs[1][lane]) + (xs[2][lane] + xs[3][lane]);
+        l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    }
     float y[4] = {x[0], x[1], x[2], x[3]};
     if (in) pg_out<T, 4>(a, hd, nullptr, r, head, 4 * lane, l, y);
     if (lane == 0) pg_out_sums(a, nullptr, r, head, top, l);
@@ -647,52 +679,66 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 // How a call is launched: the columns (rows times heads of a KV head) of a sequence
 // decide.  few: only k_paged_direct; else the rows' kernel, and, where the numbers of
 // rows differ, the former for the sequences of few.
+// k_paged_direct's workgroups share the batch's tokens evenly from PG_LONG tiles of a
+// sequence on (64 sequences of 1024 to 4096 tokens: 124 us against 133 where each is cut
+// alike), unless there are sequences enough; below, where looking up the batch costs more than
+// that gains, each sequence is cut alike (32 sequences of 5 rows that see 1028 tokens:
+// 18 us against 24).
 #define PG_FEW 32
-#define PG_FILL 256                  /* workgroups wanted of k_paged_direct */
+#define PG_FILL 512                  /* workgroups wanted of k_paged_direct: two a CU */
 #define PG_FILL_ROWS 1024            /* of the rows' kernels                */
+#define PG_LONG 64                   /* tiles of 32 tokens                  */
 #define PG_MANY 2048                 /* sequences times KV heads that need no sharing */
 struct Plan {
     bool few, both;
     int W;                           // columns of a workgroup of few
-    unsigned slots;                  // tiles of 128 columns
-    int P, S, per;
+    int wide;                        // of a workgroup of the rows' kernel
+    unsigned slots;                  // and how many
+    int P, Sf, perf, S, per;         // few: shares, or parts of a sequence; the rows' kernel's parts
     size_t po, pm, place, eo, em, bytes;
 };
-static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int H, int win, int sinks)
+static int pg_cut(long long groups, long long fill, long long tiles, long long row)
+{
+    long long S = fill / groups;
+    if (S > tiles / 8) S = tiles / 8;
+    if (S > (128ll << 20) / row) S = (128ll << 20) / row;
+    return S < 1 ? 1 : S > 64 ? 64 : (int)S;
+}
+static int pg_per(long long tiles, int S)
+{
+    const long long n = (tiles + S - 1) / S;
+    return (int)(n < 8 ? 8 : n + (n & 1));
+}
+static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int type, int H, int win, int sinks, bool alike)
 {
     Plan p = {};
     const int G = H / c->KV, rows = b->max_rows && b->max_rows < b->N ? b->max_rows : b->N;
     const long long cols = (long long)rows * G, room = (long long)b->ldt * c->page,
                     most = b->max_len && b->max_len < room ? b->max_len : room,
                     seen = win ? (long long)win + rows + (sinks < most ? sinks : most) + 64 : most,
-                    tiles = ((seen < most ? seen : most) + 31) / 32;
+                    tiles = ((seen < most ? seen : most) + 31) / 32, row = (long long)b->N * H * (c->hd + 2) * 4;
     p.few = cols <= PG_FEW;
-    p.W = cols <= 16 ? 16 : 32;
+    p.W = cols <= 16 || c->hd == 256 ? 16 : 32;            // 32 of 256 elements do not fit the registers
+    p.wide = type == TLG_F32 ? c->hd == 256 ? 64 : 128 : PGT_ROWS;
     p.both = !p.few && (long long)b->B * rows > b->N;
-    p.slots = (unsigned)((long long)b->N * G / 128 + b->B);
-    if ((p.few || p.both) && b->B <= PG_EVEN && (long long)b->B * c->KV < PG_MANY) {
-        long long P = PG_FILL / c->KV;
-        if (P < b->B) P = b->B;
-        const long long all = ((cols < PG_FEW ? cols : PG_FEW) + p.W - 1) / p.W * tiles * b->B / PG_UNITS;
-        p.P = (int)(P < all ? P : all);
-        if (p.P < b->B && b->B > 1) p.P = b->B;          // one sequence that nobody shares needs no places
-        if (p.P < 2) p.P = 0;
+    p.slots = (unsigned)((long long)b->N * G / p.wide + b->B);
+    p.S = p.Sf = 1;
+    if (p.few || p.both) {
+        // units that the batch may hold, whatever the hints say
+        const double units = ((double)b->N * G / p.W + b->B) * (room / 32 + 2);
+        if (!alike && tiles > PG_LONG && b->B <= PG_EVEN && (long long)b->B * c->KV < PG_MANY && units < 2e9) {
+            p.P = PG_FILL / c->KV;
+            if (p.P < b->B) p.P = b->B;
+        } else p.Sf = pg_cut((long long)b->B * c->KV, PG_FILL, tiles, row);
     }
-    p.S = 1;
-    if (!p.few) {
-        long long S = PG_FILL_ROWS / ((long long)p.slots * c->KV);
-        const long long row = (long long)b->N * H * (c->hd + 2) * 4;
-        if (S > tiles / 8) S = tiles / 8;
-        if (S > (128ll << 20) / row) S = (128ll << 20) / row;
-        p.S = S < 1 ? 1 : S > 64 ? 64 : (int)S;
-    }
-    p.per = (int)((tiles + p.S - 1) / p.S);
-    if (p.per < 8) p.per = 8;
-    p.per += p.per & 1;
-    const size_t parts = p.S > 1 ? (size_t)p.S * b->N * H : 0, even = (size_t)p.P * c->KV * 2 * p.W;
+    if (!p.few) p.S = pg_cut((long long)p.slots * c->KV, PG_FILL_ROWS, tiles, row);
+    p.perf = pg_per(tiles, p.Sf);
+    p.per = pg_per(tiles, p.S);
+    const int S = p.S > p.Sf ? p.S : p.Sf;
+    const size_t parts = S > 1 ? (size_t)S * b->N * H : 0, even = (size_t)p.P * c->KV * 2 * p.W;
     p.pm = parts * c->hd * 4;
     p.place = (p.pm + parts * 8 + 15) & ~(size_t)15;
-    p.eo = (p.place + (p.P ? (b->B + 2) * 8 : 0) + 15) & ~(size_t)15;
+    p.eo = (p.place + (p.P ? (b->B + 2) * 4 : 0) + 15) & ~(size_t)15;
     p.em = p.eo + even * c->hd * 4;
     p.bytes = p.em + even * 8;
     return p;
@@ -700,41 +746,49 @@ static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int H, int win, int si
 
 extern "C" size_t tlg_paged_attn_ws_bytes(const TlgPages *c, const TlgBatch *b, int type, int H)
 {
-    (void)type;
     if (!c || !b || c->KV <= 0 || H < c->KV || b->N <= 0 || b->B <= 0 || c->hd <= 0 || c->page <= 0 || b->ldt < 0 ||
         b->max_rows < 0 || b->max_len < 0)
         return 0;
-    return pg_plan(c, b, H, 0, 0).bytes;
+    // whatever the window leaves of the tokens: fewer are cut into fewer parts
+    const size_t even = pg_plan(c, b, type, H, 0, 0, false).bytes, alike = pg_plan(c, b, type, H, 0, 0, true).bytes;
+    return even > alike ? even : alike;
 }
 
-template <int T, int C, int W, bool ROWS> static void pg_direct(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
+template <int T, int C, int W> static void pg_few(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
 {
-    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<T, C, 32, W, ROWS>), grid, dim3(256), 0, st, a);
-    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<T, C, 64, W, ROWS>), grid, dim3(256), 0, st, a);
-    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<T, C, 96, W, ROWS>), grid, dim3(256), 0, st, a);
-    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<T, C, 128, W, ROWS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_paged_direct<T, C, 256, W, ROWS>), grid, dim3(256), 0, st, a);
+    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<T, C, 32, W, false>), grid, dim3(256), 0, st, a);
+    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<T, C, 64, W, false>), grid, dim3(256), 0, st, a);
+    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<T, C, 96, W, false>), grid, dim3(256), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<T, C, 128, W, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_direct<T, C, 256, 16, false>), grid, dim3(256), 0, st, a);
 }
 template <int W> static void pg_few(const AttnArgs &a, int type, int kv, int hd, dim3 grid, hipStream_t st)
 {
-    if (type == TLG_F16) pg_direct<TLG_F16, TLG_F16, W, false>(a, hd, grid, st);
-    else if (type == TLG_BF16) pg_direct<TLG_BF16, TLG_BF16, W, false>(a, hd, grid, st);
-    else if (kv == TLG_F32) pg_direct<TLG_F32, TLG_F32, W, false>(a, hd, grid, st);
-    else if (kv == TLG_F16) pg_direct<TLG_F32, TLG_F16, W, false>(a, hd, grid, st);
-    else pg_direct<TLG_F32, TLG_BF16, W, false>(a, hd, grid, st);
+    if (type == TLG_F16) pg_few<TLG_F16, TLG_F16, W>(a, hd, grid, st);
+    else if (type == TLG_BF16) pg_few<TLG_BF16, TLG_BF16, W>(a, hd, grid, st);
+    else if (kv == TLG_F32) pg_few<TLG_F32, TLG_F32, W>(a, hd, grid, st);
+    else if (kv == TLG_F16) pg_few<TLG_F32, TLG_F16, W>(a, hd, grid, st);
+    else pg_few<TLG_F32, TLG_BF16, W>(a, hd, grid, st);
+}
+template <bool EVEN, int WV> static void pg_join(const AttnArgs &a, int type, int hd, int w, int by64, hipStream_t st)
+{
+    const dim3 grid((unsigned)(((long long)a.b.N * a.H * WV + 3) / 4));
+    if (type == TLG_F32) hipLaunchKernelGGL((k_paged_join<TLG_F32, EVEN, WV>), grid, dim3(256), 0, st, a, hd, w, by64);
+    else if (type == TLG_F16) hipLaunchKernelGGL((k_paged_join<TLG_F16, EVEN, WV>), grid, dim3(256), 0, st, a, hd, w, by64);
+    else hipLaunchKernelGGL((k_paged_join<TLG_BF16, EVEN, WV>), grid, dim3(256), 0, st, a, hd, w, by64);
 }
 template <bool EVEN> static void pg_join(const AttnArgs &a, int type, int hd, int w, int by64, hipStream_t st)
 {
-    const dim3 grid((unsigned)(((long long)a.b.N * a.H + 3) / 4));
-    if (type == TLG_F32) hipLaunchKernelGGL((k_paged_join<TLG_F32, EVEN>), grid, dim3(256), 0, st, a, hd, w, by64);
-    else if (type == TLG_F16) hipLaunchKernelGGL((k_paged_join<TLG_F16, EVEN>), grid, dim3(256), 0, st, a, hd, w, by64);
-    else hipLaunchKernelGGL((k_paged_join<TLG_BF16, EVEN>), grid, dim3(256), 0, st, a, hd, w, by64);
+    if ((long long)a.b.N * a.H < 512) pg_join<EVEN, 4>(a, type, hd, w, by64, st);
+    else pg_join<EVEN, 1>(a, type, hd, w, by64, st);
 }
-static void pg_rows32(const AttnArgs &a, int kv, int hd, dim3 grid, hipStream_t st)
+template <int C> static void pg_rows32(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
 {
-    if (kv == TLG_F32) pg_direct<TLG_F32, TLG_F32, 32, true>(a, hd, grid, st);
-    else if (kv == TLG_F16) pg_direct<TLG_F32, TLG_F16, 32, true>(a, hd, grid, st);
-    else pg_direct<TLG_F32, TLG_BF16, 32, true>(a, hd, grid, st);
+    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 32, 32, true>), grid, dim3(256), 0, st, a);
+    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 64, 32, true>), grid, dim3(256), 0, st, a);
+    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 96, 32, true>), grid, dim3(256), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 128, 32, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 256, 16, true>), grid, dim3(256), 0, st, a);
 }
 
 extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const void *q, int type, long long ldq, int H,
@@ -774,31 +828,36 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
         a.K = a.V = a.q;
         a.b.head_ld = 0;
     }
-    const Plan p = pg_plan(c, b, H, a.win, a.sinks);
-    a.S = p.S;
-    a.per = p.per;
+    const Plan p = pg_plan(c, b, type, H, a.win, a.sinks, false);
     a.P = p.P;
     a.po = (float *)ws;
     a.pm = (float *)((char *)ws + p.pm);
-    a.place = (long long *)((char *)ws + p.place);
+    a.place = (int *)((char *)ws + p.place);
     a.eo = (float *)((char *)ws + p.eo);
     a.em = (float *)((char *)ws + p.em);
     hipStream_t st = ST(stream);
     if (p.few || p.both) {
         a.few = 0;
         a.many = p.few ? INT_MAX : PG_FEW;
-        const dim3 grid((unsigned)(p.P ? p.P : b->B) * c->KV);
+        a.S = p.Sf;
+        a.per = p.perf;
+        const dim3 grid((unsigned)(p.P ? p.P : b->B * p.Sf) * c->KV);
         if (p.W == 16) pg_few<16>(a, type, c->type, c->hd, grid, st);
         else pg_few<32>(a, type, c->type, c->hd, grid, st);
         if (p.P) pg_join<true>(a, type, c->hd, p.W, 0, st);
+        else if (p.Sf > 1) pg_join<false>(a, type, c->hd, p.W, 0, st);
     }
     if (!p.few) {
         a.few = p.both ? PG_FEW : 0;
         a.many = INT_MAX;
+        a.S = p.S;
+        a.per = p.per;
         const dim3 grid(p.slots * c->KV * p.S);
-        if (type == TLG_F32) pg_rows32(a, c->type, c->hd, grid, st);
+        if (type == TLG_F32 && c->type == TLG_F32) pg_rows32<TLG_F32>(a, c->hd, grid, st);
+        else if (type == TLG_F32 && c->type == TLG_F16) pg_rows32<TLG_F16>(a, c->hd, grid, st);
+        else if (type == TLG_F32) pg_rows32<TLG_BF16>(a, c->hd, grid, st);
         else pg_tile_launch(a, type, c->hd, grid.x, st);
-        if (p.S > 1) pg_join<false>(a, type, c->hd, type == TLG_F32 ? 32 : PGT_ROWS, type != TLG_F32 && PGT_TOKENS(c->hd) == 64, st);
+        if (p.S > 1) pg_join<false>(a, type, c->hd, type == TLG_F32 ? p.wide / 4 : PGT_ROWS, type != TLG_F32 && PGT_TOKENS(c->hd) == 64, st);
     }
     LAUNCH_CHECK();
     return TLG_OK;
