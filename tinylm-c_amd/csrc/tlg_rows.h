@@ -134,6 +134,14 @@ __device__ __forceinline__ float add_op(float a, float b) { return a + b; }
 WAVE_REDUCE(wave_max, fmaxf)
 WAVE_REDUCE(wave_sum, add_op)
 
+// scale (x - m); halves where the difference of finite values passes fp32 and
+// its product need not
+__device__ __forceinline__ float lp_scaled(float x, float m, float scale)
+{
+    const float d = x - m;
+    return d > -INFINITY || x == -INFINITY ? d * scale : (0.5f * x - 0.5f * m) * scale * 2.f;
+}
+
 // -------------------------------------------------------------------- checks --
 static inline size_t vb_size(int type) { return type == TLG_F32 ? 4 : 2; }
 

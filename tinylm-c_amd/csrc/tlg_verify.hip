@@ -10,7 +10,7 @@
 //
 // Two launches: the sums of every row (bound by HBM, each logit read once), then
 // for each sequence the tests of its rows, a scalar each, and the race over the one
-// row that ends it; a third joins rows that are cut over workgroups.
+// row that ends it; a third joins races that are cut over workgroups.  Short rows: one.
 #include "tlg_internal.h"
 #include "tlg_rows.h"
 #include "../../include/tlserve.h"
@@ -58,26 +58,18 @@ __device__ __forceinline__ SvSum sv_join(const SvSum *p, int n, float c)
 }
 
 // ---------------------------------------------------------------- row sums --
-// Segment blockIdx.x % S of row blockIdx.x / S; blockIdx.y 1: of the draft model's.
-template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_sums(SvArgs a)
+// The sums of vectors [lo, hi) of row x over TH threads, and, with the flag, of the
+// elements behind the last vector; the thread's own, t of TH.
+template <int TYPE, int TH>
+__device__ __forceinline__ SvSum sv_some(const char *x, int V, int lo, int hi, bool tail, float c, int t)
 {
     constexpr int VE = El<TYPE>::VE, U = 4;
-    const int r = blockIdx.x / a.S, seg = blockIdx.x % a.S, of = blockIdx.y, t = threadIdx.x;
-    if (of && a.draft[r] < 0) return;
-    const char *x = (const char *)(of ? a.y : a.x) + (long long)r * (of ? a.ldy : a.ld) * El<TYPE>::SZ;
-    const float c = of ? a.dc : a.c;
-    const int nv = a.V / VE, lo = (int)((long long)nv * seg / a.S), hi = (int)((long long)nv * (seg + 1) / a.S);
     float m = -INFINITY, s = 0.f;
-    auto take = [&](float v) {                         // one element
-        const float n = fmaxf(m, v), ref = sv_ref(n);
-        s = s * sv_term(sv_ref(m), ref, c) + sv_term(v, ref, c);
-        m = n;
-    };
-    for (int j = lo + t; j < hi; j += U * SV_THREADS) {
+    for (int j = lo + t; j < hi; j += U * TH) {
         u32x4 q[U];
 #pragma unroll
         for (int k = 0; k < U; k++) {
-            const int i = j + k * SV_THREADS;
+            const int i = j + k * TH;
             q[k] = sv_load<TYPE>(x, (i < hi ? i : j) * VE);      // beyond the end: a vector taken already, left out below
         }
         float n = m;
@@ -96,46 +88,72 @@ template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_sums(SvAr
             for (int w = VE / 2; w; w /= 2)
 #pragma unroll
                 for (int e = 0; e < w; e++) v[e] += v[e + w];
-            sum += j + k * SV_THREADS < hi ? v[0] : 0.f;
+            sum += j + k * TH < hi ? v[0] : 0.f;
         }
         s = s * sv_term(sv_ref(m), ref, c) + sum;
         m = n;
     }
-    if (seg == a.S - 1 && t < a.V % VE) take(el_load<TYPE>(x, nv * VE + t));
+    if (tail && t < V % VE) {
+        const float v = el_load<TYPE>(x, V / VE * VE + t), n = fmaxf(m, v), ref = sv_ref(n);
+        s = s * sv_term(sv_ref(m), ref, c) + sv_term(v, ref, c);
+        m = n;
+    }
+    return SvSum{m, s};
+}
+__device__ __forceinline__ SvSum sv_wave(SvSum p, float c)
+{
+    const float M = wave_max(p.m);
+    return SvSum{M, wave_sum(p.s * sv_term(sv_ref(p.m), sv_ref(M), c))};
+}
+// Segment blockIdx.x % S of row blockIdx.x / S; blockIdx.y 1: of the draft model's.
+template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_sums(SvArgs a)
+{
+    const int r = blockIdx.x / a.S, seg = blockIdx.x % a.S, of = blockIdx.y, t = threadIdx.x;
+    if (of && a.draft[r] < 0) return;
+    const char *x = (const char *)(of ? a.y : a.x) + (long long)r * (of ? a.ldy : a.ld) * El<TYPE>::SZ;
+    const float c = of ? a.dc : a.c;
+    const int nv = a.V / El<TYPE>::VE, lo = (int)((long long)nv * seg / a.S), hi = (int)((long long)nv * (seg + 1) / a.S);
+    const SvSum p = sv_wave(sv_some<TYPE, SV_THREADS>(x, a.V, lo, hi, seg == a.S - 1, c, t), c);
     __shared__ SvSum part[SV_THREADS / 64];
-    const float M = wave_max(m);
-    s = wave_sum(s * sv_term(sv_ref(m), sv_ref(M), c));
-    if (t % 64 == 0) part[t / 64] = SvSum{M, s};
+    if (t % 64 == 0) part[t / 64] = p;
     __syncthreads();
     if (t == 0) a.part[((size_t)r * 2 + of) * a.S + seg] = sv_join(part, SV_THREADS / 64, c);
 }
 
 // -------------------------------------------------------------------- tests --
 __device__ __forceinline__ bool sv_none(const SvSum &s) { return !(s.s > 0.f && s.s < INFINITY); }
-// log softmax(x)_v from its row's sums, in 64 bits: one value a row
-__device__ __forceinline__ double sv_logp(float x, const SvSum &s, float scale)
+__device__ __forceinline__ float sv_logp(float x, const SvSum &s, float scale)
 {
-    return s.s == 0.f ? -INFINITY : ((double)x - (double)s.m) * scale - log((double)s.s);
+    return x == -INFINITY ? x : lp_scaled(x, s.m, scale) - logf(s.s);
 }
 enum { SV_KEEP = 0, SV_PLAIN = 1, SV_REFUSED = 2, SV_NONE = 3 };
-// What row r does with its draft, and the draft's log probability.
-template <int TYPE> __device__ __forceinline__ int sv_test(const SvArgs &a, int r, bool last, float &lp)
+// What row r does with its draft: u q(d) < p(d) as u sum_p < sum_q e^(s (x_d - m) - s' (y_d -
+// m')), whose exponent needs 64 bits where the logits are far apart.
+struct SvTest { int how; float lp; SvSum p, q; };
+template <int TYPE> __device__ __forceinline__ SvTest sv_test(const SvArgs &a, int r, bool last)
 {
-    const SvSum p = sv_join(a.part + (size_t)r * 2 * a.S, a.S, a.c);
+    SvTest o = {SV_NONE, 0.f, sv_join(a.part + (size_t)r * 2 * a.S, a.S, a.c), {0.f, 1.f}};
     const int d = last ? -1 : a.draft[r];
-    lp = 0.f;
-    if (sv_none(p)) return SV_NONE;
-    if (d < 0) return SV_PLAIN;
-    double lpd = -INFINITY, lqd = 0.0;
-    if (d < a.V) lpd = sv_logp(el_load<TYPE>((const char *)a.x + (long long)r * a.ld * El<TYPE>::SZ, d), p, a.scale);
+    const float u = a.u[r];
+    if (sv_none(o.p)) return o;
+    o.how = SV_PLAIN;
+    if (d < 0) return o;
+    const float x = d < a.V ? el_load<TYPE>((const char *)a.x + (long long)r * a.ld * El<TYPE>::SZ, d) : -INFINITY;
+    double z = ((double)x - (double)o.p.m) * a.scale, sq = 1.0;
     if (a.y) {
-        const SvSum q = sv_join(a.part + ((size_t)r * 2 + 1) * a.S, a.S, a.dc);
-        if (!(q.s >= 0.f && q.s < INFINITY)) return SV_NONE;
-        lqd = d < a.V ? sv_logp(el_load<TYPE>((const char *)a.y + (long long)r * a.ldy * El<TYPE>::SZ, d), q, a.dscale)
-                      : -INFINITY;
+        const float y = d < a.V ? el_load<TYPE>((const char *)a.y + (long long)r * a.ldy * El<TYPE>::SZ, d) : -INFINITY;
+        o.q = sv_join(a.part + ((size_t)r * 2 + 1) * a.S, a.S, a.dc);
+        if (!(o.q.s >= 0.f && o.q.s < INFINITY)) {
+            o.how = SV_NONE;
+            return o;
+        }
+        z -= o.q.s == 0.f ? -INFINITY : ((double)y - (double)o.q.m) * a.dscale;
+        if (o.q.s > 0.f) sq = o.q.s;
     }
-    lp = (float)lpd;
-    return log((double)a.u[r]) + lqd < lpd ? SV_KEEP : SV_REFUSED;
+    o.lp = sv_logp(x, o.p, a.scale);
+    const bool keep = u == 0.f ? x > -INFINITY : (double)u * o.p.s < sq * exp(z);
+    o.how = keep ? SV_KEEP : SV_REFUSED;
+    return o;
 }
 
 // ---------------------------------------------------------------------- race --
@@ -166,18 +184,30 @@ __device__ __forceinline__ void sv_try(SvBest &b, const SvRow &w, float x, float
     if (k > b.k) b.k = k, b.v = v;
     if (kp > b.kp) b.kp = kp, b.vp = v;
 }
-template <int TYPE> __device__ __forceinline__ SvBest sv_race(const SvRow &w, int V, int seg, int T)
+// U vectors of each row in flight
+template <int TYPE, int TH> __device__ __forceinline__ SvBest sv_race(const SvRow &w, int V, int seg, int T)
 {
-    constexpr int VE = El<TYPE>::VE;
+    constexpr int VE = El<TYPE>::VE, U = 2;
     const int nv = V / VE, lo = (int)((long long)nv * seg / T), hi = (int)((long long)nv * (seg + 1) / T), t = threadIdx.x;
     SvBest b = {0.f, 0.f, V, V};
-    for (int j = lo + t; j < hi; j += blockDim.x) {
-        const u32x4 x = sv_load<TYPE>(w.x, j * VE), y = w.y ? sv_load<TYPE>(w.y, j * VE) : x;
-        f32x4 e[VE / 4];
+    for (int j = lo + t; j < hi; j += U * TH) {
+        u32x4 x[U], y[U];
+        f32x4 e[U][VE / 4];
 #pragma unroll
-        for (int k = 0; k < VE / 4; k++) e[k] = *(const f32x4_any *)(w.e + j * VE + 4 * k);
+        for (int k = 0; k < U; k++) {
+            const int i = j + k * TH < hi ? j + k * TH : j;
+            x[k] = sv_load<TYPE>(w.x, i * VE);
+            y[k] = w.y ? sv_load<TYPE>(w.y, i * VE) : x[k];
 #pragma unroll
-        for (int i = 0; i < VE; i++) sv_try(b, w, el_at<TYPE>(x, i), el_at<TYPE>(y, i), e[i / 4][i % 4], j * VE + i);
+            for (int n = 0; n < VE / 4; n++) e[k][n] = *(const f32x4_any *)(w.e + i * VE + 4 * n);
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++)
+            if (j + k * TH < hi) {
+#pragma unroll
+                for (int i = 0; i < VE; i++)
+                    sv_try(b, w, el_at<TYPE>(x[k], i), el_at<TYPE>(y[k], i), e[k][i / 4][i % 4], (j + k * TH) * VE + i);
+            }
     }
     if (seg == T - 1 && t < V % VE) {
         const int v = nv * VE + t;
@@ -192,7 +222,7 @@ __device__ __forceinline__ void sv_put(const SvArgs &a, int b, int r, int n, con
     const int v = w.v < a.V ? w.v : w.vp < a.V ? w.vp : -1;
     a.tokens[r] = v;
     if (a.logp)
-        a.logp[r] = v < 0 ? NAN : (float)sv_logp(el_load<TYPE>((const char *)a.x + (long long)r * a.ld * El<TYPE>::SZ, v),
+        a.logp[r] = v < 0 ? NAN : sv_logp(el_load<TYPE>((const char *)a.x + (long long)r * a.ld * El<TYPE>::SZ, v),
                                                  SvSum{m, s}, a.scale);
     if (a.accepted) a.accepted[b] = n;
 }
@@ -202,13 +232,14 @@ __device__ __forceinline__ void sv_rows(const SvArgs &a, int b, int &lo, int &hi
     hi = min(max(a.row0[b + 1], lo), a.N);
 }
 
-// Segment blockIdx.x % T of the race of sequence blockIdx.x / T; segment 0 writes
-// the rows besides the one that ends the sequence.
-template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_pick(SvArgs a)
+// Segment seg of the race of sequence b, TH threads; segment 0 writes the rows besides the
+// one that ends the sequence.
+template <int TYPE, int TH> __device__ __forceinline__ void sv_pick(const SvArgs &a, int b, int seg)
 {
-    const int b = blockIdx.x / a.T, seg = blockIdx.x % a.T, t = threadIdx.x;
-    __shared__ int stop, how;
-    __shared__ SvBest part[SV_THREADS / 64];
+    const int t = threadIdx.x;
+    __shared__ int stop;
+    __shared__ SvTest at_stop;
+    __shared__ SvBest part[TH / 64];
     int lo, hi;
     sv_rows(a, b, lo, hi);
     if (lo == hi) {
@@ -218,27 +249,27 @@ template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_pick(SvAr
     }
     if (t == 0) stop = hi;
     __syncthreads();
-    for (int r0 = lo; r0 < hi; r0 += SV_THREADS) {
+    for (int r0 = lo; r0 < hi; r0 += TH) {
         const int r = r0 + t;
-        float lp = 0.f;
-        const int h = r < hi ? sv_test<TYPE>(a, r, r == hi - 1, lp) : SV_KEEP;
-        if (h != SV_KEEP) atomicMin(&stop, r);
+        SvTest h = {SV_KEEP, 0.f, {0.f, 1.f}, {0.f, 1.f}};
+        if (r < hi) h = sv_test<TYPE>(a, r, r == hi - 1);
+        if (h.how != SV_KEEP) atomicMin(&stop, r);
         __syncthreads();
         const int at = stop;
-        if (r == at) how = h;
+        if (r == at) at_stop = h;
         if (seg == 0 && r < hi && r != at) {
             a.tokens[r] = r < at ? a.draft[r] : -1;
-            if (a.logp) a.logp[r] = r < at ? lp : 0.f;
+            if (a.logp) a.logp[r] = r < at ? h.lp : 0.f;
         }
         __syncthreads();
     }
     // the last row keeps nothing, so stop < hi
-    const int r = stop, h = how;
+    const int r = stop, h = at_stop.how;
     SvRow w;
     w.x = (const char *)a.x + (long long)r * a.ld * El<TYPE>::SZ;
     w.y = nullptr;
     w.e = a.noise + (long long)b * a.ldn;
-    w.p = sv_join(a.part + (size_t)r * 2 * a.S, a.S, a.c);
+    w.p = at_stop.p;
     w.q = SvSum{0.f, 1.f};
     w.c = a.c;
     w.dc = a.dc;
@@ -248,7 +279,7 @@ template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_pick(SvAr
     if (h == SV_REFUSED) {
         if (!a.y) w.point = a.draft[r];
         else {
-            w.q = sv_join(a.part + ((size_t)r * 2 + 1) * a.S, a.S, a.dc);
+            w.q = at_stop.q;
             if (w.q.s > 0.f) {
                 w.y = (const char *)a.y + (long long)r * a.ldy * El<TYPE>::SZ;
                 w.rq = 1.f / w.q.s;
@@ -256,19 +287,44 @@ template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_pick(SvAr
         }
     }
     SvBest k = {0.f, 0.f, a.V, a.V};
-    if (h != SV_NONE) k = sv_race<TYPE>(w, a.V, seg, a.T);
+    if (h != SV_NONE) k = sv_race<TYPE, TH>(w, a.V, seg, a.T);
 #pragma unroll
     for (int o = 32; o; o /= 2) sv_better(k, sv_lane(k, o));
     if (t % 64 == 0) part[t / 64] = k;
     __syncthreads();
     if (t) return;
-    for (int i = 1; i < SV_THREADS / 64; i++) sv_better(k, part[i]);
+    for (int i = 1; i < TH / 64; i++) sv_better(k, part[i]);
     if (a.T == 1) {
         sv_put<TYPE>(a, b, r, r - lo, k, w.p.m, w.p.s);
         return;
     }
     a.best[(size_t)b * a.T + seg] = f32x4{k.k, k.kp, __int_as_float(k.v), __int_as_float(k.vp)};
     if (seg == 0) a.info[b] = f32x4{__int_as_float(r), __int_as_float(r - lo), w.p.m, w.p.s};
+}
+
+// Segment blockIdx.x % T of a sequence's race, the last sequences first: their rows are
+// those that the sums read last.
+template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_pick(SvArgs a)
+{
+    sv_pick<TYPE, SV_THREADS>(a, a.B - 1 - blockIdx.x / a.T, blockIdx.x % a.T);
+}
+// Short rows: a workgroup does all of a sequence, a wave the sums of a row (3 rows of
+// 2048 fp32 values: 6.0 us; two launches 9.0).
+template <int TYPE> __global__ __launch_bounds__(1024) void k_sv_short(SvArgs a)
+{
+    const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, two = a.y ? 2 : 1;
+    int lo, hi;
+    sv_rows(a, b, lo, hi);
+    for (int i = wave; i < (hi - lo) * two; i += 16) {
+        const int r = lo + i / two, of = i % two;
+        if (of && a.draft[r] < 0) continue;
+        const char *x = (const char *)(of ? a.y : a.x) + (long long)r * (of ? a.ldy : a.ld) * El<TYPE>::SZ;
+        const float c = of ? a.dc : a.c;
+        const SvSum p = sv_wave(sv_some<TYPE, 64>(x, a.V, 0, a.V / El<TYPE>::VE, true, c, lane), c);
+        if (lane == 0) a.part[(size_t)r * 2 + of] = p;
+    }
+    __syncthreads();
+    sv_pick<TYPE, 1024>(a, b, 0);
 }
 
 // The winners of a race's segments (T <= 64), one wave a sequence.
@@ -289,18 +345,21 @@ template <int TYPE> __global__ __launch_bounds__(64) void k_sv_join(SvArgs a)
 }
 
 // -------------------------------------------------------------------- entries --
-#define SV_PIECE 1024                                  /* vectors of a segment, at least */
-#define SV_FILL 1024                                   /* workgroups wanted              */
-static int sv_cut(int type, long long rows, int V)
+// Rows of up to SV_SHORT vectors are one workgroup's a sequence.  Longer ones are cut until
+// enough workgroups work: a race's threads wait for every round of loads, so its pieces
+// are smaller.
+#define SV_SHORT 1024
+static bool sv_short(int type, int V) { return V / (type == TLG_F32 ? 4 : 8) <= SV_SHORT; }
+static int sv_cut(int type, long long rows, int V, int piece, int fill)
 {
-    const long long nv = V / (type == TLG_F32 ? 4 : 8), by_size = nv / SV_PIECE, by_rows = SV_FILL / rows;
+    const long long nv = V / (type == TLG_F32 ? 4 : 8), by_size = nv / piece, by_rows = fill / rows;
     const long long s = by_size < by_rows ? by_size : by_rows;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 static size_t sv_layout(int type, int N, int V, int B, int drafted, int *S, int *T, size_t *best, size_t *info)
 {
-    *S = sv_cut(type, (long long)N * (drafted ? 2 : 1), V);
-    *T = sv_cut(type, B, V);
+    *S = sv_short(type, V) ? 1 : sv_cut(type, (long long)N * (drafted ? 2 : 1), V, 1024, 1024);
+    *T = sv_short(type, V) ? 1 : sv_cut(type, B, V, 512, 1024);
     *best = ((size_t)N * 2 * *S * sizeof(SvSum) + 15) & ~(size_t)15;
     *info = *best + (*T > 1 ? (size_t)B * *T * 16 : 0);
     return *info + (*T > 1 ? (size_t)B * 16 : 0);
@@ -316,6 +375,10 @@ extern "C" size_t tlg_spec_verify_ws_bytes(int type, int N, int V, int B, int dr
 
 template <int TYPE> static void sv_launch(const SvArgs &a, hipStream_t st)
 {
+    if (sv_short(TYPE, a.V)) {
+        hipLaunchKernelGGL((k_sv_short<TYPE>), dim3((unsigned)a.B), dim3(1024), 0, st, a);
+        return;
+    }
     hipLaunchKernelGGL((k_sv_sums<TYPE>), dim3((unsigned)a.N * a.S, a.y ? 2 : 1), dim3(SV_THREADS), 0, st, a);
     hipLaunchKernelGGL((k_sv_pick<TYPE>), dim3((unsigned)a.B * a.T), dim3(SV_THREADS), 0, st, a);
     if (a.T > 1) hipLaunchKernelGGL((k_sv_join<TYPE>), dim3(a.B), dim3(64), 0, st, a);

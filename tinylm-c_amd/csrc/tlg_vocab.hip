@@ -279,13 +279,6 @@ template <int TYPE> __device__ __forceinline__ Given lp_given(const LpArgs &a, s
     }
     return g;
 }
-// scale (x - m); halves where the difference of finite values passes fp32 and
-// its product need not
-__device__ __forceinline__ float lp_scaled(float x, float m, float scale)
-{
-    const float d = x - m;
-    return d > -INFINITY || x == -INFINITY ? d * scale : (0.5f * x - 0.5f * m) * scale * 2.f;
-}
 __device__ __forceinline__ void lp_finish(const LpArgs &a, size_t r, const Given &g, const Sums &s, int t)
 {
     if (t < a.M) {
