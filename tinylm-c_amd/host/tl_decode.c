@@ -2,6 +2,7 @@
 #include "tl_decode.h"
 #include "../../include/tldecode.h"
 #include "../../include/tlgemm.h"
+#include "../../include/tlserve.h"
 #include "../../include/tltrain.h"
 #include <math.h>
 #include <stdlib.h>
@@ -37,6 +38,7 @@ struct TlDecode {
     int bulk, *bpos, *btok;
     void *score;                 /* tl_decode_score's buffers, grown on demand */
     size_t score_bytes;
+    void *spec;                  /* tl_decode_sample_spec's buffers, made on first use */
     float *bx, *by, *bn, *bq, *bk, *bv, *bctx, *bact;
 };
 
@@ -161,6 +163,7 @@ void tl_decode_free(TlDecode *d)
     if (!d) return;
     for (int c = 0; c < TLD_MAXPOOL; c++) if (d->graph[c]) tlg_graph_destroy(d->graph[c]);
     if (d->score) tlg_dev_free(d->score);
+    if (d->spec) tlg_dev_free(d->spec);
     if (d->arena) tlg_dev_free(d->arena);
     free(d->Kc);
     free(d->Vc);
@@ -637,6 +640,118 @@ int tl_decode_generate_spec(TlDecode *d, const int *prompt, int np, int n, int *
     }
     if (chunks) *chunks = nch;
     return 0;
+}
+
+/* Number i of the stream of 64-bit numbers with the given seed (splitmix64). */
+static unsigned long long spec_bits(unsigned long long seed, unsigned long long i)
+{
+    unsigned long long z = seed + (i + 1) * 0x9E3779B97F4A7C15ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+
+/* The device buffers of a verification: V exponentials, then TLD_MAXM of each of
+ * uniforms, drafts, tokens and log probabilities, the rows' borders, the drafts
+ * kept, and the workspace. */
+typedef struct { float *noise, *u, *logp; int *draft, *tok, *row0, *kept; void *ws; size_t ws_b; } SpecBuf;
+
+static int spec_buffers(TlDecode *d, SpecBuf *b)
+{
+    const size_t V = ((size_t)d->m.V + 3) & ~(size_t)3, head = 4 * (V + 4 * TLD_MAXM + 4);
+    b->ws_b = 0;
+    for (int m = 1; m <= d->mmax; m++) {
+        const size_t n = tlg_spec_verify_ws_bytes(TLG_F32, m, d->m.V, 1, 0);
+        if (n > b->ws_b) b->ws_b = n;
+    }
+    if (!d->spec && !(d->spec = tlg_dev_malloc(head + b->ws_b))) return TLG_ENOMEM;
+    b->noise = d->spec;
+    b->u = b->noise + V;
+    b->logp = b->u + TLD_MAXM;
+    b->draft = (int *)(b->logp + TLD_MAXM);
+    b->tok = b->draft + TLD_MAXM;
+    b->row0 = b->tok + TLD_MAXM;
+    b->kept = b->row0 + 2;
+    b->ws = (char *)d->spec + head;
+    return 0;
+}
+
+/* Verification call number `call` of a generation: rows [row, row + k] of the logits judge
+ * the k drafts.  host: the numbers' upload buffer; tok, logp: k + 1 of each. */
+static int spec_round(TlDecode *d, const SpecBuf *b, unsigned long long seed, unsigned long long call, float temp, int row,
+                      int k, const int *draft, float *host, int *tok, float *logp, int *kept, void *st)
+{
+    const int V = d->m.V, row0[2] = {0, k + 1};
+    const unsigned long long base = call * (unsigned long long)(V + TLD_MAXM);
+    for (int v = 0; v < V; v++) host[v] = (float)-log(((double)(spec_bits(seed, base + TLD_MAXM + v) >> 11) + 0.5) * 0x1p-53);
+    float *u = host + V;
+    for (int i = 0; i <= k; i++) u[i] = (float)(spec_bits(seed, base + i) >> 40) * 0x1p-24f;
+    int want[TLD_MAXM];
+    for (int i = 0; i <= k; i++) want[i] = i < k ? draft[i] : -1;
+    int rc = tlg_memcpy_h2d(b->noise, host, 4 * (size_t)V, st);
+    if (!rc) rc = tlg_memcpy_h2d(b->u, u, 4 * (size_t)(k + 1), st);
+    if (!rc) rc = tlg_memcpy_h2d(b->draft, want, 4 * (size_t)(k + 1), st);
+    if (!rc) rc = tlg_memcpy_h2d(b->row0, row0, sizeof row0, st);
+    if (!rc)
+        rc = tlg_dev_spec_verify(d->logits + (size_t)row * V, TLG_F32, V, 1.0f / temp, NULL, 0, 1.0f, k + 1, V, b->row0, 1,
+                                 b->draft, b->u, b->noise, V, b->tok, b->logp, b->kept, b->ws, b->ws_b, st);
+    if (!rc) rc = tlg_memcpy_d2h(tok, b->tok, 4 * (size_t)(k + 1), st);
+    if (!rc) rc = tlg_memcpy_d2h(logp, b->logp, 4 * (size_t)(k + 1), st);
+    if (!rc) rc = tlg_memcpy_d2h(kept, b->kept, 4, st);
+    const int rs = tlg_stream_sync(st);              /* also where a call failed: the copies read this frame */
+    if (rc || rs) return rc ? rc : rs;
+    return *kept >= 0 && *kept <= k && tok[*kept] >= 0 ? 0 : TLG_EINVAL;
+}
+
+int tl_decode_sample_spec(TlDecode *d, const int *prompt, int np, int n, float temp, unsigned long long seed, int *toks,
+                          float *logp, int *chunks, void *st)
+{
+    if (!d || !prompt || np <= 0 || n <= 0 || !toks || np > d->maxpos - (n - 1) || !(temp >= 1e-29f && temp <= 1e29f))
+        return TLG_EINVAL;
+    for (int j = 0; j < np; j++) if (prompt[j] < 0 || prompt[j] >= d->m.V) return TLG_EINVAL;
+    int heads = d->m.n_mtp;
+    if (heads > d->mmax - 1) heads = d->mmax - 1;
+    SpecBuf b;
+    CK(spec_buffers(d, &b));
+    float *host = malloc(4 * ((size_t)d->m.V + TLD_MAXM));
+    if (!host) return TLG_ENOMEM;
+    /* prefill of positions 0..np-1, as tl_decode_prime */
+    int i = 0, m = 0, rc = prime_bulk(d, prompt, np, &i, &m, st);
+    while (!rc && i < np) {
+        m = np - i < d->mmax ? np - i : d->mmax;
+        rc = tl_decode_chunk(d, prompt + i, m, i, st);
+        i += m;
+    }
+    int pos = np, cur = m - 1, got = 0, kept = 0, tok[TLD_MAXM], feed[TLD_MAXM];
+    unsigned long long call = 0;
+    float lp[TLD_MAXM];
+    /* the first token is a sample of the prompt's last row: a verification of no drafts */
+    if (!rc) rc = spec_round(d, &b, seed, call++, temp, cur, 0, NULL, host, tok, lp, &kept, st);
+    if (!rc) {
+        if (logp) logp[got] = lp[0];
+        toks[got++] = tok[0];
+    }
+    while (!rc && got < n) {
+        /* the last token and the heads' drafts of what follows it, no more than are asked for */
+        int k = n - got - 1 < heads ? n - got - 1 : heads;
+        if (k > d->maxpos - pos - 1) k = d->maxpos - pos - 1;
+        for (int h = 0; !rc && h < k; h++) rc = tl_decode_mtp_draft(d, cur, h, d->dtok + h, st);
+        if (!rc && k) rc = tlg_memcpy_d2h(feed + 1, d->dtok, 4 * (size_t)k, st);
+        if (!rc) rc = tlg_stream_sync(st);
+        feed[0] = toks[got - 1];
+        if (!rc) rc = tl_decode_chunk(d, feed, k + 1, pos, st);
+        if (!rc) rc = spec_round(d, &b, seed, call++, temp, 0, k, feed + 1, host, tok, lp, &kept, st);
+        for (int r = 0; !rc && r <= kept; r++) {
+            if (logp) logp[got] = lp[r];
+            toks[got++] = tok[r];
+        }
+        pos += kept + 1;
+        cur = kept;
+    }
+    const int rs = tlg_stream_sync(st);              /* no copy from `host` or the prompt is in flight */
+    free(host);
+    if (chunks) *chunks = (int)call - 1;
+    return rc ? rc : rs;
 }
 
 int tl_decode_greedy_step(TlDecode *d, int copy, void *st)

@@ -91,6 +91,21 @@ int tl_decode_mtp_draft(TlDecode *d, int row, int k, int *dtok_out, void *stream
  * number of verification chunks to *chunks.  Needs n_mtp >= 1 and n_mtp + 1
  * <= mmax; weights copy 0. */
 int tl_decode_generate_spec(TlDecode *d, const int *prompt, int np, int n, int *toks, int *chunks, void *stream);
+/* The same by sampling (no counterpart: the reference's self-speculative loop is greedy):
+ * n tokens of which each is a sample of softmax(logits / temp) of the row before it, temp
+ * 1e-29 .. 1e29, whatever the heads draft.  The n_mtp heads' greedy drafts (none with
+ * n_mtp = 0; at most mmax - 1 are used) go through one chunk behind the last token,
+ * and tlg_dev_spec_verify (include/tlserve.h) keeps them or puts a sample in their place.
+ * logp (host [n], or NULL): the tokens' log probabilities at that temperature.  Numbers: with s(i)
+ * = splitmix64's number i of `seed` (the finalizer of seed + (i + 1) 0x9E37..15), call c of
+ * the verification, the prompt's last row being call 0, takes as uniform of its row r (s(c
+ * (V + 8) + r) >> 40) 2^-24 and as exponential of token v -log(((s(c (V + 8) + 8 + v) >>
+ * 11) + 1/2) 2^-53), so that equal calls give equal tokens.  *chunks: the chunks that
+ * were fed after the prompt.  Needs np + n - 1 <= maxpos.  Weights copy 0; TLG_EINVAL also where
+ * a row of logits has no distribution.  Synchronous; the greedy state is undefined
+ * afterwards. */
+int tl_decode_sample_spec(TlDecode *d, const int *prompt, int np, int n, float temp, unsigned long long seed, int *toks,
+                          float *logp, int *chunks, void *stream);
 /* Capture the greedy step once per weight copy; tl_decode_graph_step
  * replays the next copy's graph. */
 int tl_decode_graph_build(TlDecode *d, void *stream);

@@ -623,6 +623,17 @@ class Decode:
                                                        ctypes.byref(ch), stream), "tl_decode_generate_spec")
         return out, ch.value
 
+    def sample_spec(self, prompt, n, stream, temp=1.0, seed=0):
+        """Self-speculative generation by sampling (tl_decode_sample_spec):
+        (tokens, their log probabilities, verification chunks)."""
+        import numpy as np
+        p = np.ascontiguousarray(prompt, np.int32)
+        out, lp = np.zeros(n, np.int32), np.zeros(n, np.float32)
+        ch = ctypes.c_int(0)
+        self._ck(self.host.dll.tl_decode_sample_spec(self.h, p.ctypes.data, p.size, n, temp, seed, out.ctypes.data,
+                                                     lp.ctypes.data, ctypes.byref(ch), stream), "tl_decode_sample_spec")
+        return out, lp, ch.value
+
     def graph_build(self, stream):
         return self._ck(self.host.dll.tl_decode_graph_build(self.h, stream), "tl_decode_graph_build")
 
@@ -852,6 +863,8 @@ class Host:
         d.tl_decode_mtp_draft.restype = _i
         d.tl_decode_generate_spec.argtypes = [_vp, _vp, _i, _i, _vp, _vp, _vp]
         d.tl_decode_generate_spec.restype = _i
+        d.tl_decode_sample_spec.argtypes = [_vp, _vp, _i, _i, _f, ctypes.c_ulonglong, _vp, _vp, _vp, _vp]
+        d.tl_decode_sample_spec.restype = _i
         self.dll = d
 
     def load_checkpoint(self, path):
