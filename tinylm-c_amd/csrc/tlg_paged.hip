@@ -621,7 +621,8 @@ static int pg_check(const char *who, const TlgPages *c, const TlgBatch *b, int t
     if (!pg_al(b->row0, 4) || !pg_al(b->len, 4) || (b->ldt && !pg_al(b->table, 4)))
         return tlg_fail(TLG_EINVAL, "%s: row0 %p len %p table %p", who, (const void *)b->row0, (const void *)b->len,
                         (const void *)b->table);
-    *o = PgBatch{b->row0, b->len, b->table, b->B, b->N, b->ldt, c->page, c->n_pages,
+    // without columns the table is not looked at, but a first entry of it may be read
+    *o = PgBatch{b->row0, b->len, b->ldt ? b->table : b->row0, b->B, b->N, b->ldt, c->page, c->n_pages,
                  0xffffffffu / (unsigned)c->page, c->page_ld, c->tok_ld, c->head_ld};
     *work = 1;
     return TLG_OK;

@@ -11,7 +11,10 @@
 // (16 modulo 32 banks).
 #include "tlg_paged.h"
 
-template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_tile(AttnArgs a)
+// ALIKE: the 16 bytes that a wave brings in one go, up to 16 tokens' in a row, lie on one page (pages
+// of a multiple of 16 tokens): their address is then one scalar and an offset that the
+// lane keeps, which saves a third of the vector instructions.
+template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_tile(AttnArgs a)
 {
     typedef typename ElT<T>::E E;
     constexpr int TT = PGT_TOKENS(HD), NB = HD / 32, NT = TT / 32, CH = HD / 8, NL = TT * CH / 256;
@@ -57,24 +60,31 @@ template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) vo
     float R = -INFINITY, l = 0.f;
 
     // the thread's pieces of a tile: token (tid + 256 i) / CH, elements 8 ((tid + 256 i) % CH)
-    int pg[NL];
+    int pg[NL], in[NL];                                  // its page, and its place there
     u32x4 kr[NL], vr[NL];
     bool lost[NL];
+    const unsigned mine = ALIKE ? (unsigned)(lane / CH * (int)a.b.tok_ld + lane % CH * 8) * 2 : 0;
     auto page = [&](int j) {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int t = pg_tile<TT>(rg, j) + (tid + 256 * i) / CH, n = pg_of(a.b, t);
-            pg[i] = j < j1 && t <= rg.pmax && n < a.b.ldt ? table[n] : -1;
+            const int t = pg_tile<TT>(rg, j) + ((ALIKE ? 64 * wave : tid) + 256 * i) / CH, n = pg_of(a.b, t);
+            pg[i] = table[max(min(n, a.b.ldt - 1), 0)];
+            in[i] = n < a.b.ldt ? t - n * a.b.page : -1;
         }
     };
-    auto load = [&](int j) {
+    auto load = [&]() {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int ch = tid + 256 * i, t = pg_tile<TT>(rg, j) + ch / CH, n = pg[i];
-            lost[i] = n < 0 || n >= a.b.n_pages;
-            const long long off = (lost[i] ? 0ll : n * a.b.page_ld + (t - pg_of(a.b, t) * a.b.page) * a.b.tok_ld) + ch % CH * 8;
-            kr[i] = *(const u32x4 *)(Kc + off);
-            vr[i] = *(const u32x4 *)(Vc + off);
+            const int n = ALIKE ? __builtin_amdgcn_readfirstlane(pg[i]) : pg[i];
+            lost[i] = n < 0 || n >= a.b.n_pages || in[i] < 0;
+            const long long off = lost[i] ? 0ll : n * a.b.page_ld + in[i] * a.b.tok_ld;
+            if constexpr (ALIKE) {
+                kr[i] = *(const u32x4 *)((const char *)(Kc + off) + (lost[i] ? 0u : mine));
+                vr[i] = *(const u32x4 *)((const char *)(Vc + off) + (lost[i] ? 0u : mine));
+            } else {
+                kr[i] = *(const u32x4 *)(Kc + off + (tid + 256 * i) % CH * 8);
+                vr[i] = *(const u32x4 *)(Vc + off + (tid + 256 * i) % CH * 8);
+            }
         }
     };
     auto whole = [&](const Range &x, int t0) { return t0 + TT - 1 <= x.pmin && (x.lomax <= t0 || t0 + TT - 1 < a.sinks); };
@@ -107,14 +117,14 @@ template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) vo
     bool odd = false;
     if (j0 < j1) {
         page(j0);
-        load(j0);
+        load();
         page(j0 + 1);
         odd = __syncthreads_or(put(j0, 0));
     }
     for (int j = j0, buf = 0; j < j1; j++, buf ^= 1) {
         const bool more = j + 1 < j1;
         if (more) {
-            load(j + 1);
+            load();
             page(j + 2);
         }
         const int t0 = pg_tile<TT>(rg, j);
@@ -161,7 +171,13 @@ template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) vo
                                           [](int blk, int m) { return 32 * blk + m; });
             }
         }
-        if (more) odd = __syncthreads_or(put(j + 1, buf ^ 1));
+        if (more) {
+            const bool hit = put(j + 1, buf ^ 1);
+            if (whole(rg, pg_tile<TT>(rg, j + 1))) {
+                odd = false;
+                __syncthreads();
+            } else odd = __syncthreads_or(hit);
+        }
     }
     l = pg_gsum<32>(l);
     if (!live) return;
@@ -177,16 +193,20 @@ template <int T, int HD> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) vo
     if (h == 0) pg_out_sums(a, pg_part(a, a.pm, 2, s, parts, r, head), r, head, R, l);
 }
 
-template <int T> static void launch(const AttnArgs &a, int hd, unsigned grid, hipStream_t st)
+template <int T, bool ALIKE> static void launch(const AttnArgs &a, int hd, unsigned grid, hipStream_t st)
 {
-    if (hd == 32) hipLaunchKernelGGL((k_paged_tile<T, 32>), dim3(grid), dim3(256), 0, st, a);
-    else if (hd == 64) hipLaunchKernelGGL((k_paged_tile<T, 64>), dim3(grid), dim3(256), 0, st, a);
-    else if (hd == 96) hipLaunchKernelGGL((k_paged_tile<T, 96>), dim3(grid), dim3(256), 0, st, a);
-    else if (hd == 128) hipLaunchKernelGGL((k_paged_tile<T, 128>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_paged_tile<T, 256>), dim3(grid), dim3(256), 0, st, a);
+    if (hd == 32) hipLaunchKernelGGL((k_paged_tile<T, 32, ALIKE>), dim3(grid), dim3(256), 0, st, a);
+    else if (hd == 64) hipLaunchKernelGGL((k_paged_tile<T, 64, ALIKE>), dim3(grid), dim3(256), 0, st, a);
+    else if (hd == 96) hipLaunchKernelGGL((k_paged_tile<T, 96, false>), dim3(grid), dim3(256), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((k_paged_tile<T, 128, ALIKE>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_tile<T, 256, ALIKE>), dim3(grid), dim3(256), 0, st, a);
 }
 void pg_tile_launch(const AttnArgs &a, int type, int hd, unsigned grid, hipStream_t st)
 {
-    if (type == TLG_F16) launch<TLG_F16>(a, hd, grid, st);
-    else launch<TLG_BF16>(a, hd, grid, st);
+    // 16 tokens' offsets in 32 bits
+    const bool alike = a.b.page % 16 == 0 && a.b.tok_ld < 1 << 24;
+    if (type == TLG_F16 && alike) launch<TLG_F16, true>(a, hd, grid, st);
+    else if (type == TLG_F16) launch<TLG_F16, false>(a, hd, grid, st);
+    else if (alike) launch<TLG_BF16, true>(a, hd, grid, st);
+    else launch<TLG_BF16, false>(a, hd, grid, st);
 }
