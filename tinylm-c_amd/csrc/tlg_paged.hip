@@ -529,9 +529,11 @@ template <int T, bool EVEN, int WV> __global__ __launch_bounds__(256) void k_pag
     long long first, second, apart;                      // places (columns) of the first sums, the second, and from one to the next
     const float *po, *pm;
     if constexpr (EVEN) {
-        const int all = a.place[a.b.B], P = a.place[a.b.B + 1], from = a.place[b], tiles = (cols + w - 1) / w,
+        // cut to what there is, should another call have written to this workspace
+        const int all = a.place[a.b.B], P = min(a.place[a.b.B + 1], a.P), from = a.place[b], tiles = (cols + w - 1) / w,
                   tot = (a.place[b + 1] - from) / tiles, u = from + rh / w * tot;
-        const long long i0 = pg_share_of(all, P, u), i1 = pg_share_of(all, P, u + tot - 1);
+        if (P < 1 || all < P || tot < 1) return;
+        const long long i0 = min(max(pg_share_of(all, P, u), 0), P - 1), i1 = min(max(pg_share_of(all, P, u + tot - 1), (int)i0), P - 1);
         parts = (int)(i1 - i0 + 1);
         first = ((i0 * a.KV + kvh) * 2 + 1) * w + rh % w;
         second = ((i0 + 1) * a.KV + kvh) * 2 * w + rh % w;

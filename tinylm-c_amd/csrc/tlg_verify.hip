@@ -219,7 +219,7 @@ template <int TYPE, int TH> __device__ __forceinline__ SvBest sv_race(const SvRo
 template <int TYPE>
 __device__ __forceinline__ void sv_put(const SvArgs &a, int b, int r, int n, const SvBest &w, float m, float s)
 {
-    const int v = w.v < a.V ? w.v : w.vp < a.V ? w.vp : -1;
+    const int v = (unsigned)w.v < (unsigned)a.V ? w.v : (unsigned)w.vp < (unsigned)a.V ? w.vp : -1;
     a.tokens[r] = v;
     if (a.logp)
         a.logp[r] = v < 0 ? NAN : sv_logp(el_load<TYPE>((const char *)a.x + (long long)r * a.ld * El<TYPE>::SZ, v),
@@ -333,7 +333,7 @@ template <int TYPE> __global__ __launch_bounds__(64) void k_sv_join(SvArgs a)
     const int b = blockIdx.x, t = threadIdx.x;
     const f32x4 i = a.info[b];
     const int r = __float_as_int(i[0]);
-    if (r < 0) return;
+    if ((unsigned)r >= (unsigned)a.N) return;            // none, or another call wrote to this workspace
     SvBest k = {0.f, 0.f, a.V, a.V};
     if (t < a.T) {
         const f32x4 p = a.best[(size_t)b * a.T + t];
