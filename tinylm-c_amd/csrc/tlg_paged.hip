@@ -421,9 +421,17 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
                 }
                 if (more) loadV(buf ^ 1);
                 pg_wave_sync();
-                u32x4 pf[NE / 8];
+                // weights in two pieces, what rounding takes from the first one and that: the products
+                // then keep 16 (bf16) or 22 bits of them, in time that the cache's bytes take anyway
+                u32x4 pf[NE / 8], pr[NE / 8];
 #pragma unroll
-                for (int i = 0; i < NE / 2; i++) pf[i / 4][i & 3] = pg_pack<T>(e[2 * i], e[2 * i + 1]);
+                for (int i = 0; i < NE / 2; i++) {
+                    typedef E e2 __attribute__((ext_vector_type(2)));
+                    const unsigned hi = pg_pack<T>(e[2 * i], e[2 * i + 1]);
+                    const e2 back = __builtin_bit_cast(e2, hi);
+                    pf[i / 4][i & 3] = hi;
+                    pr[i / 4][i & 3] = pg_pack<T>(e[2 * i] - (float)back[0], e[2 * i + 1] - (float)back[1]);
+                }
                 // sixteen lanes read four tokens of sixteen elements and get a column of them each
                 const E *vt = vs + (4 * g + (lane >> 2 & 3)) * VST + (W == 32 ? 16 * (lane >> 4 & 1) : 0) + 4 * (lane & 3);
 #pragma unroll
@@ -434,7 +442,9 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
                         const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v));
                         const u32x2 v1 =
                             __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + 4 * G * VST)));
-                        o[k] = pg_mfma<T, W>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[i], o[k]);
+                        const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+                        o[k] = pg_mfma<T, W>(vf, pf[i], o[k]);
+                        o[k] = pg_mfma<T, W>(vf, pr[i], o[k]);
                     }
             }
             if (odd)
