@@ -30,7 +30,8 @@ extern "C" {
 #define TLG_PAGED_LEN (1 << 30)     /* tokens of a sequence (ldt * page)       */
 #define TLG_PAGED_ROWS (1 << 21)    /* rows of a call                          */
 #define TLG_PAGED_SEQS (1 << 16)    /* sequences of a call                     */
-#define TLG_PAGED_HEADS 1024        /* query heads; N * H of a call is at most 2^30 */
+#define TLG_PAGED_HEADS 1024        /* query heads; N * H of an attention is at
+                                       most 2^29, B * KV at most 2^22          */
 
 /* One layer's cache: n_pages pages of `page` tokens; the hd elements of page g,
  * token t and head h start at g * page_ld + t * tok_ld + h * head_ld elements of

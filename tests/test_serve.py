@@ -83,7 +83,8 @@ def test_bad_stores_are_refused(L, bad):
                                  dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-31),
                                  dict(scale=1e31), dict(win=-1), dict(sinks=-1), dict(q=None), dict(q=P + 8),
                                  dict(ldq=248), dict(ldq=260), dict(out=None), dict(out=P + 2), dict(ldo=128),
-                                 dict(lse=P + 2)])
+                                 dict(lse=P + 2), dict(b=dict(N=1 << 20), H=514, ldq=514 * 64, ldo=514 * 64),
+                                 dict(b=dict(B=1 << 16), c=dict(KV=65), H=65, ldq=65 * 64, ldo=65 * 64)])
 def test_bad_attention_is_refused(L, bad):
     refused(L, attn(L, **bad), "paged_attn")
 

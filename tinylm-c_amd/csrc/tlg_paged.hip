@@ -13,7 +13,7 @@ struct StoreArgs {
     char *qo;
     long long ldq, ldqo, ldk, ldv;
     const float *cs, *sn;
-    int maxpos;
+    int maxpos, per;             // rows of a workgroup
 };
 template <int T> __device__ __forceinline__ void st_get(const char *p, float *x)       // 8 elements
 {
@@ -42,15 +42,18 @@ template <int T> __device__ __forceinline__ void st_put(char *p, const float *x)
     }
 }
 
-// A workgroup takes R consecutive rows; a thread eight pairs (i, i + hd/2) of a head.
+// A workgroup takes up to ST_ROWS consecutive rows; a thread eight pairs (i, i + hd/2) of
+// a head.  Bound by the bytes of many rows (16384 rows of 48 heads of 128 bf16 values: 71
+// us, 5.0 TB/s, a copy reaches 5.4), by the chain sequence - page - row of few, which one row
+// a workgroup keeps shortest (209 such rows: 6.0 us, 10.0 with four).
 #define ST_ROWS 4
 template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(StoreArgs a)
 {
     constexpr int ts = T == TLG_F32 ? 4 : 2, cs = C == TLG_F32 ? 4 : 2;
-    const int lane = threadIdx.x & 63, r0 = blockIdx.x * ST_ROWS, half = a.hd >> 1, per = half >> 3;
+    const int lane = threadIdx.x & 63, r0 = blockIdx.x * a.per, half = a.hd >> 1, per = half >> 3;
     __shared__ int pos[ST_ROWS];                      // position, -1 none: no such row
     __shared__ long long at[ST_ROWS];                 // the token's elements in the cache, -1: not stored
-    for (int k = threadIdx.x >> 6; k < ST_ROWS; k += 4) {
+    for (int k = threadIdx.x >> 6; k < a.per; k += 4) {
         const int r = r0 + k;
         int p = INT_MIN;
         long long to = -1;
@@ -72,7 +75,7 @@ template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(Sto
     }
     __syncthreads();
     const int heads = a.H + 2 * a.KV, items = heads * per;
-    for (int q = threadIdx.x; q < ST_ROWS * items; q += 256) {
+    for (int q = threadIdx.x; q < a.per * items; q += 256) {
         const int k = q / items, rem = q - k * items, h = rem / per, i = (rem - h * per) * 8, p = pos[k];
         if (p == INT_MIN) continue;
         const long long r = r0 + k;
@@ -523,13 +526,12 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
 // against 21; 1792 rows with four sums: 8.5 against 5).  EVEN:
 // those of k_paged_direct in tiles of `w` columns; else of the rows' kernels, whose tiles of `w`
 // columns had their tokens in tiles of 32 or, with the flag, 64.
-template <int T, bool EVEN, int WV> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int w, int by64)
+template <int T, bool EVEN, int WV>
+__device__ __forceinline__ void pg_join_row(const AttnArgs &a, int hd, int w, int by64, int rhd)
 {
     constexpr int U = 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rhd = __builtin_amdgcn_readfirstlane(WV == 4 ? blockIdx.x : blockIdx.x * 4 + wave), part = WV == 4 ? wave : 0;
-    const int r = rhd / a.H, head = rhd - r * a.H;
-    if (r >= a.b.N) return;
+    const int part = WV == 4 ? wave : 0, r = rhd / a.H, head = rhd - r * a.H;
     const int b = pg_search(a.b.B, r, [&](int i) { return pg_row0(a.b, i); });
     const Seq q = pg_seq(a.b, b);
     if (r < q.lo || r >= q.lo + q.n) return;
@@ -601,6 +603,13 @@ template <int T, bool EVEN, int WV> __global__ __launch_bounds__(256) void k_pag
     float y[4] = {x[0], x[1], x[2], x[3]};
     if (in) pg_out<T, 4>(a, hd, nullptr, r, head, 4 * lane, l, y);
     if (lane == 0) pg_out_sums(a, nullptr, r, head, top, l);
+}
+template <int T, bool EVEN, int WV> __global__ __launch_bounds__(256) void k_paged_join(AttnArgs a, int hd, int w, int by64)
+{
+    if constexpr (WV == 4) pg_join_row<T, EVEN, 4>(a, hd, w, by64, blockIdx.x);
+    else
+        for (int i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); i < a.b.N * a.H; i += gridDim.x * 4)
+            pg_join_row<T, EVEN, 1>(a, hd, w, by64, i);
 }
 
 // -------------------------------------------------------------------- entries --
@@ -678,7 +687,8 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
     a.cs = cos_t;
     a.sn = sin_t;
     a.maxpos = maxpos;
-    const dim3 grid((b->N + ST_ROWS - 1) / ST_ROWS), block(256);
+    a.per = b->N >= 4096 ? ST_ROWS : 1;
+    const dim3 grid((b->N + a.per - 1) / a.per), block(256);
     hipStream_t st = ST(stream);
     if (type == TLG_F16) hipLaunchKernelGGL((k_paged_store<TLG_F16, TLG_F16>), grid, block, 0, st, a);
     else if (type == TLG_BF16) hipLaunchKernelGGL((k_paged_store<TLG_BF16, TLG_BF16>), grid, block, 0, st, a);
@@ -785,7 +795,8 @@ template <int W> static void pg_few(const AttnArgs &a, int type, int kv, int hd,
 }
 template <bool EVEN, int WV> static void pg_join(const AttnArgs &a, int type, int hd, int w, int by64, hipStream_t st)
 {
-    const dim3 grid((unsigned)(((long long)a.b.N * a.H * WV + 3) / 4));
+    const long long groups = ((long long)a.b.N * a.H * WV + 3) / 4;
+    const dim3 grid((unsigned)(groups < 1 << 16 ? groups : 1 << 16));
     if (type == TLG_F32) hipLaunchKernelGGL((k_paged_join<TLG_F32, EVEN, WV>), grid, dim3(256), 0, st, a, hd, w, by64);
     else if (type == TLG_F16) hipLaunchKernelGGL((k_paged_join<TLG_F16, EVEN, WV>), grid, dim3(256), 0, st, a, hd, w, by64);
     else hipLaunchKernelGGL((k_paged_join<TLG_BF16, EVEN, WV>), grid, dim3(256), 0, st, a, hd, w, by64);
@@ -813,7 +824,8 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
     if ((rc = pg_check("paged_attn", c, b, type, &a.b, &work))) return rc;
     if (H <= 0 || H > TLG_PAGED_HEADS || H % c->KV)
         return tlg_fail(TLG_EINVAL, "paged_attn: H=%d KV=%d", H, c->KV);
-    if ((long long)b->N * H > 1 << 30) return tlg_fail(TLG_EINVAL, "paged_attn: N=%d H=%d", b->N, H);
+    if ((long long)b->N * H > 1 << 29 || (long long)b->B * c->KV > 1 << 22)           // what a grid takes
+        return tlg_fail(TLG_EINVAL, "paged_attn: N=%d H=%d B=%d KV=%d", b->N, H, b->B, c->KV);
     if (!(scale >= 1e-30f && scale <= 1e30f) || win < 0 || sinks < 0)
         return tlg_fail(TLG_EINVAL, "paged_attn: scale=%g win=%d sinks=%d", scale, win, sinks);
     if (!work) return TLG_OK;
