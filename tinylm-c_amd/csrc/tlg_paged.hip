@@ -1,4 +1,6 @@
-// tlg_paged.hip -- a paged KV cache and the attention over it (include/tlserve.h).
+// tlg_paged.hip -- a paged KV cache and the attention over it (include/tlserve.h): rows
+// into the cache, attention of few rows a sequence and of fp32 rows, the joins of shared
+// sums, and the entries.  tlg_paged_tile.hip has the attention of many 16-bit rows.
 #include "tlg_paged.h"
 
 #define ST(s) ((hipStream_t)(s))
@@ -200,6 +202,11 @@ __device__ __forceinline__ int pg_share_of(int T, int P, int u)
 // every fourth of its tiles and join their sums.  Blocks of W = 16 columns where there
 // are no more: half the registers of 32.  ROWS (fp32): every wave a block of columns of its
 // own, whose keys the waves of a workgroup find in the CU's cache.
+// Measured: 56 sequences of 1024 to 4096 tokens, 32 query and 8 KV heads of 128 bf16
+// values, 118 us for 602 MB of cache (5.1 TB/s; a plain read reaches 7.1), one row over 131072
+// tokens 102 us (5.2); 2000 sequences of up to 1024 tokens 5.3 TB/s.  256 to 512 workgroups
+// are best; with three waves a SIMD or 1024 workgroups the same bytes take 8 to 12 % longer.
+// fp32 prompts reach 70 to 93 TFLOP/s of 142.
 // One workgroup a CU where two would spill (fp32 rows of 96 elements on, 256 elements).
 template <int T, int C, int HD, int W, bool ROWS>
 __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32 ? 4 : 3) >= 384) || HD == 256 ? 1 : 2) void k_paged_direct(AttnArgs a)

@@ -9,11 +9,17 @@
 // apart by what makes the reads free of bank conflicts: keys are read 16 bytes a lane
 // down 16 tokens (row lengths 4 modulo 64 banks), values four tokens by 32 elements
 // (16 modulo 32 banks).
+// Measured: 4096 rows over 16384 tokens, 32 query and 8 KV heads of 128 bf16 values, 1.14 to 1.2
+// ms, 800 to 842 TFLOP/s (a large library product: 1210); matrix cores and vector ALUs
+// 36 % busy each, LDS about 45 %, and the two waves of a SIMD wait for each other.  The
+// weights are rounded to the rows' type, once, to nearest: their errors average out over
+// the tokens (norm error 0.0023 with bf16 outputs' own 0.0017); two pieces, as k_paged_direct
+// has them, would add half of the products.
 #include "tlg_paged.h"
 
 // ALIKE: the 16 bytes that a wave brings in one go, up to 16 tokens' in a row, lie on one page (pages
 // of a multiple of 16 tokens): their address is then one scalar and an offset that the
-// lane keeps, which saves a third of the vector instructions.
+// lane keeps (207 M vector instructions in place of 343 M, 1276 -> 1162 us).
 template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_tile(AttnArgs a)
 {
     typedef typename ElT<T>::E E;

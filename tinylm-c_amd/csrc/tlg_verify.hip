@@ -11,6 +11,9 @@
 // Two launches: the sums of every row (bound by HBM, each logit read once), then
 // for each sequence the tests of its rows, a scalar each, and the race over the one
 // row that ends it; a third joins races that are cut over workgroups.  Short rows: one.
+// Measured: 898 rows of 131072 bf16 logits of both models, 118 to 125 us (sums 72 us, 5.7
+// to 6.4 TB/s; races 44 us, whose rows are read again; join 4 us); 168 rows of 32003 fp16
+// logits 22 us, three launches of a few rounds of loads each.
 #include "tlg_internal.h"
 #include "tlg_rows.h"
 #include "../../include/tlserve.h"
@@ -308,8 +311,7 @@ template <int TYPE> __global__ __launch_bounds__(SV_THREADS) void k_sv_pick(SvAr
 {
     sv_pick<TYPE, SV_THREADS>(a, a.B - 1 - blockIdx.x / a.T, blockIdx.x % a.T);
 }
-// Short rows: a workgroup does all of a sequence, a wave the sums of a row (3 rows of
-// 2048 fp32 values: 6.0 us; two launches 9.0).
+// Short rows: a workgroup does all of a sequence, a wave the sums of a row.
 template <int TYPE> __global__ __launch_bounds__(1024) void k_sv_short(SvArgs a)
 {
     const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, two = a.y ? 2 : 1;
@@ -345,11 +347,20 @@ template <int TYPE> __global__ __launch_bounds__(64) void k_sv_join(SvArgs a)
 }
 
 // -------------------------------------------------------------------- entries --
-// Rows of up to SV_SHORT vectors are one workgroup's a sequence.  Longer ones are cut until
+// Rows of up to SV_SHORT vectors are one workgroup's a sequence, twice as long ones from
+// SV_CROWD sequences on.  In a graph that gains where sequences fill the chip (256 of 5 rows of 4096
+// fp32 values 13.2 us, in two launches 16.6; of 2048 values 11.4 and 12.1) and costs little where
+// they do not (one of 3 rows of 2048 8.8 and 8.7, 16 of 5 rows 9.6 and 9.1; of 4000 values 10.8 and
+// 9.9); a call from the host saves the second launch, 2.8 us.  Longer rows are cut until
 // enough workgroups work: a race's threads wait for every round of loads, so its pieces
 // are smaller.
-#define SV_SHORT 1024
-static bool sv_short(int type, int V) { return V / (type == TLG_F32 ? 4 : 8) <= SV_SHORT; }
+#define SV_SHORT 512
+#define SV_CROWD 128
+static bool sv_short(int type, int V, int B)
+{
+    const int nv = V / (type == TLG_F32 ? 4 : 8);
+    return nv <= SV_SHORT || (nv <= 2 * SV_SHORT && B >= SV_CROWD);
+}
 static int sv_cut(int type, long long rows, int V, int piece, int fill)
 {
     const long long nv = V / (type == TLG_F32 ? 4 : 8), by_size = nv / piece, by_rows = fill / rows;
@@ -358,8 +369,8 @@ static int sv_cut(int type, long long rows, int V, int piece, int fill)
 }
 static size_t sv_layout(int type, int N, int V, int B, int drafted, int *S, int *T, size_t *best, size_t *info)
 {
-    *S = sv_short(type, V) ? 1 : sv_cut(type, (long long)N * (drafted ? 2 : 1), V, 1024, 1024);
-    *T = sv_short(type, V) ? 1 : sv_cut(type, B, V, 512, 1024);
+    *S = sv_short(type, V, B) ? 1 : sv_cut(type, (long long)N * (drafted ? 2 : 1), V, 1024, 1024);
+    *T = sv_short(type, V, B) ? 1 : sv_cut(type, B, V, 512, 1024);
     *best = ((size_t)N * 2 * *S * sizeof(SvSum) + 15) & ~(size_t)15;
     *info = *best + (*T > 1 ? (size_t)B * *T * 16 : 0);
     return *info + (*T > 1 ? (size_t)B * 16 : 0);
@@ -375,7 +386,7 @@ extern "C" size_t tlg_spec_verify_ws_bytes(int type, int N, int V, int B, int dr
 
 template <int TYPE> static void sv_launch(const SvArgs &a, hipStream_t st)
 {
-    if (sv_short(TYPE, a.V)) {
+    if (sv_short(TYPE, a.V, a.B)) {
         hipLaunchKernelGGL((k_sv_short<TYPE>), dim3((unsigned)a.B), dim3(1024), 0, st, a);
         return;
     }
