@@ -422,6 +422,28 @@ def test_attn_bad_pages(lib, type, kv, number, rows, lens, win):
     check_attn(s, q, 2, type, 0.125, win, 0, out, ls, bad=[(b, 3)])
 
 
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("rows,hd", [([2], 32), ([70], 128), ([3, 100], 64)])
+def test_attn_cache_without_pages(lib, type, kv, rows, hd):
+    """Nothing is read of it; rows that see a token are NaN, those before position 0 are 0.
+    A store writes nothing there."""
+    s = Seqs(rows, [30] * len(rows), 1, hd, 16, kv).gpu()
+    s.pages.n_pages, s.pages.K, s.pages.V = 0, None, None
+    for ldt in (s.ldt, 0):
+        s.batch.ldt = ldt
+        s.batch.table = s.dev[2].data_ptr() if ldt else None
+        q = queries(s, 2, type)
+        out, ls = run_attn(lib, s, q, 2, type, 0.2)
+        o, l = out.cpu().float().numpy(), ls.cpu().numpy()
+        for b, n in enumerate(rows):
+            r = int(s.row0[b])
+            before = max(n - 30, 0)
+            assert (o[r:r + before] == 0).all() and np.isneginf(l[r:r + before]).all()
+            assert np.isnan(o[r + before:r + n]).all() and np.isnan(l[r + before:r + n]).all()
+        want, got, cs = run_store(lib, s, 2, type)
+        assert np.isfinite(got.cpu().float().numpy()[max(rows) - 20:max(rows)]).all()
+
+
 @pytest.mark.parametrize("type,kv", [(F32, F16), (BF16, BF16)])
 @pytest.mark.parametrize("rows,win", [([2], 0), ([90], 0), ([90], 10), ([1], 30)])
 def test_attn_table_too_short(lib, type, kv, rows, win):
@@ -489,6 +511,56 @@ def test_attn_many_sequences(lib):
             q = queries(s, 4, type)
             out, ls = run_attn(lib, s, q, 4, type, 0.2)
             check_attn(s, q, 4, type, 0.2, 0, 0, out, ls)
+
+
+@pytest.mark.parametrize("B", [130, 300, 1000, 1100])
+def test_attn_many_sequences_with_room_for_long_ones(lib, B):
+    """Tables that could hold more tokens than the sequences have, as a server's do:
+    shares of the batch that span many short sequences, and a few long ones."""
+    g = np.random.default_rng(B)
+    rows = [int(x) for x in g.integers(0, 3, B)]
+    lens = [max(r, int(x)) for r, x in zip(rows, g.integers(1, 50, B))]
+    for b in (3, B // 2, B - 1):
+        rows[b], lens[b] = 2, 1500 + b
+    for type, kv, H in ((F32, F16, 2), (BF16, BF16, 12)):
+        s = Seqs(rows, lens, 1, 32, 16, kv, hints=False, extra_ldt=60, lead=1).gpu()
+        s.batch.max_rows = 2
+        q = queries(s, H, type)
+        out, ls = run_attn(lib, s, q, H, type, 0.2)
+        check_attn(s, q, H, type, 0.2, 0, 0, out, ls)
+
+
+@pytest.mark.parametrize("type,kv", [(F32, F32), (F16, F16)])
+@pytest.mark.parametrize("rows,H,hd", [([1], 2, 32), ([9, 0, 1], 3, 64)])
+def test_attn_hundreds_of_shares(lib, type, kv, rows, H, hd):
+    """One long sequence that every workgroup takes a part of."""
+    s = Seqs(rows, [66001] + [5] * (len(rows) - 1), 1, hd, 64, kv).gpu()
+    q = queries(s, H, type)
+    out, ls = run_attn(lib, s, q, H, type, hd ** -0.5)
+    check_attn(s, q, H, type, hd ** -0.5, 0, 0, out, ls)
+
+
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("hd", [96, 128, 256])
+def test_attn_shares_of_wide_heads(lib, type, kv, hd):
+    """Ragged lengths shared evenly, in blocks of 16 and of 32 columns."""
+    for rows, H in (([1, 2, 1], 4), ([3, 1, 6], 4)):
+        s = Seqs(rows, [2600, 90, 700], 1, hd, 16, kv, head_major=True).gpu()
+        q = queries(s, H, type)
+        out, ls = run_attn(lib, s, q, H, type, hd ** -0.5)
+        check_attn(s, q, H, type, hd ** -0.5, 0, 0, out, ls)
+
+
+@pytest.mark.parametrize("page", [16, 48, 33])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_attn_long_chunks_of_two_layouts(lib, page, hd):
+    """Many 16-bit rows: pages that a wave's load does and does not stay within, in
+    both layouts, a chunk in the middle of a page."""
+    for hm in (True, False):
+        s = Seqs([100, 45], [391, 300], 2, hd, page, BF16, head_major=hm).gpu()
+        q = queries(s, 6, BF16)
+        out, ls = run_attn(lib, s, q, 6, BF16, hd ** -0.5, 150, 20)
+        check_attn(s, q, 6, BF16, hd ** -0.5, 150, 20, out, ls)
 
 
 def test_attn_pages_far_apart(lib):
