@@ -714,10 +714,17 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 // alike), unless there are sequences enough; below, where looking up the batch costs more than
 // that gains, each sequence is cut alike (32 sequences of 5 rows that see 1028 tokens:
 // 18 us against 24).
+// fp32 rows take blocks of 16 columns a wave where those of 32 do not fill the chip (4
+// prompts of 256 rows, 8 heads of 32: 18 against 14 us; of 128 elements 58 against 68).
+// Many rows' partial sums cost more than their tokens' division gains, unless the
+// chip is not filled or every part is long (4 prompts of 300 rows, 32 heads of 128 bf16: 28 us
+// whole, 68 in two parts; 512 rows over 8192 tokens 120 us in seven parts, 129 in five).
 #define PG_FEW 32
 #define PG_FILL 512                  /* workgroups wanted of k_paged_direct: two a CU */
-#define PG_FILL_ROWS 1024            /* of the rows' kernels                */
+#define PG_FILL_TILE 384             /* of k_paged_tile                     */
+#define PG_FILL_ROWS 1024            /* of k_paged_direct for fp32 rows: short waves, one SIMD each */
 #define PG_LONG 64                   /* tiles of 32 tokens                  */
+#define PG_SHORT 16                  /* tiles that the rows' kernels take for sequences of few rows too */
 #define PG_MANY 2048                 /* sequences times KV heads that need no sharing */
 struct Plan {
     bool few, both;
@@ -727,6 +734,7 @@ struct Plan {
     int P, Sf, perf, S, per;         // few: shares, or parts of a sequence; the rows' kernel's parts
     size_t po, pm, place, eo, em, bytes;
 };
+// Parts of a sequence: until `fill` workgroups work, with 8 tiles at least each.
 static int pg_cut(long long groups, long long fill, long long tiles, long long row)
 {
     long long S = fill / groups;
@@ -749,8 +757,9 @@ static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int type, int H, int w
                     tiles = ((seen < most ? seen : most) + 31) / 32, row = (long long)b->N * H * (c->hd + 2) * 4;
     p.few = cols <= PG_FEW;
     p.W = cols <= 16 || c->hd == 256 ? 16 : 32;            // 32 of 256 elements do not fit the registers
-    p.wide = type == TLG_F32 ? c->hd == 256 ? 64 : 128 : PGT_ROWS;
-    p.both = !p.few && (long long)b->B * rows > b->N;
+    p.wide = PGT_ROWS;
+    if (type == TLG_F32 && (c->hd == 256 || (c->hd <= 64 && ((long long)b->N * G / 128 + b->B) * c->KV < PG_FILL))) p.wide = 64;
+    p.both = !p.few && (long long)b->B * rows > b->N && tiles > PG_SHORT;
     p.slots = (unsigned)((long long)b->N * G / p.wide + b->B);
     p.S = p.Sf = 1;
     if (p.few || p.both) {
@@ -761,7 +770,13 @@ static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int type, int H, int w
             if (p.P < b->B) p.P = b->B;
         } else p.Sf = pg_cut((long long)b->B * c->KV, PG_FILL, tiles, row);
     }
-    if (!p.few) p.S = pg_cut((long long)p.slots * c->KV, PG_FILL_ROWS, tiles, row);
+    if (!p.few) {
+        // the tiles that there are: of each sequence's last, half, in the mean
+        const long long groups = ((long long)b->N * G / p.wide + (b->B + 1) / 2) * c->KV;
+        const int fill = type == TLG_F32 ? PG_FILL_ROWS : PG_FILL_TILE, one = pg_cut(groups, fill, tiles, row),
+                  two = pg_cut(groups, 2 * fill, tiles / 4, row);
+        p.S = one > two ? one : two;
+    }
     p.perf = pg_per(tiles, p.Sf);
     p.per = pg_per(tiles, p.S);
     const int S = p.S > p.Sf ? p.S : p.Sf;
@@ -813,13 +828,18 @@ template <bool EVEN> static void pg_join(const AttnArgs &a, int type, int hd, in
     if ((long long)a.b.N * a.H < 512) pg_join<EVEN, 4>(a, type, hd, w, by64, st);
     else pg_join<EVEN, 1>(a, type, hd, w, by64, st);
 }
-template <int C> static void pg_rows32(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
+template <int C, int W> static void pg_rows32(const AttnArgs &a, int hd, dim3 grid, hipStream_t st)
 {
-    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 32, 32, true>), grid, dim3(256), 0, st, a);
-    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 64, 32, true>), grid, dim3(256), 0, st, a);
-    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 96, 32, true>), grid, dim3(256), 0, st, a);
-    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 128, 32, true>), grid, dim3(256), 0, st, a);
+    if (hd == 32) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 32, W, true>), grid, dim3(256), 0, st, a);
+    else if (hd == 64) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 64, W, true>), grid, dim3(256), 0, st, a);
+    else if (hd == 96) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 96, W, true>), grid, dim3(256), 0, st, a);
+    else if (hd == 128) hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 128, W, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_paged_direct<TLG_F32, C, 256, 16, true>), grid, dim3(256), 0, st, a);
+}
+template <int C> static void pg_rows32(const AttnArgs &a, int wide, int hd, dim3 grid, hipStream_t st)
+{
+    if (wide == 64) pg_rows32<C, 16>(a, hd, grid, st);
+    else pg_rows32<C, 32>(a, hd, grid, st);
 }
 
 extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const void *q, int type, long long ldq, int H,
@@ -885,9 +905,9 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
         a.S = p.S;
         a.per = p.per;
         const dim3 grid(p.slots * c->KV * p.S);
-        if (type == TLG_F32 && c->type == TLG_F32) pg_rows32<TLG_F32>(a, c->hd, grid, st);
-        else if (type == TLG_F32 && c->type == TLG_F16) pg_rows32<TLG_F16>(a, c->hd, grid, st);
-        else if (type == TLG_F32) pg_rows32<TLG_BF16>(a, c->hd, grid, st);
+        if (type == TLG_F32 && c->type == TLG_F32) pg_rows32<TLG_F32>(a, p.wide, c->hd, grid, st);
+        else if (type == TLG_F32 && c->type == TLG_F16) pg_rows32<TLG_F16>(a, p.wide, c->hd, grid, st);
+        else if (type == TLG_F32) pg_rows32<TLG_BF16>(a, p.wide, c->hd, grid, st);
         else pg_tile_launch(a, type, c->hd, grid.x, st);
         if (p.S > 1) pg_join<false>(a, type, c->hd, type == TLG_F32 ? p.wide / 4 : PGT_ROWS, type != TLG_F32 && PGT_TOKENS(c->hd) == 64, st);
     }
