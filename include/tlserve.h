@@ -69,7 +69,8 @@ typedef struct {
  * by the angles of cos_t / sin_t [maxpos][hd/2], 16-byte aligned; a position outside
  * them gives NaN), computed in fp32 and rounded once.  cos_t and sin_t NULL:
  * no rotation.  q (rows of H heads; q_out its rows, which may be the same memory
- * with the same ldq) may be NULL, then H is ignored.  Rows are `type` elements, row
+ * with the same ldq, else the memory from its first to its last element must not overlap
+ * q's) may be NULL, then H is ignored.  Rows are `type` elements, row
  * r of q at q + r * ldq and so on, 16-byte aligned with distances that are
  * multiples of 16 bytes (slices of one fused projection, for instance).  The cache is
  * of the rows' type, or of any type for fp32 rows.
@@ -86,7 +87,8 @@ int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const void *q, lon
  * reads KV head h / (H / KV):
  *   out[r][h] = sum_t softmax_t(scale q . k_t) v_t,   lse[r][h] = log sum_t e^(scale q . k_t)
  * q and out have rows of H * hd elements of `type`, ldq and ldo apart (16-byte
- * aligned; out must not overlap q or the cache); lse [N][H] may be NULL.  The
+ * aligned; the memory from out's first to its last element must not overlap q's, nor
+ * the cache); lse [N][H] may be NULL.  The
  * cache is of that type, or of any type for fp32 rows.  scale lies in 1e-30 ..
  * 1e30.  Scores, softmax and sums are fp32.  For 16-bit rows the weights e^(s - max)
  * are rounded to that type before they meet v (where sequences have few rows, to

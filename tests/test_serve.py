@@ -33,7 +33,7 @@ def store(L, c={}, b={}, q=P, ldq=256, q_out=P, ldqo=256, H=4, k=P, ldk=128, v=P
     return L.tlg_dev_paged_store(*args(c, b), q, ldq, q_out, ldqo, H, k, ldk, v, ldv, type, cos, sin, maxpos, None)
 
 
-def attn(L, c={}, b={}, q=P, type=F16, ldq=256, H=4, scale=0.1, win=0, sinks=0, out=P, ldo=256, lse=P, ws=P,
+def attn(L, c={}, b={}, q=P, type=F16, ldq=256, H=4, scale=0.1, win=0, sinks=0, out=2 * P, ldo=256, lse=P, ws=P,
          ws_bytes=1 << 40):
     return L.tlg_dev_paged_attn(*args(c, b), q, type, ldq, H, scale, win, sinks, out, ldo, lse, ws, ws_bytes, None)
 
@@ -74,7 +74,8 @@ def test_no_cache_or_batch_is_refused(L, call):
 @pytest.mark.parametrize("bad", [dict(H=0), dict(H=1025), dict(q=P + 8), dict(ldq=255), dict(ldq=248), dict(ldq=260),
                                  dict(q_out=None), dict(ldqo=128), dict(k=None), dict(ldk=120), dict(ldk=132),
                                  dict(v=P + 4), dict(ldv=64), dict(cos=None), dict(sin=None), dict(cos=P + 4),
-                                 dict(sin=P + 8), dict(maxpos=-1), dict(ldk=1 << 41)])
+                                 dict(sin=P + 8), dict(maxpos=-1), dict(ldk=1 << 41), dict(ldqo=264), dict(q_out=P + 16),
+                                 dict(q_out=P - 1024)])
 def test_bad_stores_are_refused(L, bad):
     refused(L, store(L, **bad), "paged_store")
 
@@ -83,7 +84,7 @@ def test_bad_stores_are_refused(L, bad):
                                  dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-31),
                                  dict(scale=1e31), dict(win=-1), dict(sinks=-1), dict(q=None), dict(q=P + 8),
                                  dict(ldq=248), dict(ldq=260), dict(out=None), dict(out=P + 2), dict(ldo=128),
-                                 dict(lse=P + 2), dict(b=dict(N=1 << 20), H=514, ldq=514 * 64, ldo=514 * 64),
+                                 dict(lse=P + 2), dict(out=P), dict(out=P + 1024), dict(out=P - 1520), dict(b=dict(N=1 << 20), H=514, ldq=514 * 64, ldo=514 * 64),
                                  dict(b=dict(B=1 << 16), c=dict(KV=65), H=65, ldq=65 * 64, ldo=65 * 64)])
 def test_bad_attention_is_refused(L, bad):
     refused(L, attn(L, **bad), "paged_attn")

@@ -660,6 +660,13 @@ static bool pg_rows(const void *p, long long ld, long long width, int type)
     return pg_al(p, 16) && ld >= width && ld <= 1ll << 40 && ld % (16 / (long long)pg_size(type)) == 0;
 }
 
+// memory from the first to the last element of two sets of N rows meets
+static bool pg_meet(const void *a, long long lda, const void *b, long long ldb, long long width, int type, int N)
+{
+    const uintptr_t e = pg_size(type), a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    return a0 < b0 + ((uintptr_t)(N - 1) * ldb + width) * e && b0 < a0 + ((uintptr_t)(N - 1) * lda + width) * e;
+}
+
 extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const void *q, long long ldq, void *q_out,
                                    long long ldqo, int H, const void *k, long long ldk, const void *v, long long ldv,
                                    int type, const float *cos_t, const float *sin_t, int maxpos, void *stream)
@@ -677,6 +684,8 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
         return tlg_fail(TLG_EINVAL, "paged_store: k %p ldk=%lld v %p ldv=%lld", k, ldk, v, ldv);
     if (q && (!pg_rows(q, ldq, wq, type) || !pg_rows(q_out, ldqo, wq, type)))
         return tlg_fail(TLG_EINVAL, "paged_store: q %p ldq=%lld q_out %p ldqo=%lld", q, ldq, q_out, ldqo);
+    if (q && !(q == q_out && ldq == ldqo) && pg_meet(q, ldq, q_out, ldqo, wq, type, b->N))
+        return tlg_fail(TLG_EINVAL, "paged_store: q_out overlaps q without being the same rows");
     if ((rc = tlg_ensure_init())) return rc;
     a.K = (char *)c->K;
     a.V = (char *)c->V;
@@ -859,6 +868,7 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
     const long long w = (long long)H * c->hd;
     if (!pg_rows(q, ldq, w, type) || !pg_rows(out, ldo, w, type) || (lse && !pg_al(lse, 4)))
         return tlg_fail(TLG_EINVAL, "paged_attn: q %p ldq=%lld out %p ldo=%lld lse %p", q, ldq, out, ldo, (void *)lse);
+    if (pg_meet(q, ldq, out, ldo, w, type, b->N)) return tlg_fail(TLG_EINVAL, "paged_attn: out overlaps q");
     const size_t need = tlg_paged_attn_ws_bytes(c, b, type, H);
     if (need && (ws_bytes < need || !pg_al(ws, 16)))
         return tlg_fail(TLG_EINVAL, "paged_attn: workspace %p of %zu bytes, %zu needed", ws, ws_bytes, need);
