@@ -716,15 +716,17 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 }
 
 // How a call is launched: the columns (rows times heads of a KV head) of a sequence
-// decide.  few: only k_paged_direct; else the rows' kernel, and, where the numbers of
-// rows differ, the former for the sequences of few.
+// decide.  few (up to PG_FEW): only k_paged_direct; else the rows' kernel, and, where the
+// numbers of rows differ, the former for the sequences of few.  8 sequences of 8192 tokens,
+// 32 / 8 heads of 128 bf16: 24 columns 65 us so and 83 by the rows' kernel, 32 67 and 62, 36 81 and 65
+// (32 sequences of 1024: 44 and 42, 47 and 45, 66 and 48).
 // k_paged_direct's workgroups share the batch's tokens evenly from PG_LONG tiles of a
 // sequence on (64 sequences of 1024 to 4096 tokens: 124 us against 133 where each is cut
 // alike), unless there are sequences enough; below, where looking up the batch costs more than
 // that gains, each sequence is cut alike (32 sequences of 5 rows that see 1028 tokens:
 // 18 us against 24).
 // fp32 rows take blocks of 16 columns a wave where those of 32 do not fill the chip (4
-// prompts of 256 rows, 8 heads of 32: 18 against 14 us; of 128 elements 58 against 68).
+// prompts of 256 rows, 8 heads of 32: 14 us, 18 in blocks of 32; of 128 elements 68 and 58, so not there).
 // Many rows' partial sums cost more than their tokens' division gains, unless the
 // chip is not filled or every part is long (4 prompts of 300 rows, 32 heads of 128 bf16: 28 us
 // whole, 68 in two parts; 512 rows over 8192 tokens 120 us in seven parts, 129 in five).
