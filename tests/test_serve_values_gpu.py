@@ -1,0 +1,73 @@
+"""GPU tests of what attention over a paged cache (include/tlserve.h) makes of values:
+how many bits its weights keep, and what rows get of NaN and infinities that they see.
+
+Tolerances.  eps = 2^-24.  A score is off by (hd + 1) eps sum_d |q_d k_d| scale, its
+weight by that, the same of the row's maximum, and eps (4 |s - m| + 6) of the exponent:
+d_t.  16-bit rows have weights of two pieces, off by WEIGHT(type) more (twice the type's
+half step) and, for fp16, whose smallest step is 2^-24, by SMALL of the row's
+largest.  A sum of L terms in any order adds (L + 64) eps, numerator and
+denominator each, and what is written its own half step:
+  sum_t p_t |v_t| (2 d_t + WEIGHT + 2 (L + 64) eps) + SMALL sum_t |v_t| + half |out|
+"""
+import math
+
+import numpy as np
+import pytest
+
+from test_serve_gpu import BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, half, queries, run_attn, tiny
+
+pytestmark = pytest.mark.gpu
+WEIGHT = {F32: 0.0, F16: 2.0 ** -22, BF16: 2.0 ** -16}
+SMALL = {F32: 0.0, F16: 2.0 ** -36, BF16: 0.0}
+
+
+def reference(s, q, H, type, scale, win, sinks):
+    """out [N][H][hd] in float64 and its bound.  Values that are not finite count for the
+    rows that see them, whatever their weight: NaN, or infinities of one sign."""
+    G = H // s.KV
+    out, tol = np.full((s.N, H, s.hd), np.nan), np.zeros((s.N, H, s.hd))
+    for b, (n, L) in enumerate(zip(s.rows, s.lens)):
+        r0 = int(s.row0[b])
+        pos, tt = np.arange(L - n, L)[:, None], np.arange(L)[None]
+        see = tt <= pos
+        if win:
+            see &= (tt > pos - win) | (tt < sinks)
+        k, v = s.get(s.K, b, L).numpy(), s.get(s.V, b, L).numpy()
+        for h in range(H):
+            qq, kk, vv = q[r0:r0 + n, h], k[:, h // G], v[:, h // G]
+            z = np.where(see, scale * (qq @ kk.T), -np.inf)
+            mag = np.where(see, scale * (abs(qq) @ abs(kk).T), 0.0)
+            m = z.max(1, keepdims=True)
+            e = np.exp(z - m)
+            p = e / e.sum(1, keepdims=True)
+            d = (s.hd + 1) * EPS * (mag + mag.max(1, keepdims=True)) + EPS * (4 * np.where(see, m - z, 0.0) + 6)
+            ok = np.isfinite(vv)
+            w = np.where(ok, vv, 0.0)
+            o = p @ w
+            t = (p * (2 * d + WEIGHT[type] + 2 * (L + 64) * EPS)) @ abs(w) + SMALL[type] * (see @ abs(w)) + \
+                half(type) * abs(o) + tiny(type)
+            nan, up, down = (see.astype(float) @ x.astype(float) > 0 for x in (np.isnan(vv), vv == np.inf, vv == -np.inf))
+            o = np.where(nan | (up & down), np.nan, np.where(up, np.inf, np.where(down, -np.inf, o)))
+            out[r0:r0 + n, h], tol[r0:r0 + n, h] = o, t
+    return out, tol
+
+
+def compare(lib, s, H, type, scale, win=0, sinks=0, q=None):
+    q = queries(s, H, type) if q is None else q
+    out, _ = run_attn(lib, s, q, H, type, scale, win, sinks)
+    want, tol = reference(s, q.double().numpy(), H, type, scale, win, sinks)
+    inside = np.zeros(s.N, bool)
+    inside[int(s.row0[0]):int(s.row0[-1])] = True
+    check(out.cpu().double().numpy().reshape(s.N, H, s.hd)[inside], want[inside], tol[inside], "out")
+
+
+@pytest.mark.parametrize("type", [F16, BF16], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("rows,lens,KV,H,hd,page,win", [
+    ([128], [700], 1, 1, 32, 16, 0), ([150, 40], [600, 300], 2, 8, 64, 16, 0), ([70, 64], [400, 130], 1, 4, 96, 7, 0),
+    ([100, 90], [900, 90], 2, 8, 128, 64, 0), ([100], [500], 2, 4, 128, 7, 130), ([80], [333], 1, 2, 256, 16, 0),
+    ([1, 3], [900, 200], 2, 8, 128, 16, 0)])
+def test_weights_keep_twice_their_bits(lib, type, rows, lens, KV, H, hd, page, win):
+    """Rounded to the rows' type once, weights are off by 2^-8 (bf16): more than the
+    output's own rounding wherever values cancel."""
+    s = Seqs(rows, lens, KV, hd, page, type, lead=1, tail=1).gpu()
+    compare(lib, s, H, type, hd ** -0.5, win, 3 if win else 0)

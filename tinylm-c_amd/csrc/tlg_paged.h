@@ -112,6 +112,16 @@ template <int T> __device__ __forceinline__ unsigned pg_pack(float lo, float hi)
     const e2 v = {(typename ElT<T>::E)lo, (typename ElT<T>::E)hi};
     return __builtin_bit_cast(unsigned, v);
 }
+// Two weights as register k of two operands whose sum they are to twice the type's bits: rounded, and
+// what that took from them (exact in fp32), rounded.
+template <int T> __device__ __forceinline__ void pg_split(float x, float y, u32x4 &hi, u32x4 &lo, int k)
+{
+    typedef typename ElT<T>::E e2 __attribute__((ext_vector_type(2)));
+    const unsigned w = pg_pack<T>(x, y);
+    const e2 back = __builtin_bit_cast(e2, w);
+    hi[k] = w;
+    lo[k] = pg_pack<T>(x - (float)back[0], y - (float)back[1]);
+}
 // Sum and maximum over the groups of lanes that share a column, in every lane.
 template <int W, typename OP> __device__ __forceinline__ float pg_groups(float v, OP op)
 {

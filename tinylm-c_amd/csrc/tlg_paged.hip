@@ -435,13 +435,7 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
                 // then keep 16 (bf16) or 22 bits of them, in time that the cache's bytes take anyway
                 u32x4 pf[NE / 8], pr[NE / 8];
 #pragma unroll
-                for (int i = 0; i < NE / 2; i++) {
-                    typedef E e2 __attribute__((ext_vector_type(2)));
-                    const unsigned hi = pg_pack<T>(e[2 * i], e[2 * i + 1]);
-                    const e2 back = __builtin_bit_cast(e2, hi);
-                    pf[i / 4][i & 3] = hi;
-                    pr[i / 4][i & 3] = pg_pack<T>(e[2 * i] - (float)back[0], e[2 * i + 1] - (float)back[1]);
-                }
+                for (int i = 0; i < NE / 2; i++) pg_split<T>(e[2 * i], e[2 * i + 1], pf[i / 4], pr[i / 4], i & 3);
                 // sixteen lanes read four tokens of sixteen elements and get a column of them each
                 const E *vt = vs + (4 * g + (lane >> 2 & 3)) * VST + (W == 32 ? 16 * (lane >> 4 & 1) : 0) + 4 * (lane & 3);
 #pragma unroll

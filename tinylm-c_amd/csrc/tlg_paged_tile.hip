@@ -9,13 +9,14 @@
 // apart by what makes the reads free of bank conflicts: keys are read 16 bytes a lane
 // down 16 tokens (row lengths 4 modulo 64 banks), values four tokens by 32 elements
 // (16 modulo 32 banks).
-// Measured: 4096 rows over 16384 tokens, 32 query and 8 KV heads of 128 bf16 values, 1.14 to 1.2
-// ms, 800 to 842 TFLOP/s (a large library product: 1210); matrix cores and vector ALUs
-// 36 % busy each, LDS about 45 %, and the two waves of a SIMD wait for each other.  The
-// weights are rounded to the rows' type, once, to nearest: their errors average out over
-// the tokens (norm error 0.0023 with bf16 outputs' own 0.0017); two pieces, as k_paged_direct
-// has them, would add half of the products.
+// Measured: 4096 rows over 16384 tokens, 32 query and 8 KV heads of 128 bf16 values, 1.47 to 1.52
+// ms, 633 to 654 TFLOP/s of the operator's own products (a large library product: 1210).  The
+// weights are in two pieces as k_paged_direct's, which is half of the products again: rounded to
+// bf16 once they took 1.16 to 1.18 ms and left a norm error of 0.0023, where the output's own rounding is
+// 0.0017.  Exponentials and splits dealt out between the products, by hand or by
+// scheduling barriers, took 1.47 to 1.53 ms.
 #include "tlg_paged.h"
+#include <type_traits>
 
 // ALIKE: the 16 bytes that a wave brings in one go, up to 16 tokens' in a row, lie on one page (pages
 // of a multiple of 16 tokens): their address is then one scalar and an offset that the
@@ -58,13 +59,6 @@ template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256
             if (!live) qf[i] = u32x4{0, 0, 0, 0};
         }
     }
-    f32x16 o[NB];
-#pragma unroll
-    for (int k = 0; k < NB; k++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[k][i] = 0.f;
-    float R = -INFINITY, l = 0.f;
-
     // the thread's pieces of a tile: token (tid + 256 i) / CH, elements 8 ((tid + 256 i) % CH)
     int pg[NL], in[NL];                                  // its page, and its place there
     u32x4 kr[NL], vr[NL];
@@ -94,11 +88,11 @@ template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256
         }
     };
     auto whole = [&](const Range &x, int t0) { return t0 + TT - 1 <= x.pmin && (x.lomax <= t0 || t0 + TT - 1 < a.sinks); };
-    // to LDS; true if values of a tile that some column sees in part had to be cleaned
-    auto put = [&](int j, int buf) {
+    // to LDS; true if values of a tile had to be cleaned: one that some column sees in part, or any
+    auto put = [&](int j, int buf, auto every) {
         bool odd = false;
         const int t0 = pg_tile<TT>(rg, j);
-        if (!whole(rg, t0)) {
+        if (every || !whole(rg, t0)) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 bool hit = false;
@@ -120,72 +114,95 @@ template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256
         }
         return odd;
     };
-    bool odd = false;
-    if (j0 < j1) {
-        page(j0);
-        load();
-        page(j0 + 1);
-        odd = __syncthreads_or(put(j0, 0));
-    }
-    for (int j = j0, buf = 0; j < j1; j++, buf ^= 1) {
-        const bool more = j + 1 < j1;
-        if (more) {
+    // An infinite value times a weight's second piece, which may be 0 or negative, is no infinity.  Sums
+    // that are not finite are therefore formed once more, with every tile's values cleaned.
+    f32x16 o[NB];
+    float R, l;
+    auto walk = [&](auto every) {
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[k][i] = 0.f;
+        R = -INFINITY;
+        l = 0.f;
+        bool odd = false;
+        if (j0 < j1) {
+            page(j0);
             load();
-            page(j + 2);
+            page(j0 + 1);
+            odd = __syncthreads_or(put(j0, 0, every));
         }
-        const int t0 = pg_tile<TT>(rg, j);
-        if (some && t0 <= rw.pmax && (t0 + TT > lomin || t0 < a.sinks)) {
-            float e[16 * NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                f32x16 z;
-#pragma unroll
-                for (int i = 0; i < 16; i++) z[i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < HD / 16; i++)
-                    z = pg_mfma<T, 32>(*(const u32x4 *)(ks[buf] + (32 * t + col) * KST + 16 * i + 8 * h), qf[i], z);
-#pragma unroll
-                for (int i = 0; i < 16; i++) e[16 * t + i] = z[i];
+        for (int j = j0, buf = 0; j < j1; j++, buf ^= 1) {
+            const bool more = j + 1 < j1;
+            if (more) {
+                load();
+                page(j + 2);
             }
-            const bool full = whole(rw, t0);
-            if (!full) {
+            const int t0 = pg_tile<TT>(rg, j);
+            if (some && t0 <= rw.pmax && (t0 + TT > lomin || t0 < a.sinks)) {
+                float e[16 * NT];
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int t = 0; t < NT; t++) {
+                    f32x16 z;
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        e[16 * t + i] = pg_sees(a, t0 + 32 * t + pg_at<32>(i, h), p, from) ? e[16 * t + i] : -INFINITY;
-            }
-            pg_weights<32, 16 * NT, NB>(e, a.c, R, l, o);
-            u32x4 pf[2 * NT];
+                    for (int i = 0; i < 16; i++) z[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8 * NT; i++) pf[i / 4][i & 3] = pg_pack<T>(e[2 * i], e[2 * i + 1]);
-            const E *vt = vs[buf] + (4 * h + (lane >> 2 & 3)) * VST + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+                    for (int i = 0; i < HD / 16; i++)
+                        z = pg_mfma<T, 32>(*(const u32x4 *)(ks[buf] + (32 * t + col) * KST + 16 * i + 8 * h), qf[i], z);
 #pragma unroll
-            for (int i = 0; i < 2 * NT; i++)
-#pragma unroll
-                for (int k = 0; k < NB; k++) {
-                    const E *v = vt + 16 * i * VST + 32 * k;
-                    const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v));
-                    const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + 8 * VST)));
-                    o[k] = pg_mfma<T, 32>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[i], o[k]);
+                    for (int i = 0; i < 16; i++) e[16 * t + i] = z[i];
                 }
-            if (odd && !full) {
+                const bool full = whole(rw, t0);
+                if (!full) {
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-                    pg_special<T, 32, NB>(a, o, e + 16 * t, scratch[wave], (const char *)Vc, t0 + 32 * t, rg.pmax, p, from,
-                                          [&](int k) { return pg_token(a.b, table, t0 + 32 * t + k); },
-                                          [](int blk, int m) { return 32 * blk + m; });
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            e[16 * t + i] = pg_sees(a, t0 + 32 * t + pg_at<32>(i, h), p, from) ? e[16 * t + i] : -INFINITY;
+                }
+                pg_weights<32, 16 * NT, NB>(e, a.c, R, l, o);
+                const E *vt = vs[buf] + (4 * h + (lane >> 2 & 3)) * VST + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+#pragma unroll
+                for (int i = 0; i < 2 * NT; i++) {
+                    // weights in two pieces, as k_paged_direct's
+                    u32x4 pf, pr;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) pg_split<T>(e[8 * i + 2 * k], e[8 * i + 2 * k + 1], pf, pr, k);
+#pragma unroll
+                    for (int k = 0; k < NB; k++) {
+                        const E *v = vt + 16 * i * VST + 32 * k;
+                        const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v));
+                        const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + 8 * VST)));
+                        const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+                        o[k] = pg_mfma<T, 32>(vf, pf, o[k]);
+                        o[k] = pg_mfma<T, 32>(vf, pr, o[k]);
+                    }
+                }
+                if (odd && (every || !full)) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        pg_special<T, 32, NB>(a, o, e + 16 * t, scratch[wave], (const char *)Vc, t0 + 32 * t, rg.pmax, p, from,
+                                              [&](int k) { return pg_token(a.b, table, t0 + 32 * t + k); },
+                                              [](int blk, int m) { return 32 * blk + m; });
+                }
+            }
+            if (more) {
+                const bool hit = put(j + 1, buf ^ 1, every);
+                if (!every && whole(rg, pg_tile<TT>(rg, j + 1))) {
+                    odd = false;
+                    __syncthreads();
+                } else odd = __syncthreads_or(hit);
             }
         }
-        if (more) {
-            const bool hit = put(j + 1, buf ^ 1);
-            if (whole(rg, pg_tile<TT>(rg, j + 1))) {
-                odd = false;
-                __syncthreads();
-            } else odd = __syncthreads_or(hit);
-        }
-    }
-    l = pg_gsum<32>(l);
+        l = pg_gsum<32>(l);
+    };
+    walk(std::false_type());
+    bool again = false;
+#pragma unroll
+    for (int k = 0; k < NB; k++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) again |= !pg_finite(o[k][i]);
+    if (__syncthreads_or(again && live && pg_finite(l))) walk(std::true_type());
     if (!live) return;
     const int head = kvh * a.G + g;
     float *sums = pg_part(a, a.po, HD, s, parts, r, head);
