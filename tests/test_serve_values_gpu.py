@@ -14,7 +14,7 @@ import math
 import numpy as np
 import pytest
 
-from test_serve_gpu import BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, half, queries, run_attn, tiny
+from test_serve_gpu import _t, BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, half, queries, run_attn, tiny
 
 pytestmark = pytest.mark.gpu
 WEIGHT = {F32: 0.0, F16: 2.0 ** -22, BF16: 2.0 ** -16}
@@ -71,3 +71,45 @@ def test_weights_keep_twice_their_bits(lib, type, rows, lens, KV, H, hd, page, w
     output's own rounding wherever values cancel."""
     s = Seqs(rows, lens, KV, hd, page, type, lead=1, tail=1).gpu()
     compare(lib, s, H, type, hd ** -0.5, win, 3 if win else 0)
+
+
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf], ids=["nan", "inf", "minus"])
+@pytest.mark.parametrize("H,rows,lens,hd,page,win", [
+    (1, [256], [256], 64, 16, 0), (4, [256], [266], 64, 16, 0), (4, [256, 5], [276, 100], 32, 7, 0),
+    (8, [256], [276], 64, 7, 0), (1, [256], [300], 128, 16, 200), (4, [100], [310], 96, 16, 200),
+    (8, [60], [300], 256, 16, 150), (4, [100], [200], 64, 16, 30)])
+def test_visible_values_of_many_rows(lib, type, kv, value, H, rows, lens, hd, page, win):
+    """One element of some tokens' values is not finite: rows that see the token get it
+    whether its tile is seen whole or in part by them, by their wave or by the rows that share
+    their workgroup; the others' are as ever."""
+    spoiled(lib, type, kv, value, H, rows, lens, hd, page, win)
+
+
+def spoiled(lib, type, kv, value, H, rows, lens, hd, page, win):
+    s = Seqs(rows, lens, 1, hd, page, kv)
+    for b, (n, L) in enumerate(zip(rows, lens)):
+        for i, pos in enumerate((1, 10, 40, L - n + 3, L - n // 2, L - 70, L - 1)):
+            if 0 <= pos < L:
+                g, o = s.slots(b, np.array([pos]))
+                x = s.V[g, o]
+                x[..., 5 + 3 * i] = value if i < 6 else -value
+                s.V[g, o] = x
+    s.gpu()
+    compare(lib, s, H, type, hd ** -0.5, win, 2 if win else 0)
+
+
+@pytest.mark.parametrize("type", [F16, BF16], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf], ids=["nan", "inf", "minus"])
+@pytest.mark.parametrize("H,start,hd,page", [(4, 7, 64, 16), (1, 31, 128, 7), (8, 3, 32, 16)])
+def test_visible_values_of_one_wave(lib, type, value, H, start, hd, page):
+    """A tile's last token, which none but rows that see all of the tile see, while others of their
+    workgroup see it in part: the 32 columns of a wave begin at position 63 or 127."""
+    t = _t()
+    s = Seqs([250], [250 + start], 1, hd, page, type)
+    for i, pos in enumerate((63, 127)):
+        x = t.full((1, 1, hd), 0.5, dtype=s.V.dtype)
+        x[..., 9 + 4 * i] = value
+        s.put(s.V, 0, np.array([pos]), x)
+    s.gpu()
+    compare(lib, s, H, type, hd ** -0.5)

@@ -178,7 +178,7 @@ template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256
                         o[k] = pg_mfma<T, 32>(vf, pr, o[k]);
                     }
                 }
-                if (odd && (every || !full)) {
+                if (odd) {                               // also where this wave's columns see all of the tile
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         pg_special<T, 32, NB>(a, o, e + 16 * t, scratch[wave], (const char *)Vc, t0 + 32 * t, rg.pmax, p, from,
