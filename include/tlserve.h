@@ -95,6 +95,8 @@ int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const void *q, lon
  * A row that sees nothing (or only scores of -inf) is 0, its lse -inf.  A row
  * that sees a token without a valid page is NaN.  Tokens that a row does not see
  * cannot reach it, whatever their slots hold, NaN and infinities too.
+ * A value that is not finite reaches its own element of the rows that see it: NaN, an infinity as
+ * it is (NaN where its weight lies below fp32's range, or against one of the other sign).
  * ws: tlg_paged_attn_ws_bytes(c, b, type, H) bytes, 16-byte aligned, of any
  * content (NULL when that is 0; it depends on B, N, ldt, max_rows and max_len, on no
  * device memory). */

@@ -113,3 +113,12 @@ def test_visible_values_of_one_wave(lib, type, value, H, start, hd, page):
         s.put(s.V, 0, np.array([pos]), x)
     s.gpu()
     compare(lib, s, H, type, hd ** -0.5)
+
+
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf], ids=["nan", "inf", "minus"])
+@pytest.mark.parametrize("H,rows,lens,hd,page,win", [
+    (1, [1], [200], 32, 16, 0), (4, [1, 3], [300, 77], 64, 7, 0), (8, [1, 2], [2600, 130], 128, 16, 0),
+    (4, [5], [400], 96, 16, 200), (4, [2], [150], 256, 16, 0), (2, [9], [100], 64, 16, 30)])
+def test_visible_values_of_few_rows(lib, type, kv, value, H, rows, lens, hd, page, win):
+    spoiled(lib, type, kv, value, H, rows, lens, hd, page, win)

@@ -209,6 +209,18 @@ template <int C> __device__ __forceinline__ bool pg_clean(unsigned &w)
     }
     return hit;
 }
+// true if anything in these registers of 16-bit elements is not finite
+template <int C, int N, int M> __device__ __forceinline__ bool pg_odd(const unsigned (&w)[N][M])
+{
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    constexpr unsigned short X = C == TLG_F16 ? 0x7c00 : 0x7f80;
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int k = 0; k < M; k++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i][k] & 0x7fff7fffu));
+    return m[0] >= X || m[1] >= X;
+}
 __device__ __forceinline__ bool pg_finite(float v) { return fabsf(v) < INFINITY; }
 
 __device__ __forceinline__ bool pg_sees(const AttnArgs &a, int t, int p, int from)

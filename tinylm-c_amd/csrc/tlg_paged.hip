@@ -397,8 +397,11 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
                 for (int i = 0; i < NE; i++) e[i] = pg_sees(a, t0 + pg_at<W>(i, g), p, from) ? e[i] : -INFINITY;
             }
             pg_weights<W, NE, NB>(e, a.c, R, l, o);
-            bool odd = false;
-            if (!full) {
+            // 16-bit rows: in every tile, for an infinite value times a weight's second piece is none
+            bool odd = !full;
+            if constexpr (!F) odd = __any(pg_odd<C, NV, VW>(vr));
+            if (odd) {
+                odd = false;
 #pragma unroll
                 for (int i = 0; i < NV; i++) {
                     bool hit = false;
