@@ -91,7 +91,8 @@ int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const void *q, lon
  * the cache); lse [N][H] may be NULL.  The
  * cache is of that type, or of any type for fp32 rows.  scale lies in 1e-30 ..
  * 1e30.  Scores, softmax and sums are fp32.  For 16-bit rows the weights e^(s - max)
- * are rounded to twice that type's bits before they meet v; fp32 rows keep fp32 products.
+ * are rounded to twice that type's bits before they meet v (fp16: or by 2^-36 of the row's largest,
+ * whichever is more); fp32 rows keep fp32 products.
  * A row that sees nothing (or only scores of -inf) is 0, its lse -inf.  A row
  * that sees a token without a valid page is NaN.  Tokens that a row does not see
  * cannot reach it, whatever their slots hold, NaN and infinities too.

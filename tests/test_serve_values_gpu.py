@@ -14,7 +14,7 @@ import math
 import numpy as np
 import pytest
 
-from test_serve_gpu import _t, BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, half, queries, run_attn, tiny
+from test_serve_gpu import _t, dtype, BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, half, queries, run_attn, tiny
 
 pytestmark = pytest.mark.gpu
 WEIGHT = {F32: 0.0, F16: 2.0 ** -22, BF16: 2.0 ** -16}
@@ -122,3 +122,23 @@ def test_visible_values_of_one_wave(lib, type, value, H, start, hd, page):
     (4, [5], [400], 96, 16, 200), (4, [2], [150], 256, 16, 0), (2, [9], [100], 64, 16, 30)])
 def test_visible_values_of_few_rows(lib, type, kv, value, H, rows, lens, hd, page, win):
     spoiled(lib, type, kv, value, H, rows, lens, hd, page, win)
+
+
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("rows,lens,H", [([1], [1000], 1), ([2, 3], [900, 2600], 4), ([150], [1000], 2)])
+def test_small_weights_of_many_tokens(lib, type, kv, rows, lens, H):
+    """One token takes nearly all of every row and has the value 0; the others' weights, e^-15
+    each and equal, round alike, and their sum is the output."""
+    t = _t()
+    s = Seqs(rows, lens, 1, 64, 16, kv)
+    for b, L in enumerate(lens):
+        k = t.zeros(L, 1, 64, dtype=s.K.dtype)
+        v = t.full((L, 1, 64), 1000.0, dtype=s.V.dtype)
+        k[3, :, 0] = 15.0
+        v[3] = 0.0
+        s.put(s.K, b, np.arange(L), k)
+        s.put(s.V, b, np.arange(L), v)
+    s.gpu()
+    q = t.zeros(s.N, H, 64, dtype=dtype(type))
+    q[..., 0] = 1.0
+    compare(lib, s, H, type, 1.0, q=q)

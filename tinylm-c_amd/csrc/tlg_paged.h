@@ -72,12 +72,15 @@ struct AttnArgs {
     float *eo, *em;
 };
 
-// Base-2 scores against a reference: with R the largest c (q . k) of a row so far,
+// Base-2 scores against a reference: with R the largest c (q . k) of a row so far less PG_LIFT,
 // rounded once, a weight is 2^(c (q . k) - R), one fused product, and whatever R is
-// exactly, it is the same for all of a row's tokens.  R stays while no score passes it by
-// more than PG_SLACK (weights up to 2^8 lose nothing in fp16, bf16 or fp32), so that
-// the sums are rarely rescaled.
-#define PG_SLACK 8.0f
+// exactly, it is the same for all of a row's tokens.  R stays while the largest weight stays below
+// 2^(PG_LIFT + PG_SLACK), so that the sums are rarely rescaled; weights up to 2^8 lose nothing in
+// bf16 or fp32.  fp16's smallest step is 2^-24: with largest weights of 2^11 to 2^15 two pieces
+// keep 22 bits of weights above 2^-14 of the row's largest and are off by 2^-36 of that at most
+// below, which many small equal weights may add up to.
+template <int T> constexpr float PG_LIFT = T == TLG_F16 ? 11.0f : 0.0f;
+template <int T> constexpr float PG_SLACK = T == TLG_F16 ? 4.0f : 8.0f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -273,15 +276,15 @@ __device__ __forceinline__ void pg_special(const AttnArgs &a, typename AccT<W>::
 
 // The running maximum of a column and what it does to its sums: z the scores of N
 // registers (hidden ones -inf), which become weights.
-template <int W, int N, int NB>
+template <int T, int W, int N, int NB>
 __device__ __forceinline__ void pg_weights(float (&z)[N], float c, float &R, float &l, typename AccT<W>::A (&o)[NB])
 {
     float m[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
     for (int i = 4; i < N; i++) m[i & 3] = fmaxf(m[i & 3], z[i]);
     const float mx = pg_gmax<W>(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) * c;
-    if (__any(mx > R + PG_SLACK)) {
-        const float n = fmaxf(R, mx), f = __builtin_amdgcn_exp2f(R - (n == -INFINITY ? 0.f : n));
+    if (__any(mx > R + (PG_LIFT<T> + PG_SLACK<T>))) {
+        const float n = fmaxf(R, mx - PG_LIFT<T>), f = __builtin_amdgcn_exp2f(R - (n == -INFINITY ? 0.f : n));
         R = n;
         l *= f;
 #pragma unroll

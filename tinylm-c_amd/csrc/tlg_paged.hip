@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
 #pragma unroll
                 for (int i = 0; i < NE; i++) e[i] = pg_sees(a, t0 + pg_at<W>(i, g), p, from) ? e[i] : -INFINITY;
             }
-            pg_weights<W, NE, NB>(e, a.c, R, l, o);
+            pg_weights<T, W, NE, NB>(e, a.c, R, l, o);
             // 16-bit rows: in every tile, for an infinite value times a weight's second piece is none
             bool odd = !full;
             if constexpr (!F) odd = __any(pg_odd<C, NV, VW>(vr));
@@ -435,7 +435,8 @@ __global__ __launch_bounds__(256, (T == TLG_F32 && HD * (W == 32 || C == TLG_F32
                 if (more) loadV(buf ^ 1);
                 pg_wave_sync();
                 // weights in two pieces, what rounding takes from the first one and that: the products
-                // then keep 16 (bf16) or 22 bits of them, in time that the cache's bytes take anyway
+                // then keep 16 (bf16) or 22 bits of them (small fp16 ones fewer, PG_LIFT), in time that the cache's
+                // bytes take anyway
                 u32x4 pf[NE / 8], pr[NE / 8];
 #pragma unroll
                 for (int i = 0; i < NE / 2; i++) pg_split<T>(e[2 * i], e[2 * i + 1], pf[i / 4], pr[i / 4], i & 3);

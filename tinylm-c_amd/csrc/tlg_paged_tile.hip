@@ -160,7 +160,7 @@ template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256
                         for (int i = 0; i < 16; i++)
                             e[16 * t + i] = pg_sees(a, t0 + 32 * t + pg_at<32>(i, h), p, from) ? e[16 * t + i] : -INFINITY;
                 }
-                pg_weights<32, 16 * NT, NB>(e, a.c, R, l, o);
+                pg_weights<T, 32, 16 * NT, NB>(e, a.c, R, l, o);
                 const E *vt = vs[buf] + (4 * h + (lane >> 2 & 3)) * VST + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
 #pragma unroll
                 for (int i = 0; i < 2 * NT; i++) {
