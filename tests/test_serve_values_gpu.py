@@ -14,7 +14,7 @@ import math
 import numpy as np
 import pytest
 
-from test_serve_gpu import _t, dtype, BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, half, queries, run_attn, tiny
+from test_serve_gpu import _t, BF16, EPS, F16, F32, NAMES, PAIR_IDS, PAIRS, Seqs, check, dtype, half, ints, queries, run_attn, tiny
 
 pytestmark = pytest.mark.gpu
 WEIGHT = {F32: 0.0, F16: 2.0 ** -22, BF16: 2.0 ** -16}
@@ -142,3 +142,29 @@ def test_small_weights_of_many_tokens(lib, type, kv, rows, lens, H):
     q = t.zeros(s.N, H, 64, dtype=dtype(type))
     q[..., 0] = 1.0
     compare(lib, s, H, type, 1.0, q=q)
+
+
+@pytest.mark.parametrize("type,kv", [(F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("N", [32768, 65536])
+def test_decreasing_rows_whose_tiles_pass_32_bits(lib, type, kv, N):
+    """row0 must not decrease; where it does, so that 512 of 1024 sequences have all rows, their tiles number
+    more than 2^31 or 2^32: nothing is taken part in and nothing is written."""
+    s = Seqs([1] * 1024, [1] * 1024, 1, 32, 64, kv, extra_ldt=1031)
+    s.N = N
+    s.gpu()
+    s.dev[0].copy_(ints([0, N] * 512 + [0]))
+    s.dev[1].fill_(66000)
+    s.batch.N, s.batch.max_rows, s.batch.max_len = N, 1, 0
+    out, ls = run_attn(lib, s, queries(s, 1, type), 1, type, 0.2)
+    assert (out == 7.0).all() and (ls == 7.0).all()
+
+
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+def test_decreasing_rows(lib, type, kv):
+    """Sequences that share rows, over shares of the batch: any of them may have a row, rows of none
+    are left alone."""
+    s = Seqs([6, 2, 4], [2600, 2500, 2400], 1, 32, 16, kv, tail=3).gpu()
+    s.dev[0].copy_(ints([0, 9, 2, 12]))
+    s.batch.max_rows = 2
+    out, ls = run_attn(lib, s, queries(s, 2, type), 2, type, 0.2)
+    assert (out[12:] == 7.0).all() and (ls[12:] == 7.0).all()

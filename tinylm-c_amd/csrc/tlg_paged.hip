@@ -126,16 +126,19 @@ __device__ __forceinline__ int pg_units(const AttnArgs &a, const Seq &q)
     const int cols = q.n * a.G;
     return cols > a.few && cols <= a.many ? max(1, pg_range<32>(a, q, 0, cols).total) : 0;
 }
-// Where each sequence's units start, [B + 1] in LDS (their number stays below 2^31, the
-// host sees to it); the workgroups that take part, each with PG_UNITS at least.  B <=
-// PG_EVEN, 256 threads.
+// Where each sequence's units start, [B + 1] in LDS; the workgroups that take part, each with
+// PG_UNITS at least.  B <= PG_EVEN, 256 threads.  The units number less than 2^31, the host
+// sees to it, unless row0 decreases and sequences share rows: then none takes part.
 #define PG_EVEN 1024
 #define PG_UNITS 4
 template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, int *place)
 {
-    __shared__ int part[4], with[4];
+    __shared__ unsigned part[4];
+    __shared__ int with[4];
+    auto add = [](unsigned x, unsigned y) { return __builtin_elementwise_add_sat(x, y); };
     const int t = threadIdx.x, per = (a.b.B + 255) / 256, lane = t & 63;
-    int n[PG_EVEN / 256], sum = 0, some = 0;
+    unsigned n[PG_EVEN / 256], sum = 0;
+    int some = 0;
 #pragma unroll
     for (int i = 0; i < PG_EVEN / 256; i++) {
         n[i] = 0;
@@ -143,26 +146,27 @@ template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, int
             const Seq q = pg_seq(a.b, t * per + i);
             n[i] = pg_units(a, q) * ((q.n * a.G + W - 1) / W);
         }
-        sum += n[i];
+        sum = add(sum, n[i]);
         some += __popcll(__ballot(n[i] > 0));
     }
-    int upto = sum;
+    unsigned upto = sum;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-        const int v = __shfl_up(upto, o);
-        upto += lane >= o ? v : 0;
+        const unsigned v = __shfl_up(upto, o);
+        upto = add(upto, lane >= o ? v : 0);
     }
     if (lane == 63) {
         part[t >> 6] = upto;
         with[t >> 6] = some;
     }
     __syncthreads();
-    int all = 0;
+    unsigned all = 0;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
-        if (w == t >> 6) upto += all;
-        all += part[w];
+        if (w == t >> 6) upto = add(upto, all);
+        all = add(all, part[w]);
     }
+    if (all > INT_MAX) return 0;
     upto -= sum;
 #pragma unroll
     for (int i = 0; i < PG_EVEN / 256; i++) {
@@ -173,8 +177,8 @@ template <int W> __device__ __forceinline__ int pg_places(const AttnArgs &a, int
     __syncthreads();
     // Small shares of equal sequences are cut alike: a second sequence in a share costs its
     // workgroup about 4 us, as much as 8 tiles or more.
-    const int seqs = with[0] + with[1] + with[2] + with[3], P = min(a.P, max(all / PG_UNITS, all > 0));
-    return P > seqs && all < 32 * P ? P / seqs * seqs : P;
+    const int seqs = with[0] + with[1] + with[2] + with[3], P = min(a.P, max((int)all / PG_UNITS, all > 0 ? 1 : 0));
+    return P > seqs && (int)all < 32 * P ? P / seqs * seqs : P;
 }
 // Share y of T units over P: the first T % P have one more.
 __device__ __forceinline__ int pg_share(int T, int P, int y) { return T / P * y + min(y, T % P); }
