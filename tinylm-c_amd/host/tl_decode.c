@@ -642,6 +642,20 @@ int tl_decode_generate_spec(TlDecode *d, const int *prompt, int np, int n, int *
     return 0;
 }
 
+/* Drafts that may go behind the token at position pos.  A draft's key lies where the token W
+ * positions before it was, so either the ring holds every position up to the last draft's, or
+ * every layer's window ends above that token. */
+static int spec_room(const TlDecode *d, int pos)
+{
+    int widest = 0;
+    for (int l = 0; l < d->m.L; l++) {
+        const int win = dwin(&d->m, l), sees = win && win < d->W ? win : d->W;
+        if (sees > widest) widest = sees;
+    }
+    const int below = d->W - 1 - pos, behind = d->W - widest;
+    return below > behind ? below : behind;
+}
+
 /* Number i of the stream of 64-bit numbers with the given seed (splitmix64). */
 static unsigned long long spec_bits(unsigned long long seed, unsigned long long i)
 {
@@ -735,6 +749,7 @@ int tl_decode_sample_spec(TlDecode *d, const int *prompt, int np, int n, float t
         /* the last token and the heads' drafts of what follows it, no more than are asked for */
         int k = n - got - 1 < heads ? n - got - 1 : heads;
         if (k > d->maxpos - pos - 1) k = d->maxpos - pos - 1;
+        if (k > spec_room(d, pos)) k = spec_room(d, pos);
         for (int h = 0; !rc && h < k; h++) rc = tl_decode_mtp_draft(d, cur, h, d->dtok + h, st);
         if (!rc && k) rc = tlg_memcpy_d2h(feed + 1, d->dtok, 4 * (size_t)k, st);
         if (!rc) rc = tlg_stream_sync(st);

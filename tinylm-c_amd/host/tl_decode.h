@@ -96,6 +96,10 @@ int tl_decode_generate_spec(TlDecode *d, const int *prompt, int np, int n, int *
  * 1e-29 .. 1e29, whatever the heads draft.  The n_mtp heads' greedy drafts (none with
  * n_mtp = 0; at most mmax - 1 are used) go through one chunk behind the last token,
  * and tlg_dev_spec_verify (include/tlserve.h) keeps them or puts a sample in their place.
+ * Once the ring is full, no draft is fed that would take the slot of a token still seen: at
+ * most W less the widest layer's window (none with a layer that sees the whole ring), so
+ * that W >= np + n - 1 keeps all drafts.  A prompt longer than W is fed as tl_decode_prime
+ * feeds it, in chunks whose rows take the slots of their oldest tokens.
  * logp (host [n], or NULL): the tokens' log probabilities at that temperature.  Numbers: with s(i)
  * = splitmix64's number i of `seed` (the finalizer of seed + (i + 1) 0x9E37..15), call c of
  * the verification, the prompt's last row being call 0, takes as uniform of its row r (s(c
