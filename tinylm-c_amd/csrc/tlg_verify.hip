@@ -348,18 +348,26 @@ template <int TYPE> __global__ __launch_bounds__(64) void k_sv_join(SvArgs a)
 
 // -------------------------------------------------------------------- entries --
 // Rows of up to SV_SHORT vectors are one workgroup's a sequence, twice as long ones from
-// SV_CROWD sequences on.  In a graph that gains where sequences fill the chip (256 of 5 rows of 4096
-// fp32 values 13.2 us, in two launches 16.6; of 2048 values 11.4 and 12.1) and costs little where
-// they do not (one of 3 rows of 2048 8.8 and 8.7, 16 of 5 rows 9.6 and 9.1; of 4000 values 10.8 and
-// 9.9); a call from the host saves the second launch, 2.8 us.  Longer rows are cut until
-// enough workgroups work: a race's threads wait for every round of loads, so its pieces
+// SV_CROWD sequences on, where there are no more sequences than CUs and a sequence has SV_SUMS sums
+// (rows, twice with a draft model) in the mean, one of each wave, or from SV_CROWD on four.  In a
+// graph that gains where sequences fill the chip (256 of 5 rows of 4096 fp32 values 14.8 us, in two
+// launches 18.0; of 2048 values 11.7 and 12.4, of 32 rows 24.5 and 24.7) and costs little where they do
+// not (one of 3 rows of 2048 8.8 and 8.7, of 16 rows 10.0 and 9.1; 16 of 16 rows 11.5 and 9.9); a call from
+// the host saves the second launch, 2.8 us.  More rows leave the chip idle (one sequence of 64 rows
+// 18.5 and 10.0, of 2048 285 and 34; 128 of 256 rows of both models 127 and 104), more sequences
+// wait for each other's barriers (384 of 5 rows 17.6 and 13.6, 2048 64 and 35).  Longer rows are cut
+// until enough workgroups work: a race's threads wait for every round of loads, so its pieces
 // are smaller.
 #define SV_SHORT 512
 #define SV_CROWD 128
-static bool sv_short(int type, int V, int B)
+#define SV_MOST 256
+#define SV_SUMS 16
+static bool sv_short(int type, int N, int V, int B, int drafted)
 {
     const int nv = V / (type == TLG_F32 ? 4 : 8);
-    return nv <= SV_SHORT || (nv <= 2 * SV_SHORT && B >= SV_CROWD);
+    const bool crowd = B >= SV_CROWD;
+    return nv <= (crowd ? 2 : 1) * SV_SHORT && B <= SV_MOST &&
+           (long long)N * (drafted ? 2 : 1) <= (long long)B * SV_SUMS * (crowd ? 4 : 1);
 }
 static int sv_cut(int type, long long rows, int V, int piece, int fill)
 {
@@ -369,8 +377,9 @@ static int sv_cut(int type, long long rows, int V, int piece, int fill)
 }
 static size_t sv_layout(int type, int N, int V, int B, int drafted, int *S, int *T, size_t *best, size_t *info)
 {
-    *S = sv_short(type, V, B) ? 1 : sv_cut(type, (long long)N * (drafted ? 2 : 1), V, 1024, 1024);
-    *T = sv_short(type, V, B) ? 1 : sv_cut(type, B, V, 512, 1024);
+    const bool one = sv_short(type, N, V, B, drafted);
+    *S = one ? 1 : sv_cut(type, (long long)N * (drafted ? 2 : 1), V, 1024, 1024);
+    *T = one ? 1 : sv_cut(type, B, V, 512, 1024);
     *best = ((size_t)N * 2 * *S * sizeof(SvSum) + 15) & ~(size_t)15;
     *info = *best + (*T > 1 ? (size_t)B * *T * 16 : 0);
     return *info + (*T > 1 ? (size_t)B * 16 : 0);
@@ -386,7 +395,7 @@ extern "C" size_t tlg_spec_verify_ws_bytes(int type, int N, int V, int B, int dr
 
 template <int TYPE> static void sv_launch(const SvArgs &a, hipStream_t st)
 {
-    if (sv_short(TYPE, a.V, a.B)) {
+    if (sv_short(TYPE, a.N, a.V, a.B, a.y != nullptr)) {
         hipLaunchKernelGGL((k_sv_short<TYPE>), dim3((unsigned)a.B), dim3(1024), 0, st, a);
         return;
     }
