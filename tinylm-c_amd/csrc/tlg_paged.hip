@@ -46,9 +46,13 @@ template <int T> __device__ __forceinline__ void st_put(char *p, const float *x)
 
 // A workgroup takes up to ST_ROWS consecutive rows; a thread eight pairs (i, i + hd/2) of
 // a head.  Bound by the bytes of many rows (16384 rows of 48 heads of 128 bf16 values: 71
-// us, 5.0 TB/s, a copy reaches 5.4), by the chain sequence - page - row of few, which one row
-// a workgroup keeps shortest (209 such rows: 6.0 us, 10.0 with four).
+// us, 5.7 TB/s, a copy reaches 5.4), by the chain sequence - page - row of few, which one row
+// a workgroup keeps shortest (300 such rows: 6.1 us, 9.7 with four; 16384 71 and 74).  Only many
+// rows that leave half of a workgroup's threads without work are taken in fours: 24 heads of 64 fp16
+// values, one / four: 300 rows 3.7 / 4.4 us, 1024 5.2 / 6.0, 4000 10.4 / 9.2, 16384 29.9 / 26.7; 18 of
+// 32 fp32 3.7 / 3.8, 4.9 / 4.9, 8.7 / 7.9, 26.4 / 22.8; 48 of 64 bf16 4.0 / 5.7, 6.1 / 7.4, 15.9 / 15.4, 42.5 / 42.4.
 #define ST_ROWS 4
+#define ST_MANY 4096
 template <int T, int C> __global__ __launch_bounds__(256) void k_paged_store(StoreArgs a)
 {
     constexpr int ts = T == TLG_F32 ? 4 : 2, cs = C == TLG_F32 ? 4 : 2;
@@ -705,7 +709,7 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
     a.cs = cos_t;
     a.sn = sin_t;
     a.maxpos = maxpos;
-    a.per = b->N >= 4096 ? ST_ROWS : 1;
+    a.per = b->N >= ST_MANY && (a.H + 2 * a.KV) * (a.hd / 16) <= 128 ? ST_ROWS : 1;
     const dim3 grid((b->N + a.per - 1) / a.per), block(256);
     hipStream_t st = ST(stream);
     if (type == TLG_F16) hipLaunchKernelGGL((k_paged_store<TLG_F16, TLG_F16>), grid, block, 0, st, a);
