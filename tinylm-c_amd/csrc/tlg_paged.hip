@@ -722,29 +722,56 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 }
 
 // How a call is launched: the columns (rows times heads of a KV head) of a sequence
-// decide.  few (up to PG_FEW): only k_paged_direct; else the rows' kernel, and, where the
-// numbers of rows differ, the former for the sequences of few.  8 sequences of 8192 tokens,
-// 32 / 8 heads of 128 bf16: 24 columns 65 us so and 83 by the rows' kernel, 32 67 and 62, 36 81 and 65
-// (32 sequences of 1024: 44 and 42, 47 and 45, 66 and 48).
+// decide.  few: only k_paged_direct; else the rows' kernel, and, where that helps (both) and the
+// numbers of rows differ, the former for the sequences of few.
+// 16-bit rows are few up to PG_FEW.  us by k_paged_direct / by the rows' kernel, 32 / 8 heads:
+//   columns                         24         32         36         48
+//   8 x 8192 tokens, 128 bf16   64.9/88.9  66.6/64.4  80.0/68.2  81.2/69.7
+//   32 x 1024                   43.2/43.9  46.9/46.7  66.5/55.5  70.1/56.1
+//   4 x 300                     13.1/18.7  13.3/18.7  22.3/18.8  22.7/18.9
+//   8 x 8192, 64 fp16           43.6/44.8  44.2/39.5  55.1/45.9  56.2/49.6
+//   32 x 1024                   31.9/33.6  34.0/35.8  45.7/39.0  48.8/39.3
+//   8 x 8192, 32 fp16           34.5/36.7  34.8/33.2  40.9/39.0  41.5/41.8
+//   8 x 8192, 256 bf16           137/240    139/185    255/188    256/190
+// fp32 rows up to twice that, over sequences of more than PG_SHORT tiles:
+//   columns                         36         64         68        128
+//   32 x 1024, 128 fp32          148/219    163/236    219/288    301/442
+//   8 x 1000                      55/62      62/65      79/67     111/76
+//   4 x 300                       49/60      51/61      72/61      96/63
+//   8 x 8192, 32 over fp16        71/80      72/91     101/109    129/157
+//   8 x 1000                      25/28      27/30      34/30      46/33
+//   4 x 300                       23/20      24/21      33/20      43/21
+// both: over more than PG_SHORT tiles, for a row over many tokens must not be left to one of the
+// rows' kernel's workgroups.  us in two launches / by the rows' kernel alone, 32 / 8 heads:
+//   tokens of each                   256       512      1024       4000
+//   4 x 60 rows, 60 x 1, 128 bf16   39/32     58/49     97/84    273/256
+//                        64 fp16    27/18     40/27     65/42    178/138
+//                        256 bf16   71/85    109/142   188/257   516/804
+//                        128 fp32  102/147   137/253   203/458
+//                        32 fp32    38/32     59/56     80/86    230/282     (over fp16)
+//   2048 rows, 1 row over 8192 and 65536, 128 bf16: 154/290, 461/2144; 64 fp16 97/191, 165/1407
 // k_paged_direct's workgroups share the batch's tokens evenly from PG_LONG tiles of a
-// sequence on (64 sequences of 1024 to 4096 tokens: 124 us against 133 where each is cut
-// alike), unless there are sequences enough; below, where looking up the batch costs more than
-// that gains, each sequence is cut alike (32 sequences of 5 rows that see 1028 tokens:
-// 18 us against 24).
+// sequence on (64 sequences of 1024 to 4096 tokens: 139 us against 148 where each is cut
+// alike; of 525 to 2100 74 and 72), up to PG_MANY sequences times KV heads (200 of 525 to 2100: 227 and
+// 207, the price of batches of one long sequence among short ones; 512 547 and 500) and PG_EVEN
+// sequences, what the table of places holds; below PG_LONG, where looking up the batch costs
+// more than that gains, each is cut alike (32 sequences of 5 rows that see 1028 tokens: 18 us against 24).
 // fp32 rows take blocks of 16 columns a wave where those of 32 do not fill the chip (4
 // prompts of 256 rows, 8 heads of 32: 14 us, 18 in blocks of 32; of 128 elements 68 and 58, so not there).
 // Many rows' partial sums cost more than their tokens' division gains, unless the
 // chip is not filled or every part is long (4 prompts of 300 rows, 32 heads of 128 bf16: 28 us
-// whole, 68 in two parts; 512 rows over 8192 tokens 120 us in seven parts, 129 in five).
+// whole, 68 in two parts; 512 rows over 8192 tokens 120 us in seven parts, 129 in five; before weights
+// were in two pieces).
 #define PG_FEW 32
 #define PG_FILL 512                  /* workgroups wanted of k_paged_direct: two a CU */
 #define PG_FILL_TILE 384             /* of k_paged_tile                     */
 #define PG_FILL_ROWS 1024            /* of k_paged_direct for fp32 rows: short waves, one SIMD each */
 #define PG_LONG 64                   /* tiles of 32 tokens                  */
-#define PG_SHORT 16                  /* tiles that the rows' kernels take for sequences of few rows too */
+#define PG_SHORT 16                  /* tiles up to which the rows' kernels take sequences of few rows too */
 #define PG_MANY 2048                 /* sequences times KV heads that need no sharing */
 struct Plan {
     bool few, both;
+    int border;                      // columns of the sequences that are k_paged_direct's
     int W;                           // columns of a workgroup of few
     int wide;                        // of a workgroup of the rows' kernel
     unsigned slots;                  // and how many
@@ -772,7 +799,9 @@ static Plan pg_plan(const TlgPages *c, const TlgBatch *b, int type, int H, int w
                     most = b->max_len && b->max_len < room ? b->max_len : room,
                     seen = win ? (long long)win + rows + (sinks < most ? sinks : most) + 64 : most,
                     tiles = ((seen < most ? seen : most) + 31) / 32, row = (long long)b->N * H * (c->hd + 2) * 4;
-    p.few = cols <= PG_FEW;
+    // by the tokens that there are, not those in a window: the workspace is sized without one
+    p.border = type == TLG_F32 && most > 32 * PG_SHORT ? 2 * PG_FEW : PG_FEW;
+    p.few = cols <= p.border;
     p.W = cols <= 16 || c->hd == 256 ? 16 : 32;            // 32 of 256 elements do not fit the registers
     p.wide = PGT_ROWS;
     if (type == TLG_F32 && (c->hd == 256 || (c->hd <= 64 && ((long long)b->N * G / 128 + b->B) * c->KV < PG_FILL))) p.wide = 64;
@@ -877,7 +906,11 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
     if (!pg_rows(q, ldq, w, type) || !pg_rows(out, ldo, w, type) || (lse && !pg_al(lse, 4)))
         return tlg_fail(TLG_EINVAL, "paged_attn: q %p ldq=%lld out %p ldo=%lld lse %p", q, ldq, out, ldo, (void *)lse);
     if (pg_meet(q, ldq, out, ldo, w, type, b->N)) return tlg_fail(TLG_EINVAL, "paged_attn: out overlaps q");
-    const size_t need = tlg_paged_attn_ws_bytes(c, b, type, H);
+    a.win = win < TLG_PAGED_LEN + 1 ? win : 0;            // a longer one hides nothing
+    a.sinks = sinks < TLG_PAGED_LEN ? sinks : TLG_PAGED_LEN;
+    const Plan p = pg_plan(c, b, type, H, a.win, a.sinks, false);
+    size_t need = tlg_paged_attn_ws_bytes(c, b, type, H);
+    if (p.bytes > need) need = p.bytes;                  // never: a window only lessens the plan's parts
     if (need && (ws_bytes < need || !pg_al(ws, 16)))
         return tlg_fail(TLG_EINVAL, "paged_attn: workspace %p of %zu bytes, %zu needed", ws, ws_bytes, need);
     if ((rc = tlg_ensure_init())) return rc;
@@ -891,14 +924,11 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
     a.H = H;
     a.KV = c->KV;
     a.G = H / c->KV;
-    a.win = win < TLG_PAGED_LEN + 1 ? win : 0;            // a longer one hides nothing
-    a.sinks = sinks < TLG_PAGED_LEN ? sinks : TLG_PAGED_LEN;
     a.c = (float)((double)scale * 1.4426950408889634);
     if (c->n_pages == 0) {               // no token has a page: any readable memory stands for the first
         a.K = a.V = a.q;
         a.b.head_ld = 0;
     }
-    const Plan p = pg_plan(c, b, type, H, a.win, a.sinks, false);
     a.P = p.P;
     a.po = (float *)ws;
     a.pm = (float *)((char *)ws + p.pm);
@@ -908,7 +938,7 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
     hipStream_t st = ST(stream);
     if (p.few || p.both) {
         a.few = 0;
-        a.many = p.few ? INT_MAX : PG_FEW;
+        a.many = p.few ? INT_MAX : p.border;
         a.S = p.Sf;
         a.per = p.perf;
         const dim3 grid((unsigned)(p.P ? p.P : b->B * p.Sf) * c->KV);
@@ -918,7 +948,7 @@ extern "C" int tlg_dev_paged_attn(const TlgPages *c, const TlgBatch *b, const vo
         else if (p.Sf > 1) pg_join<false>(a, type, c->hd, p.W, 0, st);
     }
     if (!p.few) {
-        a.few = p.both ? PG_FEW : 0;
+        a.few = p.both ? p.border : 0;
         a.many = INT_MAX;
         a.S = p.S;
         a.per = p.per;
