@@ -93,6 +93,8 @@ int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const void *q, lon
  * 1e30.  Scores, softmax and sums are fp32.  For 16-bit rows the weights e^(s - max)
  * are rounded to twice that type's bits before they meet v (fp16: or by 2^-36 of the row's largest,
  * whichever is more); fp32 rows keep fp32 products.
+ * Sums of weights of up to 2^8 (fp16: 2^15) times values are formed before they are divided, so that
+ * values up to 1e27 cannot overflow.
  * A row that sees nothing (or only scores of -inf) is 0, its lse -inf.  A row
  * that sees a token without a valid page is NaN.  Tokens that a row does not see
  * cannot reach it, whatever their slots hold, NaN and infinities too.

@@ -168,3 +168,14 @@ def test_decreasing_rows(lib, type, kv):
     s.batch.max_rows = 2
     out, ls = run_attn(lib, s, queries(s, 2, type), 2, type, 0.2)
     assert (out[12:] == 7.0).all() and (ls[12:] == 7.0).all()
+
+
+@pytest.mark.parametrize("type,kv", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("rows,lens", [([12, 1, 16], [700, 600, 900]), ([16, 9], [2600, 150]), ([100, 12, 16, 17, 1], [600, 2500, 700, 90, 650])])
+def test_rows_around_the_launches_borders(lib, type, kv, hd, rows, lens):
+    """32 and 64 columns a sequence and some more and fewer, alone and beside longer chunks, each cut alike
+    and shared evenly."""
+    s = Seqs(rows, lens, 1, hd, 16, kv, head_major=True, lead=1, tail=1).gpu()
+    compare(lib, s, 4, type, hd ** -0.5)
+    compare(lib, s, 4, type, hd ** -0.5, 300, 5)
