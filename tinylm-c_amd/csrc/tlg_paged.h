@@ -116,11 +116,13 @@ template <int T> __device__ __forceinline__ unsigned pg_pack(float lo, float hi)
     return __builtin_bit_cast(unsigned, v);
 }
 // Two weights as register k of two operands whose sum they are to twice the type's bits: rounded, and
-// what that took from them (exact in fp32), rounded.
+// what that took from them (exact in fp32), rounded.  (The barrier: the compiler would round each
+// weight by itself a second time to have it as a float.)
 template <int T> __device__ __forceinline__ void pg_split(float x, float y, u32x4 &hi, u32x4 &lo, int k)
 {
+    unsigned w = pg_pack<T>(x, y);
+    asm("" : "+v"(w));
     typedef typename ElT<T>::E e2 __attribute__((ext_vector_type(2)));
-    const unsigned w = pg_pack<T>(x, y);
     const e2 back = __builtin_bit_cast(e2, w);
     hi[k] = w;
     lo[k] = pg_pack<T>(x - (float)back[0], y - (float)back[1]);
