@@ -726,13 +726,13 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 // numbers of rows differ, the former for the sequences of few.
 // 16-bit rows are few up to PG_FEW.  us by k_paged_direct / by the rows' kernel, 32 / 8 heads:
 //   columns                         24         32         36         48
-//   8 x 8192 tokens, 128 bf16   64.9/88.9  66.6/64.4  80.0/68.2  81.2/69.7
-//   32 x 1024                   43.2/43.9  46.9/46.7  66.5/55.5  70.1/56.1
-//   4 x 300                     13.1/18.7  13.3/18.7  22.3/18.8  22.7/18.9
-//   8 x 8192, 64 fp16           43.6/44.8  44.2/39.5  55.1/45.9  56.2/49.6
-//   32 x 1024                   31.9/33.6  34.0/35.8  45.7/39.0  48.8/39.3
-//   8 x 8192, 32 fp16           34.5/36.7  34.8/33.2  40.9/39.0  41.5/41.8
-//   8 x 8192, 256 bf16           137/240    139/185    255/188    256/190
+//   8 x 8192 tokens, 128 bf16   65.3/88.2  66.5/64.2  79.6/67.5  80.5/68.0
+//   32 x 1024                   43.3/44.0  46.8/46.7  66.4/54.8  70.0/55.3
+//   4 x 300                     13.0/18.5  13.2/18.5  22.1/18.7  22.5/18.7
+//   8 x 8192, 64 fp16           43.5/44.7  44.1/38.6  54.6/44.7  55.2/48.4
+//   32 x 1024                   31.7/33.2  34.3/35.4  45.6/37.8  48.6/37.9
+//   8 x 8192, 32 fp16           34.5/36.2  34.8/33.2  40.4/37.8  40.8/40.2
+//   8 x 8192, 256 bf16           138/236    138/181    257/186    255/186
 // fp32 rows up to twice that, over sequences of more than PG_SHORT tiles:
 //   columns                         36         64         68        128
 //   32 x 1024, 128 fp32          148/219    163/236    219/288    301/442
@@ -744,12 +744,12 @@ extern "C" int tlg_dev_paged_store(const TlgPages *c, const TlgBatch *b, const v
 // both: over more than PG_SHORT tiles, for a row over many tokens must not be left to one of the
 // rows' kernel's workgroups.  us in two launches / by the rows' kernel alone, 32 / 8 heads:
 //   tokens of each                   256       512      1024       4000
-//   4 x 60 rows, 60 x 1, 128 bf16   39/32     58/49     97/84    273/256
-//                        64 fp16    27/18     40/27     65/42    178/138
-//                        256 bf16   71/85    109/142   188/257   516/804
+//   4 x 60 rows, 60 x 1, 128 bf16   39/32     58/49     97/84    291/263
+//                        64 fp16    27/18     40/26     64/42    185/141
+//                        256 bf16   71/84    109/141   189/253   536/798
 //                        128 fp32  102/147   137/253   203/458
-//                        32 fp32    38/32     59/56     80/86    230/282     (over fp16)
-//   2048 rows, 1 row over 8192 and 65536, 128 bf16: 154/290, 461/2144; 64 fp16 97/191, 165/1407
+//                        32 fp32    38/32     59/56     80/86              (over fp16)
+//   2048 rows, 1 row over 8192 and 65536, 128 bf16: 129/284, 170/2110; 64 fp16 92/183, 113/1356
 // k_paged_direct's workgroups share the batch's tokens evenly from PG_LONG tiles of a
 // sequence on (64 sequences of 1024 to 4096 tokens: 139 us against 148 where each is cut
 // alike; of 525 to 2100 74 and 72), up to PG_MANY sequences times KV heads (200 of 525 to 2100: 227 and

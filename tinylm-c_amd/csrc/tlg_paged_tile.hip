@@ -9,18 +9,19 @@
 // apart by what makes the reads free of bank conflicts: keys are read 16 bytes a lane
 // down 16 tokens (row lengths 4 modulo 64 banks), values four tokens by 32 elements
 // (16 modulo 32 banks).
-// Measured: 4096 rows over 16384 tokens, 32 query and 8 KV heads of 128 bf16 values, 1.47 to 1.52
-// ms, 633 to 654 TFLOP/s of the operator's own products (a large library product: 1210).  The
-// weights are in two pieces as k_paged_direct's, which is half of the products again: rounded to
-// bf16 once they took 1.16 to 1.18 ms and left a norm error of 0.0023, where the output's own rounding is
-// 0.0017.  Exponentials and splits dealt out between the products, by hand or by
-// scheduling barriers, took 1.47 to 1.53 ms.
+// Measured: 4096 rows over 16384 tokens, 32 query and 8 KV heads of 128 bf16 values, 1.45 to 1.5
+// ms, 640 to 662 TFLOP/s of the operator's own products (a large library product: 1210); matrix cores 47 %
+// busy, vector ALUs 42 %, which follow each other within a wave.  The weights are in two pieces as
+// k_paged_direct's, half of the products again: rounded to bf16 once they took 1.16 to 1.18
+// ms and left a norm error of 0.0023, where the output's own rounding is 0.0017.  Exponentials and splits
+// dealt out between the products, by hand or by scheduling barriers, were no faster (1.47
+// to 1.53 ms against 1.48).
 #include "tlg_paged.h"
 #include <type_traits>
 
 // ALIKE: the 16 bytes that a wave brings in one go, up to 16 tokens' in a row, lie on one page (pages
 // of a multiple of 16 tokens): their address is then one scalar and an offset that the
-// lane keeps (207 M vector instructions in place of 343 M, 1276 -> 1162 us).
+// lane keeps (with weights in one piece: 207 M vector instructions in place of 343 M, 1276 -> 1162 us).
 template <int T, int HD, bool ALIKE> __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_tile(AttnArgs a)
 {
     typedef typename ElT<T>::E E;
